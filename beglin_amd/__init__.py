@@ -8,7 +8,8 @@ import ctypes as C
 
 from . import capi
 from .capi import (ACT_F32, ACT_W4A8, K_F16, K_F32, K_MXFP4, K_Q4G32H, K_Q4G64, K_Q4G64A,  # noqa: F401
-                   K_Q4G256P, K_Q4G256SF, K_Q8G64, K_QNG64)
+                   K_Q4G256P, K_Q4G256SF, K_Q8C, K_Q8G64, K_QNG64, NORM_LAYER, NORM_NONE, NORM_RMS, T_BF16,
+                   T_F16, T_F32)
 
 _lib = None
 
@@ -43,6 +44,36 @@ def _p(t):
         assert t.is_contiguous(), "tensor must be contiguous"
         return C.c_void_p(t.data_ptr())
     return C.c_void_p(t.ctypes.data)
+
+
+_DT = None
+
+
+def _dtypes():
+    """torch's fp32, fp16, bf16 (at their BGL_T_* places) and int8."""
+    global _DT
+    if _DT is None:
+        import torch
+        _DT = (torch.float32, torch.float16, torch.bfloat16, torch.int8)
+    return _DT
+
+
+def _type(t):
+    return _dtypes().index(t.dtype, 0, 3)
+
+
+def _rows(t, T, H):
+    """Elements between the rows of a [T][H] tensor whose rows are dense."""
+    assert t.shape == (T, H) and (t.stride(1) == 1 or H == 1), "rows must be dense, [T][H]"
+    return t.stride(0) if T > 1 else H
+
+
+def _vec(t, n):
+    """Pointer of an fp32 vector of n values, None passes through."""
+    if t is None:
+        return None
+    assert t.dtype == _dtypes()[0] and t.numel() == n and t.is_contiguous(), "fp32 vector expected"
+    return t.data_ptr()
 
 
 class Tensor:
@@ -109,7 +140,7 @@ class Context:
     def bind(self, kind, packed, scales, out, inn, bits=0, sub=None):
         """Bind host (numpy) buffers in the reference layout (sub: g256sf sub-codes or Q4G64A biases;
         scales None for the dense kinds and MXFP4, whose blocks carry their exponents)."""
-        w = capi.bgl_wt(kind, bits if kind == K_QNG64 else (8 if kind == K_Q8G64 else 4), out, inn,
+        w = capi.bgl_wt(kind, bits if kind == K_QNG64 else (8 if kind in (K_Q8G64, K_Q8C) else 4), out, inn,
                         packed.ctypes.data, scales.ctypes.data if scales is not None else None,
                         sub.ctypes.data if sub is not None else None)
         h = C.c_void_p()
@@ -134,7 +165,7 @@ class Context:
         if want_ref:
             if kind in (K_Q4G64, K_Q4G256SF, K_Q4G32H):
                 pk = np.zeros((out, inn // 2), np.uint8)
-            elif kind == K_Q8G64:
+            elif kind in (K_Q8G64, K_Q8C):
                 pk = np.zeros((out, inn), np.int8)
             else:
                 pk = np.zeros((out, inn // 64 * bits * 8), np.uint8)
@@ -142,6 +173,8 @@ class Context:
                 sc = np.zeros((out, inn // 32), np.uint16)
             elif kind == K_Q4G256SF:
                 sc = np.zeros((out, inn // 256), np.float32)
+            elif kind == K_Q8C:
+                sc = np.zeros(out, np.float32)
             else:
                 sc = np.zeros((out, inn // 64), np.float32)
             sub = np.zeros((out, inn // 64), np.uint8) if kind == K_Q4G256SF else None
@@ -191,6 +224,48 @@ class Context:
         _check(lib().bgl_quant_act_i8_dev(self.h, _p(x_dev), M, x_dev.shape[-1], gsize, _p(xq_dev), _p(ascale_dev)),
                "bgl_quant_act_i8_dev")
 
+    # ---- int8 with one scale per token and per output channel ----
+    def matmul_i8(self, ts, xq_dev, ascale_dev, ys, biases=None):
+        """ys[i] = (codes xq [M][>= in] times the K_Q8C tensor ts[i]) * scales + biases[i] (bgl_matmul_i8_dev); ys are fp32,
+        fp16 or bf16 tensors [M][out] of one type, whose rows may be apart.  A single tensor, y and bias need no lists."""
+        if isinstance(ts, Tensor):
+            ts, ys, biases = [ts], [ys], [biases]
+        n, M = len(ts), xq_dev.shape[0]
+        kind, bias = _type(ys[0]), biases or [None] * n
+        assert xq_dev.dtype == _dtypes()[3] and xq_dev.stride(-1) == 1 and len(ys) == n == len(bias)
+        for t, y in zip(ts, ys):
+            assert _type(y) == kind and y.stride(-1) == 1 and y.shape[0] == M
+        W = (C.c_void_p * n)(*[t.h.value for t in ts])
+        Y = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
+        B = (C.c_void_p * n)(*[(b.data_ptr() if b is not None else None) for b in bias])
+        S = (C.c_long * n)(*[y.stride(0) if M > 1 else y.shape[1] for y in ys])
+        _check(lib().bgl_matmul_i8_dev(self.h, n, W, C.c_void_p(xq_dev.data_ptr()), xq_dev.stride(0) if M > 1 else xq_dev.shape[1],
+                                       _p(ascale_dev), B, Y, kind, S, M), "bgl_matmul_i8_dev")
+
+    def norm(self, x, y=None, *, yq=None, yscale=None, kind=NORM_RMS, w=None, b=None, eps=1e-6, w_add=0.0, x_out=None, branch=None,
+             branch_kind=NORM_NONE, branch_w=None, branch_b=None, branch_eps=1e-6, gate=None, alpha=1.0):
+        """x_out = x + alpha * gate * branch_kind(branch), and y / (yq, yscale) = kind(x_out) (bgl_norm_dev) over [T][H] rows.
+        gate: of the branch's type, [1][H], [T][1] or [T][H].  yq: int8 [T][H up to a multiple of 16], yscale: fp32 [T]."""
+        T, H = x.shape
+        d = capi.bgl_norm(T=T, H=H, x=x.data_ptr(), ldx=_rows(x, T, H), x_type=_type(x), alpha=alpha, w_add=w_add, kind=kind,
+                          w=_vec(w, H), b=_vec(b, H), eps=eps)
+        if branch is not None:
+            d.f, d.ldf, d.f_type = branch.data_ptr(), _rows(branch, T, H), _type(branch)
+        d.post, d.post_w, d.post_b, d.post_eps = branch_kind, _vec(branch_w, H), _vec(branch_b, H), branch_eps
+        if gate is not None:
+            assert branch is not None and gate.dtype == branch.dtype and gate.dim() == 2
+            assert gate.shape[0] in (1, T) and gate.shape[1] in (1, H) and (gate.shape[1] == 1 or gate.stride(1) == 1)
+            d.gate, d.gate_t, d.gate_c = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else 0, int(gate.shape[1] > 1)
+        if x_out is not None:
+            assert x_out.dtype == x.dtype
+            d.x_out, d.ldo = x_out.data_ptr(), _rows(x_out, T, H)
+        if y is not None:
+            d.y, d.ldy, d.y_type = y.data_ptr(), _rows(y, T, H), _type(y)
+        if yq is not None:
+            assert yq.dtype == _dtypes()[3] and yq.shape[0] == T and yq.stride(-1) == 1 and yscale.numel() == T
+            d.yq, d.ldq, d.yscale = yq.data_ptr(), yq.stride(0) if T > 1 else yq.shape[1], _vec(yscale, T)
+        _check(lib().bgl_norm_dev(self.h, C.byref(d)), "bgl_norm_dev")
+
     # ---- MoE ----
     def bind_experts(self, descs):
         """descs: list of (kind, bits, packed, scales[, bias]) numpy tuples, one per expert; packed is
@@ -205,9 +280,11 @@ class Context:
                 inn = pk.shape[1]
             elif kind == K_MXFP4:                # GGUF blocks of 32 values, 17 bytes each
                 inn = pk.reshape(out, -1).shape[1] // 17 * 32
+            elif kind == K_Q8C:
+                inn = pk.shape[1]
             else:
                 inn = sc.shape[1] * (32 if kind == K_Q4G32H else 64)
-            b = bits if kind == K_QNG64 else (8 if kind == K_Q8G64 else 4)
+            b = bits if kind == K_QNG64 else (8 if kind in (K_Q8G64, K_Q8C) else 4)
             arr[e] = capi.bgl_wt(kind, b, out, inn, pk.ctypes.data, sc.ctypes.data if sc is not None else None,
                                  bi.ctypes.data if bi is not None else None)
         h = C.c_void_p()

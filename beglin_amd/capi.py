@@ -11,7 +11,9 @@ LIB_PATH = os.environ.get("BGL_LIB") or os.path.join(HERE, "libbeglin_hip.so")
 
 # mirrors of the header's enums
 K_Q4G64, K_Q8G64, K_Q4G256SF, K_QNG64, K_Q4G32H = 1, 2, 3, 4, 5
-K_Q4G64A, K_F16, K_F32, K_MXFP4, K_Q4G256P = 6, 7, 8, 9, 10
+K_Q4G64A, K_F16, K_F32, K_MXFP4, K_Q4G256P, K_Q8C = 6, 7, 8, 9, 10, 11
+T_F32, T_F16, T_BF16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 ACT_F32, ACT_W4A8 = 0, 1
 
 _P = C.c_void_p
@@ -22,6 +24,14 @@ _L = C.c_long
 class bgl_wt(C.Structure):
     _fields_ = [("kind", C.c_int), ("bits", C.c_int), ("out", C.c_int), ("in_", C.c_int),
                 ("packed", C.c_void_p), ("scales", C.c_void_p), ("sub", C.c_void_p)]
+
+
+class bgl_norm(C.Structure):
+    _fields_ = [("T", _I), ("H", _I), ("x", _P), ("ldx", _L), ("x_type", _I), ("f", _P), ("ldf", _L), ("f_type", _I),
+                ("post", _I), ("post_w", _P), ("post_b", _P), ("post_eps", C.c_float),
+                ("gate", _P), ("gate_t", _L), ("gate_c", _L), ("alpha", C.c_float), ("w_add", C.c_float),
+                ("x_out", _P), ("ldo", _L), ("kind", _I), ("w", _P), ("b", _P), ("eps", C.c_float),
+                ("y", _P), ("ldy", _L), ("y_type", _I), ("yq", _P), ("ldq", _L), ("yscale", _P)]
 
 
 # (name, restype, argtypes) for every entry point declared in include/beglin_qgemv.h
@@ -48,6 +58,8 @@ SIGNATURES = [
     ("bgl_prep_act_dev", _I, [_P, _I, _I, _P, _I, _I]),
     ("bgl_matmul_prepped_dev", _I, [_P, _P, _I, _P, _P, _I]),
     ("bgl_quant_act_i8_dev", _I, [_P, _P, _I, _I, _I, _P, _P]),
+    ("bgl_matmul_i8_dev", _I, [_P, _I, C.POINTER(_P), _P, _L, _P, C.POINTER(_P), C.POINTER(_P), _I, C.POINTER(_L), _I]),
+    ("bgl_norm_dev", _I, [_P, C.POINTER(bgl_norm)]),
     ("bgl_gemv_q4g64_mt", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),
     ("bgl_gemv_q4g64_mt_fused", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),
     ("bgl_gemv_q4g64_sdot_mt", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),

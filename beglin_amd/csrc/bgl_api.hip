@@ -14,6 +14,7 @@
 #include "../../include/beglin_qgemv.h"
 #include "bgl_kernels.h"
 #include "bgl_internal.h"
+#include "bgl_i8.h"
 
 static thread_local char g_err[512];
 static thread_local int g_code;
@@ -308,6 +309,7 @@ static int units_of(int kind, int in) {
     case BGL_Q4G64: case BGL_Q4G32H: case BGL_Q8G64: case BGL_Q4G64A: case BGL_F16: case BGL_F32: case BGL_MXFP4: return in / 64;
     case BGL_Q4G256SF: return in / 256;
     case BGL_QNG64: return (in / 64 + 1) / 2;
+    case BGL_K_Q8C: return (in + 127) / 128 * 2;         // whole stages of 128 values, zero codes behind the row
     default: return 0;
     }
 }
@@ -326,6 +328,9 @@ int check_wt(int kind, int bits, int out, int in) {
     case BGL_Q4G256SF: case BGL_K_Q4G256P:
         if (in % 256) return bgl_fail(BGL_E_ARG, "g256 in=%d %% 256 != 0", in);
         return 0;
+    case BGL_K_Q8C:
+        if (in > I8_MAX_K) return bgl_fail(BGL_E_ARG, "K_Q8C in=%d: the int32 sum holds at most %d products", in, I8_MAX_K);
+        return 0;
     default: return bgl_fail(BGL_E_UNSUPPORTED, "unknown weight kind %d", kind);
     }
 }
@@ -333,7 +338,7 @@ int check_wt(int kind, int bits, int out, int in) {
 static size_t ref_packed_bytes(int kind, int bits, int out, int in) {
     switch (kind) {
     case BGL_Q4G64: case BGL_Q4G256SF: case BGL_Q4G32H: case BGL_Q4G64A: case BGL_K_Q4G256P: return (size_t)out * in / 2;
-    case BGL_Q8G64: return (size_t)out * in;
+    case BGL_Q8G64: case BGL_K_Q8C: return (size_t)out * in;
     case BGL_F16: return (size_t)out * in * 2;
     case BGL_F32: return (size_t)out * in * 4;
     case BGL_QNG64: return (size_t)out * (in / 64) * bits * 8;
@@ -346,6 +351,7 @@ static size_t ref_scale_bytes(int kind, int out, int in) {
     case BGL_Q4G64: case BGL_Q8G64: case BGL_QNG64: case BGL_Q4G64A: return (size_t)out * (in / 64) * 4;
     case BGL_Q4G256SF: case BGL_K_Q4G256P: return (size_t)out * (in / 256) * 4;
     case BGL_Q4G32H: return (size_t)out * (in / 32) * 2;
+    case BGL_K_Q8C: return (size_t)out * 4;
     default: return 0;
     }
 }
@@ -357,17 +363,17 @@ static inline unsigned nblk(long n, int bs = 256) { return (unsigned)((n + bs - 
 void device_layout(int kind, int bits, int out, int in, BglDevTensor &T, size_t bytes[3]) {
     T = BglDevTensor{};
     T.fmt = kind;
-    T.bits = kind == BGL_QNG64 ? bits : kind == BGL_Q8G64 ? 8 : kind == BGL_F16 ? 16 : kind == BGL_F32 ? 32 : 4;
+    T.bits = kind == BGL_QNG64 ? bits : kind == BGL_Q8G64 || kind == BGL_K_Q8C ? 8 : kind == BGL_F16 ? 16 : kind == BGL_F32 ? 32 : 4;
     T.N = out; T.K = in; T.ntiles = (out + BGL_TILE - 1) / BGL_TILE;
     T.gmul = kind == BGL_Q4G256SF ? 1.0f / 63.0f : 1.0f;
     T.nunits = units_of(kind, in);
-    T.cpu = kind == BGL_Q4G256SF ? 8 : kind == BGL_Q8G64 ? 4 : kind == BGL_QNG64 ? bits : kind == BGL_F16 ? 8
+    T.cpu = kind == BGL_Q4G256SF ? 8 : kind == BGL_Q8G64 || kind == BGL_K_Q8C ? 4 : kind == BGL_QNG64 ? bits : kind == BGL_F16 ? 8
           : kind == BGL_F32 ? 16 : 2;
     T.cpr = T.nunits * T.cpu;
     const long rows = (long)T.ntiles * BGL_TILE;
     const bool dense = kind == BGL_F16 || kind == BGL_F32;
     bytes[0] = (size_t)rows * T.cpr * 16;
-    bytes[1] = dense ? 0 : (size_t)rows * T.nunits * (kind == BGL_QNG64 || kind == BGL_Q4G256SF ? 8 : 4);
+    bytes[1] = dense ? 0 : kind == BGL_K_Q8C ? (size_t)rows * 4 : (size_t)rows * T.nunits * (kind == BGL_QNG64 || kind == BGL_Q4G256SF ? 8 : 4);
     bytes[2] = kind == BGL_Q4G64A ? (size_t)rows * T.nunits * 4 : 0;
 }
 
@@ -381,11 +387,12 @@ bgl_tensor *tensor_from_parts(const BglDevTensor &T, void *w, void *s0, void *s1
 }
 
 // Repack reference-layout device buffers into a new tensor.
+// q8c_pitch: bytes between K_Q8C's code rows where they are not dense.
 static int repack_into(bgl_ctx *c, int kind, int bits, int out, int in, const void *dpk, const void *dsc,
-                       const uint8_t *dsub, bgl_tensor **res) {
+                       const uint8_t *dsub, bgl_tensor **res, long q8c_pitch = 0) {
     switch (kind) {
     case BGL_Q4G64: case BGL_Q4G32H: case BGL_Q4G256SF: case BGL_Q4G64A: case BGL_MXFP4:
-    case BGL_Q8G64: case BGL_F16: case BGL_F32: case BGL_QNG64:
+    case BGL_Q8G64: case BGL_F16: case BGL_F32: case BGL_QNG64: case BGL_K_Q8C:
         break;
     default:
         return bgl_fail(BGL_E_ARG, "repack: kind %d has no device layout of its own", kind);
@@ -424,6 +431,10 @@ static int repack_into(bgl_ctx *c, int kind, int bits, int out, int in, const vo
     case BGL_QNG64:
         bgl_repack_qng((const uint8_t *)dpk, out, in, bits, (uint8_t *)w, c->stream);
         break;
+    case BGL_K_Q8C:
+        hipLaunchKernelGGL(k_repack_q8c, dim3(nblk(nch)), dim3(256), 0, c->stream, (const int8_t *)dpk, out, in,
+                           q8c_pitch ? q8c_pitch : (long)in, T.cpr, (uint8_t *)w);
+        break;
     }
     long nu = rows * T.nunits;
     switch (kind) {
@@ -436,6 +447,9 @@ static int repack_into(bgl_ctx *c, int kind, int bits, int out, int in, const vo
     case BGL_Q4G256SF:   // wsuper and the unit's 4 sub-codes in one 8-byte word
         hipLaunchKernelGGL(k_repack_zip_u32, dim3(nblk(nu)), dim3(256), 0, c->stream, (const uint32_t *)dsc, (const uint32_t *)dsub,
                            out, T.nunits, (uint2 *)s0);
+        break;
+    case BGL_K_Q8C:      // one scale per row: [row], zero past the last
+        hipLaunchKernelGGL(k_repack_u32, dim3(nblk(rows)), dim3(256), 0, c->stream, (const uint32_t *)dsc, out, 1, (uint32_t *)s0);
         break;
     case BGL_QNG64:
         hipLaunchKernelGGL(k_repack_qng_scales, dim3(nblk(nu)), dim3(256), 0, c->stream, (const float *)dsc, out, in / 64, (float2 *)s0);
@@ -603,8 +617,9 @@ extern "C" int bgl_quantize_dev(bgl_ctx *c, int kind, int bits, int qng64_encode
     HIPCHK(hipSetDevice(c->device));
     size_t pb = ref_packed_bytes(kind, bits, out, in), sb = ref_scale_bytes(kind, out, in);
     size_t subb = kind == BGL_Q4G256SF ? (size_t)out * (in / 64) : 0;
+    const long pitch = kind == BGL_K_Q8C ? ((long)in + 15) / 16 * 16 : 0;   // the quantizer writes whole 16-byte runs
     void *dpk = nullptr, *dsc = nullptr, *dsub = nullptr;
-    HIPCHK(hipMalloc(&dpk, pb));
+    HIPCHK(hipMalloc(&dpk, pitch ? (size_t)out * pitch : pb));
     HIPCHK(hipMalloc(&dsc, sb));
     if (subb) HIPCHK(hipMalloc(&dsub, subb));
     long units;
@@ -616,6 +631,9 @@ extern "C" int bgl_quantize_dev(bgl_ctx *c, int kind, int bits, int qng64_encode
     case BGL_Q8G64:
         units = (long)out * (in / 64);
         hipLaunchKernelGGL(k_quant_q8g64, dim3(nblk(units, PK_THREADS)), dim3(PK_THREADS), 0, c->stream, w_dev, out, in, (int8_t *)dpk, (float *)dsc);
+        break;
+    case BGL_K_Q8C:      // a row is a column of the per-token quantizer: the same codes and scale
+        rc = run_quant_rows(c, w_dev, nullptr, nullptr, out, in, (int8_t *)dpk, pitch, (float *)dsc);
         break;
     case BGL_QNG64:
         units = (long)out * (in / 64);
@@ -633,9 +651,11 @@ extern "C" int bgl_quantize_dev(bgl_ctx *c, int kind, int bits, int qng64_encode
         break;
     }
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) rc = bgl_fail(BGL_E_HIP, "quantize launch: %s", hipGetErrorString(e));
-    if (!rc) rc = repack_into(c, kind, bits, out, in, dpk, dsc, (const uint8_t *)dsub, t);
-    if (!rc && ref_packed) rc = hipMemcpyAsync(ref_packed, dpk, pb, hipMemcpyDeviceToHost, c->stream) ? BGL_E_HIP : 0;
+    if (!rc && e != hipSuccess) rc = bgl_fail(BGL_E_HIP, "quantize launch: %s", hipGetErrorString(e));
+    if (!rc) rc = repack_into(c, kind, bits, out, in, dpk, dsc, (const uint8_t *)dsub, t, pitch);
+    if (!rc && ref_packed)
+        rc = (pitch ? hipMemcpy2DAsync(ref_packed, in, dpk, pitch, in, out, hipMemcpyDeviceToHost, c->stream)
+                    : hipMemcpyAsync(ref_packed, dpk, pb, hipMemcpyDeviceToHost, c->stream)) ? BGL_E_HIP : 0;
     if (!rc && ref_scales) rc = hipMemcpyAsync(ref_scales, dsc, sb, hipMemcpyDeviceToHost, c->stream) ? BGL_E_HIP : 0;
     if (!rc && ref_sub && subb) rc = hipMemcpyAsync(ref_sub, dsub, subb, hipMemcpyDeviceToHost, c->stream) ? BGL_E_HIP : 0;
     e = hipStreamSynchronize(c->stream);
@@ -674,7 +694,7 @@ extern "C" int bgl_tensor_info(const bgl_tensor *t, int *kind, int *bits, int *o
 extern "C" int bgl_dequant_dev(bgl_ctx *c, const bgl_tensor *t, int row0, int nrows, float *out_dev) {
     if (!c || !t || !out_dev || !t->experts.empty()) return bgl_fail(BGL_E_ARG, "bgl_dequant_dev: bad argument");
     if (row0 < 0 || nrows <= 0 || row0 + nrows > t->T.N) return bgl_fail(BGL_E_ARG, "bgl_dequant_dev: rows out of range");
-    hipLaunchKernelGGL(k_dequant, dim3((unsigned)((long)(t->T.K / 64) * ((nrows + 15) / 16))), dim3(256), 0, c->stream, t->T, row0, nrows, out_dev);
+    hipLaunchKernelGGL(k_dequant, dim3((unsigned)((long)((t->T.K + 63) / 64) * ((nrows + 15) / 16))), dim3(256), 0, c->stream, t->T, row0, nrows, out_dev);
     HIPCHK(hipGetLastError());
     return 0;
 }
@@ -732,6 +752,11 @@ int prep_act(bgl_ctx *c, int act, int gq, const float *x_dev, int M, int K, Gemv
 
 extern "C" int bgl_quant_act_i8_dev(bgl_ctx *c, const float *x_dev, int M, int in, int gsize, int8_t *xq_dev, float *ascale_dev) {
     if (!c || !x_dev || !xq_dev || !ascale_dev || M <= 0) return bgl_fail(BGL_E_ARG, "bgl_quant_act_i8_dev: bad argument");
+    if (gsize == in && gsize != 64 && gsize != 256 && in >= 16 && in % 16 == 0) {    // one scale per token
+        if ((uintptr_t)xq_dev % 16) return bgl_fail(BGL_E_ARG, "bgl_quant_act_i8_dev: one scale per token needs a 16-byte aligned xq");
+        HIPCHK(hipSetDevice(c->device));
+        return run_quant_rows(c, x_dev, nullptr, nullptr, M, in, xq_dev, in, ascale_dev);
+    }
     if ((gsize != 64 && gsize != 256) || in % gsize) return bgl_fail(BGL_E_ARG, "bgl_quant_act_i8_dev: in=%d gsize=%d", in, gsize);
     if (dbuf_reserve(c, c->act_sum, (size_t)M * (in / 64) * 4, false)) return bgl_last_code();
     hipLaunchKernelGGL(k_act_w4a8, dim3(nblk((long)M * (in / gsize) * 64)), dim3(256), 0, c->stream, x_dev, M, in, gsize, xq_dev,
@@ -1054,7 +1079,10 @@ extern "C" int bgl_matmul_group_dev(bgl_ctx *c, int n, const bgl_tensor *const *
         return bgl_fail(BGL_E_UNSUPPORTED, "K_Q4G256SF requires W4A8 activations -- no fp32-activation path exists for g256sf");
     if ((kind == BGL_Q4G32H || kind == BGL_QNG64) && act != BGL_ACT_F32)
         return bgl_fail(BGL_E_UNSUPPORTED, "kind %d has fp32-activation kernels only", kind);
+    if (kind == BGL_K_Q8C && act != BGL_ACT_W4A8)
+        return bgl_fail(BGL_E_UNSUPPORTED, "K_Q8C multiplies int8 activations only (BGL_ACT_W4A8)");
     HIPCHK(hipSetDevice(c->device));
+    if (kind == BGL_K_Q8C) return run_i8_cols(c, n, Ts, x_dev, nullptr, nullptr, M, bias_dev, y_dev);
     if (act == BGL_ACT_W4A8 && fused_q_ok(c, kind, Ts[0].K, M)) return run_gemv_q(c, n, Ts, x_dev, M, bias_dev, y_dev);
     if (act == BGL_ACT_F32 && mfma_takes(c, n, Ts, M)) return run_gemm_mfma(c, n, Ts, x_dev, M, bias_dev, y_dev, nullptr);
     // one fp32 column over a short K: the GEMV makes the activation digits itself (no prep launch)
@@ -1102,6 +1130,13 @@ extern "C" int bgl_matmul_group_noalloc_dev(bgl_ctx *c, int n, const bgl_tensor 
 extern "C" int bgl_prep_act_dev(bgl_ctx *c, int act, int kind, const float *x_dev, int M, int in) {
     if (!c || !x_dev || M < 1) return bgl_fail(BGL_E_ARG, "bgl_prep_act_dev: bad argument");
     if (act != BGL_ACT_F32 && act != BGL_ACT_W4A8) return bgl_fail(BGL_E_ARG, "unknown activation mode %d", act);
+    if (kind == BGL_K_Q8C) {
+        if (act != BGL_ACT_W4A8) return bgl_fail(BGL_E_UNSUPPORTED, "K_Q8C multiplies int8 activations only (BGL_ACT_W4A8)");
+        int rc = check_wt(kind, 8, 1, in);
+        if (rc) return rc;
+        HIPCHK(hipSetDevice(c->device));
+        return prep_i8_cols(c, x_dev, nullptr, nullptr, M, in, true);
+    }
     const int gq = act_group(kind);
     if (in % 64 || in % gq) return bgl_fail(BGL_E_ARG, "bgl_prep_act_dev: in=%d not a multiple of the group", in);
     HIPCHK(hipSetDevice(c->device));
@@ -1128,7 +1163,8 @@ extern "C" int bgl_matmul_prepped_dev(bgl_ctx *c, const bgl_tensor *w, int act, 
     if (T.fmt == BGL_Q4G64A || T.fmt == BGL_F16 || T.fmt == BGL_F32 || T.fmt == BGL_MXFP4)
         return bgl_fail(BGL_E_UNSUPPORTED, "kind %d runs in the MoE gather only", T.fmt);
     const int kind = T.fmt == BGL_Q4G256SF && T.gmul == 1.0f ? BGL_K_Q4G256P : T.fmt;
-    if (!c->prep_reuse || c->prep_act != act || c->prep_K != T.K || c->prep_gq != act_group(kind) || M > c->prep_M)
+    if (!c->prep_reuse || c->prep_act != act || c->prep_K != T.K || M > c->prep_M ||
+        c->prep_gq != (kind == BGL_K_Q8C ? PREP_GQ_TOKEN : act_group(kind)))
         return bgl_fail(BGL_E_ARG, "bgl_matmul_prepped_dev: no activation prepared by bgl_prep_act_dev matches (act %d, in %d, M %d)",
                         act, T.K, M);
     if (T.fmt == BGL_Q4G256SF && act != BGL_ACT_W4A8)
@@ -1136,6 +1172,12 @@ extern "C" int bgl_matmul_prepped_dev(bgl_ctx *c, const bgl_tensor *w, int act, 
     HIPCHK(hipSetDevice(c->device));
     GemvAct A;
     memset(&A, 0, sizeof A);
+    if (kind == BGL_K_Q8C) {
+        if (M < 1) return bgl_fail(BGL_E_ARG, "bgl_matmul_prepped_dev: M=%d", M);
+        void *yv = y_dev;
+        return run_i8(c, 1, &T, (const int8_t *)c->act_w.p, i8_ld_scratch(T.K), (const float *)c->act_s.p, &bias_dev, &yv,
+                      BGL_T_F32, nullptr, M);
+    }
     if (act == BGL_ACT_F32) f32_act_ptrs(c->act_w.p, c->act_s.p, c->act_sum.p, c->prep_M, T.K, c->prep_x, A);
     else { A.xw = (const int *)c->act_w.p; A.xs = (const float *)c->act_s.p; A.xsum = (const int *)c->act_sum.p; A.gq = c->prep_gq; }
     const float *b[1] = {bias_dev};

@@ -1,0 +1,384 @@
+// bgl_i8.hip -- products of int8 codes with one scale per token and per output channel (BGL_K_Q8C):
+//
+//   y[m][r] = (float)(sum_c xq[m][c] * wq[r][c]) * (xs[m] * ws[r]) + bias[r]
+//
+// The sum is an int32 and exact, so neither its order nor a split of K changes a bit: waves may take any
+// share of K.  The device layout is that of int8 group-64 tensors ([64-row tile][16-byte chunk][row]), K
+// padded to 128 with zero codes: four chunks of 16 rows are the A operand of v_mfma_i32_16x16x64_i8 as
+// they lie in memory (lane l: row l % 16, values 16 (l / 16) .. + 15), the codes of a token row are its B
+// operand, and a lane's four results are four neighbouring channels of one token.  The zero padding of
+// the weights also means that what an activation row holds past K never counts.
+#include <string.h>
+
+#include <algorithm>
+
+#include "../../include/beglin_qgemv.h"
+#include "bgl_i8.h"
+
+#define HIPCHK(expr)                                                                             \
+    do {                                                                                         \
+        hipError_t e_ = (expr);                                                                  \
+        if (e_ != hipSuccess) return bgl_fail(BGL_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+    } while (0)
+
+struct I8Task {
+    BglDevTensor T;
+    const float *bias;
+    void *y;
+    long ldy;
+    int blk0;                 // first workgroup row block of this tensor
+};
+struct I8Launch {
+    I8Task t[BGL_MAX_TASKS];
+    int n, M, K16, y_type, vec;   // K16: K rounded up to 16; vec: four outputs of a lane go in one store
+    const int8_t *xq;
+    long ldq;
+    const float *xs;
+};
+
+__device__ __forceinline__ i8_i4 i8_mfma(i8_u4 a, i8_u4 b, i8_i4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i8_i4, a), __builtin_bit_cast(i8_i4, b), c, 0, 0, 0);
+}
+
+// The workgroup's tensor, picked by selects so that its fields come in one round of scalar loads.
+__device__ __forceinline__ I8Task i8_task(const I8Launch &L, int blk) {
+    I8Task t = L.t[0];
+#pragma unroll
+    for (int i = 1; i < BGL_MAX_TASKS; i++)
+        if (i < L.n && blk >= L.t[i].blk0) t = L.t[i];
+    return t;
+}
+
+// Four neighbouring channels r .. r + 3 of token m.
+__device__ __forceinline__ void i8_store4(const I8Launch &L, const I8Task &t, int m, int r, i8_i4 acc, float as, i8_f4 ws, i8_f4 b) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = i8_out(acc[i], as, ws[i]);
+    if (t.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __fadd_rn(v[i], b[i]);
+    }
+    const size_t at = (size_t)m * t.ldy + r;
+    if (L.vec && r + 4 <= t.T.N) {
+        if (L.y_type == BGL_T_F32) *(i8_f4 *)((float *)t.y + at) = i8_f4{v[0], v[1], v[2], v[3]};
+        else
+            *(uint2 *)((uint16_t *)t.y + at) = make_uint2((uint32_t)i8_h16(v[0], L.y_type) | ((uint32_t)i8_h16(v[1], L.y_type) << 16),
+                                                          (uint32_t)i8_h16(v[2], L.y_type) | ((uint32_t)i8_h16(v[3], L.y_type) << 16));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (r + i < t.T.N) i8_st(t.y, L.y_type, at + i, v[i]);
+    }
+}
+// scales (the device copy is padded to whole tiles) and biases of channels r .. r + 3
+__device__ __forceinline__ i8_f4 i8_ws(const I8Task &t, int r) { return *(const i8_f4 *)((const float *)t.T.s0 + r); }
+__device__ __forceinline__ i8_f4 i8_bias(const I8Task &t, int r) {
+    i8_f4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (t.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) b[i] = t.bias[min(r + i, t.T.N - 1)];
+    }
+    return b;
+}
+
+// ================================================================================== few columns
+// A workgroup owns RB blocks of 16 channels and up to 16 CB tokens; its waves split K.  Weights and codes
+// go straight from memory to the operand registers, D units ahead; the waves' int32 sums meet in LDS.
+template <int RB, int CB>
+constexpr int i8_s_waves() { return RB * CB <= 4 ? 16 : 64 / (RB * CB); }    // 64 KB of sums at most
+template <int RB, int CB, int D>
+__global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L) {
+    extern __shared__ __align__(16) i8_i4 red[];               // [wave][RB * CB][64]
+    const int nw = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const I8Task t = i8_task(L, blockIdx.x);
+    const int rb0 = (blockIdx.x - t.blk0) * RB, U = t.T.nunits;     // RB divides 4: the blocks lie in one tile
+    const uint8_t *wp = t.T.w + ((size_t)(rb0 >> 2) * t.T.cpr + (lane >> 4)) * 1024 + ((rb0 & 3) * 16 + (lane & 15)) * 16;
+    const int8_t *xp[CB];
+    const int kq = (lane >> 4) * 16;
+#pragma unroll
+    for (int j = 0; j < CB; j++) xp[j] = L.xq + (size_t)min(16 * j + (lane & 15), L.M - 1) * L.ldq;
+    i8_i4 acc[RB][CB];
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) acc[i][j] = i8_i4{0, 0, 0, 0};
+    i8_u4 a[D][RB], b[D][CB];
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int s = 0; s < D; s++) {
+            const int u = min(u0 + s * nw, U - 1);
+#pragma unroll
+            for (int i = 0; i < RB; i++) a[s][i] = *(const i8_u4 *)(wp + (size_t)u * 4096 + 256 * i);
+            const int k = min(64 * u + kq, L.K16 - 16);              // past the row: the weights are zero there
+#pragma unroll
+            for (int j = 0; j < CB; j++) b[s][j] = *(const i8_u4 *)(xp[j] + k);
+        }
+    };
+    load(wave);
+    for (int u0 = wave; u0 < U; u0 += D * nw) {
+        i8_u4 ca[D][RB], cb[D][CB];
+#pragma unroll
+        for (int s = 0; s < D; s++) {
+#pragma unroll
+            for (int i = 0; i < RB; i++) ca[s][i] = a[s][i];
+#pragma unroll
+            for (int j = 0; j < CB; j++) cb[s][j] = b[s][j];
+        }
+        if (u0 + D * nw < U) load(u0 + D * nw);
+#pragma unroll
+        for (int s = 0; s < D; s++) {
+            if (u0 + s * nw < U) {
+#pragma unroll
+                for (int i = 0; i < RB; i++)
+#pragma unroll
+                    for (int j = 0; j < CB; j++) acc[i][j] = i8_mfma(ca[s][i], cb[s][j], acc[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) red[(wave * RB * CB + i * CB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int o = threadIdx.x; o < RB * CB * 64; o += blockDim.x) {
+        const int l = o & 63, j = (o >> 6) % CB, i = (o >> 6) / CB;
+        const int m = 16 * j + (l & 15), r = (rb0 + i) * 16 + 4 * (l >> 4);
+        if (m >= L.M || r >= t.T.N) continue;
+        i8_i4 s = {0, 0, 0, 0};
+        for (int w = 0; w < nw; w++) s += red[(w * RB * CB + i * CB + j) * 64 + l];
+        i8_store4(L, t, m, r, s, L.xs[m], i8_ws(t, r), i8_bias(t, r));
+    }
+}
+
+// ================================================================================== many columns
+// Tiles of 16 CM NWM tokens by 16 CN NWN channels, NWM x NWN waves; both operands go through LDS in
+// stages of 128 values of K, copied there without passing through registers (buffer loads to LDS), the
+// next stage while this one is multiplied.
+//
+// A stage of weights keeps the device layout ([64-row tile][chunk][row], 1 KB runs).  A stage of token
+// rows is [row][128 bytes] with chunk c of row r at place c ^ (r / 2 % 8): an instruction copies 8 whole
+// rows (128-byte runs of memory), and the 16 rows that an operand read touches lie in different banks.
+#define I8_BK 128
+
+typedef unsigned int i8_rsrc __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i8_rsrc i8_mkrsrc(const void *p, uint32_t bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    i8_rsrc r;
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    r.z = __builtin_amdgcn_readfirstlane(bytes);
+    r.w = 0x00020000u;
+    return r;
+}
+// 64 lanes x 16 bytes at rsrc + voff + soff into LDS at lds + 16 * lane.  Written as asm because the compiler
+// would wait for every copy in flight before each LDS read; i8_wait below is the wait that counts.  (m0 is
+// never live across code of the compiler's: it sets m0 right before an instruction that reads it.)
+__device__ __forceinline__ void i8_copy(i8_rsrc rs, uint32_t voff, uint32_t soff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff)
+                 : "memory");
+}
+// every copy of this wave has landed and every LDS read of it has returned
+__device__ __forceinline__ void i8_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// Workgroup b of nt: each XCD (workgroups go round the 8 of them) takes a run of neighbouring tiles, and
+// within it 8 tiles of tokens share the weights that they read from its L2.
+__device__ __forceinline__ void i8_tile(int b, int ntm, int ntn, int &tm, int &tn) {
+    const int nt = ntm * ntn, x = b & 7, q = nt >> 3, rem = nt & 7;
+    const int id = x * q + min(x, rem) + (b >> 3);
+    const int gw = 8 * ntn, g = id / gw, in = id % gw, gm = min(8, ntm - 8 * g);
+    tm = 8 * g + in % gm;
+    tn = in / gm;
+}
+
+template <int CM, int CN, int NWM, int NWN>
+__global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, int ntn) {
+    constexpr int BM = 16 * CM * NWM, BN = 16 * CN * NWN, NW = NWM * NWN;
+    constexpr int XB = BM * I8_BK, WB = BN * I8_BK, SB = XB + WB;             // bytes of a stage
+    constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;                   // copies of a wave per stage
+    static_assert(XI * NW * 1024 == XB && WI * NW * 1024 == WB && BN % 64 == 0, "whole copies");
+    extern __shared__ __align__(1024) uint8_t sm[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int tm, tn;
+    i8_tile(blockIdx.x, ntm, ntn, tm, tn);
+    const I8Task t = i8_task(L, tn);
+    const int m0 = tm * BM, n0 = (tn - t.blk0) * BN;
+    const int nk = t.T.nunits / 2;                                            // K is padded to whole stages
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm;
+
+    // token rows: copy j of the stage is rows 8 j .. 8 j + 7; rows past M repeat the last one
+    const int rows = min(BM, L.M - m0);
+    const i8_rsrc xr = i8_mkrsrc(L.xq + (size_t)m0 * L.ldq, (uint32_t)((rows - 1) * L.ldq + L.K16));
+    uint32_t xo[XI];
+#pragma unroll
+    for (int i = 0; i < XI; i++) {
+        const int r = 8 * (wave + NW * i) + (lane >> 3);
+        xo[i] = (uint32_t)(min(r, rows - 1) * (int)L.ldq + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
+    }
+    // weights: copy j is chunk j % 8 of tile j / 8; tiles past the tensor's last repeat it
+    const int tile0 = n0 / 64, tb = t.T.cpr * 1024;
+    const i8_rsrc wr = i8_mkrsrc(t.T.w + (size_t)tile0 * tb, (uint32_t)(min(BN / 64, t.T.ntiles - tile0) * tb));
+    uint32_t wo[WI];
+#pragma unroll
+    for (int i = 0; i < WI; i++) {
+        const int j = wave + NW * i;
+        wo[i] = (uint32_t)(min(j >> 3, t.T.ntiles - 1 - tile0) * tb + (j & 7) * 1024);
+    }
+    auto stage = [&](int k, uint32_t base) {
+#pragma unroll
+        for (int i = 0; i < WI; i++) i8_copy(wr, lane * 16, wo[i] + k * 8192, base + (wave + NW * i) * 1024);
+#pragma unroll
+        for (int i = 0; i < XI; i++) i8_copy(xr, xo[i] + k * I8_BK, 0, base + WB + (wave + NW * i) * 1024);
+    };
+
+    const int wm = wave / NWN, wn = wave % NWN;
+    i8_i4 acc[CM][CN];
+#pragma unroll
+    for (int i = 0; i < CM; i++)
+#pragma unroll
+        for (int j = 0; j < CN; j++) acc[i][j] = i8_i4{0, 0, 0, 0};
+    const int key = ((lane & 15) >> 1), xl = WB + (wm * CM * 16 + (lane & 15)) * I8_BK;
+    const int wl = (lane >> 4) * 1024 + (lane & 15) * 16;
+
+    stage(0, lds0);
+    for (int k = 0; k < nk; k++) {
+        i8_wait();
+        __builtin_amdgcn_s_barrier();
+        const int cur = (k & 1) * SB;
+        if (k + 1 < nk) stage(k + 1, lds0 + (SB - cur));
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            i8_u4 a[CN], b[CM];
+#pragma unroll
+            for (int j = 0; j < CN; j++) {
+                const int nb = wn * CN + j;
+                a[j] = *(const i8_u4 *)(sm + cur + (nb >> 2) * 8192 + (nb & 3) * 256 + kk * 4096 + wl);
+            }
+#pragma unroll
+            for (int i = 0; i < CM; i++)
+                b[i] = *(const i8_u4 *)(sm + cur + xl + i * 16 * I8_BK + (((kk * 4 + (lane >> 4)) ^ key) << 4));
+#pragma unroll
+            for (int i = 0; i < CM; i++)
+#pragma unroll
+                for (int j = 0; j < CN; j++) acc[i][j] = i8_mfma(a[j], b[i], acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CN; j++) {
+        const int r = n0 + (wn * CN + j) * 16 + 4 * (lane >> 4);
+        if (r >= t.T.N) continue;
+        const i8_f4 ws = i8_ws(t, r), bias = i8_bias(t, r);
+#pragma unroll
+        for (int i = 0; i < CM; i++) {
+            const int m = m0 + (wm * CM + i) * 16 + (lane & 15);
+            if (m < L.M) i8_store4(L, t, m, r, acc[i][j], L.xs[m], ws, bias);
+        }
+    }
+}
+
+// ================================================================================== host side
+template <int RB, int CB>
+static void s_go(const I8Launch &L, int blocks, int units, hipStream_t st) {
+    constexpr int D = RB + CB <= 2 ? 4 : 2;
+    const int nw = std::min(i8_s_waves<RB, CB>(), units);
+    hipLaunchKernelGGL((k_i8_s<RB, CB, D>), dim3(blocks), dim3(nw * 64), (size_t)nw * RB * CB * 1024, st, L);
+}
+
+template <int CM, int CN, int NWM, int NWN>
+static int l_go(bgl_ctx *c, I8Launch &L) {
+    constexpr int BM = 16 * CM * NWM, BN = 16 * CN * NWN;
+    int ntn = 0;
+    for (int i = 0; i < L.n; i++) {
+        L.t[i].blk0 = ntn;
+        ntn += (L.t[i].T.N + BN - 1) / BN;
+    }
+    const int ntm = (L.M + BM - 1) / BM;
+    const size_t lds = 2 * (size_t)(BM + BN) * I8_BK;
+    auto kern = k_i8_l<CM, CN, NWM, NWN>;
+    HIPCHK(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kern, dim3((unsigned)ntm * ntn), dim3(NWM * NWN * 64), lds, c->stream, L, ntm, ntn);
+    return 0;
+}
+
+#define I8_S_COLS 64          // columns that a launch of k_i8_s takes
+
+int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
+           void *const *y, int y_type, const long *ldy, int M) {
+    I8Launch L;
+    memset(&L, 0, sizeof L);
+    L.n = n; L.M = M; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
+    L.xq = xq; L.ldq = ldq; L.xs = xs;
+    L.vec = 1;
+    for (int i = 0; i < n; i++) {
+        I8Task &t = L.t[i];
+        t.T = Ts[i];
+        t.bias = bias ? bias[i] : nullptr;
+        t.y = y[i];
+        t.ldy = ldy ? ldy[i] : Ts[i].N;
+        if (((uintptr_t)t.y | (uintptr_t)t.ldy * i8_elem(y_type)) % (4 * i8_elem(y_type))) L.vec = 0;
+    }
+    int tok = prof_begin(c, 1), rc = 0;
+    if (M <= I8_S_COLS) {
+        const int CB = (M + 15) / 16;
+        long tiles = 0;
+        for (int i = 0; i < n; i++) tiles += Ts[i].ntiles;
+        int RB = 1;                                            // 16 channels a workgroup, more once that leaves 512 of them
+        while (RB < 4 && tiles * 4 / (2 * RB) >= 512) RB *= 2;
+        int blocks = 0;
+        for (int i = 0; i < n; i++) {
+            L.t[i].blk0 = blocks;
+            blocks += ((Ts[i].N + 15) / 16 + RB - 1) / RB;
+        }
+#define GO(R, C) if (RB == R && CB == C) s_go<R, C>(L, blocks, Ts[0].nunits, c->stream)
+        GO(1, 1); GO(1, 2); GO(1, 3); GO(1, 4); GO(2, 1); GO(2, 2); GO(2, 3); GO(2, 4); GO(4, 1); GO(4, 2); GO(4, 3); GO(4, 4);
+#undef GO
+    } else {
+        rc = l_go<8, 4, 2, 4>(c, L);
+    }
+    prof_end(c, tok);
+    if (rc) return rc;
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int prep_i8_cols(bgl_ctx *c, const float *x, const float *u, float *h, int M, int K, bool reuse) {
+    const long ldq = i8_ld_scratch(K);
+    if (dbuf_reserve(c, c->act_w, (size_t)M * ldq, false) || dbuf_reserve(c, c->act_s, (size_t)M * 4, false)) return bgl_last_code();
+    c->prep_reuse = false;
+    int rc = run_quant_rows(c, x, u, h, M, K, (int8_t *)c->act_w.p, ldq, (float *)c->act_s.p);
+    if (rc) return rc;
+    c->prep_act = BGL_ACT_W4A8; c->prep_gq = PREP_GQ_TOKEN; c->prep_M = M; c->prep_K = K; c->prep_x = nullptr;
+    c->prep_reuse = reuse;
+    return 0;
+}
+
+int run_i8_cols(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x, const float *u, float *h, int M,
+                const float *const *bias, float *const *y) {
+    int rc = prep_i8_cols(c, x, u, h, M, Ts[0].K, false);
+    if (rc) return rc;
+    void *yv[BGL_MAX_TASKS];
+    for (int i = 0; i < n; i++) yv[i] = y[i];
+    return run_i8(c, n, Ts, (const int8_t *)c->act_w.p, i8_ld_scratch(Ts[0].K), (const float *)c->act_s.p, bias, yv, BGL_T_F32,
+                  nullptr, M);
+}
+
+extern "C" int bgl_matmul_i8_dev(bgl_ctx *c, int n, const bgl_tensor *const *w, const int8_t *xq, long ldq, const float *xs,
+                                 const float *const *bias, void *const *y, int y_type, const long *ldy, int M) {
+    if (!c || n < 1 || n > BGL_MAX_TASKS || !w || !xq || !xs || !y || M < 1)
+        return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: bad argument");
+    if (y_type != BGL_T_F32 && y_type != BGL_T_F16 && y_type != BGL_T_BF16)
+        return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: unknown element type %d", y_type);
+    BglDevTensor Ts[BGL_MAX_TASKS];
+    for (int i = 0; i < n; i++) {
+        if (!w[i] || !w[i]->experts.empty() || !y[i]) return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: tensor %d invalid", i);
+        Ts[i] = w[i]->T;
+        if (Ts[i].fmt != BGL_K_Q8C) return bgl_fail(BGL_E_UNSUPPORTED, "bgl_matmul_i8_dev: kind %d is not K_Q8C", Ts[i].fmt);
+        if (Ts[i].K != Ts[0].K) return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: fused tensors must share in");
+        if (ldy && ldy[i] < Ts[i].N) return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: y rows %ld apart, %d values each", ldy[i], Ts[i].N);
+    }
+    if (ldq < Ts[0].K || ldq % 16 || (uintptr_t)xq % 16)
+        return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: code rows are 16-byte aligned, a multiple of 16 and at least in=%d bytes apart (ldq=%ld)",
+                        Ts[0].K, ldq);
+    if (ldq > (1l << 22)) return bgl_fail(BGL_E_ARG, "bgl_matmul_i8_dev: code rows %ld bytes apart (at most %ld)", ldq, 1l << 22);
+    HIPCHK(hipSetDevice(c->device));
+    return run_i8(c, n, Ts, xq, ldq, xs, bias, y, y_type, ldy, M);
+}

@@ -10,6 +10,7 @@
 //           diagnostic kind is this layout with every sub-code 1 and gmul 1 instead of 1/63.
 //   Q8G64   64 elements, 4 chunks, s0 = fp32 scale
 //   QNG64   128 elements (a pair of 64-groups), n chunks, s0 = float2 (the two group scales)
+//   Q8C     64 elements, 4 chunks (an even number of units, zero codes behind the row); s0 = fp32 [row]
 //   MXFP4   64 elements (two GGUF blocks), 2 chunks (Q4G64's nibble order), s0 = u32 holding the
 //           two E8M0 exponent bytes (low = first block)
 struct BglDevTensor {
@@ -219,6 +220,7 @@ __global__ void k_quant_q4g32h(const float *w, int N, int K, uint8_t *packed, ui
 __global__ void k_quant_g256sf(const float *w, int N, int K, uint8_t *packed, float *wsuper, uint8_t *sub);
 __global__ void k_repack_nib(const uint8_t *src, int N, int K, uint32_t flip, uint8_t *dst);
 __global__ void k_repack_q8(const int8_t *src, int N, int K, uint8_t *dst);
+__global__ void k_repack_q8c(const int8_t *src, int N, int K, long pitch, int cpr, uint8_t *dst);
 void bgl_repack_qng(const uint8_t *src, int N, int K, int n, uint8_t *dst, hipStream_t st);
 __global__ void k_repack_u32(const uint32_t *src, int N, int U, uint32_t *dst);
 __global__ void k_repack_u64(const uint64_t *src, int N, int U, uint64_t *dst);

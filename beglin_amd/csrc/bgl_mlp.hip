@@ -21,6 +21,7 @@
 
 #include "../../include/beglin_qgemv.h"
 #include "bgl_internal.h"
+#include "bgl_i8.h"
 
 #define HIPCHK(expr)                                                                             \
     do {                                                                                         \
@@ -79,6 +80,8 @@ extern "C" int bgl_mlp_dev(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor 
     }
     int rc = bgl_matmul_group_dev(c, 2, gu, act, x_dev, nob, ys, M);
     if (rc) return rc;
+    // K_Q8C: the launch that quantizes h forms it
+    if (act == BGL_ACT_W4A8 && down->T.fmt == BGL_K_Q8C) return run_i8_cols(c, 1, &down->T, g, u, h, M, nullptr, &y_dev);
     // several W4A8 columns whose down projection quantizes them up front: that launch forms h too
     if (act == BGL_ACT_W4A8) {
         rc = run_down_swiglu_w4a8(c, down->T, g, u, h, M, y_dev);

@@ -470,6 +470,12 @@ static int expert_check(const bgl_tensor *t, const char *what) {
     return 0;
 }
 
+static bool stack_i8(const bgl_tensor *t) {
+    for (const bgl_tensor *e : t->experts)
+        if (e->T.fmt == BGL_K_Q8C) return true;
+    return false;
+}
+
 static void max_units(const bgl_tensor *t, int &tiles, int &units) {
     tiles = 0; units = 0;
     for (const bgl_tensor *e : t->experts) {
@@ -483,6 +489,8 @@ extern "C" int bgl_gather_matvec_dev(bgl_ctx *c, const bgl_tensor *experts, cons
     if (!c || !x_dev || !idx_dev || !y_dev || N < 1) return bgl_fail(BGL_E_ARG, "bgl_gather_matvec_dev: bad argument");
     int rc = expert_check(experts, "bgl_gather_matvec_dev: experts");
     if (rc) return rc;
+    if (stack_i8(experts))
+        return bgl_fail(BGL_E_UNSUPPORTED, "bgl_gather_matvec_dev: K_Q8C experts take int8 activations only (bgl_moe_ffn_dev)");
     HIPCHK(hipSetDevice(c->device));
     const int E = (int)experts->experts.size();
     MoeScratch S;
@@ -642,6 +650,8 @@ static int moe_ffn(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, con
     for (int e = 0; e < E; e++)
         if (gate->experts[e]->T.fmt != up->experts[e]->T.fmt || gate->experts[e]->T.bits != up->experts[e]->T.bits)
             return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: expert %d gate and up differ in format", e);
+    if (stack_i8(gate) || stack_i8(up) || stack_i8(down))
+        return bgl_fail(BGL_E_UNSUPPORTED, "bgl_moe_ffn_dev: K_Q8C experts");
     const int nsh = (sg != nullptr) + (su != nullptr) + (sd != nullptr);
     if (nsh != 0 && nsh != 3) return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: give all three shared tensors or none");
     int Ish = 0;

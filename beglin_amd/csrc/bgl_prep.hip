@@ -401,6 +401,22 @@ __global__ void k_repack_q8(const int8_t *__restrict__ src, int N, int K, uint8_
     *reinterpret_cast<uint4 *>(dst + (((size_t)tile * cpr + c) * BGL_TILE + lane) * 16) = v;
 }
 
+// K_Q8C: the same interleave for rows of any length, `pitch` bytes apart in src; zero codes behind each row
+// and behind the last one.
+__global__ void k_repack_q8c(const int8_t *__restrict__ src, int N, int K, long pitch, int cpr, uint8_t *__restrict__ dst) {
+    const long t = (long)blockIdx.x * blockDim.x + threadIdx.x, ntiles = (N + BGL_TILE - 1) / BGL_TILE;
+    if (t >= ntiles * BGL_TILE * cpr) return;
+    const int r = (int)(t / cpr), c = (int)(t % cpr);
+    union { int8_t b[16]; uint4 v; } o;
+    o.v = make_uint4(0, 0, 0, 0);
+    if (r < N) {
+        const int8_t *s = src + (size_t)r * pitch + (size_t)c * 16;
+        const int n = min(16, K - c * 16);
+        for (int i = 0; i < n; i++) o.b[i] = s[i];
+    }
+    *reinterpret_cast<uint4 *>(dst + (((size_t)(r / BGL_TILE) * cpr + c) * BGL_TILE + r % BGL_TILE) * 16) = o.v;
+}
+
 // qNg64 bit planes -> field chunks.  One thread per (row, pair of 64-groups).  Per pair (128
 // elements) the device stores n chunks: the 8-bit field (8 chunks, element 16k+i in byte i of chunk
 // k, stored as f ^ 0x80 i.e. f-128 as a signed byte), the 4-bit field (4 chunks, int4 device nibble
@@ -559,11 +575,17 @@ __global__ void k_repack_qng_scales(const float *__restrict__ src, int N, int ng
 // 64-bit division to find it, took 150 us for 14336 x 4096 q4g64; 40 us so, 46 for a plain write).
 // int4: the 4 columns are the low or the high nibbles of one dword.
 __global__ __launch_bounds__(256) void k_dequant(BglDevTensor T, int row0, int nrows, float *__restrict__ out) {
-    const unsigned ng = T.K / 64;                            // workgroups along the columns
+    const unsigned ng = (T.K + 63) / 64;                     // workgroups along the columns
     const int rl = (int)(blockIdx.x / ng) * 16 + (threadIdx.x >> 4), c = (int)(blockIdx.x % ng) * 64 + 4 * (threadIdx.x & 15);
     if (rl >= nrows) return;
     const int r = row0 + rl, tile = r / BGL_TILE, lane = r % BGL_TILE;
     pk_f4 v;
+    if (T.fmt == BGL_K_Q8C) {                                // any number of columns, rows of any alignment
+        const uint32_t d = *reinterpret_cast<const uint32_t *>(T.w + (((size_t)tile * T.cpr + c / 16) * BGL_TILE + lane) * 16 + c % 16);
+        const float s = reinterpret_cast<const float *>(T.s0)[r];
+        for (int i = 0; i < 4 && c + i < T.K; i++) out[(size_t)rl * T.K + c + i] = __fmul_rn((float)(int8_t)(d >> (8 * i)), s);
+        return;
+    }
     if (T.fmt == BGL_Q4G64 || T.fmt == BGL_Q4G32H || T.fmt == BGL_Q4G256SF) {
         const uint32_t d = *reinterpret_cast<const uint32_t *>(T.w + (((size_t)tile * T.cpr + c / 32) * BGL_TILE + lane) * 16 + 4 * ((c % 32) / 8));
         uint32_t n4 = c % 8 ? (d >> 4) & 0x0F0F0F0Fu : d & 0x0F0F0F0Fu;

@@ -17,6 +17,9 @@
  *     blocks of 32, an E8M0 exponent byte then 16 bytes of E2M1 nibbles (gguf_quants.c:284-327).
  *     Kinds 6..9 run in the MoE gather only (fp32 activations).  10 BGL_K_Q4G256P is the plain-g256
  *     diagnostic of q4gemv_g256.h:102-130 (q4 nibbles, one fp32 scale per 256 values, W4A8 only).
+ *     11 BGL_K_Q8C has no counterpart in the reference: int8 codes with one fp32 scale per output
+ *     channel, multiplied by int8 activations with one scale per token (BGL_ACT_W4A8 only; any in
+ *     up to 131071, where the int32 sum cannot overflow).
  *   - *_dev entry points take DEVICE pointers and are asynchronous on the context's stream;
  *     host-pointer entry points (the drop-ins with the reference's exact argument lists) copy
  *     x in and y out and return after y is on the host.
@@ -39,7 +42,9 @@ extern "C" {
 #endif
 
 enum { BGL_K_Q4G64 = 1, BGL_K_Q8G64 = 2, BGL_K_Q4G256SF = 3, BGL_K_QNG64 = 4, BGL_K_Q4G32H = 5,
-       BGL_K_Q4G64A = 6, BGL_K_F16 = 7, BGL_K_F32 = 8, BGL_K_MXFP4 = 9, BGL_K_Q4G256P = 10 };
+       BGL_K_Q4G64A = 6, BGL_K_F16 = 7, BGL_K_F32 = 8, BGL_K_MXFP4 = 9, BGL_K_Q4G256P = 10, BGL_K_Q8C = 11 };
+enum { BGL_T_F32 = 0, BGL_T_F16 = 1, BGL_T_BF16 = 2 };          /* element types of rows in device memory */
+enum { BGL_NORM_NONE = 0, BGL_NORM_RMS = 1, BGL_NORM_LAYER = 2 };
 enum { BGL_ACT_F32 = 0, BGL_ACT_W4A8 = 1 };
 enum { BGL_OK = 0, BGL_E_ARG = -1, BGL_E_UNSUPPORTED = -2, BGL_E_HIP = -3, BGL_E_NODEV = -4, BGL_E_NOMEM = -5,
        BGL_E_CAPTURE = -6 /* per-call scratch would have to grow inside a stream capture */,
@@ -51,10 +56,10 @@ typedef struct bgl_tensor bgl_tensor;
 /* Weight descriptor: the fields of the engine's WT (qwen_infer.c:208-222).
  *   packed: K_Q4G64/K_Q4G256SF/Q4G32H/Q4G64A nibbles [out][in/2] (low nibble = even column; the
  *           AF int4 u32 words [out][in/8] are the same bytes, mlx_moe.cpp:238-257);
- *           K_Q8G64 int8 codes [out][in]; K_QNG64 bit planes [out][in/64][n][8];
+ *           K_Q8G64 and K_Q8C int8 codes [out][in]; K_QNG64 bit planes [out][in/64][n][8];
  *           F16 / F32: dense fp16 / fp32 rows [out][in]; MXFP4: the GGUF blocks [out][in/32][17].
  *   scales: fp32 [out][in/64] (K_Q4G64, K_Q8G64, K_QNG64, Q4G64A); fp32 wsuper [out][in/256]
- *           (K_Q4G256SF; the plain scale for Q4G256P); fp16 bits [out][in/32] (Q4G32H); unused (may be NULL) for F16 / F32 / MXFP4.
+ *           (K_Q4G256SF; the plain scale for Q4G256P); fp16 bits [out][in/32] (Q4G32H); fp32 [out] (K_Q8C); unused (may be NULL) for F16 / F32 / MXFP4.
  *   sub:    K_Q4G256SF: sub-codes u8 [out][in/64]; Q4G64A: fp32 biases [out][in/64] (read as bytes).
  *   bits:   K_QNG64 only: n in 2..15. */
 typedef struct {
@@ -114,7 +119,8 @@ int  bgl_dequant_dev(bgl_ctx *ctx, const bgl_tensor *t, int row0, int nrows, flo
  *         q4gemv.h:672-769; qng64_matvec_f32 / qng64_matmul_f32, qng64_dense.c:70-100).
  *   act = BGL_ACT_W4A8: the reference's dynamic int8 activations (gemv_q4g64_sdot_mt,
  *         gemv_q8g64_sdot_mt, gemm_qXg64_sdot_mt, q4gemv.h:701-791; gemv/gemm_q4g256sf_sdot_mt,
- *         q4gemv_g256.h:339-383).  K_Q4G256SF accepts only this mode (qwen_infer.c:697-702).
+ *         q4gemv_g256.h:339-383).  K_Q4G256SF accepts only this mode (qwen_infer.c:697-702), and so
+ *         does K_Q8C, whose columns are quantized as one group each.
  * This is the matvec_t / matmul_t / matmul_sdot backend switch (qwen_infer.c:687-708,
  * :1608-1655, :1852-1900) with the format taken from the bound tensor. */
 int  bgl_matmul_dev(bgl_ctx *ctx, const bgl_tensor *w, int act, const float *x_dev, const float *bias_dev,
@@ -157,8 +163,55 @@ int  bgl_read_probe_dev(bgl_ctx *ctx, int n, const bgl_tensor *const *w, int nbl
 int  bgl_prep_act_dev(bgl_ctx *ctx, int act, int kind, const float *x_dev, int M, int in);
 int  bgl_matmul_prepped_dev(bgl_ctx *ctx, const bgl_tensor *w, int act, const float *bias_dev, float *y_dev, int M);
 /* W4A8 activation quantizer on device (q4_quant_act_i8, q4gemv.h:177-213; _g256,
- * q4gemv_g256.h:72-99): xq [M][in] int8, ascale [M][in/gsize]. */
+ * q4gemv_g256.h:72-99): xq [M][in] int8, ascale [M][in/gsize].  gsize 64, 256, or in itself: one scale
+ * per token, the columns of K_Q8C (then in % 16 == 0 and xq 16-byte aligned; bgl_norm_dev writes rows
+ * of other widths). */
 int  bgl_quant_act_i8_dev(bgl_ctx *ctx, const float *x_dev, int M, int in, int gsize, int8_t *xq_dev, float *ascale_dev);
+
+/* ---------------- int8 with one scale per token and per output channel ----------------
+ * K_Q8C products over columns that the caller quantized (bgl_norm_dev, bgl_quant_act_i8_dev): for
+ * n <= 4 tensors of one `in`
+ *     y[i][m][r] = (fp32)(sum_c xq[m][c] * W_i[r][c]) * (ascale[m] * wscale_i[r]) + bias_i[r]
+ * with an exact int32 sum; every fp32 operation is rounded, and the result is rounded once more to
+ * y_type (BGL_T_*).  xq: rows ldq bytes apart, ldq % 16 == 0, ldq >= in, 16-byte aligned; the bytes
+ * between in and the row's next multiple of 16 may hold anything.  ascale [M].  bias_dev, or an entry
+ * of it, may be NULL.  y[i]: rows ldy[i] values apart (ldy NULL: dense), so a group may fill the parts of
+ * one wider row.  No scratch for up to 64 columns and none that a capture would have to grow; no
+ * counterpart in the reference.  bgl_matmul_dev, bgl_matmul_group_dev, bgl_mlp_dev,
+ * bgl_prep_act_dev / bgl_matmul_prepped_dev, bgl_quantize_dev (largest |w| of a row = 127) and
+ * bgl_dequant_dev take K_Q8C as any kind; bgl_moe_ffn_dev and bgl_moe_layer_dev take stacks of it. */
+int  bgl_matmul_i8_dev(bgl_ctx *ctx, int n, const bgl_tensor *const *w, const int8_t *xq_dev, long ldq, const float *ascale_dev,
+                       const float *const *bias_dev, void *const *y_dev, int y_type, const long *ldy, int M);
+/* The end of a block and the norm before the next one, in one launch over T rows of H values
+ * (the residual adds and rmsnorm calls of forward_token, qwen_infer.c:1435-1585; the norm after the
+ * block, the gate, the residual scale and the int8 output have no counterpart there):
+ *     n = post(f)                    f: the block's output, or NULL: then v = x
+ *     v = x + alpha * gate * n       rounded to x_type, written to x_out (which may be x itself)
+ *     y = norm(v)                    written to y, and / or as int8 codes to yq with a scale per row
+ *     BGL_NORM_RMS     v / sqrt(mean(v^2) + eps) * (w + w_add) + b
+ *     BGL_NORM_LAYER   (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * (w + w_add) + b
+ *     BGL_NORM_NONE    v             (w and b unused)
+ * Values are computed in double and rounded to fp32, then to the output's type; the codes are those
+ * that bgl_quant_act_i8_dev gives for the fp32 values (a row holding NaN or an infinity: codes 0 and a
+ * scale that is not finite, so its products are NaN).  w, b: fp32 [H], NULL: 1 and 0.  gate: values
+ * gate_t * t + gate_c * h of f's type -- per channel (0, 1), per token (1, 0), per both (>= H, 1);
+ * NULL: 1.  Strides are in elements (ldq: bytes, a multiple of 16, the bytes from H to the next
+ * multiple of 16 are zeroed).  Apart from x_out == x the rows that are written overlap nothing that is
+ * read. */
+typedef struct {
+    int T, H;
+    const void *x; long ldx; int x_type;
+    const void *f; long ldf; int f_type;
+    int post; const float *post_w, *post_b; float post_eps;
+    const void *gate; long gate_t, gate_c;
+    float alpha;
+    float w_add;                                   /* of both norms: 1 where weights are stored as w - 1 */
+    void *x_out; long ldo;
+    int kind; const float *w, *b; float eps;
+    void *y; long ldy; int y_type;
+    int8_t *yq; long ldq; float *yscale;
+} bgl_norm;
+int  bgl_norm_dev(bgl_ctx *ctx, const bgl_norm *d);
 
 /* ---------------- host-pointer drop-ins with the reference's argument lists ----------------
  * The q4pool* argument becomes the context.  The weight pointer identifies the tensor: the first
