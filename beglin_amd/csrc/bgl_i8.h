@@ -85,3 +85,9 @@ int run_i8_cols(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x, const
                 const float *const *bias, float *const *y);
 // bytes between the codes' rows in the context's scratch: whole 64-value units
 static inline long i8_ld_scratch(int K) { return ((long)K + 63) / 64 * 64; }
+// The routed FFN of K_Q8C experts (bgl_moe_i8.hip), shapes checked by the caller: routing given (rw null), or from the
+// router rw [E][H] (+ rb).
+#define MOE_I8_MAX_E 1024
+int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down, const bgl_tensor *sg, const bgl_tensor *su,
+               const bgl_tensor *sd, const float *rw, const float *rb, int renorm, const float *x, const int32_t *idx, const float *w, int T,
+               int K, float *out);

@@ -21,6 +21,8 @@
 
 #include "bgl_gemv_impl.h"
 #include "bgl_internal.h"
+#include "bgl_i8.h"
+#include "bgl_route.h"
 
 #define HIPCHK(expr)                                                                             \
     do {                                                                                         \
@@ -631,12 +633,9 @@ static int moe_ffn_m(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, c
     return 0;
 }
 
-// The routed FFN; pre: the pairs' bucketing when the caller already made it (the whole-layer entry).
-static int moe_ffn(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down, const bgl_tensor *sg,
-                   const bgl_tensor *su, const bgl_tensor *sd, const float *x_dev, const int32_t *idx_dev, const float *w_dev,
-                   int T, int K, float *out_dev, const MoeScratch *pre) {
-    if (!c || !x_dev || !idx_dev || !w_dev || !out_dev || T < 1 || K < 1 || K > MOE_MAX_K)
-        return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: bad argument (T=%d, K=%d; 1 <= K <= %d)", T, K, MOE_MAX_K);
+// Whether the tensors form a routed FFN, and one that its kernels take; i8: its experts are K_Q8C.
+static int moe_check(const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down, const bgl_tensor *sg, const bgl_tensor *su,
+                     const bgl_tensor *sd, bool &i8) {
     int rc;
     if ((rc = expert_check(gate, "bgl_moe_ffn_dev: gate")) || (rc = expert_check(up, "bgl_moe_ffn_dev: up")) ||
         (rc = expert_check(down, "bgl_moe_ffn_dev: down")))
@@ -650,8 +649,6 @@ static int moe_ffn(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, con
     for (int e = 0; e < E; e++)
         if (gate->experts[e]->T.fmt != up->experts[e]->T.fmt || gate->experts[e]->T.bits != up->experts[e]->T.bits)
             return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: expert %d gate and up differ in format", e);
-    if (stack_i8(gate) || stack_i8(up) || stack_i8(down))
-        return bgl_fail(BGL_E_UNSUPPORTED, "bgl_moe_ffn_dev: K_Q8C experts");
     const int nsh = (sg != nullptr) + (su != nullptr) + (sd != nullptr);
     if (nsh != 0 && nsh != 3) return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: give all three shared tensors or none");
     int Ish = 0;
@@ -666,7 +663,28 @@ static int moe_ffn(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, con
         if (sg->T.fmt == BGL_Q4G256SF || sd->T.fmt == BGL_Q4G256SF || Ish % 64)
             return bgl_fail(BGL_E_UNSUPPORTED, "bgl_moe_ffn_dev: shared experts need fp32-activation formats, in %% 64 == 0");
     }
+    i8 = stack_i8(gate);
+    auto all = [&](const bgl_tensor *s) { return std::all_of(s->experts.begin(), s->experts.end(), [](const bgl_tensor *e) { return e->T.fmt == BGL_K_Q8C; }); };
+    if (i8 || stack_i8(up) || stack_i8(down) || (nsh && (sg->T.fmt == BGL_K_Q8C || sd->T.fmt == BGL_K_Q8C))) {
+        if (!all(gate) || !all(up) || !all(down) || (nsh && (sg->T.fmt != BGL_K_Q8C || sd->T.fmt != BGL_K_Q8C)))
+            return bgl_fail(BGL_E_UNSUPPORTED, "bgl_moe_ffn_dev: K_Q8C experts (shared ones included) do not mix with other kinds");
+        if (E > MOE_I8_MAX_E) return bgl_fail(BGL_E_UNSUPPORTED, "bgl_moe_ffn_dev: %d K_Q8C experts (at most %d)", E, MOE_I8_MAX_E);
+    }
+    return 0;
+}
+
+// The routed FFN; pre: the pairs' bucketing when the caller already made it (the whole-layer entry).
+static int moe_ffn(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down, const bgl_tensor *sg,
+                   const bgl_tensor *su, const bgl_tensor *sd, const float *x_dev, const int32_t *idx_dev, const float *w_dev,
+                   int T, int K, float *out_dev, const MoeScratch *pre) {
+    if (!c || !x_dev || !idx_dev || !w_dev || !out_dev || T < 1 || K < 1 || K > MOE_MAX_K)
+        return bgl_fail(BGL_E_ARG, "bgl_moe_ffn_dev: bad argument (T=%d, K=%d; 1 <= K <= %d)", T, K, MOE_MAX_K);
+    int rc;
+    bool i8;
+    if ((rc = moe_check(gate, up, down, sg, su, sd, i8))) return rc;
+    const int E = (int)gate->experts.size(), H = gate->T.K, I = gate->T.N, nsh = sg ? 3 : 0, Ish = sg ? sg->T.N : 0;
     HIPCHK(hipSetDevice(c->device));
+    if (i8) return run_moe_i8(c, gate, up, down, sg, su, sd, nullptr, nullptr, 0, x_dev, idx_dev, w_dev, T, K, out_dev);
     const int P = T * K;
     MoeScratch S;
     if (pre) S = *pre;
@@ -773,104 +791,17 @@ extern "C" int bgl_moe_ffn_dev(bgl_ctx *c, const bgl_tensor *gate, const bgl_ten
 // The router dot products run in double on every lane (fma with exact float products) and are
 // combined across the wave; the softmax sum runs sequentially in expert order as the reference's.
 // exp is evaluated in double and rounded once to float.
-#define ROUTE_MAXE 256
 #define ROUTE_EPW 4          // experts per scores workgroup: one per wave
 
 // scores[t][e] = (float)(sum_c (double)W[e][c] * x[t][c]) (+ b[e]); grid (T, ceil(E/4)), one wave
-// per expert so the router matrix is read by many CUs at once.  Each lane sums its elements
-// 4*lane + 256*i in ascending order; a round's 8 row and 8 x loads all go out before the first fma
-// (buffer loads: the ones past H return zero, so none is conditional and one round trip serves
-// H <= 2048).
-#define ROUTE_RND 8
+// per expert so the router matrix is read by many CUs at once (route_dot_wave, bgl_route.h).
 __global__ __launch_bounds__(ROUTE_EPW * 64) void k_moe_router_scores(const float *__restrict__ W, const float *__restrict__ bias,
                                                                       int E, int H, const float *__restrict__ x,
                                                                       float *__restrict__ scores) {
     const int t = blockIdx.x, e = blockIdx.y * ROUTE_EPW + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (e >= E) return;
-    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(W + (size_t)e * H), (short)0, H * 4, 0x00020000);
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(x + (size_t)t * H), (short)0, H * 4, 0x00020000);
-    typedef float rf4 __attribute__((ext_vector_type(4)));
-    double acc = 0.0;
-    for (int c0 = 0; c0 < H; c0 += ROUTE_RND * 256) {
-        rf4 wv[ROUTE_RND], xv[ROUTE_RND];
-#pragma unroll
-        for (int i = 0; i < ROUTE_RND; i++) {
-            const int off = (c0 + 256 * i + 4 * lane) * 4;
-            wv[i] = __builtin_bit_cast(rf4, __builtin_amdgcn_raw_buffer_load_b128(wr, off, 0, 0));
-            xv[i] = __builtin_bit_cast(rf4, __builtin_amdgcn_raw_buffer_load_b128(xr, off, 0, 0));
-        }
-#pragma unroll
-        for (int i = 0; i < ROUTE_RND; i++) {
-            acc = fma((double)wv[i].x, (double)xv[i].x, acc);
-            acc = fma((double)wv[i].y, (double)xv[i].y, acc);
-            acc = fma((double)wv[i].z, (double)xv[i].z, acc);
-            acc = fma((double)wv[i].w, (double)xv[i].w, acc);
-        }
-    }
-    for (int o = 32; o; o >>= 1) acc += __shfl_xor(acc, o);
+    const double acc = route_dot_wave(W + (size_t)e * H, x + (size_t)t * H, H, lane);
     if (lane == 0) scores[(size_t)t * E + e] = bias ? __fadd_rn((float)acc, bias[e]) : (float)acc;
-}
-
-// Softmax, top-K and renorm of one token's E scores by one wave; lane 0 returns the K picks.
-__device__ __forceinline__ void route_topk_wave(const float *__restrict__ sc_t, int E, int K, int renorm, int lane,
-                                                int *sel_i, float *sel_w, float *lbuf) {
-    constexpr int PL = ROUTE_MAXE / 64;                      // scores per lane: expert lane + 64j
-    float v[PL];
-    float mx = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < PL; j++) {
-        const int e = lane + 64 * j;
-        v[j] = e < E ? sc_t[e] : 0.0f;
-        if (e < E) mx = fmaxf(mx, v[j]);
-    }
-    mx = wave_max_f32(mx);
-#pragma unroll
-    for (int j = 0; j < PL; j++) {
-        const int e = lane + 64 * j;
-        if (e < E) v[j] = (float)exp((double)__fsub_rn(v[j], mx));
-    }
-    // the double sum in expert order: the values go through the wave's LDS row (lbuf, 16-byte
-    // aligned, ROUTE_MAXE floats) and every lane reads them all at the same addresses (broadcast
-    // reads, 16 values per round); a wave's LDS accesses complete in order
-#pragma unroll
-    for (int j = 0; j < PL; j++)
-        if (lane + 64 * j < E) lbuf[lane + 64 * j] = v[j];
-    __builtin_amdgcn_wave_barrier();
-    typedef float lf4 __attribute__((ext_vector_type(4)));
-    const lf4 *l4 = reinterpret_cast<const lf4 *>(lbuf);
-    double sum = 0.0;
-    int e16 = 0;
-    for (; e16 + 16 <= E; e16 += 16) {
-        const lf4 q0 = l4[e16 / 4], q1 = l4[e16 / 4 + 1], q2 = l4[e16 / 4 + 2], q3 = l4[e16 / 4 + 3];
-        sum += (double)q0.x; sum += (double)q0.y; sum += (double)q0.z; sum += (double)q0.w;
-        sum += (double)q1.x; sum += (double)q1.y; sum += (double)q1.z; sum += (double)q1.w;
-        sum += (double)q2.x; sum += (double)q2.y; sum += (double)q2.z; sum += (double)q2.w;
-        sum += (double)q3.x; sum += (double)q3.y; sum += (double)q3.z; sum += (double)q3.w;
-    }
-    for (; e16 < E; e16++) sum += (double)lbuf[e16];
-    unsigned used = 0;                                       // bit j: expert lane + 64j selected
-#pragma unroll
-    for (int j = 0; j < PL; j++) v[j] = (float)((double)v[j] / sum);
-    for (int k = 0; k < K; k++) {
-        // this lane's best unselected expert (lowest id first among equal values), then the wave's
-        float bv = -1.0f;
-        int bi = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < PL; j++) {
-            const int e = lane + 64 * j;
-            if (e < E && !((used >> j) & 1u) && v[j] > bv) { bv = v[j]; bi = e; }
-        }
-        wave_argmax(bv, bi);                                  // DPP and readlane: no LDS round trips
-        if ((bi & 63) == lane) used |= 1u << (bi >> 6);
-        sel_w[k] = bv;
-        sel_i[k] = bi;
-    }
-    if (lane == 0 && renorm) {
-        double s = 0.0;
-        for (int k = 0; k < K; k++) s += (double)sel_w[k];
-        if (s > 0.0)
-            for (int k = 0; k < K; k++) sel_w[k] = (float)((double)sel_w[k] / s);
-    }
 }
 
 // softmax, top-K and renorm of one token per wave (grid T, 64 threads).
@@ -886,6 +817,10 @@ __global__ __launch_bounds__(64) void k_moe_route_topk(const float *__restrict__
         idx_out[(size_t)t * K + k] = sel_i[k];
         w_out[(size_t)t * K + k] = sel_w[k];
     }
+}
+
+void bgl_launch_route_topk(const float *scores, int T, int E, int K, int renorm, int32_t *idx, float *w, hipStream_t st) {
+    hipLaunchKernelGGL(k_moe_route_topk, dim3(T), dim3(64), 0, st, scores, E, K, renorm, idx, w);
 }
 
 // The top-K of every token (one wave per token in turn) and the bucketing of the T*K pairs by
@@ -932,13 +867,18 @@ __global__ __launch_bounds__(1024) void k_moe_route_bucket(const float *__restri
 }
 
 // The router's checks and its scores kernel; *scores: the [T][E] scores in the context's scratch.
-static int route_scores(bgl_ctx *c, const char *who, const float *rw_dev, const float *rb_dev, int E, int in,
-                        const float *x_dev, int T, int K, float **scores) {
+static int route_check(bgl_ctx *c, const char *who, const float *rw_dev, int E, int in, const float *x_dev, int T, int K) {
     if (!c || !rw_dev || !x_dev || T < 1) return bgl_fail(BGL_E_ARG, "%s: bad argument", who);
     if (E < 1 || E > ROUTE_MAXE || K < 1 || K > E || K > MOE_MAX_K)
         return bgl_fail(BGL_E_ARG, "%s: need 1 <= K <= min(E, %d) and E <= %d (E=%d, K=%d)", who, MOE_MAX_K, ROUTE_MAXE, E, K);
     if (in < 4 || in % 4 || ((uintptr_t)rw_dev | (uintptr_t)x_dev) % 16)
         return bgl_fail(BGL_E_ARG, "%s: in=%d must be a multiple of 4 with 16-byte aligned rows", who, in);
+    return 0;
+}
+static int route_scores(bgl_ctx *c, const char *who, const float *rw_dev, const float *rb_dev, int E, int in,
+                        const float *x_dev, int T, int K, float **scores) {
+    const int rc = route_check(c, who, rw_dev, E, in, x_dev, T, K);
+    if (rc) return rc;
     HIPCHK(hipSetDevice(c->device));
     if (dbuf_reserve(c, c->moe_scores, (size_t)T * E * 4, false)) return bgl_last_code();
     *scores = (float *)c->moe_scores.p;
@@ -970,6 +910,13 @@ extern "C" int bgl_moe_layer_dev(bgl_ctx *c, const float *rw_dev, const float *r
     int rc;
     if ((rc = expert_check(gate, "bgl_moe_layer_dev: gate"))) return rc;
     const int E = (int)gate->experts.size(), H = gate->T.K;
+    if (stack_i8(gate)) {
+        bool i8;
+        if (!out_dev || K > MOE_MAX_K) return bgl_fail(BGL_E_ARG, "bgl_moe_layer_dev: bad argument (K=%d)", K);
+        if ((rc = moe_check(gate, up, down, sg, su, sd, i8)) || (rc = route_check(c, "bgl_moe_layer_dev", rw_dev, E, H, x_dev, T, K))) return rc;
+        HIPCHK(hipSetDevice(c->device));
+        return run_moe_i8(c, gate, up, down, sg, su, sd, rw_dev, rb_dev, renorm ? 1 : 0, x_dev, nullptr, nullptr, T, K, out_dev);
+    }
     HIPCHK(hipSetDevice(c->device));
     if (dbuf_reserve(c, c->moe_route, (size_t)T * K * 8, false)) return bgl_last_code();
     int32_t *idx = (int32_t *)c->moe_route.p;

@@ -56,3 +56,24 @@ def normed(kind, v, w=None, b=None, eps=1e-6, w_add=0.0):
 def weights(rng, out, inn):
     """Codes over their whole range and scales of their own for each channel."""
     return rng.integers(-127, 128, (out, inn)).astype(np.int8), rng.uniform(2e-4, 9e-4, out).astype(F)
+
+
+def routed(x, idx, w, gate, up, down, shared=None):
+    """The routed FFN of int8 experts: gate / up / down are lists of (codes, scales), idx / w [T][K]; ids outside the stack
+    are skipped.  Experts are added in ascending order, then k, each step one fp32 operation."""
+    T, K = idx.shape
+    q, s = quantize(x)
+    out = np.zeros((T, x.shape[1]), F)
+    pair = {}
+    for e in range(len(gate)):
+        ts, ks = np.nonzero(idx == e)
+        if len(ts):
+            h = swiglu(product(q[ts], s[ts], *gate[e]), product(q[ts], s[ts], *up[e]))
+            y = product(*quantize(h), *down[e])
+            pair.update({(t, k): y[i] for i, (t, k) in enumerate(zip(ts, ks))})
+    for t in range(T):
+        for e, k in sorted((int(idx[t, k]), k) for k in range(K) if (t, k) in pair):
+            out[t] = out[t] + w[t, k] * pair[t, k]
+    if shared:
+        out = out + mlp(x, *shared)[1]
+    return out
