@@ -12,12 +12,12 @@
 // Every value is computed in double and rounded once to fp32 (and from there to a 16-bit type): a code
 // of the int8 output changes by one where a value lies within rounding of a border between codes, and
 // with the values right to fp32's last bit the codes are those of the formula.  gfx950 issues double
-// multiply-adds at the rate of single ones, and the launch is bound by memory.
+// multiply-adds at the rate of single ones, and the launch is bound by memory: 4096 rows of 4096 in bf16
+// (residual add, RMS norm) take 31 us, 4.3 TB/s of what they read and write, where a large copy moves 5.1.
 //
-// The row stays in registers between its two passes (statistics, then the output): 16 values a thread,
-// 64 threads to a row up to H = 1024, 256 up to 4096, 1024 up to 16384.  Wider rows (the quantizer takes
-// MLP rows) go through k_norm_wide, which reads the row again for each pass.  A workgroup walks several
-// rows, so the norm weights are read once per workgroup and kept.
+// The row stays in registers between its passes (statistics, then the output): a wave to a row up to H = 512, then
+// workgroups of 256, 512 or 1024 threads with 8 or 16 values each.  Wider
+// rows (the quantizer takes MLP rows) go through k_norm_wide, which reads the row again for each pass.
 #include <string.h>
 
 #include <algorithm>
@@ -36,68 +36,168 @@ struct NormLaunch {
     const float *glu_u;      // x is an MLP block's gate row: v = silu(x) * u, which goes to x_out (bgl_mlp.hip's h)
 };
 
-#define NORM_V 8             // consecutive values of a thread
-#define NORM_NV 2            // such runs
+// What a row is before the norm: itself, x + a gated block, x + a normed and gated block, or SwiGLU of two rows.
+enum { ROW_X = 0, ROW_ADD = 1, ROW_POST = 2, ROW_GLU = 3 };
 
-template <bool VEC>
-__device__ __forceinline__ void norm_ld8(float (&o)[NORM_V], const void *p, int type, size_t at, int left) {
-    if constexpr (VEC) {
-        if (left <= 0) {
+// 16 bytes of a row, wherever the row starts (gfx950 loads and stores them at any address)
+typedef float nr_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int nr_u4 __attribute__((ext_vector_type(4), aligned(2)));
+
+// A thread's values of a row of at least 8: NV chunks of 8 consecutive ones, NT chunks apart.  A chunk that the row's
+// end cuts, or that lies behind it, loads the row's last 8 values instead and shifts its own to the front (values past
+// the end are 0 and stay so): every load is a full one and none is conditional.
+template <int NT, int NV>
+struct RowMap {
+    static constexpr int N = 8 * NV;
+    int lt, H;
+    __device__ __forceinline__ int at(int i) const { return (i * NT + lt) * 8; }
+    __device__ __forceinline__ int has(int i) const { return H - at(i); }        // values of chunk i that exist (>= 8: all)
+    // An access is a uniform address plus the thread's 32-bit offset: no address registers per pointer and value.
+    template <typename V>
+    __device__ __forceinline__ V get(const void *row, int i, int per, int j = 0) const {
+        return *(const V *)((const char *)row + (uint32_t)(min(at(i), H - 8) + j) * (uint32_t)per);
+    }
+    template <typename V>
+    __device__ __forceinline__ void put(void *row, int i, int per, V v, int j = 0) const {
+        *(V *)((char *)row + (uint32_t)(at(i) + j) * (uint32_t)per) = v;
+    }
+    __device__ __forceinline__ void load(float *q, int i, const void *row, int type) const {
+        if (type == BGL_T_F32) {
+            const nr_f4 u = get<nr_f4>(row, i, 4), v = get<nr_f4>(row, i, 4, 4);
 #pragma unroll
-            for (int j = 0; j < NORM_V; j++) o[j] = 0.0f;
-        } else if (type == BGL_T_F32) {
-            const i8_f4 *q = (const i8_f4 *)((const float *)p + at);
-            const i8_f4 a = q[0], b = q[1];
-#pragma unroll
-            for (int j = 0; j < 4; j++) { o[j] = a[j]; o[4 + j] = b[j]; }
+            for (int j = 0; j < 4; j++) { q[j] = u[j]; q[4 + j] = v[j]; }
         } else {
-            const i8_u4 a = *(const i8_u4 *)((const uint16_t *)p + at);
+            const nr_u4 u = get<nr_u4>(row, i, 2);
+            if (type == BGL_T_F16) {
 #pragma unroll
-            for (int j = 0; j < NORM_V; j++) {
-                const uint16_t h = (uint16_t)(a[j / 2] >> (16 * (j & 1)));
-                o[j] = type == BGL_T_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+                for (int j = 0; j < 8; j++) q[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[j / 2] >> (16 * (j & 1))));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) q[j] = __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
             }
         }
-    } else {
+        const int s = 8 - has(i);
+        if (s > 0) {
 #pragma unroll
-        for (int j = 0; j < NORM_V; j++) o[j] = j < left ? i8_ld(p, type, at + j) : 0.0f;
-    }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void norm_st8(void *p, int type, size_t at, int left, const float (&v)[NORM_V]) {
-    if constexpr (VEC) {
-        if (left <= 0) return;
-        if (type == BGL_T_F32) {
-            i8_f4 *q = (i8_f4 *)((float *)p + at);
-            q[0] = i8_f4{v[0], v[1], v[2], v[3]};
-            q[1] = i8_f4{v[4], v[5], v[6], v[7]};
-        } else {
-            i8_u4 a;
+            for (int step = 4; step; step >>= 1) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) a[j] = (uint32_t)i8_h16(v[2 * j], type) | ((uint32_t)i8_h16(v[2 * j + 1], type) << 16);
-            *(i8_u4 *)((uint16_t *)p + at) = a;
+                for (int j = 0; j < 8; j++) q[j] = s & step ? (j + step < 8 ? q[j + step] : 0.0f) : q[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) q[j] = s >= 8 ? 0.0f : q[j];
         }
+    }
+    // zeroes what a computation made of the values past the end
+    __device__ __forceinline__ void cut(float *q, int i) const {
+        const int n = has(i);
+        if (n >= 8) return;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q[j] = j < n ? q[j] : 0.0f;
+    }
+    // chunk i rounded to the type and stored; with KEEP, q becomes what was stored
+    template <bool KEEP>
+    __device__ __forceinline__ void store(void *row, int type, float *q, int i) const {
+        const int n = has(i);
+        if (type == BGL_T_F32) {
+            if (!row) return;
+            if (n >= 8) {
+                put(row, i, 4, nr_f4{q[0], q[1], q[2], q[3]});
+                put(row, i, 4, nr_f4{q[4], q[5], q[6], q[7]}, 4);
+            } else if (n > 0) {
+#pragma unroll
+                for (int j = 0; j < 7; j++)
+                    if (j < n) put(row, i, 4, q[j], j);
+            }
+            return;
+        }
+        uint16_t h[8];
+        if (type == BGL_T_F16) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                h[j] = __builtin_bit_cast(uint16_t, (_Float16)q[j]);
+                if (KEEP) q[j] = (float)__builtin_bit_cast(_Float16, h[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                h[j] = __builtin_bit_cast(uint16_t, (__bf16)q[j]);
+                if (KEEP) q[j] = __uint_as_float((uint32_t)h[j] << 16);
+            }
+        }
+        if (!row) return;
+        if (n >= 8) {
+            nr_u4 u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[j] = (uint32_t)h[2 * j] | ((uint32_t)h[2 * j + 1] << 16);
+            put(row, i, 2, u);
+        } else if (n > 0) {
+#pragma unroll
+            for (int j = 0; j < 7; j++)
+                if (j < n) put(row, i, 2, h[j], j);
+        }
+    }
+};
+// row `row` of rows ld values of a type apart
+__device__ __forceinline__ const void *norm_row(const void *p, long row, long ld, int type) { return (const char *)p + row * ld * (type == BGL_T_F32 ? 4 : 2); }
+
+// n = (v - mean) * inv * (w + w_add) + b of a chunk, for any of its parts (the conditions are the launch's, outside the
+// loops over values)
+template <typename Map>
+__device__ __forceinline__ void norm_chunk(double (&n)[8], const Map &m, int i, const float *v, int kind, double mean, double inv, const float *w,
+                                           float w_add, const float *b) {
+    float p[8];
+    if (kind == BGL_NORM_LAYER) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) n[j] = ((double)v[j] - mean) * inv;
     } else {
 #pragma unroll
-        for (int j = 0; j < NORM_V; j++)
-            if (j < left) i8_st(p, type, at + j, v[j]);
+        for (int j = 0; j < 8; j++) n[j] = (double)v[j] * inv;
+    }
+    if (w) {
+        m.load(p, i, w, BGL_T_F32);
+        if (w_add == 0.0f) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) n[j] *= (double)p[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) n[j] *= (double)p[j] + (double)w_add;
+        }
+    }
+    if (b) {
+        m.load(p, i, b, BGL_T_F32);
+#pragma unroll
+        for (int j = 0; j < 8; j++) n[j] += (double)p[j];
     }
 }
 
+// Sums over a wave through DPP and readlane (a shuffle would go through the LDS, twice for a double).
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const int2 p = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(dpp_i<CTRL>(p.x), dpp_i<CTRL>(p.y)));
+}
+__device__ __forceinline__ double rlane_d(double v, int l) {
+    const int2 p = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(p.x, l), __builtin_amdgcn_readlane(p.y, l)));
+}
+__device__ __forceinline__ double row16_sum(double v) {
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    return v + dpp_d<0x140>(v);
+}
 // Sums over the NT threads of a row, in every one of them, in one order whatever the launch.
 template <int NT>
 __device__ __forceinline__ double row_sum(double v, double *red) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    v = row16_sum(v);
+    v = (rlane_d(v, 0) + rlane_d(v, 16)) + (rlane_d(v, 32) + rlane_d(v, 48));
     if constexpr (NT > 64) {
-        const int wave = threadIdx.x >> 6;
         __syncthreads();                       // the last round's reads are done
-        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.0;
-#pragma unroll
-        for (int i = 0; i < NT / 64; i++) v += red[i];
+        // lane l % 16 takes wave l % 16's sum (0 past the last wave)
+        const int w = threadIdx.x & 15;
+        v = rlane_d(row16_sum(w < NT / 64 ? red[w] : 0.0), 0);
     }
     return v;
 }
@@ -109,166 +209,148 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, double *red) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NT / 64; i++) v = max(v, r[i]);
+        v = wave_max_u32(r[threadIdx.x & (NT / 64 - 1)]);
     }
     return v;
 }
 
-// mean and 1 / sqrt(... + eps) of a norm over the thread's values (0 past the row's end)
-template <int NT, int NVAL>
-__device__ __forceinline__ void norm_stats(int kind, const float (&v)[NVAL], const bool (&in)[NVAL], int H, float eps, double *red,
+// mean and 1 / sqrt(... + eps) of a norm over the thread's values (0 past the row's end); rows: 1 / H
+template <int NT, typename Map>
+__device__ __forceinline__ void norm_stats(int kind, const float (&v)[Map::N], const Map &m, float eps, double rows, double *red,
                                            double &mean, double &inv) {
     mean = 0.0;
+    double q = 0.0;
     if (kind == BGL_NORM_LAYER) {
         double s = 0.0;
 #pragma unroll
-        for (int i = 0; i < NVAL; i++) s += (double)v[i];
-        mean = row_sum<NT>(s, red) / H;
-    }
-    double q = 0.0;
+        for (int k = 0; k < Map::N; k++) s += (double)v[k];
+        mean = row_sum<NT>(s, red) * rows;
 #pragma unroll
-    for (int i = 0; i < NVAL; i++) {
-        const double d = in[i] ? (double)v[i] - mean : 0.0;
-        q = fma(d, d, q);
+        for (int i = 0; i < Map::N / 8; i++) {
+            const int n = m.has(i);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double d = (double)v[8 * i + j] - mean;
+                if (n >= 8 || j < n) q = fma(d, d, q);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < Map::N; k++) q = fma((double)v[k], (double)v[k], q);
     }
-    inv = 1.0 / sqrt(row_sum<NT>(q, red) / H + (double)eps);
+    inv = rsqrt(row_sum<NT>(q, red) * rows + (double)eps);
 }
 
-template <int NT, bool VEC>
+template <int NT, int NV, int ROW>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormLaunch L) {
-    constexpr int RPW = NT < 256 ? 256 / NT : 1, NVAL = NORM_V * NORM_NV;
+    constexpr int RPW = NT < 256 ? 256 / NT : 1;
+    using Map = RowMap<NT, NV>;
+    constexpr int N = Map::N;
     const bgl_norm &d = L.d;
-    __shared__ double red[16];
-    const int lt = NT < 256 ? threadIdx.x % NT : threadIdx.x;
-    int at[NORM_NV], left[NORM_NV];
-    bool in[NVAL];
+    __shared__ double reds[RPW][16];
+    const int sub = NT < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+    double *const red = reds[sub];
+    const Map m{(int)threadIdx.x % NT, d.H};
+    static_assert(NT == 64 || NT >= 256, "a row is a wave's or a workgroup's");
+    const double rows = 1.0 / d.H;
+    const long row = (long)blockIdx.x * RPW + sub;
+    if (row >= d.T) return;                                  // whole waves (RPW > 1: no barrier follows)
+    {
+        float v[N], f[N];
 #pragma unroll
-    for (int i = 0; i < NORM_NV; i++) {
-        at[i] = (i * NT + lt) * NORM_V;
-        left[i] = d.H - at[i];
+        for (int i = 0; i < NV; i++) m.load(v + 8 * i, i, norm_row(d.x, row, d.ldx, d.x_type), d.x_type);
+        if constexpr (ROW == ROW_GLU) {
 #pragma unroll
-        for (int j = 0; j < NORM_V; j++) in[i * NORM_V + j] = j < left[i];
-    }
-    // the weights of the norm before the next block stay for every row of the workgroup
-    float w[NVAL];
+            for (int i = 0; i < NV; i++) {
+                m.load(f, i, norm_row(L.glu_u, row, d.ldx, BGL_T_F32), BGL_T_F32);
 #pragma unroll
-    for (int i = 0; i < NVAL; i++) w[i] = 1.0f;
-    if (d.w) {
-#pragma unroll
-        for (int i = 0; i < NORM_NV; i++)
-            norm_ld8<VEC>(*(float(*)[NORM_V])(w + i * NORM_V), d.w, BGL_T_F32, at[i], left[i]);
-    }
-    for (long row = (long)blockIdx.x * RPW + (NT < 256 ? threadIdx.x / NT : 0); row < d.T; row += (long)gridDim.x * RPW) {
-        float v[NVAL];
-#pragma unroll
-        for (int i = 0; i < NORM_NV; i++)
-            norm_ld8<VEC>(*(float(*)[NORM_V])(v + i * NORM_V), d.x, d.x_type, (size_t)row * d.ldx + at[i], left[i]);
-        if (L.glu_u) {
-            float u[NVAL];
-#pragma unroll
-            for (int i = 0; i < NORM_NV; i++)
-                norm_ld8<VEC>(*(float(*)[NORM_V])(u + i * NORM_V), L.glu_u, BGL_T_F32, (size_t)row * d.ldx + at[i], left[i]);
-#pragma unroll
-            for (int k = 0; k < NVAL; k++) v[k] = in[k] ? i8_swiglu(v[k], u[k]) : 0.0f;
-        }
-        if (d.f) {
-            float f[NVAL], g[NVAL];
-#pragma unroll
-            for (int i = 0; i < NORM_NV; i++)
-                norm_ld8<VEC>(*(float(*)[NORM_V])(f + i * NORM_V), d.f, d.f_type, (size_t)row * d.ldf + at[i], left[i]);
-            if (d.gate) {
-                if (d.gate_c) {
-#pragma unroll
-                    for (int i = 0; i < NORM_NV; i++)
-                        norm_ld8<VEC>(*(float(*)[NORM_V])(g + i * NORM_V), d.gate, d.f_type, (size_t)row * d.gate_t + at[i], left[i]);
-                } else {
-                    const float g1 = i8_ld(d.gate, d.f_type, (size_t)row * d.gate_t);
-#pragma unroll
-                    for (int i = 0; i < NVAL; i++) g[i] = g1;
-                }
+                for (int j = 0; j < 8; j++) v[8 * i + j] = i8_swiglu(v[8 * i + j], f[j]);      // of zeros: 0
             }
+        }
+        if constexpr (ROW == ROW_ADD || ROW == ROW_POST) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) m.load(f + 8 * i, i, norm_row(d.f, row, d.ldf, d.f_type), d.f_type);
             double mean = 0.0, inv = 1.0;
-            if (d.post != BGL_NORM_NONE) norm_stats<NT, NVAL>(d.post, f, in, d.H, d.post_eps, red, mean, inv);
+            if constexpr (ROW == ROW_POST) norm_stats<NT>(d.post, f, m, d.post_eps, rows, red, mean, inv);
 #pragma unroll
-            for (int i = 0; i < NORM_NV; i++) {
-                float pw[NORM_V], pb[NORM_V];
-                if (d.post != BGL_NORM_NONE && d.post_w) norm_ld8<VEC>(pw, d.post_w, BGL_T_F32, at[i], left[i]);
-                if (d.post != BGL_NORM_NONE && d.post_b) norm_ld8<VEC>(pb, d.post_b, BGL_T_F32, at[i], left[i]);
+            for (int i = 0; i < NV; i++) {
+                float *const vi = v + 8 * i;
+                if (ROW == ROW_ADD && !d.gate) {             // one rounding without the way through double
 #pragma unroll
-                for (int j = 0; j < NORM_V; j++) {
-                    const int k = i * NORM_V + j;
-                    double n = (double)f[k];
-                    if (d.post != BGL_NORM_NONE) {
-                        n = (n - mean) * inv;
-                        if (d.post_w) n *= (double)pw[j] + (double)d.w_add;
-                        if (d.post_b) n += (double)pb[j];
+                    for (int j = 0; j < 8; j++) vi[j] = fmaf(d.alpha, f[8 * i + j], vi[j]);
+                } else {
+                    double n[8];
+                    if constexpr (ROW == ROW_POST) norm_chunk(n, m, i, f + 8 * i, d.post, mean, inv, d.post_w, d.w_add, d.post_b);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) n[j] = (double)f[8 * i + j];
                     }
-                    if (d.gate) n *= (double)g[k];
-                    v[k] = in[k] ? i8_kept((float)((double)v[k] + (double)d.alpha * n), d.x_type) : 0.0f;
+                    if (d.gate) {
+                        float g[8];
+                        if (d.gate_c) m.load(g, i, norm_row(d.gate, row, d.gate_t, d.f_type), d.f_type);
+                        else {
+                            const float g1 = i8_ld(d.gate, d.f_type, (size_t)row * d.gate_t);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) g[j] = g1;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j++) n[j] *= (double)g[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++) vi[j] = (float)fma((double)d.alpha, n[j], (double)vi[j]);
+                    m.cut(vi, i);                            // a post norm's bias
                 }
             }
         }
-        if (d.x_out) {
+        if (ROW != ROW_X || d.x_out) {
+            void *const to = d.x_out ? const_cast<void *>(norm_row(d.x_out, row, d.ldo, d.x_type)) : nullptr;
 #pragma unroll
-            for (int i = 0; i < NORM_NV; i++)
-                norm_st8<VEC>(d.x_out, d.x_type, (size_t)row * d.ldo + at[i], left[i], *(float(*)[NORM_V])(v + i * NORM_V));
+            for (int i = 0; i < NV; i++) m.template store<true>(to, d.x_type, v + 8 * i, i);
         }
-        if (!d.y && !d.yq) continue;
+        if (!d.y && !d.yq) return;
         if (d.kind != BGL_NORM_NONE) {
             double mean, inv;
-            norm_stats<NT, NVAL>(d.kind, v, in, d.H, d.eps, red, mean, inv);
+            norm_stats<NT>(d.kind, v, m, d.eps, rows, red, mean, inv);
 #pragma unroll
-            for (int i = 0; i < NORM_NV; i++) {
-                float b[NORM_V];
-                if (d.b) norm_ld8<VEC>(b, d.b, BGL_T_F32, at[i], left[i]);
+            for (int i = 0; i < NV; i++) {
+                double n[8];
+                norm_chunk(n, m, i, v + 8 * i, d.kind, mean, inv, d.w, d.w_add, d.b);
 #pragma unroll
-                for (int j = 0; j < NORM_V; j++) {
-                    const int k = i * NORM_V + j;
-                    double n = ((double)v[k] - mean) * inv;
-                    if (d.w) n *= (double)w[k] + (double)d.w_add;
-                    if (d.b) n += (double)b[j];
-                    v[k] = (float)n;
-                }
+                for (int j = 0; j < 8; j++) v[8 * i + j] = (float)n[j];
+                m.cut(v + 8 * i, i);
             }
         }
         if (d.y) {
 #pragma unroll
-            for (int i = 0; i < NORM_NV; i++)
-                norm_st8<VEC>(d.y, d.y_type, (size_t)row * d.ldy + at[i], left[i], *(float(*)[NORM_V])(v + i * NORM_V));
+            for (int i = 0; i < NV; i++) m.template store<false>(const_cast<void *>(norm_row(d.y, row, d.ldy, d.y_type)), d.y_type, v + 8 * i, i);
         }
         if (d.yq) {
             uint32_t mb = I8_MX0;
 #pragma unroll
-            for (int k = 0; k < NVAL; k++)
-                if (in[k]) mb = max(mb, __float_as_uint(v[k]) & 0x7fffffffu);
+            for (int k = 0; k < N; k++) mb = max(mb, __float_as_uint(v[k]) & 0x7fffffffu);
             const I8Scale s = i8_scale(row_max<NT>(mb, red));
-            if (lt == 0) d.yscale[row] = s.sc;
+            if (m.lt == 0) d.yscale[row] = s.sc;
             int8_t *q = d.yq + (size_t)row * d.ldq;
+            const int H16 = (d.H + 15) & ~15;              // the bytes up to the row's next multiple of 16 are zeroed
 #pragma unroll
-            for (int i = 0; i < NORM_NV; i++) {
-                uint32_t c2[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float *t = v + i * NORM_V + 4 * j;
-                    const bool *u = in + i * NORM_V + 4 * j;
-                    c2[j] = i8_pack4(u[0] ? i8_code(t[0], s) : 0, u[1] ? i8_code(t[1], s) : 0, u[2] ? i8_code(t[2], s) : 0,
-                                     u[3] ? i8_code(t[3], s) : 0);
-                }
-                // rows are 16 bytes apart at least: whole runs of 8, the bytes up to the row's next multiple of 16 zeroed
-                if (at[i] < ((d.H + 15) & ~15)) *(uint2 *)(q + at[i]) = make_uint2(c2[0], c2[1]);
+            for (int i = 0; i < NV; i++) {
+                const float *t = v + 8 * i;
+                if (m.at(i) < H16)
+                    m.put(q, i, 1, make_uint2(i8_pack4(i8_code(t[0], s), i8_code(t[1], s), i8_code(t[2], s), i8_code(t[3], s)),
+                                              i8_pack4(i8_code(t[4], s), i8_code(t[5], s), i8_code(t[6], s), i8_code(t[7], s))));
             }
         }
     }
 }
 
-// Rows wider than 16384: 1024 threads a row, one value at a time, the row read again for each pass.
+// Rows wider than 16384 or narrower than 8: 1024 threads a row, one value at a time, the row read again for each pass.
 // Only the thread that wrote a value of x_out reads it back.
 __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
     const bgl_norm &d = L.d;
     __shared__ double red[16];
     const int tid = threadIdx.x;
-    for (long row = blockIdx.x; row < d.T; row += gridDim.x) {
+    {
+        const long row = blockIdx.x;
         double fmean = 0.0, finv = 1.0;
         if (d.f && d.post != BGL_NORM_NONE) {
             if (d.post == BGL_NORM_LAYER) {
@@ -300,7 +382,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
             for (int h = tid; h < d.H; h += 1024) i8_st(d.x_out, d.x_type, (size_t)row * d.ldo + h, fresh(h));
         // x_out may be x itself: from here on its new values are read
         auto value = [&](int h) -> float { return d.x_out ? i8_ld(d.x_out, d.x_type, (size_t)row * d.ldo + h) : fresh(h); };
-        if (!d.y && !d.yq) continue;
+        if (!d.y && !d.yq) return;
         double mean = 0.0, inv = 1.0;
         if (d.kind == BGL_NORM_LAYER) {
             double s = 0.0;
@@ -329,7 +411,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
             if (d.y) i8_st(d.y, d.y_type, (size_t)row * d.ldy + h, v);
             mb = max(mb, __float_as_uint(v) & 0x7fffffffu);
         }
-        if (!d.yq) continue;
+        if (!d.yq) return;
         const I8Scale s = i8_scale(row_max<1024>(mb, red));
         if (tid == 0) d.yscale[row] = s.sc;
         int8_t *q = d.yq + (size_t)row * d.ldq;
@@ -338,19 +420,29 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
 }
 
 // ================================================================================== host side
-#define NORM_BLOCKS 2048         // workgroups of a launch at most (8 a CU): each then walks its rows
+template <int ROW>
+static void norm_go(const NormLaunch &L, hipStream_t st) {
+    auto go = [&](auto kernel, int threads, int rows) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long)L.d.T + rows - 1) / rows)), dim3(threads), 0, st, L);
+    };
+    // (4096 bf16 rows of 4096 with 16 values a thread 31.2 us, with 8 33.1; 2048 normed-twice rows of 8192 36.8 and 42.7)
+    const int H = L.d.H;
+    if (H < 8) go(k_norm_wide, 1024, 1);
+    else if (H <= 512) go(k_norm<64, 1, ROW>, 256, 4);
+    else if (H <= 2048) go(k_norm<256, 1, ROW>, 256, 1);
+    else if (H <= 4096) go(k_norm<256, 2, ROW>, 256, 1);
+    else if (H <= 8192) go(k_norm<512, 2, ROW>, 512, 1);
+    else if (H <= 16384) go(k_norm<1024, 2, ROW>, 1024, 1);
+    else go(k_norm_wide, 1024, 1);
+}
 
-static int norm_launch(bgl_ctx *c, const NormLaunch &L, bool vec) {
+static int norm_launch(bgl_ctx *c, const NormLaunch &L) {
     const bgl_norm &d = L.d;
     int tok = prof_begin(c, L.glu_u || d.kind == BGL_NORM_NONE ? 0 : 2);
-    auto go = [&](auto kernel, int threads, int rows) {
-        const long blocks = std::min<long>(NORM_BLOCKS, ((long)d.T + rows - 1) / rows);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, c->stream, L);
-    };
-    if (d.H <= 1024) vec ? go(k_norm<64, true>, 256, 4) : go(k_norm<64, false>, 256, 4);
-    else if (d.H <= 4096) vec ? go(k_norm<256, true>, 256, 1) : go(k_norm<256, false>, 256, 1);
-    else if (d.H <= 16384) vec ? go(k_norm<1024, true>, 1024, 1) : go(k_norm<1024, false>, 1024, 1);
-    else go(k_norm_wide, 1024, 1);
+    if (L.glu_u) norm_go<ROW_GLU>(L, c->stream);
+    else if (!d.f) norm_go<ROW_X>(L, c->stream);
+    else if (d.post == BGL_NORM_NONE) norm_go<ROW_ADD>(L, c->stream);
+    else norm_go<ROW_POST>(L, c->stream);
     prof_end(c, tok);
     HIPCHK(hipGetLastError());
     return 0;
@@ -364,7 +456,7 @@ int run_quant_rows(bgl_ctx *c, const float *x, const float *u, float *h, int M, 
     L.glu_u = u;
     L.d.x_out = u ? h : nullptr; L.d.ldo = K;
     L.d.yq = xq; L.d.ldq = ldq; L.d.yscale = xs;
-    return norm_launch(c, L, K % 8 == 0 && (((uintptr_t)x | (uintptr_t)u | (uintptr_t)h) & 15) == 0);
+    return norm_launch(c, L);
 }
 
 extern "C" int bgl_norm_dev(bgl_ctx *c, const bgl_norm *d) {
@@ -396,10 +488,5 @@ extern "C" int bgl_norm_dev(bgl_ctx *c, const bgl_norm *d) {
     NormLaunch L;
     memset(&L, 0, sizeof L);
     L.d = *d;
-    // 16-byte accesses where every row starts on 16 bytes and holds whole runs of 8 values
-    auto al = [](const void *p, long ld, int type) { return !p || (((uintptr_t)p | (uintptr_t)ld * i8_elem(type)) & 15) == 0; };
-    const bool vec = h % 8 == 0 && al(d->x, d->ldx, d->x_type) && al(d->f, d->ldf, d->f_type) && al(d->x_out, d->ldo, d->x_type) &&
-                     al(d->y, d->ldy, d->y_type) && al(d->gate_c ? d->gate : nullptr, d->gate_t, d->f_type) &&
-                     al(d->w, 0, BGL_T_F32) && al(d->b, 0, BGL_T_F32) && al(d->post_w, 0, BGL_T_F32) && al(d->post_b, 0, BGL_T_F32);
-    return norm_launch(c, L, vec);
+    return norm_launch(c, L);
 }
