@@ -27,9 +27,11 @@ struct I8Task {
     void *y;
     long ldy;
     int blk0;                 // first workgroup row block of this tensor
+    int *part;                // K split: the slices' sums [slice][M][N rounded up to 4], joined by k_i8_join
 };
 struct I8Launch {
     I8Task t[BGL_MAX_TASKS];
+    int ks;                       // slices of K (grid z); 1: the outputs are written at once
     int n, M, K16, y_type, vec;   // K16: K rounded up to 16; vec: four outputs of a lane go in one store
     const int8_t *xq;
     long ldq;
@@ -70,6 +72,7 @@ __device__ __forceinline__ void i8_store4(const I8Launch &L, const I8Task &t, in
             if (r + i < t.T.N) i8_st(t.y, L.y_type, at + i, v[i]);
     }
 }
+__device__ __forceinline__ int i8_np(int N) { return (N + 3) & ~3; }
 // scales (the device copy is padded to whole tiles) and biases of channels r .. r + 3
 __device__ __forceinline__ i8_f4 i8_ws(const I8Task &t, int r) { return *(const i8_f4 *)((const float *)t.T.s0 + r); }
 __device__ __forceinline__ i8_f4 i8_bias(const I8Task &t, int r) {
@@ -84,19 +87,25 @@ __device__ __forceinline__ i8_f4 i8_bias(const I8Task &t, int r) {
 // ================================================================================== few columns
 // A workgroup owns RB blocks of 16 channels and up to 16 CB tokens; its waves split K.  Weights and codes
 // go straight from memory to the operand registers, D units ahead; the waves' int32 sums meet in LDS.
+// Partial sums of at most I8_S_PART / (RB * CB) waves lie in LDS at once: a workgroup of twice that many waves first
+// adds the upper half's to the lower half's.
+#define I8_S_PART 64          // KB
 template <int RB, int CB>
-constexpr int i8_s_waves() { return RB * CB <= 4 ? 16 : 64 / (RB * CB); }    // 64 KB of sums at most
+constexpr int i8_s_waves() { return RB * CB <= 4 ? 16 : 8; }
 template <int RB, int CB, int D>
 __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L) {
     extern __shared__ __align__(16) i8_i4 red[];               // [wave][RB * CB][64]
+    constexpr int Q = RB * CB, G = I8_S_PART / Q;
     const int nw = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const I8Task t = i8_task(L, blockIdx.x);
-    const int rb0 = (blockIdx.x - t.blk0) * RB, U = t.T.nunits;     // RB divides 4: the blocks lie in one tile
+    const int m0 = blockIdx.y * 64;
+    const int rb0 = (blockIdx.x - t.blk0) * RB;                     // RB divides 4: the blocks lie in one tile
+    const int U0 = t.T.nunits * blockIdx.z / L.ks, U = t.T.nunits * (blockIdx.z + 1) / L.ks;
     const uint8_t *wp = t.T.w + ((size_t)(rb0 >> 2) * t.T.cpr + (lane >> 4)) * 1024 + ((rb0 & 3) * 16 + (lane & 15)) * 16;
     const int8_t *xp[CB];
     const int kq = (lane >> 4) * 16;
 #pragma unroll
-    for (int j = 0; j < CB; j++) xp[j] = L.xq + (size_t)min(16 * j + (lane & 15), L.M - 1) * L.ldq;
+    for (int j = 0; j < CB; j++) xp[j] = L.xq + (size_t)min(m0 + 16 * j + (lane & 15), L.M - 1) * L.ldq;
     i8_i4 acc[RB][CB];
 #pragma unroll
     for (int i = 0; i < RB; i++)
@@ -114,8 +123,8 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
             for (int j = 0; j < CB; j++) b[s][j] = *(const i8_u4 *)(xp[j] + k);
         }
     };
-    load(wave);
-    for (int u0 = wave; u0 < U; u0 += D * nw) {
+    load(U0 + wave);
+    for (int u0 = U0 + wave; u0 < U; u0 += D * nw) {
         i8_u4 ca[D][RB], cb[D][CB];
 #pragma unroll
         for (int s = 0; s < D; s++) {
@@ -135,31 +144,52 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
             }
         }
     }
+    auto put = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < RB; i++)
+        for (int i = 0; i < RB; i++)
 #pragma unroll
-        for (int j = 0; j < CB; j++) red[(wave * RB * CB + i * CB + j) * 64 + lane] = acc[i][j];
+            for (int j = 0; j < CB; j++) red[(at * Q + i * CB + j) * 64 + lane] = acc[i][j];
+    };
+    if (i8_s_waves<RB, CB>() > G && nw > G) {
+        if (wave >= G) put(wave - G);
+        __syncthreads();
+        if (wave < nw - G) {
+#pragma unroll
+            for (int i = 0; i < RB; i++)
+#pragma unroll
+                for (int j = 0; j < CB; j++) acc[i][j] += red[(wave * Q + i * CB + j) * 64 + lane];
+        }
+        __syncthreads();
+    }
+    if (wave < G) put(wave);
     __syncthreads();
-    for (int o = threadIdx.x; o < RB * CB * 64; o += blockDim.x) {
+    const int parts = min(nw, G);
+    for (int o = threadIdx.x; o < Q * 64; o += blockDim.x) {
         const int l = o & 63, j = (o >> 6) % CB, i = (o >> 6) / CB;
-        const int m = 16 * j + (l & 15), r = (rb0 + i) * 16 + 4 * (l >> 4);
+        const int m = m0 + 16 * j + (l & 15), r = (rb0 + i) * 16 + 4 * (l >> 4);
         if (m >= L.M || r >= t.T.N) continue;
         i8_i4 s = {0, 0, 0, 0};
-        for (int w = 0; w < nw; w++) s += red[(w * RB * CB + i * CB + j) * 64 + l];
-        i8_store4(L, t, m, r, s, L.xs[m], i8_ws(t, r), i8_bias(t, r));
+        for (int w = 0; w < parts; w++) s += red[(w * Q + i * CB + j) * 64 + l];
+        if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = s;
+        else i8_store4(L, t, m, r, s, L.xs[m], i8_ws(t, r), i8_bias(t, r));
     }
 }
 
 // ================================================================================== many columns
 // Tiles of 16 CM NWM tokens by 16 CN NWN channels, NWM x NWN waves; both operands go through LDS in
-// stages of 128 values of K, copied there without passing through registers (buffer loads to LDS), the
-// next stage while this one is multiplied.
+// two stages of 128 values of K, copied there without passing through registers (buffer loads to LDS).  A wave reads
+// the operands of half a stage from LDS while it multiplies the half before, so that its products wait neither for
+// LDS nor at the barrier, of which there is one a stage: between the halves, when every wave has read the whole stage
+// and the next one has landed; the copies of the stage after that go out among the products that follow.
 //
 // A stage of weights keeps the device layout ([64-row tile][chunk][row], 1 KB runs).  A stage of token
 // rows is [row][128 bytes] with chunk c of row r at place c ^ (r / 2 % 8): an instruction copies 8 whole
-// rows (128-byte runs of memory), and the 16 rows that an operand read touches lie in different banks.
-#define I8_BK 128
-
+// rows, and the 16 rows that an operand read touches lie in different banks (none in conflict, by the counters).  Stages
+// of 64 values, four of them, took as long for the copies alone as the products do: a copy of 64-byte pieces of 16 rows
+// moves half of what one of 128-byte pieces does (4096 x 4096 x 14336: 206 us so, 190 now).
+//
+// 256 x 256 tiles: 8192 x 8192 x 8192 in 464 us, 2.37 POP/s (the library's int8 product: 474 us); a wave's products
+// without copies and reads would take 262 us at the clock that the card holds there (2.0 GHz).
 typedef unsigned int i8_rsrc __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i8_rsrc i8_mkrsrc(const void *p, uint32_t bytes) {
     const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -192,8 +222,8 @@ __device__ __forceinline__ void i8_tile(int b, int ntm, int ntn, int &tm, int &t
 
 template <int CM, int CN, int NWM, int NWN>
 __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, int ntn) {
-    constexpr int BM = 16 * CM * NWM, BN = 16 * CN * NWN, NW = NWM * NWN;
-    constexpr int XB = BM * I8_BK, WB = BN * I8_BK, SB = XB + WB;             // bytes of a stage
+    constexpr int BK = 128, BM = 16 * CM * NWM, BN = 16 * CN * NWN, NW = NWM * NWN;
+    constexpr int XB = BM * BK, WB = BN * BK, SB = XB + WB;                   // bytes of a stage
     constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;                   // copies of a wave per stage
     static_assert(XI * NW * 1024 == XB && WI * NW * 1024 == WB && BN % 64 == 0, "whole copies");
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -202,7 +232,7 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
     i8_tile(blockIdx.x, ntm, ntn, tm, tn);
     const I8Task t = i8_task(L, tn);
     const int m0 = tm * BM, n0 = (tn - t.blk0) * BN;
-    const int nk = t.T.nunits / 2;                                            // K is padded to whole stages
+    const int all = t.T.nunits / 2, s0 = all * blockIdx.z / L.ks, ns = all * (blockIdx.z + 1) / L.ks;   // K is padded to whole stages
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm;
 
     // token rows: copy j of the stage is rows 8 j .. 8 j + 7; rows past M repeat the last one
@@ -223,44 +253,63 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
         const int j = wave + NW * i;
         wo[i] = (uint32_t)(min(j >> 3, t.T.ntiles - 1 - tile0) * tb + (j & 7) * 1024);
     }
-    auto stage = [&](int k, uint32_t base) {
-#pragma unroll
-        for (int i = 0; i < WI; i++) i8_copy(wr, lane * 16, wo[i] + k * 8192, base + (wave + NW * i) * 1024);
-#pragma unroll
-        for (int i = 0; i < XI; i++) i8_copy(xr, xo[i] + k * I8_BK, 0, base + WB + (wave + NW * i) * 1024);
+    auto copy = [&](int i, int s, uint32_t base) {                            // the wave's i-th copy of stage s
+        if (i < WI) i8_copy(wr, lane * 16, wo[i] + s * 8192, base + (wave + NW * i) * 1024);
+        else i8_copy(xr, xo[i - WI] + s * BK, 0, base + WB + (wave + NW * (i - WI)) * 1024);
     };
-
     const int wm = wave / NWN, wn = wave % NWN;
     i8_i4 acc[CM][CN];
 #pragma unroll
     for (int i = 0; i < CM; i++)
 #pragma unroll
         for (int j = 0; j < CN; j++) acc[i][j] = i8_i4{0, 0, 0, 0};
-    const int key = ((lane & 15) >> 1), xl = WB + (wm * CM * 16 + (lane & 15)) * I8_BK;
+    // a lane's operand addresses in a stage, for each of its halves of 64 values
+    const int key = (lane & 15) >> 1, xl = WB + (wm * CM * 16 + (lane & 15)) * BK;
+    const int xh[2] = {xl + (((lane >> 4) ^ key) << 4), xl + (((4 + (lane >> 4)) ^ key) << 4)};
     const int wl = (lane >> 4) * 1024 + (lane & 15) * 16;
-
-    stage(0, lds0);
-    for (int k = 0; k < nk; k++) {
+    i8_u4 a[2][CN], b[2][CM];
+    auto ld_a = [&](int h, int j, const uint8_t *st) {
+        const int nb = wn * CN + j;
+        a[h][j] = *(const i8_u4 *)(st + (nb >> 2) * 8192 + (nb & 3) * 256 + h * 4096 + wl);
+    };
+    auto ld_b = [&](int h, int i, const uint8_t *st) { b[h][i] = *(const i8_u4 *)(st + xh[h] + i * 16 * BK); };
+    // The products of half h, with the operands of the other half (of the stage at st) read among them, and with
+    // `from` the copies of stage s into the stage at base.
+    auto half = [&](int h, const uint8_t *st, bool more, int s, uint32_t base) {
+#pragma unroll
+        for (int i = 0; i < CM; i++) {
+#pragma unroll
+            for (int j = i * CN / CM; j < (i + 1) * CN / CM; j++) ld_a(h ^ 1, j, st);
+            ld_b(h ^ 1, i, st);
+#pragma unroll
+            for (int j = 0; j < CN; j++) acc[i][j] = i8_mfma(a[h][j], b[h][i], acc[i][j]);
+            if (more) {
+#pragma unroll
+                for (int q = i * (WI + XI) / CM; q < (i + 1) * (WI + XI) / CM; q++) copy(q, s, base);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < WI + XI; q++) copy(q, s0, lds0);
+    i8_wait();
+    __builtin_amdgcn_s_barrier();
+    if (s0 + 1 < ns) {
+#pragma unroll
+        for (int q = 0; q < WI + XI; q++) copy(q, s0 + 1, lds0 + SB);
+    }
+#pragma unroll
+    for (int j = 0; j < CN; j++) ld_a(0, j, sm);
+#pragma unroll
+    for (int i = 0; i < CM; i++) ld_b(0, i, sm);
+    uint32_t cur = 0;                                                         // the stage that is multiplied: 0 or SB
+    for (int s = s0; s < ns; s++) {
+        half(0, sm + cur, false, 0, 0);
+        // every wave has read the whole stage, and the next one has landed: it is read while this one's place is filled
         i8_wait();
         __builtin_amdgcn_s_barrier();
-        const int cur = (k & 1) * SB;
-        if (k + 1 < nk) stage(k + 1, lds0 + (SB - cur));
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            i8_u4 a[CN], b[CM];
-#pragma unroll
-            for (int j = 0; j < CN; j++) {
-                const int nb = wn * CN + j;
-                a[j] = *(const i8_u4 *)(sm + cur + (nb >> 2) * 8192 + (nb & 3) * 256 + kk * 4096 + wl);
-            }
-#pragma unroll
-            for (int i = 0; i < CM; i++)
-                b[i] = *(const i8_u4 *)(sm + cur + xl + i * 16 * I8_BK + (((kk * 4 + (lane >> 4)) ^ key) << 4));
-#pragma unroll
-            for (int i = 0; i < CM; i++)
-#pragma unroll
-                for (int j = 0; j < CN; j++) acc[i][j] = i8_mfma(a[j], b[i], acc[i][j]);
-        }
+        half(1, sm + (SB - cur), s + 2 < ns, s + 2, lds0 + cur);              // (the last stage reads what lies there)
+        cur = SB - cur;
     }
 #pragma unroll
     for (int j = 0; j < CN; j++) {
@@ -270,36 +319,147 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
 #pragma unroll
         for (int i = 0; i < CM; i++) {
             const int m = m0 + (wm * CM + i) * 16 + (lane & 15);
-            if (m < L.M) i8_store4(L, t, m, r, acc[i][j], L.xs[m], ws, bias);
+            if (m >= L.M) continue;
+            if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = acc[i][j];
+            else i8_store4(L, t, m, r, acc[i][j], L.xs[m], ws, bias);
         }
     }
 }
 
-// ================================================================================== host side
-template <int RB, int CB>
-static void s_go(const I8Launch &L, int blocks, int units, hipStream_t st) {
-    constexpr int D = RB + CB <= 2 ? 4 : 2;
-    const int nw = std::min(i8_s_waves<RB, CB>(), units);
-    hipLaunchKernelGGL((k_i8_s<RB, CB, D>), dim3(blocks), dim3(nw * 64), (size_t)nw * RB * CB * 1024, st, L);
+// The slices' sums added (integers: in any order the same) and the outputs written, four channels a thread.
+__global__ __launch_bounds__(256) void k_i8_join(I8Launch L) {
+    const I8Task t = i8_task(L, blockIdx.z);                   // (blk0 holds the tensor's place in the group)
+    const int np = i8_np(t.T.N), r = (blockIdx.x * 256 + threadIdx.x) * 4, m = blockIdx.y;
+    if (r >= np) return;
+    const size_t slice = (size_t)L.M * np;
+    const int *p = t.part + (size_t)m * np + r;
+    i8_i4 s = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int z = 0; z < L.ks; z++) s += *(const i8_i4 *)(p + z * slice);
+    i8_store4(L, t, m, r, s, L.xs[m], i8_ws(t, r), i8_bias(t, r));
 }
 
-template <int CM, int CN, int NWM, int NWN>
-static int l_go(bgl_ctx *c, I8Launch &L) {
-    constexpr int BM = 16 * CM * NWM, BN = 16 * CN * NWN;
-    int ntn = 0;
+// ================================================================================== host side
+#define I8_CUS 256
+#define I8_SLICE 512          // values of K that a slice has at least
+#define I8_JOIN 1.6e6         // bytes of slices' sums that are written and joined in a us
+// Room for the slices' sums, the same for every call that could split K at its or at fewer columns, so that those may
+// be captured after it.  A choice that does not fit (many columns in many slices, which would cost more than they give)
+// keeps K whole.
+#define I8_PART_BYTES ((size_t)32 << 20)
+
+static size_t i8_part(const I8Launch &L, int ks) {
+    size_t v = 0;
+    for (int i = 0; i < L.n; i++) v += (size_t)ks * L.M * ((L.t[i].T.N + 3) & ~3) * 4;
+    return v;
+}
+// Points the tensors at their slices' sums; with no room for them (the no-alloc entry's fixed scratch) K stays whole.
+static int i8_split(bgl_ctx *c, I8Launch &L, int ks) {
+    L.ks = 1;
+    const int units = L.t[0].T.nunits;
+    if (units * 64 < 2 * I8_SLICE) return 0;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (!c->fixed_base) HIPCHK(hipStreamIsCapturing(c->stream, &cs));
+    if (!c->fixed_base && cs == hipStreamCaptureStatusNone && dbuf_reserve(c, c->part, I8_PART_BYTES, false)) return bgl_last_code();
+    if (ks <= 1) return 0;
+    const size_t need = i8_part(L, ks);
+    if (need > I8_PART_BYTES || (c->fixed_base && c->fixed_used + need + 256 > c->fixed_cap)) return 0;
+    if (dbuf_reserve(c, c->part, c->fixed_base ? need : I8_PART_BYTES, false)) return bgl_last_code();
+    int *p = (int *)c->part.p;
     for (int i = 0; i < L.n; i++) {
-        L.t[i].blk0 = ntn;
-        ntn += (L.t[i].T.N + BN - 1) / BN;
+        L.t[i].part = p;
+        p += (size_t)ks * L.M * ((L.t[i].T.N + 3) & ~3);
     }
-    const int ntm = (L.M + BM - 1) / BM;
-    const size_t lds = 2 * (size_t)(BM + BN) * I8_BK;
-    auto kern = k_i8_l<CM, CN, NWM, NWN>;
-    HIPCHK(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kern, dim3((unsigned)ntm * ntn), dim3(NWM * NWN * 64), lds, c->stream, L, ntm, ntn);
+    L.ks = ks;
     return 0;
 }
 
-#define I8_S_COLS 64          // columns that a launch of k_i8_s takes
+template <int RB, int CB>
+static void s_go(const I8Launch &L, int blocks, hipStream_t st) {
+    constexpr int D = RB + CB <= 2 ? 4 : 2;
+    const int nw = std::min(i8_s_waves<RB, CB>(), std::max(1, L.t[0].T.nunits / L.ks));
+    hipLaunchKernelGGL((k_i8_s<RB, CB, D>), dim3(blocks, (L.M + 63) / 64, L.ks), dim3(nw * 64), (size_t)std::min(nw * RB * CB, I8_S_PART) * 1024, st, L);
+}
+static long s_blocks(I8Launch &L, int RB) {
+    long blocks = 0;
+    for (int i = 0; i < L.n; i++) {
+        L.t[i].blk0 = (int)blocks;
+        blocks += ((L.t[i].T.N + 15) / 16 + RB - 1) / RB;
+    }
+    return blocks;
+}
+static int run_s(bgl_ctx *c, I8Launch &L, int RB, int ks) {
+    const int rc = i8_split(c, L, ks), CB = std::min(4, (L.M + 15) / 16);
+    if (rc) return rc;
+    const int blocks = (int)s_blocks(L, RB);
+#define GO(R, C) if (RB == R && CB == C) s_go<R, C>(L, blocks, c->stream)
+    GO(1, 1); GO(1, 2); GO(1, 3); GO(1, 4); GO(2, 1); GO(2, 2); GO(2, 3); GO(2, 4); GO(4, 1); GO(4, 2); GO(4, 3); GO(4, 4);
+#undef GO
+    return 0;
+}
+
+static long l_tiles(I8Launch &L, int BM, int BN) {
+    long ntn = 0;
+    for (int i = 0; i < L.n; i++) {
+        L.t[i].blk0 = (int)ntn;
+        ntn += (L.t[i].T.N + BN - 1) / BN;
+    }
+    return ntn * ((L.M + BM - 1) / BM);
+}
+template <int CM, int CN, int NWM, int NWN>
+static int run_l(bgl_ctx *c, I8Launch &L, int ks) {
+    constexpr int BM = 16 * CM * NWM, BN = 16 * CN * NWN;
+    const int rc = i8_split(c, L, ks);
+    if (rc) return rc;
+    const int ntm = (L.M + BM - 1) / BM, ntn = (int)(l_tiles(L, BM, BN) / ntm);
+    const size_t lds = 2 * (size_t)(BM + BN) * 128;
+    auto kern = k_i8_l<CM, CN, NWM, NWN>;
+    HIPCHK(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kern, dim3((unsigned)ntm * ntn, 1, L.ks), dim3(NWM * NWN * 64), lds, c->stream, L, ntm, ntn);
+    return 0;
+}
+
+// Which kernel runs a product of M columns, by the time in us that each would take: the launch and the sums of a tile
+// (constant), what a CU reads or multiplies for its tiles, and with K split the launch that joins the slices.  The
+// constants were fitted to 37 shapes from 1 x 256 x 1536 to 4096 x 14336 x 4096, where the choice is the fastest of all
+// or within a tenth; us of both sides of each line (columns x channels x K):
+//   up to 64 columns, k_i8_s with 16 / 32 / 64 channels a workgroup: 1 x 4096 x 4096 5.5 / 5.8 / 6.4, 1 x 8960 x 1536
+//     8.0 / 6.5 / 5.5, 64 x 14336 x 4096 40.8 / 26.6 / 21.0; 64 with K in 1 / 4 / 8 slices: 64 x 1536 x 8960
+//     24.8 / 13.1 / 12.1, 64 x 14336 x 4096 21.5 / 34.0 / 51.7
+//   k_i8_s with 64 x 64 outputs / 128 x 128 tiles / 256 x 256: 512 x 1536 x 1536 9.3 / 12.8 / 31.8, 2048 x 2048 x 2048
+//     34.8 / 17.9 / 37.9, 2048 x 14336 x 4096 369 / 157 / 146
+//   128 x 128 tiles with K in 1 / 4 slices: 1024 x 1536 x 8960 48.7 / 31.1, 128 x 8960 x 1536 14.0 / 19.9
+static int run_any(bgl_ctx *c, I8Launch &L) {
+    const int K = L.t[0].T.K, M = L.M;
+    auto up = [](long v) { return (double)((v + I8_CUS - 1) / I8_CUS); };
+    auto join = [&](int ks) { return ks > 1 ? 3.0 + i8_part(L, ks) / I8_JOIN : 0.0; };
+    if (M <= 64) {
+        int best = 0, bks = 1;
+        double least = 1e30;
+        for (int RB = 1; RB <= 4; RB *= 2) {
+            const long blocks = s_blocks(L, RB);
+            for (int ks = 1; ks <= 8 && (ks == 1 || K / ks >= I8_SLICE); ks *= 2) {
+                const double us = up(blocks * ks) * ((double)(16 * RB + M) * K / ks / 40e3 + 1.5) + join(ks);
+                if (us < least) { least = us; best = RB; bks = ks; }
+            }
+        }
+        return run_s(c, L, best, bks);
+    }
+    const double ns = (K + 127) / 128;
+    const long t256 = l_tiles(L, 256, 256), t128 = l_tiles(L, 128, 128), t64 = s_blocks(L, 4) * ((M + 63) / 64);
+    int ks = 1;
+    double c128 = 1e30;
+    for (int k = 1; k <= 8 && (k == 1 || (t128 < I8_CUS && K / k >= I8_SLICE)); k *= 2) {
+        const double r = (double)t128 * k / I8_CUS;
+        const double us = 4.0 + (r <= 1.0 ? 0.62 + 0.25 * r : 0.6 * up(t128 * k)) * ns / k + join(k);
+        if (us < c128) { c128 = us; ks = k; }
+    }
+    const double c256 = 6.0 + 1.9 * ns * up(t256);
+    const double c64 = 3.0 + (t64 <= I8_CUS ? 0.4 : 0.62 * up(t64)) * ns;
+    if (c64 <= c128 && c64 <= c256 && (M + 63) / 64 <= 65535) return run_s(c, L, 4, 1);
+    if (c128 <= c256) return run_l<4, 2, 2, 4>(c, L, ks);
+    return run_l<8, 4, 2, 4>(c, L, 1);
+}
 
 int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
            void *const *y, int y_type, const long *ldy, int M) {
@@ -308,31 +468,21 @@ int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq
     L.n = n; L.M = M; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
     L.xq = xq; L.ldq = ldq; L.xs = xs;
     L.vec = 1;
+    int widest = 0;
     for (int i = 0; i < n; i++) {
         I8Task &t = L.t[i];
         t.T = Ts[i];
         t.bias = bias ? bias[i] : nullptr;
         t.y = y[i];
         t.ldy = ldy ? ldy[i] : Ts[i].N;
+        widest = std::max(widest, Ts[i].N);
         if (((uintptr_t)t.y | (uintptr_t)t.ldy * i8_elem(y_type)) % (4 * i8_elem(y_type))) L.vec = 0;
     }
-    int tok = prof_begin(c, 1), rc = 0;
-    if (M <= I8_S_COLS) {
-        const int CB = (M + 15) / 16;
-        long tiles = 0;
-        for (int i = 0; i < n; i++) tiles += Ts[i].ntiles;
-        int RB = 1;                                            // 16 channels a workgroup, more once that leaves 512 of them
-        while (RB < 4 && tiles * 4 / (2 * RB) >= 512) RB *= 2;
-        int blocks = 0;
-        for (int i = 0; i < n; i++) {
-            L.t[i].blk0 = blocks;
-            blocks += ((Ts[i].N + 15) / 16 + RB - 1) / RB;
-        }
-#define GO(R, C) if (RB == R && CB == C) s_go<R, C>(L, blocks, Ts[0].nunits, c->stream)
-        GO(1, 1); GO(1, 2); GO(1, 3); GO(1, 4); GO(2, 1); GO(2, 2); GO(2, 3); GO(2, 4); GO(4, 1); GO(4, 2); GO(4, 3); GO(4, 4);
-#undef GO
-    } else {
-        rc = l_go<8, 4, 2, 4>(c, L);
+    int tok = prof_begin(c, 1);
+    const int rc = run_any(c, L);
+    if (!rc && L.ks > 1) {
+        for (int i = 0; i < n; i++) L.t[i].blk0 = i;
+        hipLaunchKernelGGL(k_i8_join, dim3((unsigned)((widest + 1023) / 1024), M, n), dim3(256), 0, c->stream, L);
     }
     prof_end(c, tok);
     if (rc) return rc;
