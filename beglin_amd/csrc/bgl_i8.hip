@@ -111,38 +111,34 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
     for (int i = 0; i < RB; i++)
 #pragma unroll
         for (int j = 0; j < CB; j++) acc[i][j] = i8_i4{0, 0, 0, 0};
-    i8_u4 a[D][RB], b[D][CB];
-    auto load = [&](int u0) {
+    struct Ops { i8_u4 a[D][RB], b[D][CB]; } even, odd;             // in turn: no copy waits for a load
+    auto load = [&](Ops &o, int u0) {
 #pragma unroll
         for (int s = 0; s < D; s++) {
             const int u = min(u0 + s * nw, U - 1);
 #pragma unroll
-            for (int i = 0; i < RB; i++) a[s][i] = *(const i8_u4 *)(wp + (size_t)u * 4096 + 256 * i);
+            for (int i = 0; i < RB; i++) o.a[s][i] = *(const i8_u4 *)(wp + (size_t)u * 4096 + 256 * i);
             const int k = min(64 * u + kq, L.K16 - 16);              // past the row: the weights are zero there
 #pragma unroll
-            for (int j = 0; j < CB; j++) b[s][j] = *(const i8_u4 *)(xp[j] + k);
+            for (int j = 0; j < CB; j++) o.b[s][j] = *(const i8_u4 *)(xp[j] + k);
         }
     };
-    load(U0 + wave);
-    for (int u0 = U0 + wave; u0 < U; u0 += D * nw) {
-        i8_u4 ca[D][RB], cb[D][CB];
-#pragma unroll
-        for (int s = 0; s < D; s++) {
-#pragma unroll
-            for (int i = 0; i < RB; i++) ca[s][i] = a[s][i];
-#pragma unroll
-            for (int j = 0; j < CB; j++) cb[s][j] = b[s][j];
-        }
-        if (u0 + D * nw < U) load(u0 + D * nw);
+    auto step = [&](int u0, const Ops &cur, Ops &nxt) {
+        if (u0 + D * nw < U) load(nxt, u0 + D * nw);
 #pragma unroll
         for (int s = 0; s < D; s++) {
             if (u0 + s * nw < U) {
 #pragma unroll
                 for (int i = 0; i < RB; i++)
 #pragma unroll
-                    for (int j = 0; j < CB; j++) acc[i][j] = i8_mfma(ca[s][i], cb[s][j], acc[i][j]);
+                    for (int j = 0; j < CB; j++) acc[i][j] = i8_mfma(cur.a[s][i], cur.b[s][j], acc[i][j]);
             }
         }
+    };
+    load(even, U0 + wave);
+    for (int u0 = U0 + wave; u0 < U; u0 += 2 * D * nw) {
+        step(u0, even, odd);
+        if (u0 + D * nw < U) step(u0 + D * nw, odd, even);
     }
     auto put = [&](int at) {
 #pragma unroll

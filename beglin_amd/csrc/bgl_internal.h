@@ -50,6 +50,7 @@ struct bgl_ctx {
     DevBuf moe_a, moe_b, moe_c, moe_d, moe_e, moe_f, moe_g, moe_meta;   // MoE digits x2, fp32 h/down, bucket scratch
     DevBuf moe_route;                     // routing of bgl_moe_layer_dev: idx [T][K] + w [T][K]
     DevBuf moe_scores;                    // router scores [T][E]
+    DevBuf moe_ticket;                    // K_Q8C experts: workgroups of each token that have their scores, 0 between launches
     DevBuf mlp;                           // bgl_mlp_dev: gate and up outputs [M][I] each, then h [M][I]
     std::unordered_map<uint64_t, DevBuf> mlp_sync;   // single-launch MLP, per shape (in << 32 | down workgroups): counters, generations, flag
     bool no_qmfma = false;                // BGL_NO_QMFMA=1: W4A8 at 2..16 columns through the dot4 kernel (k_gemv_q)

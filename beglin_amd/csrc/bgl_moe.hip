@@ -819,10 +819,6 @@ __global__ __launch_bounds__(64) void k_moe_route_topk(const float *__restrict__
     }
 }
 
-void bgl_launch_route_topk(const float *scores, int T, int E, int K, int renorm, int32_t *idx, float *w, hipStream_t st) {
-    hipLaunchKernelGGL(k_moe_route_topk, dim3(T), dim3(64), 0, st, scores, E, K, renorm, idx, w);
-}
-
 // The top-K of every token (one wave per token in turn) and the bucketing of the T*K pairs by
 // expert (k_moe_bucket's outputs, stable in pair order) in one workgroup: the whole routing after
 // the scores is one launch.

@@ -9,12 +9,15 @@
 // row's bits depend neither on the other tokens nor on how the work is split.
 //
 // What bounds it is the experts' bytes: each touched expert is read once, whatever the number of its tokens
-// (64 at the most; more go in chunks).  A gate+up workgroup owns 16 rows of both tensors of one expert and all
-// of its tokens, its waves splitting K; a down workgroup owns 16 output channels, its waves taking whole
-// experts, and holds every pair's sum in LDS until the combine, so there is no launch and no memory traffic
-// for partial sums.  Workgroups find their expert and its pairs from the routing themselves; up to
-// MOE_I8_ROUTE tokens they also make it from the scores (softmax, top-K: about a microsecond a token and
-// wave), so that a layer needs no launch for it.
+// (64 at the most; more go in chunks).
+//   k_moe_i8_pre   the codes of x; the router's scores, a wave an expert, and the softmax and top-K of a token by
+//                  whichever workgroup finishes its last score (a ticket per token; no workgroup waits)
+//   k_moe_i8_gu    16-row blocks of both tensors of an expert and all of its tokens, in equal runs over two workgroups a
+//                  CU, whose waves split K; the next block's weights are on their way while one is multiplied
+//   k_moe_i8_hq    the codes of h, where a down workgroup would spend longer on making them all (MOE_I8_LDSQ)
+//   k_moe_i8_down  a workgroup owns 16 output channels; its waves take pieces of the experts' K and add the int32 sums in
+//                  LDS, which holds every pair's until the combine: no launch and no memory traffic for partial sums
+// Workgroups find their expert and its pairs from the routing themselves.
 #include <string.h>
 
 #include <algorithm>
@@ -31,28 +34,31 @@
 
 #define MOE_I8_TOK 64             // tokens of a chunk
 #define MOE_I8_PAIRS (MOE_I8_TOK * MOE_MAX_K)
-#define MOE_I8_ROUTE 8            // up to this many tokens every workgroup makes the routing: one wave a token
-#define MOE_I8_LDSQ (64 * 1024)   // h codes that a down workgroup makes for itself; more take a launch
-#define MOE_I8_NW 8               // waves of a workgroup
+#define MOE_I8_LDSQ (24 * 1024)   // h codes that a down workgroup makes for itself; more take a launch
+#define MOE_I8_NW 8               // waves of a gate+up workgroup
+#define MOE_I8_DW 16              // waves of a down workgroup
+#define MOE_I8_DC 8               // units of 64 values that one of them takes at a time at most
+#define MOE_I8_GU_WGS 512         // gate+up workgroups at most: two a CU
 
 struct MoeI8Launch {
     const BglDevTensor *tg, *tu, *td;    // expert tables
     BglDevTensor sg, su, sd;             // shared experts (shared != 0)
-    int shared, E, K, T, P, H, I, Ish, nslots, parts;
+    int shared, E, K, T, P, H, I, Ish, nslots, piece;   // nslots: the most slots; piece: units a down wave takes
     const float *x, *rw, *rb;            // token rows; router
     float *scores;                       // [T][E], null: idx / w are given
+    int *ticket;                         // [T] workgroups of a token that have their scores; 0 between launches
     int renorm;
-    const int32_t *idx;                  // [P] where the scores are not routed by the workgroups
-    const float *w;
+    int32_t *idx;                        // [P]
+    float *w;
     int8_t *xq;
     float *xs;
     float *h, *hsh;                      // [P][I], [T][Ish]
-    uint32_t *amax;                      // [P + T] bits of the largest |h| of a row
-    int8_t *hq, *hshq;                   // codes of h; null: the down workgroups make them
+    int8_t *hq, *hshq;                   // codes of h and their scales [P + T]; null: the down workgroups make them
+    float *hs;
     float *out;
 };
 
-// ------------------------------------------------------------------ codes of x, scores, cleared maxima
+// ------------------------------------------------------------------ codes of x, routing
 __global__ __launch_bounds__(256) void k_moe_i8_pre(MoeI8Launch L) {
     const int tid = threadIdx.x, lane = tid & 63;
     if ((int)blockIdx.x < L.T) {
@@ -68,68 +74,102 @@ __global__ __launch_bounds__(256) void k_moe_i8_pre(MoeI8Launch L) {
         if (tid == 0) L.xs[t] = s.sc;
         for (int k = 4 * tid; k < L.H; k += 1024)
             *(uint32_t *)(L.xq + (size_t)t * L.H + k) = i8_pack4(i8_code(x[k], s), i8_code(x[k + 1], s), i8_code(x[k + 2], s), i8_code(x[k + 3], s));
-        for (int k = tid; k < L.K; k += 256) L.amax[t * L.K + k] = 0;
-        if (tid == 0) L.amax[L.P + t] = 0;
         return;
     }
+    // scores and ticket pass the L2s of the eight dies (agent scope), so no cache is written back for them: a score is in
+    // memory before its workgroup's ticket is drawn, and who draws the last one reads them there
     const int per = (L.E + 3) / 4, b = blockIdx.x - L.T, t = b / per, e = (b % per) * 4 + (tid >> 6);
-    if (e >= L.E) return;
-    const double acc = route_dot_wave(L.rw + (size_t)e * L.H, L.x + (size_t)t * L.H, L.H, lane);
-    if (lane == 0) L.scores[(size_t)t * L.E + e] = L.rb ? __fadd_rn((float)acc, L.rb[e]) : (float)acc;
+    __shared__ int last;
+    __shared__ __align__(16) float lbuf[ROUTE_MAXE], sc[ROUTE_MAXE];
+    if (e < L.E) {
+        const double acc = route_dot_wave(L.rw + (size_t)e * L.H, L.x + (size_t)t * L.H, L.H, lane);
+        const float s = L.rb ? __fadd_rn((float)acc, L.rb[e]) : (float)acc;
+        if (lane == 0) __hip_atomic_store(L.scores + (size_t)t * L.E + e, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) last = __hip_atomic_fetch_add(L.ticket + t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == per - 1;
+    __syncthreads();
+    if (!last || tid >= 64) return;
+    for (int i = lane; i < L.E; i += 64)
+        sc[i] = __hip_atomic_load(L.scores + (size_t)t * L.E + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lane == 0) __hip_atomic_store(L.ticket + t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    __builtin_amdgcn_wave_barrier();
+    float sel_w[MOE_MAX_K];
+    int sel_i[MOE_MAX_K];
+    route_topk_wave(sc, L.E, L.K, L.renorm, lane, sel_i, sel_w, lbuf);
+    if (lane == 0)
+        for (int k = 0; k < L.K; k++) {
+            L.idx[t * L.K + k] = sel_i[k];
+            L.w[t * L.K + k] = sel_w[k];
+        }
 }
 
 // ------------------------------------------------------------------ the routing in LDS
+// The used experts in ascending order ("slots") and each one's pairs.  (The order of a slot's pairs is that of LDS
+// atomics; no value depends on it.)
+#define MOE_I8_NONE 0xffff
 struct MoeI8Route {
-    int ids[MOE_I8_PAIRS];               // expert of each pair
-    float w[MOE_I8_PAIRS];
-    uint32_t used[32];                   // experts that have a pair (E <= 1024)
+    uint16_t slot[MOE_I8_PAIRS];         // of each pair; MOE_I8_NONE: its id lies outside the stack
+    uint16_t list[MOE_I8_PAIRS];         // the pairs by slot
+    uint16_t expert[MOE_I8_PAIRS];       // of each slot
+    int off[MOE_I8_PAIRS + 1], at[MOE_I8_PAIRS];
+    uint32_t used[32], base[32];         // experts that have a pair (E <= 1024), slots before each 32 of them
+    int n;                               // slots
 };
-__device__ __forceinline__ void i8_routing(const MoeI8Launch &L, MoeI8Route &R, float (*lbuf)[ROUTE_MAXE]) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (threadIdx.x < 32) R.used[threadIdx.x] = 0;
-    if (!L.idx) {
-        if (wave < L.T) route_topk_wave(L.scores + (size_t)wave * L.E, L.E, L.K, L.renorm, lane, R.ids + wave * L.K, R.w + wave * L.K, lbuf[wave]);
-    } else {
-        for (int p = threadIdx.x; p < L.P; p += blockDim.x) {
-            R.ids[p] = L.idx[p];
-            R.w[p] = L.w[p];
-        }
+__device__ __forceinline__ void i8_routing(const MoeI8Launch &L, MoeI8Route &R) {
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63;
+    if (tid < 32) R.used[tid] = 0;
+    for (int s = tid; s < L.nslots; s += nt) R.at[s] = 0;
+    __syncthreads();
+    for (int p = tid; p < L.P; p += nt) {
+        const int e = L.idx[p];
+        R.slot[p] = e >= 0 && e < L.E ? (uint16_t)e : (uint16_t)MOE_I8_NONE;     // the expert, for now
+        if (e >= 0 && e < L.E) atomicOr(&R.used[e >> 5], 1u << (e & 31));
     }
     __syncthreads();
-    for (int p = threadIdx.x; p < L.P; p += blockDim.x) {
-        const int e = R.ids[p];
-        if (e >= 0 && e < L.E) atomicOr(&R.used[e >> 5], 1u << (e & 31));   // others are skipped
-    }
-    __syncthreads();
-}
-// the s-th used expert in ascending order (-1: there are fewer), by a whole wave
-__device__ __forceinline__ int i8_slot(const MoeI8Route &R, int s) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t word = lane < 32 ? R.used[lane] : 0u;
-    int incl = __popc(word);
+    if (tid < 64) {
+        const int c = lane < 32 ? __popc(R.used[lane]) : 0;
+        int incl = c;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up(incl, o);
-        if (lane >= o) incl += v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up(incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane < 32) R.base[lane] = incl - c;
+        if (lane == 31) R.n = incl;
     }
-    const unsigned long long m = __ballot(incl > s);
-    if (!m) return -1;
-    const int l = __ffsll(m) - 1;
-    uint32_t wd = __shfl(word, l);
-    for (int left = s - (__shfl(incl, l) - __popc(wd)); left > 0; left--) wd &= wd - 1;
-    return __builtin_amdgcn_readfirstlane(32 * l + __ffs(wd) - 1);
-}
-// the pairs of expert e in ascending order into list, by a whole wave; returns how many
-__device__ __forceinline__ int i8_pairs(const MoeI8Launch &L, const MoeI8Route &R, int e, uint16_t *list) {
-    const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int p0 = 0; p0 < L.P; p0 += 64) {
-        const bool hit = p0 + lane < L.P && R.ids[p0 + lane] == e;
-        const unsigned long long m = __ballot(hit);
-        if (hit) list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(p0 + lane);
-        n += __popcll(m);
+    __syncthreads();
+    for (int p = tid; p < L.P; p += nt) {
+        const uint32_t e = R.slot[p];
+        if (e == MOE_I8_NONE) continue;
+        const int s = R.base[e >> 5] + __popc(R.used[e >> 5] & ((1u << (e & 31)) - 1));
+        R.slot[p] = (uint16_t)s;
+        R.expert[s] = (uint16_t)e;
+        atomicAdd(&R.at[s], 1);
     }
-    return n;
+    __syncthreads();
+    if (tid < 64) {
+        int before = 0;
+        for (int s0 = 0; s0 < R.n; s0 += 64) {
+            const int c = s0 + lane < R.n ? R.at[s0 + lane] : 0;
+            int incl = c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (s0 + lane < R.n) R.off[s0 + lane] = R.at[s0 + lane] = before + incl - c;
+            before += __shfl(incl, 63);
+        }
+        if (lane == 0) R.off[R.n] = before;
+    }
+    __syncthreads();
+    for (int p = tid; p < L.P; p += nt) {
+        const int s = R.slot[p];
+        if (s != MOE_I8_NONE) R.list[atomicAdd(&R.at[s], 1)] = (uint16_t)p;
+    }
+    __syncthreads();
 }
 
 __device__ __forceinline__ i8_i4 mi_mfma(i8_u4 a, i8_u4 b, i8_i4 c) {
@@ -141,243 +181,259 @@ __device__ __forceinline__ const uint8_t *mi_rows(const uint8_t *w, int cpr, int
 }
 
 // ------------------------------------------------------------------ gate + up
-// h of rows 16 rb .. + 15 for columns c0 .. of the n in list (a pair, or with list null a token)
-template <int CB>
-__device__ __forceinline__ void i8_gu(const MoeI8Launch &L, const BglDevTensor &G, const BglDevTensor &Up, int rb, const uint16_t *list, int c0,
-                                      int n, float *h, int width, uint32_t *amax, i8_i4 *red) {
+// h of the 16-row blocks rb0 .. rb1 - 1 for columns c0 .. of the n in list (a pair, or with list null a token): a wave
+// takes every eighth unit of K, D at a time, and has the weights of the next D on their way while it multiplies.
+template <int CB, int D>
+__device__ __forceinline__ void i8_gu(const MoeI8Launch &L, const BglDevTensor &G, const BglDevTensor &Up, int rb0, int rb1, const uint16_t *list,
+                                      int c0, int n, float *h, int width, i8_i4 *red) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int U = L.H / 64;
-    const uint8_t *gp = mi_rows(G.w, G.cpr, rb, lane), *up = mi_rows(Up.w, Up.cpr, rb, lane);
+    const int U = L.H / 64, NC = (U + D * MOE_I8_NW - 1) / (D * MOE_I8_NW), its = (rb1 - rb0) * NC;
     const int8_t *xp[CB];
 #pragma unroll
     for (int j = 0; j < CB; j++) {
         const int c = min(c0 + 16 * j + (lane & 15), n - 1), tok = list ? list[c] / L.K : c;
         xp[j] = L.xq + (size_t)tok * L.H + (lane >> 4) * 16;
     }
-    i8_i4 ga[CB], ua[CB];
-#pragma unroll
-    for (int j = 0; j < CB; j++) ga[j] = ua[j] = i8_i4{0, 0, 0, 0};
-    constexpr int D = CB == 1 ? 4 : 2;
-    for (int u0 = wave; u0 < U; u0 += D * MOE_I8_NW) {
-        i8_u4 a[D], b[D], x[D][CB];
+    struct Ops { i8_u4 a[D], b[D]; } even, odd;                // in turn: no copy waits for a load
+    auto load = [&](Ops &o, int it) {
+        const int rb = rb0 + it / NC, u0 = (it % NC) * D * MOE_I8_NW + wave;
+        const uint8_t *gp = mi_rows(G.w, G.cpr, rb, lane), *up = mi_rows(Up.w, Up.cpr, rb, lane);
 #pragma unroll
         for (int s = 0; s < D; s++) {
             const int u = min(u0 + s * MOE_I8_NW, U - 1);
-            a[s] = *(const i8_u4 *)(gp + (size_t)u * 4096);
-            b[s] = *(const i8_u4 *)(up + (size_t)u * 4096);
-#pragma unroll
-            for (int j = 0; j < CB; j++) x[s][j] = *(const i8_u4 *)(xp[j] + u * 64);
+            o.a[s] = *(const i8_u4 *)(gp + (size_t)u * 4096);
+            o.b[s] = *(const i8_u4 *)(up + (size_t)u * 4096);
         }
+    };
+    i8_i4 ga[CB], ua[CB];
+    // the outputs that a thread forms, one for each NO: channel och of a block for column oc (a wave: 16 columns, 4 channels)
+    constexpr int NO = CB <= 2 ? 1 : CB / 2;
+    const int och = 4 * (wave & 3) + (lane & 3);
+    int oc[NO], orow[NO];
+    float xs[NO], gs, us;
+#pragma unroll
+    for (int i = 0; i < NO; i++) {
+        oc[i] = c0 + 16 * ((wave >> 2) + 2 * i) + (lane >> 2);
+        orow[i] = list ? list[min(oc[i], n - 1)] : min(oc[i], n - 1);
+        xs[i] = L.xs[list ? orow[i] / L.K : orow[i]];
+    }
+    auto step = [&](int it, Ops &cur, Ops &nxt) {
+        const int ch = it % NC, rb = rb0 + it / NC, u0 = ch * D * MOE_I8_NW + wave;
+        i8_u4 x[D][CB];
+#pragma unroll
+        for (int s = 0; s < D; s++)
+#pragma unroll
+            for (int j = 0; j < CB; j++) x[s][j] = *(const i8_u4 *)(xp[j] + min(u0 + s * MOE_I8_NW, U - 1) * 64);
+        if (ch == 0) {
+#pragma unroll
+            for (int j = 0; j < CB; j++) ga[j] = ua[j] = i8_i4{0, 0, 0, 0};
+            gs = ((const float *)G.s0)[16 * rb + och];
+            us = ((const float *)Up.s0)[16 * rb + och];
+        }
+        load(nxt, min(it + 1, its - 1));
 #pragma unroll
         for (int s = 0; s < D; s++)
             if (u0 + s * MOE_I8_NW < U) {
 #pragma unroll
                 for (int j = 0; j < CB; j++) {
-                    ga[j] = mi_mfma(a[s], x[s][j], ga[j]);
-                    ua[j] = mi_mfma(b[s], x[s][j], ua[j]);
+                    ga[j] = mi_mfma(cur.a[s], x[s][j], ga[j]);
+                    ua[j] = mi_mfma(cur.b[s], x[s][j], ua[j]);
                 }
             }
-    }
-    __syncthreads();                                   // an earlier chunk's sums have been read
+        if (ch != NC - 1) return;
+        __syncthreads();                                       // an earlier block's sums have been read
 #pragma unroll
-    for (int j = 0; j < CB; j++) {
-        red[((wave * CB + j) * 2) * 64 + lane] = ga[j];
-        red[((wave * CB + j) * 2 + 1) * 64 + lane] = ua[j];
-    }
-    __syncthreads();
-    for (int o = threadIdx.x; o < CB * 64; o += MOE_I8_NW * 64) {
-        const int j = o >> 6, l = o & 63, c = c0 + 16 * j + (l & 15), r = 16 * rb + 4 * (l >> 4);
-        uint32_t mb = 0;
-        int row = 0;
-        if (c < n) {
-            i8_i4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+        for (int j = 0; j < CB; j++) {
+            red[((wave * CB + j) * 2) * 64 + lane] = ga[j];
+            red[((wave * CB + j) * 2 + 1) * 64 + lane] = ua[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NO; i++) {
+            const int j = (wave >> 2) + 2 * i;
+            if (j >= CB) continue;
+            const int *s = (const int *)red + j * 512 + (wave & 3) * 64 + lane;      // int (wave & 3) * 64 + lane of a block's 256
+            int g = 0, u = 0;
 #pragma unroll
             for (int w = 0; w < MOE_I8_NW; w++) {
-                g += red[((w * CB + j) * 2) * 64 + l];
-                u += red[((w * CB + j) * 2 + 1) * 64 + l];
+                g += s[w * CB * 512];
+                u += s[w * CB * 512 + 256];
             }
-            row = list ? list[c] : c;
-            const float xs = L.xs[list ? row / L.K : row];
-            const i8_f4 gs = *(const i8_f4 *)((const float *)G.s0 + r), us = *(const i8_f4 *)((const float *)Up.s0 + r);
-            i8_f4 v;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i] = i8_swiglu(i8_out(g[i], xs, gs[i]), i8_out(u[i], xs, us[i]));
-                mb = max(mb, __float_as_uint(v[i]) & 0x7fffffffu);
-            }
-            *(i8_f4 *)(h + (size_t)row * width + r) = v;
+            if (oc[i] < n) h[(size_t)orow[i] * width + 16 * rb + och] = i8_swiglu(i8_out(g, xs[i], gs), i8_out(u, xs[i], us));
         }
-        mb = max(mb, (uint32_t)__shfl_xor((int)mb, 16));
-        mb = max(mb, (uint32_t)__shfl_xor((int)mb, 32));
-        if (c < n && l < 16) atomicMax(&amax[row], mb);      // a maximum: the order of the workgroups does not matter
+    };
+    load(even, 0);
+    for (int it = 0; it < its; it += 2) {
+        step(it, even, odd);
+        if (it + 1 < its) step(it + 1, odd, even);
     }
 }
 
-__global__ __launch_bounds__(MOE_I8_NW * 64, 4) void k_moe_i8_gu(MoeI8Launch L, int cbmax) {
+// The 16-row blocks of the shared experts and then of each used expert, in equal runs over the workgroups.
+template <int CB, int D>
+__global__ __launch_bounds__(MOE_I8_NW * 64, 4) void k_moe_i8_gu(MoeI8Launch L) {
     extern __shared__ __align__(16) i8_i4 red[];               // [wave][column block][gate, up][64]
     __shared__ MoeI8Route R;
-    __shared__ __align__(16) float lbuf[MOE_I8_ROUTE][ROUTE_MAXE];
-    __shared__ uint16_t list[MOE_I8_PAIRS];
-    __shared__ int found[2];
-    const int nsh = L.shared ? L.Ish / 16 : 0;
-    BglDevTensor G, U;
-    int rb, n;
-    const uint16_t *ls = nullptr;
-    float *h;
-    int width;
-    uint32_t *amax;
-    if ((int)blockIdx.x < nsh) {
-        G = L.sg; U = L.su; rb = blockIdx.x; n = L.T; h = L.hsh; width = L.Ish; amax = L.amax + L.P;
-    } else {
-        i8_routing(L, R, lbuf);
-        const int b = blockIdx.x - nsh, per = L.I / 16;
-        if (threadIdx.x < 64) {
-            const int e = i8_slot(R, b / per), m = e < 0 ? 0 : i8_pairs(L, R, e, list);
-            if (threadIdx.x == 0) { found[0] = e; found[1] = m; }
-        }
-        __syncthreads();
-        const int e = __builtin_amdgcn_readfirstlane(found[0]);
-        if (e < 0) return;
-        n = __builtin_amdgcn_readfirstlane(found[1]);
-        rb = b % per;
-        G = L.tg[e]; U = L.tu[e]; ls = list; h = L.h; width = L.I; amax = L.amax;
-    }
-    for (int c0 = 0; c0 < n; c0 += 16 * cbmax) {
-        const int left = n - c0;
-        if (left <= 16 || cbmax == 1) i8_gu<1>(L, G, U, rb, ls, c0, n, h, width, amax, red);
-        else if (left <= 32 || cbmax == 2) i8_gu<2>(L, G, U, rb, ls, c0, n, h, width, amax, red);
-        else i8_gu<4>(L, G, U, rb, ls, c0, n, h, width, amax, red);
+    i8_routing(L, R);
+    const int nsh = L.shared ? L.Ish / 16 : 0, per = L.I / 16;
+    const long all = nsh + (long)__builtin_amdgcn_readfirstlane(R.n) * per;
+    const int end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    for (int it = (int)(all * blockIdx.x / gridDim.x); it < end;) {
+        const bool sh = it < nsh;
+        const int slot = sh ? 0 : (it - nsh) / per, first = sh ? 0 : nsh + slot * per;    // (uniform)
+        const int rb = it - first, rb1 = min(end - first, sh ? nsh : per);
+        const int e = sh ? 0 : __builtin_amdgcn_readfirstlane((int)R.expert[slot]);
+        const int l0 = sh ? 0 : __builtin_amdgcn_readfirstlane(R.off[slot]);
+        const int n = sh ? L.T : __builtin_amdgcn_readfirstlane(R.off[slot + 1]) - l0;
+        const BglDevTensor G = sh ? L.sg : L.tg[e], U = sh ? L.su : L.tu[e];
+        const uint16_t *const list = sh ? nullptr : R.list + l0;
+        float *const h = sh ? L.hsh : L.h;
+        const int width = sh ? L.Ish : L.I;
+        for (int c0 = 0; c0 < n; c0 += 16 * CB) i8_gu<CB, D>(L, G, U, rb, rb1, list, c0, n, h, width, red);
+        it = first + rb1;
     }
 }
 
 // ------------------------------------------------------------------ codes of h where they take a launch
-// Four values a thread; rows [0, P) of I, then [0, T) of Ish.  The maxima came with h.
+// A workgroup a row: rows [0, P) of I, then [0, T) of Ish.
 __global__ __launch_bounds__(256) void k_moe_i8_hq(MoeI8Launch L) {
-    const long q = (long)blockIdx.x * 256 + threadIdx.x, n0 = (long)L.P * L.I / 4;
-    const bool sh = q >= n0;
-    const long i = (sh ? q - n0 : q) * 4;
+    __shared__ uint32_t red[4];
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const bool sh = row >= L.P;
     const int width = sh ? L.Ish : L.I;
-    if (sh && (!L.shared || i >= (long)L.T * L.Ish)) return;
-    const int row = (int)(i / width);
-    const I8Scale s = i8_scale(max(L.amax[(sh ? L.P : 0) + row], I8_MX0));
-    const i8_f4 v = *(const i8_f4 *)((sh ? L.hsh : L.h) + i);
-    *(uint32_t *)((sh ? L.hshq : L.hq) + i) = i8_pack4(i8_code(v.x, s), i8_code(v.y, s), i8_code(v.z, s), i8_code(v.w, s));
+    const size_t at = (size_t)(sh ? row - L.P : row) * width;
+    const float *h = (sh ? L.hsh : L.h) + at;
+    uint32_t mb = I8_MX0;
+    for (int k = 4 * tid; k < width; k += 1024) {
+        const i8_f4 v = *(const i8_f4 *)(h + k);
+#pragma unroll
+        for (int i = 0; i < 4; i++) mb = max(mb, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+    mb = wave_max_u32(mb);
+    if ((tid & 63) == 0) red[tid >> 6] = mb;
+    __syncthreads();
+    const I8Scale s = i8_scale(max(max(red[0], red[1]), max(red[2], red[3])));
+    if (tid == 0) L.hs[row] = s.sc;
+    for (int k = 4 * tid; k < width; k += 1024) {
+        const i8_f4 v = *(const i8_f4 *)(h + k);
+        *(uint32_t *)((sh ? L.hshq : L.hq) + at + k) = i8_pack4(i8_code(v.x, s), i8_code(v.y, s), i8_code(v.z, s), i8_code(v.w, s));
+    }
 }
 
 // ------------------------------------------------------------------ down + combine
-// Sums of units [u0, u1) of 16 channels for columns c0 .. of the n rows (list, or row = column) of codes into LDS:
-// sums[row * 16 + channel]
-template <int CB, typename Rows>
-__device__ __forceinline__ void i8_down(const uint8_t *wp, const int8_t *codes, int width, Rows rowof, int u0, int u1, int c0, int n, int *sums) {
-    const int lane = threadIdx.x & 63;
-    const int8_t *xp[CB];
-#pragma unroll
-    for (int j = 0; j < CB; j++) xp[j] = codes + (size_t)rowof(min(c0 + 16 * j + (lane & 15), n - 1)) * width + (lane >> 4) * 16;
-    i8_i4 acc[CB];
-#pragma unroll
-    for (int j = 0; j < CB; j++) acc[j] = i8_i4{0, 0, 0, 0};
-    constexpr int D = CB == 1 ? 8 : 4;
-    for (int u = u0; u < u1; u += D) {
-        i8_u4 a[D], x[D][CB];
-#pragma unroll
-        for (int s = 0; s < D; s++) {
-            const int v = min(u + s, u1 - 1);
-            a[s] = *(const i8_u4 *)(wp + (size_t)v * 4096);
-#pragma unroll
-            for (int j = 0; j < CB; j++) x[s][j] = *(const i8_u4 *)(xp[j] + v * 64);
-        }
-#pragma unroll
-        for (int s = 0; s < D; s++)
-            if (u + s < u1) {
-#pragma unroll
-                for (int j = 0; j < CB; j++) acc[j] = mi_mfma(a[s], x[s][j], acc[j]);
-            }
-    }
-#pragma unroll
-    for (int j = 0; j < CB; j++) {
-        const int c = c0 + 16 * j + (lane & 15);
-        if (c < n) *(i8_i4 *)(sums + rowof(c) * 16 + 4 * (lane >> 4)) = acc[j];
-    }
-}
-
 template <bool LDSQ>
-__global__ __launch_bounds__(MOE_I8_NW * 64) void k_moe_i8_down(MoeI8Launch L) {
+__global__ __launch_bounds__(MOE_I8_DW * 64) void k_moe_i8_down(MoeI8Launch L) {
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ MoeI8Route R;
-    __shared__ __align__(16) float lbuf[MOE_I8_ROUTE][ROUTE_MAXE];
-    __shared__ uint16_t lists[MOE_I8_NW][MOE_I8_PAIRS];
-    int *const sums = (int *)dyn;                                        // [part][P + T][16]
-    const int rows = L.P + (L.shared ? L.T : 0);
-    int8_t *const q = (int8_t *)dyn + (size_t)L.parts * rows * 64;       // LDSQ: the codes [P][I], [T][Ish]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, rb = blockIdx.x;
-    i8_routing(L, R, lbuf);
-    if constexpr (LDSQ) {
-        const int n0 = L.P * L.I / 4, n1 = n0 + (L.shared ? L.T * L.Ish / 4 : 0);
-        for (int i = threadIdx.x; i < n1; i += MOE_I8_NW * 64) {
-            const bool sh = i >= n0;
-            const int at = (sh ? i - n0 : i) * 4, row = at / (sh ? L.Ish : L.I);
-            const I8Scale s = i8_scale(max(L.amax[(sh ? L.P : 0) + row], I8_MX0));
-            const i8_f4 v = *(const i8_f4 *)((sh ? L.hsh : L.h) + at);
-            ((uint32_t *)q)[i] = i8_pack4(i8_code(v.x, s), i8_code(v.y, s), i8_code(v.z, s), i8_code(v.w, s));
-        }
-        __syncthreads();
-    }
+    __shared__ const uint8_t *tw[MOE_I8_PAIRS];                          // each slot's weights and scales
+    __shared__ const float *ts[MOE_I8_PAIRS];
+    __shared__ uint16_t order[MOE_I8_PAIRS];
+    __shared__ float hs[LDSQ ? MOE_I8_LDSQ / 64 : 1];                     // LDSQ: the scales of the rows (64 codes at least)
+    int *const sums = (int *)dyn;                                        // [P + T][16]
+    const int rows = L.P + (L.shared ? L.T : 0), tid = threadIdx.x;
+    int8_t *const q = (int8_t *)dyn + (size_t)rows * 64;                 // LDSQ: the codes [P][I], [T][Ish]
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, rb = blockIdx.x;
     const int8_t *const hq = LDSQ ? q : L.hq, *const shq = LDSQ ? q + (size_t)L.P * L.I : L.hshq;
-    // the shared experts first (the longest rows), then the routed ones
-    const int nsh = L.shared ? L.parts : 0;
-    for (int task = wave; task < nsh + L.nslots * L.parts; task += MOE_I8_NW) {
-        const bool sh = task < nsh;
-        const int slot = sh ? 0 : (task - nsh) / L.parts, part = sh ? task : (task - nsh) % L.parts;
-        const int e = sh ? 0 : i8_slot(R, slot);
-        if (e < 0) break;                                                // slots past the last used expert
-        const BglDevTensor *const T = sh ? &L.sd : L.td + e;
-        const int n = sh ? L.T : i8_pairs(L, R, e, lists[wave]), width = sh ? L.Ish : L.I, U = width / 64;
-        const uint8_t *wp = mi_rows(T->w, T->cpr, rb, lane);
-        const int u0 = U * part / L.parts, u1 = U * (part + 1) / L.parts;
-        int *const to = sums + (part * rows + (sh ? L.P : 0)) * 16;
-        __builtin_amdgcn_wave_barrier();
-        if (u0 == u1) {                                                  // fewer units than parts
-            for (int i = lane; i < n * 16; i += 64) to[(sh ? i >> 4 : lists[wave][i >> 4]) * 16 + (i & 15)] = 0;
-            continue;
-        }
-        for (int c0 = 0; c0 < n; c0 += 64) {
-            const int left = n - c0;
-            const uint16_t *ls = lists[wave];
-            auto go = [&](auto rowof) {
-                if (left <= 16) i8_down<1>(wp, sh ? shq : hq, width, rowof, u0, u1, c0, n, to);
-                else if (left <= 32) i8_down<2>(wp, sh ? shq : hq, width, rowof, u0, u1, c0, n, to);
-                else i8_down<4>(wp, sh ? shq : hq, width, rowof, u0, u1, c0, n, to);
-            };
-            if (sh) go([](int c) { return c; });
-            else go([ls](int c) { return (int)ls[c]; });
+    for (int i = tid; i < rows * 16; i += MOE_I8_DW * 64) sums[i] = 0;
+    i8_routing(L, R);
+    const int nslots = __builtin_amdgcn_readfirstlane(R.n);
+    for (int s = tid; s < nslots; s += MOE_I8_DW * 64) {
+        tw[s] = L.td[R.expert[s]].w;
+        ts[s] = (const float *)L.td[R.expert[s]].s0;
+    }
+    __syncthreads();
+    // pieces of the shared experts first (the longest rows), then of the routed ones
+    const int np = (L.I / 64 + L.piece - 1) / L.piece, nps = L.shared ? (L.Ish / 64 + L.piece - 1) / L.piece : 0;
+    const int tasks = nps + nslots * np, cpr = (L.I + 127) / 128 * 8, scpr = (L.Ish + 127) / 128 * 8;
+    struct Piece { int slot, u0, nu; i8_u4 a[MOE_I8_DC]; } even, odd;      // in turn: no copy waits for a load
+    // a piece's place and weights
+    auto fetch = [&](Piece &p, int task) {
+        const bool sh = task < nps;
+        p.slot = sh ? -1 : (task - nps) / np;
+        p.u0 = (sh ? task : (task - nps) % np) * L.piece;
+        p.nu = min(L.piece, (sh ? L.Ish : L.I) / 64 - p.u0);
+        const uint8_t *wp = mi_rows(sh ? L.sd.w : tw[p.slot], sh ? scpr : cpr, rb, lane) + (size_t)p.u0 * 4096;
+#pragma unroll
+        for (int s = 0; s < MOE_I8_DC; s++) p.a[s] = *(const i8_u4 *)(wp + (size_t)min(s, p.nu - 1) * 4096);
+    };
+    if (wave < tasks) fetch(even, wave);                                 // on its way while the codes are made
+    // a token's pairs by expert, then k: the order in which they are added
+    for (int p = tid; p < L.P; p += MOE_I8_DW * 64) {
+        const int t = p / L.K, me = R.slot[p];
+        int before = 0;
+        for (int o = t * L.K; o < (t + 1) * L.K; o++) before += R.slot[o] < me || (R.slot[o] == me && o < p);
+        order[t * L.K + before] = (uint16_t)p;
+    }
+    if constexpr (LDSQ) {
+        for (int row = wave; row < rows; row += MOE_I8_DW) {             // a wave a row
+            const bool sh = row >= L.P;
+            const int width = sh ? L.Ish : L.I;
+            const float *h = sh ? L.hsh + (size_t)(row - L.P) * width : L.h + (size_t)row * width;
+            int8_t *to = sh ? q + (size_t)L.P * L.I + (size_t)(row - L.P) * width : q + (size_t)row * width;
+            uint32_t mb = I8_MX0;
+            for (int k = 4 * lane; k < width; k += 256) {
+                const i8_f4 v = *(const i8_f4 *)(h + k);
+#pragma unroll
+                for (int i = 0; i < 4; i++) mb = max(mb, __float_as_uint(v[i]) & 0x7fffffffu);
+            }
+            const I8Scale s = i8_scale(wave_max_u32(mb));
+            if (lane == 0) hs[row] = s.sc;
+            for (int k = 4 * lane; k < width; k += 256) {
+                const i8_f4 v = *(const i8_f4 *)(h + k);
+                *(uint32_t *)(to + k) = i8_pack4(i8_code(v.x, s), i8_code(v.y, s), i8_code(v.z, s), i8_code(v.w, s));
+            }
         }
     }
     __syncthreads();
-    // k_moe_combine's order: ascending expert id, then k; then the shared experts
-    for (int o = threadIdx.x; o < L.T * 16; o += MOE_I8_NW * 64) {
-        const int t = o >> 4, ch = o & 15, r = 16 * rb + ch;
-        const int *ids = R.ids + t * L.K;
-        auto value = [&](int row, const BglDevTensor *T) {
-            int s = 0;
-            for (int i = 0; i < L.parts; i++) s += sums[(i * rows + row) * 16 + ch];
-            return i8_out(s, i8_scale(max(L.amax[row], I8_MX0)).sc, ((const float *)T->s0)[r]);
-        };
-        float acc = 0.0f;
-        int last = -1, lastk = -1;                                        // the pair added last
-        for (int a = 0; a < L.K; a++) {
-            int be = 0x7fffffff, bk = -1;
-            for (int k = 0; k < L.K; k++) {
-                const int e = ids[k];
-                if (e < 0 || e >= L.E) continue;
-                if ((e > last || (e == last && k > lastk)) && e < be) { be = e; bk = k; }
+    auto piece = [&](int task, const Piece &cur, Piece &nxt) {
+        const bool sh = cur.slot < 0;
+        const int l0 = sh ? 0 : R.off[cur.slot], n = sh ? L.T : R.off[cur.slot + 1] - l0;
+        const int8_t *const codes = (sh ? shq : hq) + cur.u0 * 64 + (lane >> 4) * 16;
+        for (int c0 = 0; c0 < n; c0 += 16) {
+            const int c = min(c0 + (lane & 15), n - 1), row = sh ? c : R.list[l0 + c];
+            const int8_t *xp = codes + (size_t)row * (sh ? L.Ish : L.I);
+            i8_i4 acc = {0, 0, 0, 0};
+            i8_u4 x[MOE_I8_DC];
+#pragma unroll
+            for (int s = 0; s < MOE_I8_DC; s++) x[s] = *(const i8_u4 *)(xp + min(s, cur.nu - 1) * 64);
+            // behind the codes: loads return in order, and these are waited for in the next piece
+            if (c0 == 0 && task + MOE_I8_DW < tasks) fetch(nxt, task + MOE_I8_DW);
+#pragma unroll
+            for (int s = 0; s < MOE_I8_DC; s++)
+                if (s < cur.nu) acc = mi_mfma(cur.a[s], x[s], acc);
+            if (c0 + (lane & 15) < n) {
+                int *to = sums + ((sh ? L.P : 0) + row) * 16 + 4 * (lane >> 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) atomicAdd(to + i, acc[i]);   // integers: in any order the same
             }
-            if (bk < 0) break;
-            acc = __fadd_rn(acc, __fmul_rn(R.w[t * L.K + bk], value(t * L.K + bk, L.td + be)));
-            last = be;
-            lastk = bk;
         }
-        if (L.shared) acc = __fadd_rn(acc, value(L.P + t, &L.sd));
-        L.out[(size_t)t * L.H + r] = acc;
+    };
+    for (int task = wave; task < tasks; task += 2 * MOE_I8_DW) {
+        piece(task, even, odd);
+        if (task + MOE_I8_DW < tasks) piece(task + MOE_I8_DW, odd, even);
+    }
+    __syncthreads();
+    // each sum becomes its weighted output, then a token's are added as k_moe_combine does: ascending expert id, then k;
+    // then the shared experts
+    for (int i = tid; i < rows * 16; i += MOE_I8_DW * 64) {
+        const int row = i >> 4, r = 16 * rb + (i & 15);
+        const bool sh = row >= L.P;
+        const int s = sh ? 0 : R.slot[row];
+        if (s == MOE_I8_NONE) continue;
+        const float ws = sh ? ((const float *)L.sd.s0)[r] : ts[s][r];
+        const float v = i8_out(sums[i], LDSQ ? hs[row] : L.hs[row], ws);
+        sums[i] = __float_as_int(sh ? v : __fmul_rn(L.w[row], v));
+    }
+    __syncthreads();
+    for (int o = tid; o < L.T * 16; o += MOE_I8_DW * 64) {
+        const int t = o >> 4, ch = o & 15;
+        float acc = 0.0f;
+        for (int i = 0; i < L.K; i++) {
+            const int p = order[t * L.K + i];
+            if (R.slot[p] != MOE_I8_NONE) acc = __fadd_rn(acc, __int_as_float(sums[p * 16 + ch]));
+        }
+        if (L.shared) acc = __fadd_rn(acc, __int_as_float(sums[(L.P + t) * 16 + ch]));
+        L.out[(size_t)t * L.H + 16 * rb + ch] = acc;
     }
 }
 
@@ -397,12 +453,13 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
     const size_t P = (size_t)most * K, rows = P + most;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) & ~(size_t)255; return o; };
-    const size_t o_amax = take(rows * 4), o_xs = take((size_t)most * 4), o_xq = take((size_t)most * L.H), o_h = take(P * L.I * 4),
+    const size_t o_hs = take(rows * 4), o_xs = take((size_t)most * 4), o_xq = take((size_t)most * L.H), o_h = take(P * L.I * 4),
                  o_hsh = take((size_t)most * L.Ish * 4), o_hq = take(P * L.I), o_hshq = take((size_t)most * L.Ish),
                  o_idx = take(P * 4), o_w = take(P * 4), o_sc = take((size_t)most * L.E * 4);
-    if (dbuf_reserve(c, c->moe_g, at, false)) return bgl_last_code();
+    if (dbuf_reserve(c, c->moe_g, at, false) || (rw && dbuf_reserve(c, c->moe_ticket, MOE_I8_TOK * 4, true))) return bgl_last_code();
+    L.ticket = (int *)c->moe_ticket.p;
     uint8_t *base = (uint8_t *)c->moe_g.p;
-    L.amax = (uint32_t *)(base + o_amax); L.xs = (float *)(base + o_xs); L.xq = (int8_t *)(base + o_xq);
+    L.hs = (float *)(base + o_hs); L.xs = (float *)(base + o_xs); L.xq = (int8_t *)(base + o_xq);
     L.h = (float *)(base + o_h); L.hsh = (float *)(base + o_hsh);
     for (int t0 = 0; t0 < T; t0 += MOE_I8_TOK) {
         L.T = std::min(MOE_I8_TOK, T - t0);
@@ -411,31 +468,29 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
         L.x = x + (size_t)t0 * L.H;
         L.out = out + (size_t)t0 * L.H;
         L.scores = rw ? (float *)(base + o_sc) : nullptr;
-        L.idx = rw ? nullptr : idx + (size_t)t0 * K;
-        L.w = rw ? nullptr : w + (size_t)t0 * K;
+        L.idx = rw ? (int32_t *)(base + o_idx) : const_cast<int32_t *>(idx) + (size_t)t0 * K;
+        L.w = rw ? (float *)(base + o_w) : const_cast<float *>(w) + (size_t)t0 * K;
         int tok = prof_begin(c, 2);
         hipLaunchKernelGGL(k_moe_i8_pre, dim3((unsigned)(L.T + (rw ? L.T * ((L.E + 3) / 4) : 0))), dim3(256), 0, c->stream, L);
-        if (rw && L.T > MOE_I8_ROUTE) {
-            bgl_launch_route_topk(L.scores, L.T, L.E, K, renorm, (int32_t *)(base + o_idx), (float *)(base + o_w), c->stream);
-            L.idx = (const int32_t *)(base + o_idx);
-            L.w = (const float *)(base + o_w);
-        }
         prof_end(c, tok);
         tok = prof_begin(c, 1);
-        const int cbmax = L.T <= 16 ? 1 : L.T <= 32 ? 2 : 4;
-        hipLaunchKernelGGL(k_moe_i8_gu, dim3((unsigned)((L.shared ? L.Ish / 16 : 0) + L.nslots * (L.I / 16))), dim3(MOE_I8_NW * 64),
-                           (size_t)MOE_I8_NW * cbmax * 2048, c->stream, L, cbmax);
+        const unsigned wgs = (unsigned)std::min(MOE_I8_GU_WGS, (L.shared ? L.Ish / 16 : 0) + L.nslots * (L.I / 16));
+        // Columns at a time: 2 blocks of 16 keep every register through the epilogue; 4 read a popular expert's weights once
+        // instead of twice and keep less of them on their way.  64 experts of 2048 x 1408, 6 a token and a shared 2816:
+        // 32 tokens 161 us with 2, 164 with 4; 64 tokens 214, 204.  (1 block runs into spills: 139 us for 129 at 16.)
+        if (L.T <= 32) hipLaunchKernelGGL((k_moe_i8_gu<2, 2>), dim3(wgs), dim3(MOE_I8_NW * 64), MOE_I8_NW * 4096, c->stream, L);
+        else hipLaunchKernelGGL((k_moe_i8_gu<4, 1>), dim3(wgs), dim3(MOE_I8_NW * 64), MOE_I8_NW * 8192, c->stream, L);
         const size_t q = (size_t)L.P * L.I + (size_t)(L.shared ? L.T * L.Ish : 0);
         const bool ldsq = q <= MOE_I8_LDSQ;
         L.hq = ldsq ? nullptr : (int8_t *)(base + o_hq);
         L.hshq = ldsq ? nullptr : (int8_t *)(base + o_hshq);
-        if (!ldsq) hipLaunchKernelGGL(k_moe_i8_hq, dim3((unsigned)((q / 4 + 255) / 256)), dim3(256), 0, c->stream, L);
-        // few pairs: K is split as well, so that every wave has work
-        L.parts = L.T == 1 ? 4 : L.T <= 4 ? 2 : 1;
-        const size_t lds = (size_t)L.parts * (L.P + (L.shared ? L.T : 0)) * 64 + (ldsq ? q : 0);
+        if (!ldsq) hipLaunchKernelGGL(k_moe_i8_hq, dim3((unsigned)(L.P + (L.shared ? L.T : 0))), dim3(256), 0, c->stream, L);
+        const int pieces = (L.I / 64 + MOE_I8_DC - 1) / MOE_I8_DC;            // of equal length
+        L.piece = (L.I / 64 + pieces - 1) / pieces;
+        const size_t lds = (size_t)(L.P + (L.shared ? L.T : 0)) * 64 + (ldsq ? q : 0);
         auto kern = ldsq ? k_moe_i8_down<true> : k_moe_i8_down<false>;
         HIPCHK(hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        hipLaunchKernelGGL(kern, dim3((unsigned)(L.H / 16)), dim3(MOE_I8_NW * 64), lds, c->stream, L);
+        hipLaunchKernelGGL(kern, dim3((unsigned)(L.H / 16)), dim3(MOE_I8_DW * 64), lds, c->stream, L);
         prof_end(c, tok);
         HIPCHK(hipGetLastError());
     }

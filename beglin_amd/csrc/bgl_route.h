@@ -3,9 +3,6 @@
 #pragma once
 #include "bgl_internal.h"
 
-// T tokens' scores [T][E] to their K picks (bgl_moe.hip)
-void bgl_launch_route_topk(const float *scores, int T, int E, int K, int renorm, int32_t *idx, float *w, hipStream_t st);
-
 #define ROUTE_MAXE 256
 #define ROUTE_RND 8
 
