@@ -50,7 +50,7 @@ struct bgl_ctx {
     DevBuf moe_a, moe_b, moe_c, moe_d, moe_e, moe_f, moe_g, moe_meta;   // MoE digits x2, fp32 h/down, bucket scratch
     DevBuf moe_route;                     // routing of bgl_moe_layer_dev: idx [T][K] + w [T][K]
     DevBuf moe_scores;                    // router scores [T][E]
-    DevBuf moe_ticket;                    // K_Q8C experts: workgroups of each token that have their scores, 0 between launches
+    DevBuf moe_sync;                      // K_Q8C experts: what the workgroups of a launch tell each other (MoeI8Sync)
     DevBuf mlp;                           // bgl_mlp_dev: gate and up outputs [M][I] each, then h [M][I]
     std::unordered_map<uint64_t, DevBuf> mlp_sync;   // single-launch MLP, per shape (in << 32 | down workgroups): counters, generations, flag
     bool no_qmfma = false;                // BGL_NO_QMFMA=1: W4A8 at 2..16 columns through the dot4 kernel (k_gemv_q)
@@ -58,10 +58,10 @@ struct bgl_ctx {
     int qm_prb = 0, qm_ps = 0;            // BGL_QM_PRB / BGL_QM_PS: the same for its launches over prepared codes
     int mlp_gu = 0;                       // BGL_MLP_GU: gate+up workgroups of the single-launch MLP (tuning; 0 by shape)
     bool no_fused_mlp = false;            // BGL_NO_FUSED_MLP=1: the MLP block as three launches at every M
-    int mlp_spin = 1 << 20;               // BGL_MLP_SPIN: polls of the single-launch MLP's bounded wait
+    int mlp_spin = 1 << 20;               // BGL_MLP_SPIN: polls of the bounded waits of a single-launch MLP or MoE layer
     int mlp_delay = -1;                   // BGL_MLP_DELAY: ns the single-launch MLP's down waves wait before loading their weights (tuning; -1 by shape)
     int mlp_waves = 0;                    // BGL_MLP_WAVES: wavefronts per single-launch MLP workgroup (tuning; 0 by shape)
-    int mlp_test_timeout = 0;             // BGL_MLP_TEST_TIMEOUT=n: the next n such launches wait for a count never reached (tests of the give-up path)
+    int mlp_test_timeout = 0;             // BGL_MLP_TEST_TIMEOUT=n: the next n such launches wait for what is never written (tests of the give-up path)
     std::vector<void *> retired;          // outgrown scratch, kept for captured graphs until destroy / epoch reset
     uint8_t *fixed_base = nullptr;        // set during bgl_matmul_group_noalloc_dev: scratch comes from here
     size_t fixed_cap = 0, fixed_used = 0;
@@ -110,6 +110,8 @@ bool mfma_takes(const bgl_ctx *c, int n, const BglDevTensor *Ts, int M);
 // into glu_h [M][N] (k_swiglu's arithmetic), so the caller needs no SwiGLU launch.
 int run_gemm_mfma(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x_dev, int M, const float *const *bias,
                   float *const *y, const int *ystride, float *glu_h = nullptr);
+int moe_i8_recount(bgl_ctx *c);              // bgl_ctx_check, after a wait in a layer of K_Q8C experts gave up (bgl_moe_i8.hip)
+
 // The dense MLP block at one W4A8 column in one launch (bgl_mlp_q.hip): the formats it takes, and the call.
 int run_down_swiglu_w4a8(bgl_ctx *c, const BglDevTensor &down, const float *g, const float *u, float *h, int M, float *y);
 // W4A8 products of more than 16 columns (bgl_gemm_q.hip): the calls it takes, and the call.

@@ -434,19 +434,26 @@ extern "C" int bgl_ctx_check(bgl_ctx *c) {
     if (!c) return bgl_fail(BGL_E_ARG, "bgl_ctx_check: NULL context");
     HIPCHK(hipSetDevice(c->device));
     HIPCHK(hipStreamSynchronize(c->stream));
-    bool gave_up = false;
-    for (auto &kv : c->mlp_sync) {
-        const DevBuf &sb = kv.second;
-        if (!sb.p) continue;
-        int *flag = (int *)sb.p;
+    int *flags[2] = {nullptr, (int *)c->moe_sync.p};             // a sync buffer begins with its flag
+    bool gave_up[2] = {false, false};
+    auto check = [&](int which) {
         int f = 0;
-        HIPCHK(hipMemcpy(&f, flag, sizeof f, hipMemcpyDeviceToHost));
-        if (!f) continue;
         const int zero = 0;
-        HIPCHK(hipMemcpy(flag, &zero, sizeof zero, hipMemcpyHostToDevice));
-        gave_up = true;
+        if (!flags[which]) return hipSuccess;
+        hipError_t e = hipMemcpy(&f, flags[which], sizeof f, hipMemcpyDeviceToHost);
+        if (e != hipSuccess || !f) return e;
+        gave_up[which] = true;
+        return hipMemcpy(flags[which], &zero, sizeof zero, hipMemcpyHostToDevice);
+    };
+    for (auto &kv : c->mlp_sync) {
+        flags[0] = (int *)kv.second.p;
+        HIPCHK(check(0));
     }
-    if (gave_up)
+    HIPCHK(check(1));
+    if (gave_up[1] && moe_i8_recount(c)) return bgl_last_code();
+    if (gave_up[0])
         return bgl_fail(BGL_E_TIMEOUT, "a single-launch MLP block stopped waiting for its gate+up workgroups: its outputs are invalid");
+    if (gave_up[1])
+        return bgl_fail(BGL_E_TIMEOUT, "a single-launch MoE layer stopped waiting for some of its workgroups: its outputs and later layers' are invalid");
     return 0;
 }

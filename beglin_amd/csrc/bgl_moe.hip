@@ -809,13 +809,12 @@ __global__ __launch_bounds__(64) void k_moe_route_topk(const float *__restrict__
                                                        int32_t *__restrict__ idx_out, float *__restrict__ w_out) {
     __shared__ __align__(16) float lbuf[ROUTE_MAXE];
     const int t = blockIdx.x, lane = threadIdx.x;
-    float sel_w[MOE_MAX_K];
-    int sel_i[MOE_MAX_K];
+    float sel_w;
+    int sel_i;
     route_topk_wave(scores + (size_t)t * E, E, K, renorm, lane, sel_i, sel_w, lbuf);
-    if (lane != 0) return;
-    for (int k = 0; k < K; k++) {
-        idx_out[(size_t)t * K + k] = sel_i[k];
-        w_out[(size_t)t * K + k] = sel_w[k];
+    if (lane < K) {
+        idx_out[(size_t)t * K + lane] = sel_i;
+        w_out[(size_t)t * K + lane] = sel_w;
     }
 }
 
@@ -833,15 +832,14 @@ __global__ __launch_bounds__(1024) void k_moe_route_bucket(const float *__restri
     const int P = T * K, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, nw = blockDim.x >> 6;
     for (int e = threadIdx.x; e <= E; e += blockDim.x) start[e] = 0;
     for (int t = wave; t < T; t += nw) {
-        float sel_w[MOE_MAX_K];
-        int sel_i[MOE_MAX_K];
+        float sel_w;
+        int sel_i;
         route_topk_wave(scores + (size_t)t * E, E, K, renorm, lane, sel_i, sel_w, lbuf[wave]);
-        if (lane == 0)
-            for (int k = 0; k < K; k++) {
-                idx_out[(size_t)t * K + k] = sel_i[k];
-                w_out[(size_t)t * K + k] = sel_w[k];
-                ids[t * K + k] = sel_i[k] < E ? sel_i[k] : -1;   // a slot no score filled
-            }
+        if (lane < K) {
+            idx_out[(size_t)t * K + lane] = sel_i;
+            w_out[(size_t)t * K + lane] = sel_w;
+            ids[t * K + lane] = sel_i < E ? sel_i : -1;          // a slot no score filled
+        }
     }
     __syncthreads();
     for (int p = threadIdx.x; p < P; p += blockDim.x)

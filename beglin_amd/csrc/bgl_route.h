@@ -35,9 +35,9 @@ __device__ __forceinline__ double route_dot_wave(const float *w, const float *x,
     return acc;
 }
 
-// Softmax, top-K and renorm of one token's E scores by one wave; lane 0 returns the K picks.
+// Softmax, top-K and renorm of one token's E scores by one wave; lane k < K returns pick k.
 __device__ __forceinline__ void route_topk_wave(const float *__restrict__ sc_t, int E, int K, int renorm, int lane,
-                                                int *sel_i, float *sel_w, float *lbuf) {
+                                                int &sel_i, float &sel_w, float *lbuf) {
     constexpr int PL = ROUTE_MAXE / 64;                      // scores per lane: expert lane + 64j
     float v[PL];
     float mx = -INFINITY;
@@ -72,6 +72,8 @@ __device__ __forceinline__ void route_topk_wave(const float *__restrict__ sc_t, 
         sum += (double)q3.x; sum += (double)q3.y; sum += (double)q3.z; sum += (double)q3.w;
     }
     for (; e16 < E; e16++) sum += (double)lbuf[e16];
+    sel_i = 0;
+    sel_w = 0.0f;
     unsigned used = 0;                                       // bit j: expert lane + 64j selected
 #pragma unroll
     for (int j = 0; j < PL; j++) v[j] = (float)((double)v[j] / sum);
@@ -86,13 +88,11 @@ __device__ __forceinline__ void route_topk_wave(const float *__restrict__ sc_t, 
         }
         wave_argmax(bv, bi);                                  // DPP and readlane: no LDS round trips
         if ((bi & 63) == lane) used |= 1u << (bi >> 6);
-        sel_w[k] = bv;
-        sel_i[k] = bi;
+        if (lane == k) { sel_w = bv; sel_i = bi; }
     }
-    if (lane == 0 && renorm) {
+    if (renorm) {
         double s = 0.0;
-        for (int k = 0; k < K; k++) s += (double)sel_w[k];
-        if (s > 0.0)
-            for (int k = 0; k < K; k++) sel_w[k] = (float)((double)sel_w[k] / s);
+        for (int k = 0; k < K; k++) s += (double)rlane_f(sel_w, k);
+        if (s > 0.0) sel_w = (float)((double)sel_w / s);
     }
 }

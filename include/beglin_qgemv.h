@@ -76,9 +76,10 @@ int  bgl_ctx_create(int device, void *hip_stream, bgl_ctx **out);   /* q4pool_in
 void bgl_ctx_destroy(bgl_ctx *ctx);                         /* q4pool_destroy (q4gemv.h:623-637) */
 int  bgl_synchronize(bgl_ctx *ctx);                         /* mlx_gpu_synchronize (mlx_moe.h:29) */
 /* Synchronize the context's stream, then report (and clear) a bounded in-kernel wait that gave up
- * since the last check: BGL_E_TIMEOUT means the outputs of that call are invalid.  No counterpart in
+ * since the last check: BGL_E_TIMEOUT means the outputs of that call are invalid, and for a layer of
+ * K_Q8C experts those of later such layers before the check too.  No counterpart in
  * the reference (its CPU kernels never wait on each other); the single-launch MLP block of
- * bgl_mlp_dev is the call that waits. */
+ * bgl_mlp_dev and the K_Q8C layers of bgl_moe_ffn_dev and bgl_moe_layer_dev are the calls that wait. */
 int  bgl_ctx_check(bgl_ctx *ctx);
 void *bgl_ctx_stream(bgl_ctx *ctx);                          /* the hipStream_t work is queued on */
 
@@ -176,8 +177,8 @@ int  bgl_quant_act_i8_dev(bgl_ctx *ctx, const float *x_dev, int M, int in, int g
  * y_type (BGL_T_*).  xq: rows ldq bytes apart, ldq % 16 == 0, ldq >= in, 16-byte aligned; the bytes
  * between in and the row's next multiple of 16 may hold anything.  ascale [M].  bias_dev, or an entry
  * of it, may be NULL.  y[i]: rows ldy[i] values apart (ldy NULL: dense), so a group may fill the parts of
- * one wider row.  No scratch for up to 64 columns and none that a capture would have to grow; no
- * counterpart in the reference.  bgl_matmul_dev, bgl_matmul_group_dev, bgl_mlp_dev,
+ * one wider row.  A product whose K is split over workgroups keeps its sums in the context's scratch,
+ * which a capture must not have to grow; no counterpart in the reference.  bgl_matmul_dev, bgl_matmul_group_dev, bgl_mlp_dev,
  * bgl_prep_act_dev / bgl_matmul_prepped_dev, bgl_quantize_dev (largest |w| of a row = 127) and
  * bgl_dequant_dev take K_Q8C as any kind; bgl_moe_ffn_dev and bgl_moe_layer_dev take stacks of it. */
 int  bgl_matmul_i8_dev(bgl_ctx *ctx, int n, const bgl_tensor *const *w, const int8_t *xq_dev, long ldq, const float *ascale_dev,
@@ -288,7 +289,11 @@ int bgl_gather_matvec_dev(bgl_ctx *ctx, const bgl_tensor *experts, const float *
 /* Routed SwiGLU FFN for T tokens with top-K routing given (moe_ffn_batched, qwen_infer.c:5238-5350):
  * out[t] = sum_k w[t][k] * down_e(silu(gate_e x_t) * up_e x_t) + shared(x_t), e = idx[t][k];
  * the weighted sum runs in ascending expert order per token like the reference's bucket loop.
- * shared_* may be NULL (no shared experts). x_dev [T][in], idx/w [T][K] on device, out [T][in]. */
+ * shared_* may be NULL (no shared experts). x_dev [T][in], idx/w [T][K] on device, out [T][in].
+ * Stacks of K_Q8C (all of gate, up, down and shared_*, up to 1024 experts; any other mixture with it is
+ * refused): x and h are quantized with one scale per row, as bgl_quant_act_i8_dev does, and the products
+ * are bgl_matmul_i8_dev's, so a token's bits do not depend on the others.  For few tokens: 64 at a
+ * time, each of which reads the experts that it touches once; a bounded wait, see bgl_ctx_check. */
 int bgl_moe_ffn_dev(bgl_ctx *ctx, const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down,
                     const bgl_tensor *shared_gate, const bgl_tensor *shared_up, const bgl_tensor *shared_down,
                     const float *x_dev, const int32_t *topk_idx_dev, const float *topk_w_dev, int T, int K,

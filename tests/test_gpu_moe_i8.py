@@ -173,6 +173,100 @@ def test_captured_layer(torch_dev, T):
     c.close()
 
 
+def test_launches_of_changing_sizes(ctx, torch_dev):
+    """Launches of many and of few workgroups after each other leave nothing behind: the same bits each time."""
+    torch = torch_dev
+    E, K, H, W = 24, 4, 256, 192
+    lay = Layer(ctx, 77, E, H, W, 320)
+    rw = torch.from_numpy((lay.rng.standard_normal((E, H)) / H ** 0.5).astype(np.float32)).cuda()
+    xs = [torch.from_numpy(lay.rng.standard_normal((T, H)).astype(np.float32)).cuda() for T in (1, 64, 2, 7, 33, 1, 70, 16)]
+    first = None
+    for r in range(6):
+        outs = [torch.full_like(x, float("nan")) for x in xs]
+        torch.cuda.synchronize()
+        for x, o in list(zip(xs, outs))[::1 if r % 2 else -1]:
+            ctx.moe_layer(rw, *lay.stacks, lay.sh, x, K, o)
+        ctx.check()
+        outs = [o.cpu().numpy() for o in outs]
+        if first is None:
+            first = outs
+            for x, o in zip(xs, outs):
+                idx, w = torch.empty((len(x), K), dtype=torch.int32, device="cuda"), torch.empty((len(x), K), device="cuda")
+                torch.cuda.synchronize()
+                ctx.moe_route(rw, x, K, idx, w)
+                ctx.sync()
+                same(torch.from_numpy(o), lay.want(x.cpu().numpy(), idx.cpu().numpy(), w.cpu().numpy()))
+        assert all(np.array_equal(a.view(np.uint32), b.view(np.uint32)) for a, b in zip(first, outs)), r
+    lay.free()
+
+
+def test_two_contexts_at_once(torch_dev):
+    """Two contexts on streams of their own, whose launches share the CUs."""
+    import beglin_amd as B
+    torch = torch_dev
+    E, K, H, W = 16, 4, 512, 256
+    cs, lays, rws, xs = [], [], [], []
+    for i in range(2):
+        cs.append(B.Context(0))
+        lays.append(Layer(cs[i], 90 + i, E, H, W, 256))
+        rws.append(torch.from_numpy((lays[i].rng.standard_normal((E, H)) / H ** 0.5).astype(np.float32)).cuda())
+        xs.append([torch.from_numpy(lays[i].rng.standard_normal((T, H)).astype(np.float32)).cuda() for T in (1, 12, 40)])
+    outs = [[[torch.full_like(x, float("nan")) for x in xs[i]] for _ in range(20)] for i in range(2)]
+    torch.cuda.synchronize()
+    for r in range(20):
+        for i in range(2):
+            for x, o in zip(xs[i], outs[i][r]):
+                cs[i].moe_layer(rws[i], *lays[i].stacks, lays[i].sh, x, K, o)
+    for c in cs:
+        c.check()
+    for i in range(2):
+        for j, x in enumerate(xs[i]):
+            idx, w = torch.empty((len(x), K), dtype=torch.int32, device="cuda"), torch.empty((len(x), K), device="cuda")
+            torch.cuda.synchronize()
+            cs[i].moe_route(rws[i], x, K, idx, w)
+            cs[i].sync()
+            want = lays[i].want(x.cpu().numpy(), idx.cpu().numpy(), w.cpu().numpy())
+            for r in range(20):
+                same(outs[i][r][j], want)
+    for c, l in zip(cs, lays):
+        l.free()
+        c.close()
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_bounded_waits_give_up(torch_dev, monkeypatch, T):
+    """A launch whose waits are for what is never written (set from the host, with a few polls) still ends, is reported by
+    bgl_ctx_check, and leaves the context ready for the next."""
+    import beglin_amd as B
+    torch = torch_dev
+    print("[case] bounded waits", T, flush=True)
+    monkeypatch.setenv("BGL_MLP_TEST_TIMEOUT", "1")
+    monkeypatch.setenv("BGL_MLP_SPIN", "64")
+    c = B.Context(0)
+    monkeypatch.delenv("BGL_MLP_TEST_TIMEOUT")
+    monkeypatch.delenv("BGL_MLP_SPIN")
+    E, K, H, W = 16, 4, 256, 128
+    lay = Layer(c, 41, E, H, W, 64)
+    x = lay.rng.standard_normal((T, H)).astype(np.float32)
+    xd, out = torch.from_numpy(x).cuda(), torch.empty((T, H), device="cuda")
+    idx, w = lay.rng.integers(0, E, (T, K)).astype(np.int32), lay.rng.uniform(0, 1, (T, K)).astype(np.float32)
+    idd, wd = torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda()
+    torch.cuda.synchronize()
+    c.moe_ffn(*lay.stacks, lay.sh, xd, idd, wd, out)
+    with pytest.raises(B.BglError) as e:
+        c.check()
+    assert e.value.code == B.E_TIMEOUT
+    c.check()                                             # the flag was cleared
+    for _ in range(2):
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        c.moe_ffn(*lay.stacks, lay.sh, xd, idd, wd, out)
+        c.check()
+        same(out, lay.want(x, idx, w))
+    lay.free()
+    c.close()
+
+
 def test_refusals(ctx, torch_dev):
     import beglin_amd as B
     torch = torch_dev
