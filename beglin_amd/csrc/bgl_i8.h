@@ -75,7 +75,7 @@ __device__ __forceinline__ float i8_out(int acc, float as, float ws) { return __
 int run_quant_rows(bgl_ctx *c, const float *x, const float *u, float *h, int M, int K, int8_t *xq, long ldq, float *xs);
 // n <= 4 tensors of the int8 kind over M columns of codes (bgl_i8.hip); y[i] rows ldy[i] values apart
 int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
-           void *const *y, int y_type, const long *ldy, int M);
+           void *const *y, int y_type, const long *ldy, int M, const float *xf = nullptr);
 // M fp32 columns (u, h as run_quant_rows) quantized into the context's act_w / act_s; reuse: for
 // bgl_matmul_prepped_dev, as columns with one scale per token
 #define PREP_GQ_TOKEN -1

@@ -36,6 +36,8 @@ struct I8Launch {
     const int8_t *xq;
     long ldq;
     const float *xs;
+    const float *xf;              // the columns before quantization, [M][K]: each workgroup makes the codes it needs; or null
+    float *xs_out;                // then K split: where their scales go
 };
 
 __device__ __forceinline__ i8_i4 i8_mfma(i8_u4 a, i8_u4 b, i8_i4 c) {
@@ -85,16 +87,18 @@ __device__ __forceinline__ i8_f4 i8_bias(const I8Task &t, int r) {
 }
 
 // ================================================================================== few columns
-// A workgroup owns RB blocks of 16 channels and up to 16 CB tokens; its waves split K.  Weights and codes
+// A workgroup owns RB blocks of 16 channels and up to 16 CB tokens; its waves split K.  F32: the tokens come in fp32, and
+// every workgroup makes their codes in LDS (bgl_norm.hip's arithmetic) while its first weights are on their way.  Weights and codes
 // go straight from memory to the operand registers, D units ahead; the waves' int32 sums meet in LDS.
 // Partial sums of at most I8_S_PART / (RB * CB) waves lie in LDS at once: a workgroup of twice that many waves first
 // adds the upper half's to the lower half's.
 #define I8_S_PART 64          // KB
+#define I8_S_RND 4            // F32: 4 values a thread this often at most
 template <int RB, int CB>
 constexpr int i8_s_waves() { return RB * CB <= 4 ? 16 : 8; }
-template <int RB, int CB, int D>
+template <int RB, int CB, int D, bool F32>
 __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L) {
-    extern __shared__ __align__(16) i8_i4 red[];               // [wave][RB * CB][64]
+    extern __shared__ __align__(16) i8_i4 red[];               // [wave][RB * CB][64]; F32: codes [M][K + 16], a word a column
     constexpr int Q = RB * CB, G = I8_S_PART / Q;
     const int nw = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const I8Task t = i8_task(L, blockIdx.x);
@@ -104,6 +108,18 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
     const uint8_t *wp = t.T.w + ((size_t)(rb0 >> 2) * t.T.cpr + (lane >> 4)) * 1024 + ((rb0 & 3) * 16 + (lane & 15)) * 16;
     const int8_t *xp[CB];
     const int kq = (lane >> 4) * 16;
+    int8_t *const codes = (int8_t *)(red + min(nw * Q, I8_S_PART) * 64);
+    uint32_t *const mx = (uint32_t *)(codes + L.M * (t.T.K + 16));
+    const int grp = nw * 4, per = t.T.K / 64, nch = F32 ? L.M * per : 0;
+    i8_f4 xv[I8_S_RND];
+    if constexpr (F32) {
+        // 16 lanes take 64 values of a column; these loads go out before the weights, which need not be there for the codes
+#pragma unroll
+        for (int r = 0; r < I8_S_RND; r++)
+            if (r * grp < nch) xv[r] = *(const i8_f4 *)(L.xf + (size_t)min(r * grp + (int)(threadIdx.x >> 4), nch - 1) * 64 + 4 * (threadIdx.x & 15));
+        if (threadIdx.x < L.M) mx[threadIdx.x] = I8_MX0;
+        xp[0] = codes + min(lane & 15, L.M - 1) * (t.T.K + 16);
+    } else
 #pragma unroll
     for (int j = 0; j < CB; j++) xp[j] = L.xq + (size_t)min(m0 + 16 * j + (lane & 15), L.M - 1) * L.ldq;
     i8_i4 acc[RB][CB];
@@ -120,7 +136,8 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
             for (int i = 0; i < RB; i++) o.a[s][i] = *(const i8_u4 *)(wp + (size_t)u * 4096 + 256 * i);
             const int k = min(64 * u + kq, L.K16 - 16);              // past the row: the weights are zero there
 #pragma unroll
-            for (int j = 0; j < CB; j++) o.b[s][j] = *(const i8_u4 *)(xp[j] + k);
+            for (int j = 0; j < CB; j++)
+                if (!F32) o.b[s][j] = *(const i8_u4 *)(xp[j] + k);
         }
     };
     auto step = [&](int u0, const Ops &cur, Ops &nxt) {
@@ -128,6 +145,12 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
 #pragma unroll
         for (int s = 0; s < D; s++) {
             if (u0 + s * nw < U) {
+                if constexpr (F32) {
+                    const i8_u4 b = *(const i8_u4 *)(xp[0] + min(64 * (u0 + s * nw) + kq, L.K16 - 16));
+#pragma unroll
+                    for (int i = 0; i < RB; i++) acc[i][0] = i8_mfma(cur.a[s][i], b, acc[i][0]);
+                    continue;
+                }
 #pragma unroll
                 for (int i = 0; i < RB; i++)
 #pragma unroll
@@ -136,6 +159,33 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
         }
     };
     load(even, U0 + wave);
+    if constexpr (F32) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < I8_S_RND; r++) {
+            if (r * grp >= nch) break;
+            uint32_t mb = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) mb = max(mb, __float_as_uint(xv[r][i]) & 0x7fffffffu);
+            mb = max(mb, (uint32_t)dpp_i<0xB1>((int)mb));
+            mb = max(mb, (uint32_t)dpp_i<0x4E>((int)mb));
+            mb = max(mb, (uint32_t)dpp_i<0x141>((int)mb));
+            mb = max(mb, (uint32_t)dpp_i<0x140>((int)mb));
+            if ((threadIdx.x & 15) == 0) atomicMax(&mx[min(r * grp + (int)(threadIdx.x >> 4), nch - 1) / per], mb);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < I8_S_RND; r++) {
+            const int ch = r * grp + (threadIdx.x >> 4);
+            if (ch >= nch) break;
+            const int m = ch / per;
+            const I8Scale s = i8_scale(mx[m]);
+            *(uint32_t *)(codes + m * (t.T.K + 16) + (ch - m * per) * 64 + 4 * (threadIdx.x & 15)) =
+                i8_pack4(i8_code(xv[r].x, s), i8_code(xv[r].y, s), i8_code(xv[r].z, s), i8_code(xv[r].w, s));
+        }
+        if (L.ks > 1 && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x < L.M) L.xs_out[threadIdx.x] = i8_scale(mx[threadIdx.x]).sc;
+        __syncthreads();
+    }
     for (int u0 = U0 + wave; u0 < U; u0 += 2 * D * nw) {
         step(u0, even, odd);
         if (u0 + D * nw < U) step(u0 + D * nw, odd, even);
@@ -167,7 +217,7 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
         i8_i4 s = {0, 0, 0, 0};
         for (int w = 0; w < parts; w++) s += red[(w * Q + i * CB + j) * 64 + l];
         if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = s;
-        else i8_store4(L, t, m, r, s, L.xs[m], i8_ws(t, r), i8_bias(t, r));
+        else i8_store4(L, t, m, r, s, F32 ? i8_scale(mx[m]).sc : L.xs[m], i8_ws(t, r), i8_bias(t, r));
     }
 }
 
@@ -358,7 +408,7 @@ static int i8_split(bgl_ctx *c, I8Launch &L, int ks) {
     if (!c->fixed_base) HIPCHK(hipStreamIsCapturing(c->stream, &cs));
     if (!c->fixed_base && cs == hipStreamCaptureStatusNone && dbuf_reserve(c, c->part, I8_PART_BYTES, false)) return bgl_last_code();
     if (ks <= 1) return 0;
-    const size_t need = i8_part(L, ks);
+    const size_t need = i8_part(L, ks) + (L.xf ? L.M * 4 : 0);
     if (need > I8_PART_BYTES || (c->fixed_base && c->fixed_used + need + 256 > c->fixed_cap)) return 0;
     if (dbuf_reserve(c, c->part, c->fixed_base ? need : I8_PART_BYTES, false)) return bgl_last_code();
     int *p = (int *)c->part.p;
@@ -366,15 +416,31 @@ static int i8_split(bgl_ctx *c, I8Launch &L, int ks) {
         L.t[i].part = p;
         p += (size_t)ks * L.M * ((L.t[i].T.N + 3) & ~3);
     }
+    if (L.xf) L.xs = L.xs_out = (float *)p;
     L.ks = ks;
     return 0;
+}
+
+// Columns whose codes each workgroup of k_i8_s makes itself, where it has registers for all values: it costs less than the
+// launch that quantizes them up to 8192 values, and in one column, which that launch gives to one CU, up to 16384.  us with
+// this / with the launch (columns x channels x K): 1 x 4096 x 4096 6.2 / 8.2, 1 x 14336 x 4096 14.0 / 16.6, 1 x 4096 x 14336
+// 16.3 / 17.2, 2 x 4096 x 4096 7.1 / 8.4, 4 x 4096 x 4096 8.9 / 8.6, 16 x 8960 x 1024 8.8 / 8.3.
+static bool f32_fits(int M, int K, int units, int ks) {
+    return M <= 16 && K % 64 == 0 && M * (long)K <= (M == 1 ? 16384 : 8192) && M * (long)(K / 64) <= 4l * I8_S_RND * std::min(16, std::max(1, units / ks));
 }
 
 template <int RB, int CB>
 static void s_go(const I8Launch &L, int blocks, hipStream_t st) {
     constexpr int D = RB + CB <= 2 ? 4 : 2;
     const int nw = std::min(i8_s_waves<RB, CB>(), std::max(1, L.t[0].T.nunits / L.ks));
-    hipLaunchKernelGGL((k_i8_s<RB, CB, D>), dim3(blocks, (L.M + 63) / 64, L.ks), dim3(nw * 64), (size_t)std::min(nw * RB * CB, I8_S_PART) * 1024, st, L);
+    const size_t lds = (size_t)std::min(nw * RB * CB, I8_S_PART) * 1024;
+    const dim3 grid(blocks, (L.M + 63) / 64, L.ks);
+    if constexpr (CB == 1)
+        if (L.xf) {
+            hipLaunchKernelGGL((k_i8_s<RB, 1, D, true>), grid, dim3(nw * 64), lds + (size_t)L.M * (L.t[0].T.K + 16) + L.M * 4, st, L);
+            return;
+        }
+    hipLaunchKernelGGL((k_i8_s<RB, CB, D, false>), grid, dim3(nw * 64), lds, st, L);
 }
 static long s_blocks(I8Launch &L, int RB) {
     long blocks = 0;
@@ -435,6 +501,7 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
         for (int RB = 1; RB <= 4; RB *= 2) {
             const long blocks = s_blocks(L, RB);
             for (int ks = 1; ks <= 8 && (ks == 1 || K / ks >= I8_SLICE); ks *= 2) {
+                if (L.xf && !f32_fits(M, K, L.t[0].T.nunits, ks)) break;
                 const double us = up(blocks * ks) * ((double)(16 * RB + M) * K / ks / 40e3 + 1.5) + join(ks);
                 if (us < least) { least = us; best = RB; bks = ks; }
             }
@@ -458,11 +525,11 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
 }
 
 int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
-           void *const *y, int y_type, const long *ldy, int M) {
+           void *const *y, int y_type, const long *ldy, int M, const float *xf) {
     I8Launch L;
     memset(&L, 0, sizeof L);
     L.n = n; L.M = M; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
-    L.xq = xq; L.ldq = ldq; L.xs = xs;
+    L.xq = xq; L.ldq = ldq; L.xs = xs; L.xf = xf;
     L.vec = 1;
     int widest = 0;
     for (int i = 0; i < n; i++) {
@@ -499,10 +566,12 @@ int prep_i8_cols(bgl_ctx *c, const float *x, const float *u, float *h, int M, in
 
 int run_i8_cols(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x, const float *u, float *h, int M,
                 const float *const *bias, float *const *y) {
-    int rc = prep_i8_cols(c, x, u, h, M, Ts[0].K, false);
-    if (rc) return rc;
     void *yv[BGL_MAX_TASKS];
     for (int i = 0; i < n; i++) yv[i] = y[i];
+    if (!u && f32_fits(M, Ts[0].K, Ts[0].nunits, 1) && (uintptr_t)x % 16 == 0)
+        return run_i8(c, n, Ts, nullptr, 0, nullptr, bias, yv, BGL_T_F32, nullptr, M, x);
+    int rc = prep_i8_cols(c, x, u, h, M, Ts[0].K, false);
+    if (rc) return rc;
     return run_i8(c, n, Ts, (const int8_t *)c->act_w.p, i8_ld_scratch(Ts[0].K), (const float *)c->act_s.p, bias, yv, BGL_T_F32,
                   nullptr, M);
 }

@@ -141,6 +141,81 @@ def test_fp32_columns(ctx, torch_dev, M, rows, K):
         t.free()
 
 
+@pytest.mark.parametrize("M,rows,K", [(1, [64], 64), (1, [300, 70], 8192), (1, [17], 16384), (1, [4000], 16320), (2, [130], 4096), (8, [33, 900], 1024),
+                                      (16, [40], 512), (15, [65, 1], 448), (3, [500], 2688), (5, [9000], 1600), (2, [20, 20, 20, 20], 4032)])
+def test_few_fp32_columns(ctx, torch_dev, M, rows, K):
+    """Few values, whose codes each workgroup makes (K whole and split): the bits of quantizing first, also where the columns
+    begin off 16 bytes, and rows of NaN, infinities, zeros."""
+    say("few columns", M, rows, K)
+    rng = np.random.default_rng([M, K, 7])
+    ws, bs = [I.weights(rng, n, K) for n in rows], [rng.standard_normal(n).astype(np.float32) for n in rows]
+    ts, bd = [bind(ctx, w) for w in ws], [torch_dev.from_numpy(b).cuda() for b in bs]
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    x[:, K // 3] *= 40
+    wild = x.copy()
+    wild[0, K - 1] = np.nan
+    wild[M // 2, 3] = -np.inf
+    for v in (x, wild, np.zeros_like(x)):
+        for off in (0, 1, 3):
+            xd = torch_dev.zeros(M * K + 8, device="cuda")[off:off + M * K].view(M, K)
+            xd.copy_(torch_dev.from_numpy(v))
+            ys = [torch_dev.empty((M, n), device="cuda") for n in rows]
+            torch_dev.cuda.synchronize()
+            ctx.matmul_group(ts, xd, ys, act=1, biases=bd)
+            ctx.sync()
+            q, s = I.quantize(v)
+            for y, w, b in zip(ys, ws, bs):
+                same(y, I.product(q, s, *w, b))
+    for t in ts:
+        t.free()
+
+
+@pytest.mark.parametrize("M", [1, 20, 64, 200])
+def test_split_sums_are_joined(ctx, torch_dev, M):
+    """Few channels and a long K, which several workgroups share: groups, biases, strided 16-bit rows, then fewer columns in
+    a graph after the larger eager call."""
+    say("split K", M)
+    torch = torch_dev
+    rng = np.random.default_rng(M)
+    K, rows = 9000, [70, 5, 130]
+    ws, bs = [I.weights(rng, n, K) for n in rows], [rng.standard_normal(rows[0]).astype(np.float32), None, rng.standard_normal(rows[2]).astype(np.float32)]
+    import beglin_amd as B
+    stream = torch.cuda.Stream()
+    c = B.Context(0, stream.cuda_stream)
+    ts = [bind(c, w) for w in ws]
+    bd = [torch.from_numpy(b).cuda() if b is not None else None for b in bs]
+    q, s, qd, sd = codes(torch, rng, M, K)
+    for dt in (torch.float32, torch.bfloat16):
+        wide = torch.full((M, 301), 7.0, dtype=dt, device="cuda")
+        ys = [wide[:, 1:71], wide[:, 80:85], wide[:, 100:230]]
+        torch.cuda.synchronize()
+        c.matmul_i8(ts, qd, sd, ys, biases=bd)
+        c.sync()
+        want = torch.full((M, 301), 7.0)
+        for at, w, b in zip((1, 80, 100), ws, bs):
+            want[:, at:at + w[0].shape[0]] = torch.from_numpy(I.product(q[:, :K], s, *w, b))
+        assert torch.equal(wide.cpu(), want.to(dt))
+    m = (M + 1) // 2
+    y = torch.empty((m, rows[2]), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            c.matmul_i8(ts[2], qd[:m], sd[:m], y)
+    for r in range(3):
+        y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+            c.matmul_i8(ts[0], qd, sd, torch.empty((M, rows[0]), device="cuda"))       # eager work that uses the same sums
+        torch.cuda.synchronize()
+        same(y, I.product(q[:m, :K], s[:m], *ws[2]))
+    del graph
+    for t in ts:
+        t.free()
+    c.close()
+
+
 def test_columns_at_the_ends_of_fp32(ctx, torch_dev):
     """Zeros, subnormals, 1e38, infinities and NaN: a row that holds one of the last two gives NaN, the others nothing of it."""
     rng = np.random.default_rng(3)
