@@ -73,16 +73,18 @@ __device__ __forceinline__ float i8_out(int acc, float as, float ws) { return __
 // M fp32 rows to codes [M][ldq] (bytes K .. ldq zeroed) and scales [M]; u != null: the rows are h = silu(x) * u,
 // also written to h.  (bgl_norm.hip)
 int run_quant_rows(bgl_ctx *c, const float *x, const float *u, float *h, int M, int K, int8_t *xq, long ldq, float *xs);
-// n <= 4 tensors of the int8 kind over M columns of codes (bgl_i8.hip); y[i] rows ldy[i] values apart
+// n <= 4 tensors of the int8 kind over M columns of codes (bgl_i8.hip); y[i] rows ldy[i] values apart.  xf: fp32 columns in
+// place of the codes (run_i8_cols)
 int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
-           void *const *y, int y_type, const long *ldy, int M, const float *xf = nullptr);
+           void *const *y, int y_type, const long *ldy, int M, const float *xf = nullptr, bool glu = false);
 // M fp32 columns (u, h as run_quant_rows) quantized into the context's act_w / act_s; reuse: for
 // bgl_matmul_prepped_dev, as columns with one scale per token
 #define PREP_GQ_TOKEN -1
 int prep_i8_cols(bgl_ctx *c, const float *x, const float *u, float *h, int M, int K, bool reuse);
-// run_i8 over fp32 columns, quantized first
+// run_i8 over fp32 columns, quantized first; glu (M <= 64): Ts are gate and up of one h = silu(gate x) * up x, written to
+// y[0]
 int run_i8_cols(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x, const float *u, float *h, int M,
-                const float *const *bias, float *const *y);
+                const float *const *bias, float *const *y, bool glu = false);
 // bytes between the codes' rows in the context's scratch: whole 64-value units
 static inline long i8_ld_scratch(int K) { return ((long)K + 63) / 64 * 64; }
 // The routed FFN of K_Q8C experts (bgl_moe_i8.hip), shapes checked by the caller: routing given (rw null), or from the

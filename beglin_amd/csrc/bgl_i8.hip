@@ -31,6 +31,7 @@ struct I8Task {
 };
 struct I8Launch {
     I8Task t[BGL_MAX_TASKS];
+    int glu;                      // t[0] and t[1] are gate and up of one h = silu(gate x) * up x, written to t[0].y
     int ks;                       // slices of K (grid z); 1: the outputs are written at once
     int n, M, K16, y_type, vec;   // K16: K rounded up to 16; vec: four outputs of a lane go in one store
     const int8_t *xq;
@@ -96,16 +97,18 @@ __device__ __forceinline__ i8_f4 i8_bias(const I8Task &t, int r) {
 #define I8_S_RND 4            // F32: 4 values a thread this often at most
 template <int RB, int CB>
 constexpr int i8_s_waves() { return RB * CB <= 4 ? 16 : 8; }
-template <int RB, int CB, int D, bool F32>
+template <int RB, int CB, int D, bool F32, bool GLU>
 __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L) {
     extern __shared__ __align__(16) i8_i4 red[];               // [wave][RB * CB][64]; F32: codes [M][K + 16], a word a column
     constexpr int Q = RB * CB, G = I8_S_PART / Q;
     const int nw = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const I8Task t = i8_task(L, blockIdx.x);
+    constexpr int RP = GLU ? RB / 2 : RB;
+    const I8Task t = GLU ? L.t[0] : i8_task(L, blockIdx.x);
     const int m0 = blockIdx.y * 64;
-    const int rb0 = (blockIdx.x - t.blk0) * RB;                     // RB divides 4: the blocks lie in one tile
+    const int rb0 = (blockIdx.x - t.blk0) * RP;                     // RP divides 4: the blocks lie in one tile
     const int U0 = t.T.nunits * blockIdx.z / L.ks, U = t.T.nunits * (blockIdx.z + 1) / L.ks;
-    const uint8_t *wp = t.T.w + ((size_t)(rb0 >> 2) * t.T.cpr + (lane >> 4)) * 1024 + ((rb0 & 3) * 16 + (lane & 15)) * 16;
+    const size_t wo = ((size_t)(rb0 >> 2) * t.T.cpr + (lane >> 4)) * 1024 + ((rb0 & 3) * 16 + (lane & 15)) * 16;
+    const uint8_t *wp = t.T.w + wo, *wu = GLU ? L.t[1].T.w + wo : nullptr;
     const int8_t *xp[CB];
     const int kq = (lane >> 4) * 16;
     int8_t *const codes = (int8_t *)(red + min(nw * Q, I8_S_PART) * 64);
@@ -133,7 +136,7 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
         for (int s = 0; s < D; s++) {
             const int u = min(u0 + s * nw, U - 1);
 #pragma unroll
-            for (int i = 0; i < RB; i++) o.a[s][i] = *(const i8_u4 *)(wp + (size_t)u * 4096 + 256 * i);
+            for (int i = 0; i < RB; i++) o.a[s][i] = *(const i8_u4 *)((i < RP ? wp : wu) + (size_t)u * 4096 + 256 * (i % RP));
             const int k = min(64 * u + kq, L.K16 - 16);              // past the row: the weights are zero there
 #pragma unroll
             for (int j = 0; j < CB; j++)
@@ -210,13 +213,28 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
     if (wave < G) put(wave);
     __syncthreads();
     const int parts = min(nw, G);
-    for (int o = threadIdx.x; o < Q * 64; o += blockDim.x) {
+    for (int o = threadIdx.x; o < RP * CB * 64; o += blockDim.x) {
         const int l = o & 63, j = (o >> 6) % CB, i = (o >> 6) / CB;
         const int m = m0 + 16 * j + (l & 15), r = (rb0 + i) * 16 + 4 * (l >> 4);
         if (m >= L.M || r >= t.T.N) continue;
         i8_i4 s = {0, 0, 0, 0};
         for (int w = 0; w < parts; w++) s += red[(w * Q + i * CB + j) * 64 + l];
-        if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = s;
+        if constexpr (GLU) {
+            i8_i4 s2 = {0, 0, 0, 0};
+            for (int w = 0; w < parts; w++) s2 += red[(w * Q + (i + RP) * CB + j) * 64 + l];
+            const float as = F32 ? i8_scale(mx[m]).sc : L.xs[m];
+            const i8_f4 gs = i8_ws(t, r), us = i8_ws(L.t[1], r);
+            i8_f4 h;
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[e] = i8_swiglu(i8_out(s[e], as, gs[e]), i8_out(s2[e], as, us[e]));
+            float *y = (float *)t.y + (size_t)m * t.ldy + r;
+            if (L.vec && r + 4 <= t.T.N) *(i8_f4 *)y = h;
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (r + e < t.T.N) y[e] = h[e];
+            }
+        } else if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = s;
         else i8_store4(L, t, m, r, s, F32 ? i8_scale(mx[m]).sc : L.xs[m], i8_ws(t, r), i8_bias(t, r));
     }
 }
@@ -429,7 +447,7 @@ static bool f32_fits(int M, int K, int units, int ks) {
     return M <= 16 && K % 64 == 0 && M * (long)K <= (M == 1 ? 16384 : 8192) && M * (long)(K / 64) <= 4l * I8_S_RND * std::min(16, std::max(1, units / ks));
 }
 
-template <int RB, int CB>
+template <int RB, int CB, bool GLU>
 static void s_go(const I8Launch &L, int blocks, hipStream_t st) {
     constexpr int D = RB + CB <= 2 ? 4 : 2;
     const int nw = std::min(i8_s_waves<RB, CB>(), std::max(1, L.t[0].T.nunits / L.ks));
@@ -437,12 +455,14 @@ static void s_go(const I8Launch &L, int blocks, hipStream_t st) {
     const dim3 grid(blocks, (L.M + 63) / 64, L.ks);
     if constexpr (CB == 1)
         if (L.xf) {
-            hipLaunchKernelGGL((k_i8_s<RB, 1, D, true>), grid, dim3(nw * 64), lds + (size_t)L.M * (L.t[0].T.K + 16) + L.M * 4, st, L);
+            hipLaunchKernelGGL((k_i8_s<RB, 1, D, true, GLU>), grid, dim3(nw * 64), lds + (size_t)L.M * (L.t[0].T.K + 16) + L.M * 4, st, L);
             return;
         }
-    hipLaunchKernelGGL((k_i8_s<RB, CB, D, false>), grid, dim3(nw * 64), lds, st, L);
+    hipLaunchKernelGGL((k_i8_s<RB, CB, D, false, GLU>), grid, dim3(nw * 64), lds, st, L);
 }
+// workgroups of RB blocks of 16 channels; of a pair, half of them gate's
 static long s_blocks(I8Launch &L, int RB) {
+    if (L.glu) return ((L.t[0].T.N + 15) / 16 + RB / 2 - 1) / (RB / 2);
     long blocks = 0;
     for (int i = 0; i < L.n; i++) {
         L.t[i].blk0 = (int)blocks;
@@ -451,10 +471,17 @@ static long s_blocks(I8Launch &L, int RB) {
     return blocks;
 }
 static int run_s(bgl_ctx *c, I8Launch &L, int RB, int ks) {
-    const int rc = i8_split(c, L, ks), CB = std::min(4, (L.M + 15) / 16);
+    const int rc = L.glu ? 0 : i8_split(c, L, ks), CB = std::min(4, (L.M + 15) / 16);
     if (rc) return rc;
+    if (L.glu) L.ks = 1;
     const int blocks = (int)s_blocks(L, RB);
-#define GO(R, C) if (RB == R && CB == C) s_go<R, C>(L, blocks, c->stream)
+#define GO(R, C) if (RB == R && CB == C) s_go<R, C, true>(L, blocks, c->stream)
+    if (L.glu) {
+        GO(2, 1); GO(2, 2); GO(2, 3); GO(2, 4); GO(4, 1); GO(4, 2); GO(4, 3); GO(4, 4);
+        return 0;
+    }
+#undef GO
+#define GO(R, C) if (RB == R && CB == C) s_go<R, C, false>(L, blocks, c->stream)
     GO(1, 1); GO(1, 2); GO(1, 3); GO(1, 4); GO(2, 1); GO(2, 2); GO(2, 3); GO(2, 4); GO(4, 1); GO(4, 2); GO(4, 3); GO(4, 4);
 #undef GO
     return 0;
@@ -498,9 +525,9 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
     if (M <= 64) {
         int best = 0, bks = 1;
         double least = 1e30;
-        for (int RB = 1; RB <= 4; RB *= 2) {
+        for (int RB = L.glu ? 2 : 1; RB <= 4; RB *= 2) {
             const long blocks = s_blocks(L, RB);
-            for (int ks = 1; ks <= 8 && (ks == 1 || K / ks >= I8_SLICE); ks *= 2) {
+            for (int ks = 1; ks <= 8 && (ks == 1 || (!L.glu && K / ks >= I8_SLICE)); ks *= 2) {
                 if (L.xf && !f32_fits(M, K, L.t[0].T.nunits, ks)) break;
                 const double us = up(blocks * ks) * ((double)(16 * RB + M) * K / ks / 40e3 + 1.5) + join(ks);
                 if (us < least) { least = us; best = RB; bks = ks; }
@@ -525,10 +552,10 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
 }
 
 int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq, const float *xs, const float *const *bias,
-           void *const *y, int y_type, const long *ldy, int M, const float *xf) {
+           void *const *y, int y_type, const long *ldy, int M, const float *xf, bool glu) {
     I8Launch L;
     memset(&L, 0, sizeof L);
-    L.n = n; L.M = M; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
+    L.n = n; L.M = M; L.glu = glu; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
     L.xq = xq; L.ldq = ldq; L.xs = xs; L.xf = xf;
     L.vec = 1;
     int widest = 0;
@@ -565,15 +592,15 @@ int prep_i8_cols(bgl_ctx *c, const float *x, const float *u, float *h, int M, in
 }
 
 int run_i8_cols(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x, const float *u, float *h, int M,
-                const float *const *bias, float *const *y) {
+                const float *const *bias, float *const *y, bool glu) {
     void *yv[BGL_MAX_TASKS];
-    for (int i = 0; i < n; i++) yv[i] = y[i];
+    for (int i = 0; i < n; i++) yv[i] = y[glu ? 0 : i];
     if (!u && f32_fits(M, Ts[0].K, Ts[0].nunits, 1) && (uintptr_t)x % 16 == 0)
-        return run_i8(c, n, Ts, nullptr, 0, nullptr, bias, yv, BGL_T_F32, nullptr, M, x);
+        return run_i8(c, n, Ts, nullptr, 0, nullptr, bias, yv, BGL_T_F32, nullptr, M, x, glu);
     int rc = prep_i8_cols(c, x, u, h, M, Ts[0].K, false);
     if (rc) return rc;
     return run_i8(c, n, Ts, (const int8_t *)c->act_w.p, i8_ld_scratch(Ts[0].K), (const float *)c->act_s.p, bias, yv, BGL_T_F32,
-                  nullptr, M);
+                  nullptr, M, nullptr, glu);
 }
 
 extern "C" int bgl_matmul_i8_dev(bgl_ctx *c, int n, const bgl_tensor *const *w, const int8_t *xq, long ldq, const float *xs,

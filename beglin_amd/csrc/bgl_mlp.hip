@@ -65,6 +65,14 @@ extern "C" int bgl_mlp_dev(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor 
         }
         return run_mlp_q(c, gate->T, up->T, down->T, x_dev, hq, y_dev);
     }
+    // few columns of K_Q8C: the gate+up products form h themselves
+    if (act == BGL_ACT_W4A8 && gate->T.fmt == BGL_K_Q8C && up->T.fmt == BGL_K_Q8C && M <= 64) {
+        if (!h_dev && dbuf_reserve(c, c->mlp, n * 4, false)) return bgl_last_code();
+        float *hq = h_dev ? h_dev : (float *)c->mlp.p;
+        const BglDevTensor Ts[2] = {gate->T, up->T};
+        const int rc = run_i8_cols(c, 2, Ts, x_dev, nullptr, nullptr, M, nullptr, &hq, true);
+        return rc ? rc : bgl_matmul_dev(c, down, act, hq, nullptr, y_dev, M);
+    }
     // g and u side by side, then h unless the caller keeps it
     if (dbuf_reserve(c, c->mlp, n * 4 * (h_dev ? 2 : 3), false)) return bgl_last_code();
     float *g = (float *)c->mlp.p, *u = g + n, *h = h_dev ? h_dev : u + n;
