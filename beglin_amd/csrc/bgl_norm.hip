@@ -425,24 +425,41 @@ static void norm_go(const NormLaunch &L, hipStream_t st) {
     auto go = [&](auto kernel, int threads, int rows) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(((long)L.d.T + rows - 1) / rows)), dim3(threads), 0, st, L);
     };
-    // (4096 bf16 rows of 4096 with 16 values a thread 31.2 us, with 8 33.1; 2048 normed-twice rows of 8192 36.8 and 42.7)
+    // (4096 bf16 rows of 4096 with 16 values a thread 31.2 us, with 8 33.1; 2048 normed-twice rows of 8192 36.8 and 42.7; few
+    // rows wait for one row's passes: 1 of 4096 4.1 and 3.5, 300 5.9 and 5.6, 1024 9.0 and 9.4)
     const int H = L.d.H;
     if (H < 8) go(k_norm_wide, 1024, 1);
     else if (H <= 512) go(k_norm<64, 1, ROW>, 256, 4);
     else if (H <= 2048) go(k_norm<256, 1, ROW>, 256, 1);
+    else if (H <= 4096 && L.d.T <= 512) go(k_norm<512, 1, ROW>, 512, 1);
     else if (H <= 4096) go(k_norm<256, 2, ROW>, 256, 1);
     else if (H <= 8192) go(k_norm<512, 2, ROW>, 512, 1);
     else if (H <= 16384) go(k_norm<1024, 2, ROW>, 1024, 1);
     else go(k_norm_wide, 1024, 1);
 }
 
-static int norm_launch(bgl_ctx *c, const NormLaunch &L) {
-    const bgl_norm &d = L.d;
-    int tok = prof_begin(c, L.glu_u || d.kind == BGL_NORM_NONE ? 0 : 2);
-    if (L.glu_u) norm_go<ROW_GLU>(L, c->stream);
-    else if (!d.f) norm_go<ROW_X>(L, c->stream);
-    else if (d.post == BGL_NORM_NONE) norm_go<ROW_ADD>(L, c->stream);
-    else norm_go<ROW_POST>(L, c->stream);
+// A launch has less than 2^32 threads, and up to 1024 take a row.
+#define NORM_ROWS (1 << 21)
+static int norm_launch(bgl_ctx *c, const NormLaunch &all) {
+    const bgl_norm &a = all.d;
+    int tok = prof_begin(c, all.glu_u || a.kind == BGL_NORM_NONE ? 0 : 2);
+    for (long t = 0; t < a.T; t += NORM_ROWS) {
+        NormLaunch L = all;
+        bgl_norm &d = L.d;
+        d.T = (int)std::min<long>(NORM_ROWS, a.T - t);
+        auto at = [&](const void *p, long ld, int type) { return p ? const_cast<char *>((const char *)p) + t * ld * i8_elem(type) : nullptr; };
+        d.x = at(a.x, a.ldx, a.x_type);
+        d.f = at(a.f, a.ldf, a.f_type);
+        d.gate = at(a.gate, a.gate_t, a.f_type);
+        d.x_out = at(a.x_out, a.ldo, a.x_type);
+        d.y = at(a.y, a.ldy, a.y_type);
+        if (a.yq) { d.yq = a.yq + t * a.ldq; d.yscale = a.yscale + t; }
+        if (all.glu_u) L.glu_u = all.glu_u + t * a.ldx;
+        if (L.glu_u) norm_go<ROW_GLU>(L, c->stream);
+        else if (!d.f) norm_go<ROW_X>(L, c->stream);
+        else if (d.post == BGL_NORM_NONE) norm_go<ROW_ADD>(L, c->stream);
+        else norm_go<ROW_POST>(L, c->stream);
+    }
     prof_end(c, tok);
     HIPCHK(hipGetLastError());
     return 0;

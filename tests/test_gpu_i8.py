@@ -350,6 +350,27 @@ def test_captured_call(ctx, torch_dev, M):
     c.close()
 
 
+@pytest.mark.parametrize("M,N,K", [(70000, 33000, 64), (70000, 64, 65536)])
+def test_rows_past_4_gib(ctx, torch_dev, M, N, K):
+    """Outputs, then codes, of more than 2^32 bytes."""
+    say("past 4 GiB", M, N, K)
+    torch = torch_dev
+    rng = np.random.default_rng(N)
+    w = I.weights(rng, N, K)
+    t, y = bind(ctx, w), torch.full((M, N), 9.0, dtype=torch.float16, device="cuda")
+    q, s = torch.zeros((M, K), dtype=torch.int8, device="cuda"), torch.full((M,), 0.01, device="cuda")
+    some = np.array([0, 1, 32768, 65535, 65536, M - 1])
+    part = rng.integers(-20, 21, (len(some), K)).astype(np.int8)
+    q[torch.from_numpy(some).cuda()] = torch.from_numpy(part).cuda()
+    torch.cuda.synchronize()
+    ctx.matmul_i8(t, q, s, y)
+    ctx.sync()
+    want = torch.from_numpy(I.product(part, np.full(len(some), 0.01, np.float32), *w)).half()
+    assert torch.equal(y[torch.from_numpy(some).cuda()].cpu(), want)
+    assert int((y != 0).any(1).sum()) == len(some)
+    t.free()
+
+
 def test_noalloc(ctx, torch_dev):
     import ctypes as C
 

@@ -106,6 +106,22 @@ def test_given_routings(ctx, torch_dev, T):
         lay.free()
 
 
+def test_most_experts_and_picks(ctx, torch_dev):
+    """1024 experts, 16 a token, 64 tokens: as many experts as pairs."""
+    torch = torch_dev
+    E, K, H, W, T = 1024, 16, 64, 64, 64
+    lay = Layer(ctx, 6, E, H, W, 128)
+    x, w = lay.rng.standard_normal((T, H)).astype(np.float32), lay.rng.standard_normal((T, K)).astype(np.float32)
+    for idx in (lay.rng.permutation(E).reshape(T, K).astype(np.int32), lay.rng.integers(0, E, (T, K)).astype(np.int32)):
+        xd, wd, idd = (torch.from_numpy(v).cuda() for v in (x, w, idx))
+        out = torch.full((T, H), float("nan"), device="cuda")
+        torch.cuda.synchronize()
+        ctx.moe_ffn(*lay.stacks, lay.sh, xd, idd, wd, out)
+        ctx.check()
+        same(out, lay.want(x, idx, w))
+    lay.free()
+
+
 def test_rows_at_the_ends_of_fp32(ctx, torch_dev):
     """A token of NaN, infinities or zeros changes no other token's bits."""
     torch = torch_dev

@@ -62,6 +62,7 @@ CASES = [  # T, H, x, f, post, pre, gate, out, padding behind each row, w_add
     (2, 40000, "bfloat16", "float16", 1, 1, "channel", "bfloat16", 0, 0.0),
     (5000, 96, "bfloat16", "bfloat16", 0, 1, None, "bfloat16", 0, 0.0),     # more rows than a launch has workgroups
     (2500, 1536, "float32", "float32", 1, 1, "token", "float32", 0, 0.0),
+    (512, 4095, "bfloat16", "bfloat16", 0, 1, None, "bfloat16", 1, 0.0), (513, 2049, "float16", "float16", 2, 1, "full", "float16", 0, 0.0),
 ]
 
 
@@ -175,3 +176,41 @@ def test_non_finite_and_extreme_rows(ctx, torch_dev):
         assert np.isnan(got[3]).all() and np.isnan(s[3])
         assert np.isnan(got[4][1]) and not np.isfinite(s[4])
         assert not yq[3].any() and not yq[4].any()
+
+
+def test_rows_past_4_gib(ctx, torch_dev):
+    torch = torch_dev
+    T, H = 140000, 16384
+    x = torch.zeros((T, H), dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 65537, 131071, 131072, T - 1])
+    part = torch.from_numpy(np.random.default_rng(2).standard_normal((len(some), H)).astype(np.float32)).bfloat16()
+    x[some.cuda()] = part.cuda()
+    y, yq, ys = torch.empty_like(x), torch.empty((T, H), dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    torch.cuda.synchronize()
+    ctx.norm(x, y=y, yq=yq, yscale=ys)
+    ctx.sync()
+    want = I.normed(1, host(part))
+    near(y[some.cuda()], want, "y")
+    q, s = I.quantize(want.astype(np.float32))
+    assert np.array_equal(yq[some.cuda()].cpu().numpy(), q) and np.array_equal(ys[some.cuda()].cpu().numpy(), s)
+    assert int((y != 0).any(1).sum()) == len(some) == int((yq != 0).any(1).sum())
+
+
+def test_more_rows_than_a_launch_takes(ctx, torch_dev):
+    torch = torch_dev
+    T, H = (1 << 22) + 5, 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    rand = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    x, f, g = rand(T, H), rand(T, H).half(), rand(T, 1).half()
+    y, xo, yq, ys = torch.empty_like(x), torch.empty_like(x), torch.zeros((T, 16), dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    torch.cuda.synchronize()
+    ctx.norm(x, y=y, yq=yq, yscale=ys, x_out=xo, branch=f, gate=g)
+    ctx.sync()
+    v = (x.double() + f.double() * g.double()).float()
+    assert torch.equal(xo, v)
+    n = v.double() / (v.double().square().mean(-1, keepdim=True) + float(np.float32(1e-6))).sqrt()
+    assert ((y.double() - n).abs() <= n.abs() * (2.0 ** -24 * (1 + 1e-6)) + 1e-45).all()
+    # (a tensor of 127s: torch multiplies by 1 / 127, rounded, where the divisor is a Python number)
+    assert torch.equal(ys, y.abs().amax(-1) / torch.full_like(ys, 127.0))
+    # half a code, and up to 127 codes times the roundings of the scale, its inverse, the two products and the difference
+    assert ((yq[:, :H].float() * ys[:, None] - y).abs() <= ys[:, None] * (0.5 + 127 * 5 * 2.0 ** -24)).all()
