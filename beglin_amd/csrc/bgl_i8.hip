@@ -240,7 +240,7 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
 }
 
 // ================================================================================== many columns
-// Tiles of 16 CM NWM tokens by 16 CN NWN channels, NWM x NWN waves; both operands go through LDS in
+// Tiles of 16 CM NWM tokens by 16 CN NWN channels (128 x 128, 128 x 192, 256 x 256), NWM x NWN waves; both operands go through LDS in
 // two stages of 128 values of K, copied there without passing through registers (buffer loads to LDS).  A wave reads
 // the operands of half a stage from LDS while it multiplies the half before, so that its products wait neither for
 // LDS nor at the barrier, of which there is one a stage: between the halves, when every wave has read the whole stage
@@ -517,6 +517,8 @@ static int run_l(bgl_ctx *c, I8Launch &L, int ks) {
 //     24.8 / 13.1 / 12.1, 64 x 14336 x 4096 21.5 / 34.0 / 51.7
 //   k_i8_s with 64 x 64 outputs / 128 x 128 tiles / 256 x 256: 512 x 1536 x 1536 9.3 / 12.8 / 31.8, 2048 x 2048 x 2048
 //     34.8 / 17.9 / 37.9, 2048 x 14336 x 4096 369 / 157 / 146
+//   128 x 192 tiles / 128 x 128, where the last round of the latter leaves most CUs idle: 512 x 17920 x 1536 27.2 / 30.7,
+//     1500 x 6144 x 4096 49.1 / 59.5, 2048 x 8960 x 1536 44.2 / 48.8; where it does not: 512 x 14336 x 4096 52.7 / 43.3
 //   128 x 128 tiles with K in 1 / 4 slices: 1024 x 1536 x 8960 48.7 / 31.1, 128 x 8960 x 1536 14.0 / 19.9
 static int run_any(bgl_ctx *c, I8Launch &L) {
     const int K = L.t[0].T.K, M = L.M;
@@ -546,7 +548,10 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
     }
     const double c256 = 6.0 + 1.9 * ns * up(t256);
     const double c64 = 3.0 + (t64 <= I8_CUS ? 0.4 : 0.62 * up(t64)) * ns;
-    if (c64 <= c128 && c64 <= c256 && (M + 63) / 64 <= 65535) return run_s(c, L, 4, 1);
+    const double u192 = up(l_tiles(L, 128, 192));
+    const double c192 = 6.0 + (u192 == 2.0 ? 1.44 : 0.85 * u192) * ns;
+    if (c64 <= c128 && c64 <= c192 && c64 <= c256 && (M + 63) / 64 <= 65535) return run_s(c, L, 4, 1);
+    if (c192 < c128 && c192 <= c256) return run_l<4, 3, 2, 4>(c, L, 1);
     if (c128 <= c256) return run_l<4, 2, 2, 4>(c, L, ks);
     return run_l<8, 4, 2, 4>(c, L, 1);
 }

@@ -52,7 +52,8 @@ def codes(torch, rng, M, K, pad=0):
 SHAPES = [(1, 1, 1), (1, 64, 64), (1, 8960, 1536), (2, 17, 100), (3, 63, 127), (5, 65, 128), (16, 256, 129), (17, 1001, 1411),
           (31, 15, 16), (33, 4096, 500), (48, 130, 4096), (49, 9000, 192), (64, 1024, 14336), (64, 33000, 80), (12, 40000, 256),
           (20, 33000, 128), (65, 64, 64), (65, 1, 1), (100, 257, 255), (128, 512, 256), (129, 300, 1000), (255, 255, 384),
-          (256, 256, 4096), (257, 1030, 640), (333, 1001, 1411), (1000, 96, 2048), (640, 2600, 512), (2049, 520, 272)]
+          (256, 256, 4096), (257, 1030, 640), (333, 1001, 1411), (1000, 96, 2048), (640, 2600, 512), (2049, 520, 272), (1500, 6144, 1024),
+          (1411, 6001, 1090)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
