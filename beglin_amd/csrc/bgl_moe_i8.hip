@@ -10,8 +10,8 @@
 //
 // What bounds it is the experts' bytes: each touched expert is read once for up to 16 of its tokens (64 tokens
 // at the most; more go in chunks).  All of it is one launch, k_moe_i8, whose workgroups have four roles:
-//   i8_pre           codes of x; the router's scores, a wave an expert, and the softmax and top-K of a token by whichever
-//                    workgroup finishes its last score
+//   i8_pre           codes of x; the router's scores, a wave an expert, and the softmax and top-K of a token by
+//                    its last workgroup
 //   i8_gate_up       16-row blocks of both tensors, the shared experts' while the routing is made, then the used experts'
 //                    in equal runs, whose waves split K; the next block's operands are on their way while one is
 //                    multiplied.  Whoever finishes an expert's last block makes the codes of its h rows.
@@ -22,10 +22,10 @@
 // Workgroups wait only for ones with lower ids, and find their expert and its pairs from the routing themselves.  1024
 // threads with up to 128 registers fill a CU, so that equal shares take equal times (with 512 threads a CU often had two
 // workgroups of down and its neighbour none: 173 us for 32 tokens, and 161 as four launches).
-// 64 experts of 2048 x 1408, 6 a token, a shared 2816: 1 token 33 us (four launches 41), 8 tokens 81 (96), 32 tokens 130
+// 64 experts of 2048 x 1408, 6 a token, a shared 2816: 1 token 31 us (four launches 41), 8 tokens 76 (96), 32 tokens 129
 // (161), 64 tokens 153 (204).  32 tokens' gate and up move 4.9 TB/s, a large copy 5.1; what is above the bytes' time is the
-// routing (12 us from the first load to the last workgroup's list), the wait between the last h and its codes (8) and the
-// slowest CU's share.
+// routing (9 us at one token from the first load to the last workgroup's list, of which 2.4 the top-K), the codes between
+// the last h and down's products (6) and the slowest CU's share.
 #include <string.h>
 
 #include <algorithm>
@@ -54,14 +54,14 @@
 // What the workgroups of a launch tell each other.  Each flag holds the number of the last launch that set it.
 struct MoeI8Sync {
     int gave_up, pad[15];                // a wait ended at its limit (bgl_ctx_check)
-    int ticket[MOE_I8_TOK];              // workgroups of a token that have its scores; 0 between launches
     int codes[MOE_I8_TOK];               // a token's codes are there
-    int routed[MOE_I8_TOK];              // its experts are
     int shared[MOE_I8_GU_WGS];           // a gate+up workgroup's share of the shared experts is done
     int gu[MOE_I8_GU_WGS];               // all it does
     int sq[MOE_I8_SQ_WGS];               // codes of the shared experts' h are there
     int blocks[MOE_I8_PAIRS];            // 16-row blocks of a slot that are done; 0 between launches
     int gen[MOE_I8_WGS];                 // launches so far: the same in every element between launches
+    // values that carry the number of their launch in the upper half
+    uint64_t score[MOE_I8_TOK * ROUTE_MAXE], idx[MOE_I8_PAIRS], w[MOE_I8_PAIRS];
 };
 
 struct MoeI8Launch {
@@ -73,10 +73,9 @@ struct MoeI8Launch {
     int never, spin;                     // a test's launch whose waits give up; polls before a wait does
     MoeI8Sync *sync;
     const float *x, *rw, *rb;            // token rows; router
-    float *scores;                       // [T][E], null: idx / w are given
     int renorm;
-    int32_t *idx;                        // [P]
-    float *w;
+    const int32_t *idx;                  // [P] and their weights, or null: the router's, in sync
+    const float *w;
     int8_t *xq;
     float *xs;
     float *h, *hsh;                      // [P][I], [T][Ish]
@@ -93,6 +92,20 @@ __device__ __forceinline__ i8_f4 i8_get4(const float *p) {
     const uint64_t a = i8_get((const uint64_t *)p), b = i8_get((const uint64_t *)p + 1);
     return i8_f4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))};
 }
+// A value and the number of its launch in one store; and the wait for it, by one lane.
+__device__ __forceinline__ void i8_put_now(uint64_t *p, int gen, uint32_t v) { i8_put(p, (uint64_t)(uint32_t)gen << 32 | v); }
+__device__ __forceinline__ uint32_t i8_get_now(const MoeI8Launch &L, const uint64_t *p, int gen) {
+    for (int s = 0;;) {
+        const uint64_t v = i8_get(p);
+        if ((int)(v >> 32) == gen + L.never) return (uint32_t)v;
+        if (++s >= L.spin) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    i8_put(&L.sync->gave_up, 1);
+    return 0xffffffffu;
+}
+__device__ __forceinline__ int i8_idx(const MoeI8Launch &L, int p, int gen) { return L.idx ? L.idx[p] : (int)i8_get_now(L, L.sync->idx + p, gen); }
+__device__ __forceinline__ float i8_weight(const MoeI8Launch &L, int p, int gen) { return L.w ? L.w[p] : __uint_as_float(i8_get_now(L, L.sync->w + p, gen)); }
 // the workgroup's stores are in memory, and then its flag
 __device__ __forceinline__ void i8_done(int *flag, int gen) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -174,8 +187,8 @@ __device__ __forceinline__ void i8_row_codes(const float *x, int width, int8_t *
     for (int i = tid; i < n; i += MOE_I8_NT) i8_put(scale + row(i), i8_scale(mx[i]).sc);
 }
 
-// Workgroups [0, T): a token's codes.  The others: a wave an expert's score; a workgroup that finds its token's ticket to
-// be the last takes the softmax and the top-K.
+// Workgroups [0, T): a token's codes.  The others: a wave an expert's score; a token's last one takes the softmax and the
+// top-K when the others' scores are there.
 __device__ __forceinline__ void i8_pre(const MoeI8Launch &L, int b, int gen, uint8_t *lds) {
     const int tid = threadIdx.x, lane = tid & 63;
     if (b < L.T) {
@@ -184,30 +197,22 @@ __device__ __forceinline__ void i8_pre(const MoeI8Launch &L, int b, int gen, uin
         return;
     }
     const int per = (L.E + MOE_I8_NW - 1) / MOE_I8_NW, t = (b - L.T) / per, e = ((b - L.T) % per) * MOE_I8_NW + (tid >> 6);
-    int *const last = (int *)lds;
-    float *const lbuf = (float *)(lds + 16), *const sc = lbuf + ROUTE_MAXE;
+    float *const lbuf = (float *)lds, *const sc = lbuf + ROUTE_MAXE;
     if (e < L.E) {
         const double acc = route_dot_wave(L.rw + (size_t)e * L.H, L.x + (size_t)t * L.H, L.H, lane);
         const float s = L.rb ? __fadd_rn((float)acc, L.rb[e]) : (float)acc;
-        if (lane == 0) i8_put(L.scores + (size_t)t * L.E + e, s);
+        if (lane == 0) i8_put_now(L.sync->score + t * ROUTE_MAXE + e, gen, __float_as_uint(s));
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // a score is in memory before its workgroup's ticket is drawn
-    __syncthreads();
-    if (tid == 0) *last = __hip_atomic_fetch_add(L.sync->ticket + t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == per - 1;
-    __syncthreads();
-    if (!*last || tid >= 64) return;
-    for (int i = lane; i < L.E; i += 64) sc[i] = i8_get(L.scores + (size_t)t * L.E + i);
-    if (lane == 0) i8_put(L.sync->ticket + t, 0);              // for the next launch
+    if ((b - L.T) % per != per - 1 || tid >= 64) return;
+    for (int i = lane; i < L.E; i += 64) sc[i] = __uint_as_float(i8_get_now(L, L.sync->score + t * ROUTE_MAXE + i, gen));
     __builtin_amdgcn_wave_barrier();
     float sel_w;
     int sel_i;
     route_topk_wave(sc, L.E, L.K, L.renorm, lane, sel_i, sel_w, lbuf);
     if (lane < L.K) {
-        i8_put(L.idx + t * L.K + lane, sel_i);
-        i8_put(L.w + t * L.K + lane, sel_w);
+        i8_put_now(L.sync->idx + t * L.K + lane, gen, (uint32_t)sel_i);
+        i8_put_now(L.sync->w + t * L.K + lane, gen, __float_as_uint(sel_w));
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (lane == 0) i8_put(L.sync->routed + t, gen);
 }
 
 // ------------------------------------------------------------------ the routing in LDS
@@ -222,12 +227,12 @@ struct MoeI8Route {
     uint32_t used[32], base[32];         // experts that have a pair (E <= 1024), slots before each 32 of them
     int n;                               // slots
 };
-__device__ __forceinline__ void i8_routing(const MoeI8Launch &L, MoeI8Route &R) {
+__device__ __forceinline__ void i8_routing(const MoeI8Launch &L, MoeI8Route &R, int gen) {
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63;
     // few pairs: a lane each, without the barriers
     if (L.P <= MOE_I8_FEW) {
         if (tid < 64) {
-            const int got = lane < L.P ? i8_get(L.idx + lane) : -1, e = got >= 0 && got < L.E ? got : 0x7fffffff;
+            const int got = lane < L.P ? i8_idx(L, lane, gen) : -1, e = got >= 0 && got < L.E ? got : 0x7fffffff;
             int s = 0, less = 0, n = 0;
             uint64_t same = 0;
             for (int p = 0; p < L.P; p++) {
@@ -258,7 +263,7 @@ __device__ __forceinline__ void i8_routing(const MoeI8Launch &L, MoeI8Route &R) 
     for (int s = tid; s < L.nslots; s += nt) R.at[s] = 0;
     __syncthreads();
     for (int p = tid; p < L.P; p += nt) {
-        const int e = i8_get(L.idx + p);
+        const int e = i8_idx(L, p, gen);
         R.slot[p] = e >= 0 && e < L.E ? (uint16_t)e : (uint16_t)MOE_I8_NONE;     // the expert, for now
         if (e >= 0 && e < L.E) atomicOr(&R.used[e >> 5], 1u << (e & 31));
     }
@@ -403,8 +408,7 @@ __device__ __forceinline__ void i8_gate_up(const MoeI8Launch &L, int b, int gen,
             for (int c0 = 0; c0 < L.T; c0 += 16) i8_gu(L, L.sg, L.su, rb0, rb1, nullptr, c0, L.T, L.hsh, L.Ish, red, par);
         i8_done(L.sync->shared + b, gen);
     }
-    if (L.scores) i8_wait(L, L.sync->routed, L.T, gen);
-    i8_routing(L, R);
+    i8_routing(L, R, gen);
     const int per = L.I / 16;
     const long all = (long)__builtin_amdgcn_readfirstlane(R.n) * per;
     const int begin = (int)(all * b / L.ngu), end = (int)(all * (b + 1) / L.ngu);
@@ -470,8 +474,7 @@ __device__ __forceinline__ void i8_down(const MoeI8Launch &L, int rb, int gen, M
     const int rows = L.P + (L.shared ? L.T : 0), tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     for (int i = tid; i < rows * 8; i += MOE_I8_NT) sums[i] = 0;
-    if (L.scores) i8_wait(L, L.sync->routed, L.T, gen);
-    i8_routing(L, R);
+    i8_routing(L, R, gen);
     const int nslots = __builtin_amdgcn_readfirstlane(R.n);
     for (int s = tid; s < nslots; s += MOE_I8_NT) {
         tw[s] = L.td[R.expert[s]].w;
@@ -544,7 +547,7 @@ __device__ __forceinline__ void i8_down(const MoeI8Launch &L, int rb, int gen, M
         if (s == MOE_I8_NONE) continue;
         const float ws = mi_float((i8_gp)(sh ? (const float *)L.sd.s0 : ts[s]), r);
         const float v = i8_out(sums[i], i8_get(L.hs + row), ws);
-        sums[i] = __float_as_int(sh ? v : __fmul_rn(i8_get(L.w + row), v));
+        sums[i] = __float_as_int(sh ? v : __fmul_rn(i8_weight(L, row, gen), v));
     }
     __syncthreads();
     for (int o = tid; o < L.T * 8; o += MOE_I8_NT) {
@@ -594,8 +597,7 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) & ~(size_t)255; return o; };
     L.hp = (L.H + 127) & ~127; L.ip = (L.I + 127) & ~127; L.ishp = (L.Ish + 127) & ~127;
     const size_t o_hs = take(rows * 4), o_xs = take((size_t)most * 4), o_xq = take((size_t)most * L.hp), o_h = take(P * L.I * 4),
-                 o_hsh = take((size_t)most * L.Ish * 4), o_hq = take(P * L.ip), o_hshq = take((size_t)most * L.ishp),
-                 o_idx = take(P * 4), o_w = take(P * 4), o_sc = take((size_t)most * L.E * 4);
+                 o_hsh = take((size_t)most * L.Ish * 4), o_hq = take(P * L.ip), o_hshq = take((size_t)most * L.ishp);
     if (dbuf_reserve(c, c->moe_g, at, false) || dbuf_reserve(c, c->moe_sync, sizeof(MoeI8Sync), true)) return bgl_last_code();
     L.sync = (MoeI8Sync *)c->moe_sync.p;
     uint8_t *base = (uint8_t *)c->moe_g.p;
@@ -609,9 +611,8 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
         L.nslots = std::min(L.E, L.P);
         L.x = x + (size_t)t0 * L.H;
         L.out = out + (size_t)t0 * L.H;
-        L.scores = rw ? (float *)(base + o_sc) : nullptr;
-        L.idx = rw ? (int32_t *)(base + o_idx) : const_cast<int32_t *>(idx) + (size_t)t0 * K;
-        L.w = rw ? (float *)(base + o_w) : const_cast<float *>(w) + (size_t)t0 * K;
+        L.idx = rw ? nullptr : idx + (size_t)t0 * K;
+        L.w = rw ? nullptr : w + (size_t)t0 * K;
         L.never = c->mlp_test_timeout > 0 ? 1 : 0;                  // a test's launch whose waits must give up
         if (c->mlp_test_timeout > 0) c->mlp_test_timeout--;
         L.npre = L.T + (rw ? L.T * ((L.E + MOE_I8_NW - 1) / MOE_I8_NW) : 0);
@@ -627,10 +628,9 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
     return 0;
 }
 
-// After a wait gave up, workgroups may have counted by different routings: the counts begin at 0 again (the stream is idle).
+// After a wait gave up, workgroups may have counted blocks by different routings: the counts begin at 0 again (the stream is idle).
 int moe_i8_recount(bgl_ctx *c) {
     MoeI8Sync *s = (MoeI8Sync *)c->moe_sync.p;
-    HIPCHK(hipMemset(s->ticket, 0, sizeof s->ticket));
     HIPCHK(hipMemset(s->blocks, 0, sizeof s->blocks));
     return 0;
 }

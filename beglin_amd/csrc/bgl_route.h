@@ -74,20 +74,26 @@ __device__ __forceinline__ void route_topk_wave(const float *__restrict__ sc_t, 
     for (; e16 < E; e16++) sum += (double)lbuf[e16];
     sel_i = 0;
     sel_w = 0.0f;
-    unsigned used = 0;                                       // bit j: expert lane + 64j selected
 #pragma unroll
-    for (int j = 0; j < PL; j++) v[j] = (float)((double)v[j] / sum);
+    for (int j = 0; j < PL; j++) {
+        if (64 * j < E) v[j] = (float)((double)v[j] / sum);
+        if (!(lane + 64 * j < E && v[j] >= 0.0f)) v[j] = -1.0f;     // not there, or NaN: never picked
+    }
     for (int k = 0; k < K; k++) {
-        // this lane's best unselected expert (lowest id first among equal values), then the wave's
-        float bv = -1.0f;
+        // the wave's largest value left, of the lowest expert that has it; none left: -1 and no expert
+        float bv = v[0];
+#pragma unroll
+        for (int j = 1; j < PL; j++) bv = fmaxf(bv, v[j]);
+        bv = wave_max_f32(bv);
         int bi = 0x7fffffff;
 #pragma unroll
-        for (int j = 0; j < PL; j++) {
-            const int e = lane + 64 * j;
-            if (e < E && !((used >> j) & 1u) && v[j] > bv) { bv = v[j]; bi = e; }
+        for (int j = PL - 1; j >= 0; j--) {
+            const uint64_t m = __builtin_amdgcn_ballot_w64(v[j] == bv);
+            if (m != 0 && bv >= 0.0f) bi = 64 * j + __builtin_ctzll(m);
         }
-        wave_argmax(bv, bi);                                  // DPP and readlane: no LDS round trips
-        if ((bi & 63) == lane) used |= 1u << (bi >> 6);
+#pragma unroll
+        for (int j = 0; j < PL; j++)
+            if (lane + 64 * j == bi) v[j] = -1.0f;
         if (lane == k) { sel_w = bv; sel_i = bi; }
     }
     if (renorm) {
