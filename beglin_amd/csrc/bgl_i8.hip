@@ -252,7 +252,7 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
 // of 64 values, four of them, took as long for the copies alone as the products do: a copy of 64-byte pieces of 16 rows
 // moves half of what one of 128-byte pieces does (4096 x 4096 x 14336: 206 us so, 190 now).
 //
-// 256 x 256 tiles: 8192 x 8192 x 8192 in 464 us, 2.37 POP/s (the library's int8 product: 474 us); a wave's products
+// 256 x 256 tiles: 8192 x 8192 x 8192 in 438 us, 2.51 POP/s (the library's int8 product: 474 us); a wave's products
 // without copies and reads would take 262 us at the clock that the card holds there (2.0 GHz).
 typedef unsigned int i8_rsrc __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i8_rsrc i8_mkrsrc(const void *p, uint32_t bytes) {
@@ -375,17 +375,26 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
         half(1, sm + (SB - cur), s + 2 < ns, s + 2, lds0 + cur);              // (the last stage reads what lies there)
         cur = SB - cur;
     }
+    // a token's channels one after the other: the pieces of a line meet in the L2 (the other way round 4096 x 14336 bf16
+    // outputs were 224 MB of writes, and are their 117 so: 270 us -> 242)
+    i8_f4 ws[CN], bias[CN];
 #pragma unroll
     for (int j = 0; j < CN; j++) {
-        const int r = n0 + (wn * CN + j) * 16 + 4 * (lane >> 4);
-        if (r >= t.T.N) continue;
-        const i8_f4 ws = i8_ws(t, r), bias = i8_bias(t, r);
+        const int r = min(n0 + (wn * CN + j) * 16 + 4 * (lane >> 4), t.T.ntiles * 64 - 4);
+        ws[j] = i8_ws(t, r);
+        bias[j] = i8_bias(t, r);
+    }
 #pragma unroll
-        for (int i = 0; i < CM; i++) {
-            const int m = m0 + (wm * CM + i) * 16 + (lane & 15);
-            if (m >= L.M) continue;
+    for (int i = 0; i < CM; i++) {
+        const int m = m0 + (wm * CM + i) * 16 + (lane & 15);
+        if (m >= L.M) continue;
+        const float as = L.ks > 1 ? 0.0f : L.xs[m];
+#pragma unroll
+        for (int j = 0; j < CN; j++) {
+            const int r = n0 + (wn * CN + j) * 16 + 4 * (lane >> 4);
+            if (r >= t.T.N) continue;
             if (L.ks > 1) *(i8_i4 *)(t.part + ((size_t)blockIdx.z * L.M + m) * i8_np(t.T.N) + r) = acc[i][j];
-            else i8_store4(L, t, m, r, acc[i][j], L.xs[m], ws, bias);
+            else i8_store4(L, t, m, r, acc[i][j], as, ws[j], bias[j]);
         }
     }
 }
@@ -516,9 +525,9 @@ static int run_l(bgl_ctx *c, I8Launch &L, int ks) {
 //     8.0 / 6.5 / 5.5, 64 x 14336 x 4096 40.8 / 26.6 / 21.0; 64 with K in 1 / 4 / 8 slices: 64 x 1536 x 8960
 //     24.8 / 13.1 / 12.1, 64 x 14336 x 4096 21.5 / 34.0 / 51.7
 //   k_i8_s with 64 x 64 outputs / 128 x 128 tiles / 256 x 256: 512 x 1536 x 1536 9.3 / 12.8 / 31.8, 2048 x 2048 x 2048
-//     34.8 / 17.9 / 37.9, 2048 x 14336 x 4096 369 / 157 / 146
-//   128 x 192 tiles / 128 x 128, where the last round of the latter leaves most CUs idle: 512 x 17920 x 1536 27.2 / 30.7,
-//     1500 x 6144 x 4096 49.1 / 59.5, 2048 x 8960 x 1536 44.2 / 48.8; where it does not: 512 x 14336 x 4096 52.7 / 43.3
+//     34.8 / 16.4 / 33.3, 2048 x 14336 x 4096 369 / 153 / 126
+//   128 x 192 tiles / 128 x 128, where the last round of the latter leaves most CUs idle: 512 x 17920 x 1536 24.6 / 29.4,
+//     1500 x 6144 x 4096 45.5 / 59.0, 2048 x 8960 x 1536 38.1 / 44.6; where it does not: 512 x 14336 x 4096 50.8 / 41.7
 //   128 x 128 tiles with K in 1 / 4 slices: 1024 x 1536 x 8960 48.7 / 31.1, 128 x 8960 x 1536 14.0 / 19.9
 static int run_any(bgl_ctx *c, I8Launch &L) {
     const int K = L.t[0].T.K, M = L.M;
