@@ -565,7 +565,8 @@ __device__ __forceinline__ void i8_down(const MoeI8Launch &L, int rb, int gen, M
 __global__ __launch_bounds__(MOE_I8_NT, 4) void k_moe_i8(MoeI8Launch L) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeI8Route R;
-    const int b = blockIdx.x, gen = L.sync->gen[b] + 1, gu = b - L.npre, sq = gu - L.ngu, rb = sq - L.nsq;
+    const int b = blockIdx.x, gu = b - L.npre, sq = gu - L.ngu, rb = sq - L.nsq;
+    const int gen = max(1u, (uint32_t)L.sync->gen[b] + 1u);    // 0: what was never set
     if (gu < 0) i8_pre(L, b, gen, lds);
     else if (sq < 0) i8_gate_up(L, gu, gen, R, lds);
     else if (rb < 0) i8_shared_codes(L, sq, gen, lds);

@@ -53,7 +53,8 @@ SHAPES = [  # E, K, H, W, Wsh, T
     (4, 1, 64, 64, 0, 1), (8, 2, 128, 192, 64, 1), (64, 6, 512, 320, 640, 1), (8, 8, 192, 128, 128, 2), (16, 3, 256, 448, 0, 3),
     (64, 6, 256, 320, 128, 4), (60, 4, 320, 1408, 704, 5), (16, 4, 128, 64, 64, 8), (33, 2, 192, 256, 0, 9), (64, 6, 320, 192, 256, 16),
     (7, 3, 64, 128, 64, 17), (64, 8, 128, 128, 128, 33), (3, 3, 128, 64, 192, 64), (2, 1, 64, 64, 0, 64), (16, 16, 64, 128, 64, 64),
-    (8, 2, 64, 64, 64, 65), (16, 5, 128, 64, 0, 130), (256, 8, 64, 64, 64, 12)]
+    (8, 2, 64, 64, 64, 65), (16, 5, 128, 64, 0, 130), (256, 8, 64, 64, 64, 12),
+    (3, 2, 16448, 64, 64, 3), (3, 2, 64, 16448, 8256, 5), (4, 2, 64, 192, 33024, 2)]
 
 
 @pytest.mark.parametrize("E,K,H,W,Wsh,T", SHAPES)
@@ -214,6 +215,48 @@ def test_launches_of_changing_sizes(ctx, torch_dev):
                 same(torch.from_numpy(o), lay.want(x.cpu().numpy(), idx.cpu().numpy(), w.cpu().numpy()))
         assert all(np.array_equal(a.view(np.uint32), b.view(np.uint32)) for a, b in zip(first, outs)), r
     lay.free()
+
+
+@pytest.mark.parametrize("T", [1, 9, 40])
+def test_layers_back_to_back(torch_dev, T):
+    """Launches with nothing between them, in one graph, whose codes and sums lie in the same scratch: each reads its own."""
+    import beglin_amd as B
+    torch = torch_dev
+    E, K, H, W, N = 12, 3, 512, 320, 8
+    stream = torch.cuda.Stream()
+    c = B.Context(0, stream.cuda_stream)
+    lay = Layer(c, [8, T], E, H, W, 384)
+    rw = torch.from_numpy((lay.rng.standard_normal((E, H)) / H ** 0.5).astype(np.float32)).cuda()
+    xs, outs = [torch.zeros((T, H), device="cuda") for _ in range(N)], [torch.zeros((T, H), device="cuda") for _ in range(N)]
+    idx, w = torch.empty((T, K), dtype=torch.int32, device="cuda"), torch.empty((T, K), device="cuda")
+    torch.cuda.synchronize()
+
+    def step():
+        for x, o in zip(xs, outs):
+            c.moe_layer(rw, *lay.stacks, lay.sh, x, K, o)
+
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for r in range(3):
+        for x in xs:
+            x.copy_(torch.from_numpy(lay.rng.standard_normal((T, H)).astype(np.float32)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay() if r != 1 else step()
+        torch.cuda.synchronize()
+        c.check()
+        for x, o in zip(xs, outs):
+            with torch.cuda.stream(stream):
+                c.moe_route(rw, x, K, idx, w)
+            c.sync()
+            same(o, lay.want(x.cpu().numpy(), idx.cpu().numpy(), w.cpu().numpy()))
+    del graph
+    lay.free()
+    c.close()
 
 
 def test_two_contexts_at_once(torch_dev):
