@@ -33,7 +33,7 @@ struct I8Launch {
     I8Task t[BGL_MAX_TASKS];
     int glu;                      // t[0] and t[1] are gate and up of one h = silu(gate x) * up x, written to t[0].y
     int ks;                       // slices of K (grid z); 1: the outputs are written at once
-    int n, M, K16, y_type, vec;   // K16: K rounded up to 16; vec: four outputs of a lane go in one store
+    int n, M, K16, y_type;        // K16: K rounded up to 16
     const int8_t *xq;
     long ldq;
     const float *xs;
@@ -54,6 +54,10 @@ __device__ __forceinline__ I8Task i8_task(const I8Launch &L, int blk) {
     return t;
 }
 
+// Four outputs of a lane in one store, wherever their row begins (gfx950 stores 8 and 16 bytes at any address; as single
+// values the outputs of 3101 x 8030 x 523, whose rows begin off 8 bytes, took 64 us in all, 42 so).
+typedef float i8_sf4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int i8_su2 __attribute__((ext_vector_type(2), aligned(2)));
 // Four neighbouring channels r .. r + 3 of token m.
 __device__ __forceinline__ void i8_store4(const I8Launch &L, const I8Task &t, int m, int r, i8_i4 acc, float as, i8_f4 ws, i8_f4 b) {
     float v[4];
@@ -64,11 +68,11 @@ __device__ __forceinline__ void i8_store4(const I8Launch &L, const I8Task &t, in
         for (int i = 0; i < 4; i++) v[i] = __fadd_rn(v[i], b[i]);
     }
     const size_t at = (size_t)m * t.ldy + r;
-    if (L.vec && r + 4 <= t.T.N) {
-        if (L.y_type == BGL_T_F32) *(i8_f4 *)((float *)t.y + at) = i8_f4{v[0], v[1], v[2], v[3]};
+    if (r + 4 <= t.T.N) {
+        if (L.y_type == BGL_T_F32) *(i8_sf4 *)((float *)t.y + at) = i8_sf4{v[0], v[1], v[2], v[3]};
         else
-            *(uint2 *)((uint16_t *)t.y + at) = make_uint2((uint32_t)i8_h16(v[0], L.y_type) | ((uint32_t)i8_h16(v[1], L.y_type) << 16),
-                                                          (uint32_t)i8_h16(v[2], L.y_type) | ((uint32_t)i8_h16(v[3], L.y_type) << 16));
+            *(i8_su2 *)((uint16_t *)t.y + at) = i8_su2{(uint32_t)i8_h16(v[0], L.y_type) | ((uint32_t)i8_h16(v[1], L.y_type) << 16),
+                                                       (uint32_t)i8_h16(v[2], L.y_type) | ((uint32_t)i8_h16(v[3], L.y_type) << 16)};
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -228,7 +232,7 @@ __global__ __launch_bounds__((i8_s_waves<RB, CB>() * 64)) void k_i8_s(I8Launch L
 #pragma unroll
             for (int e = 0; e < 4; e++) h[e] = i8_swiglu(i8_out(s[e], as, gs[e]), i8_out(s2[e], as, us[e]));
             float *y = (float *)t.y + (size_t)m * t.ldy + r;
-            if (L.vec && r + 4 <= t.T.N) *(i8_f4 *)y = h;
+            if (r + 4 <= t.T.N) *(i8_sf4 *)y = i8_sf4{h[0], h[1], h[2], h[3]};
             else {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
@@ -571,7 +575,6 @@ int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq
     memset(&L, 0, sizeof L);
     L.n = n; L.M = M; L.glu = glu; L.K16 = (Ts[0].K + 15) & ~15; L.y_type = y_type;
     L.xq = xq; L.ldq = ldq; L.xs = xs; L.xf = xf;
-    L.vec = 1;
     int widest = 0;
     for (int i = 0; i < n; i++) {
         I8Task &t = L.t[i];
@@ -580,7 +583,6 @@ int run_i8(bgl_ctx *c, int n, const BglDevTensor *Ts, const int8_t *xq, long ldq
         t.y = y[i];
         t.ldy = ldy ? ldy[i] : Ts[i].N;
         widest = std::max(widest, Ts[i].N);
-        if (((uintptr_t)t.y | (uintptr_t)t.ldy * i8_elem(y_type)) % (4 * i8_elem(y_type))) L.vec = 0;
     }
     int tok = prof_begin(c, 1);
     const int rc = run_any(c, L);
