@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256) void k_i8_join(I8Launch L) {
 // ================================================================================== host side
 #define I8_CUS 256
 #define I8_SLICE 512          // values of K that a slice has at least
-#define I8_JOIN 1.6e6         // bytes of slices' sums that are written and joined in a us
+#define I8_JOIN 3.2e6         // bytes of slices' sums that are written and joined in a us
 // Room for the slices' sums, the same for every call that could split K at its or at fewer columns, so that those may
 // be captured after it.  A choice that does not fit (many columns in many slices, which would cost more than they give)
 // keeps K whole.
