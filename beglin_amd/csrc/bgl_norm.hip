@@ -46,11 +46,12 @@ typedef unsigned int nr_u4 __attribute__((ext_vector_type(4), aligned(2)));
 // A thread's values of a row of at least 8: NV chunks of 8 consecutive ones, NT chunks apart.  A chunk that the row's
 // end cuts, or that lies behind it, loads the row's last 8 values instead and shifts its own to the front (values past
 // the end are 0 and stay so): every load is a full one and none is conditional.
+// NT: threads of a row, or 0: as many as the workgroup has.
 template <int NT, int NV>
 struct RowMap {
     static constexpr int N = 8 * NV;
     int lt, H;
-    __device__ __forceinline__ int at(int i) const { return (i * NT + lt) * 8; }
+    __device__ __forceinline__ int at(int i) const { return (i * (NT ? NT : (int)blockDim.x) + lt) * 8; }
     __device__ __forceinline__ int has(int i) const { return H - at(i); }        // values of chunk i that exist (>= 8: all)
     // An access is a uniform address plus the thread's 32-bit offset: no address registers per pointer and value.
     template <typename V>
@@ -186,36 +187,36 @@ __device__ __forceinline__ double row16_sum(double v) {
     v += dpp_d<0x141>(v);
     return v + dpp_d<0x140>(v);
 }
-// Sums over the NT threads of a row, in every one of them, in one order whatever the launch.
-template <int NT>
+// Sums over the threads of a row (a wave, or with WG the workgroup), in every one of them, in one order whatever the launch.
+template <bool WG>
 __device__ __forceinline__ double row_sum(double v, double *red) {
     v = row16_sum(v);
     v = (rlane_d(v, 0) + rlane_d(v, 16)) + (rlane_d(v, 32) + rlane_d(v, 48));
-    if constexpr (NT > 64) {
+    if constexpr (WG) {
         __syncthreads();                       // the last round's reads are done
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         // lane l % 16 takes wave l % 16's sum (0 past the last wave)
         const int w = threadIdx.x & 15;
-        v = rlane_d(row16_sum(w < NT / 64 ? red[w] : 0.0), 0);
+        v = rlane_d(row16_sum(w < (int)(blockDim.x >> 6) ? red[w] : 0.0), 0);
     }
     return v;
 }
-template <int NT>
+template <bool WG>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, double *red) {
     v = wave_max_u32(v);
-    if constexpr (NT > 64) {
+    if constexpr (WG) {
         uint32_t *r = (uint32_t *)red;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = wave_max_u32(r[threadIdx.x & (NT / 64 - 1)]);
+        v = wave_max_u32(r[threadIdx.x & ((blockDim.x >> 6) - 1)]);
     }
     return v;
 }
 
 // mean and 1 / sqrt(... + eps) of a norm over the thread's values (0 past the row's end); rows: 1 / H
-template <int NT, typename Map>
+template <bool WG, typename Map>
 __device__ __forceinline__ void norm_stats(int kind, const float (&v)[Map::N], const Map &m, float eps, double rows, double *red,
                                            double &mean, double &inv) {
     mean = 0.0;
@@ -224,7 +225,7 @@ __device__ __forceinline__ void norm_stats(int kind, const float (&v)[Map::N], c
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < Map::N; k++) s += (double)v[k];
-        mean = row_sum<NT>(s, red) * rows;
+        mean = row_sum<WG>(s, red) * rows;
 #pragma unroll
         for (int i = 0; i < Map::N / 8; i++) {
             const int n = m.has(i);
@@ -238,23 +239,23 @@ __device__ __forceinline__ void norm_stats(int kind, const float (&v)[Map::N], c
 #pragma unroll
         for (int k = 0; k < Map::N; k++) q = fma((double)v[k], (double)v[k], q);
     }
-    inv = rsqrt(row_sum<NT>(q, red) * rows + (double)eps);
+    inv = rsqrt(row_sum<WG>(q, red) * rows + (double)eps);
 }
 
+// NT 64: a wave a row, four in a workgroup of 256; 0: a workgroup a row, of as many threads as it has (one kernel for 256,
+// 512 and 1024: as fast as one each, within a twentieth for rows normed twice).
 template <int NT, int NV, int ROW>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormLaunch L) {
-    constexpr int RPW = NT < 256 ? 256 / NT : 1;
+__global__ __launch_bounds__(NT ? 256 : 1024) void k_norm(NormLaunch L) {
+    constexpr bool WG = NT != 64;
     using Map = RowMap<NT, NV>;
     constexpr int N = Map::N;
     const bgl_norm &d = L.d;
-    __shared__ double reds[RPW][16];
-    const int sub = NT < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
-    double *const red = reds[sub];
-    const Map m{(int)threadIdx.x % NT, d.H};
-    static_assert(NT == 64 || NT >= 256, "a row is a wave's or a workgroup's");
+    __shared__ double red[16];
+    const int sub = WG ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Map m{WG ? (int)threadIdx.x : (int)(threadIdx.x & 63), d.H};
     const double rows = 1.0 / d.H;
-    const long row = (long)blockIdx.x * RPW + sub;
-    if (row >= d.T) return;                                  // whole waves (RPW > 1: no barrier follows)
+    const long row = (long)blockIdx.x * (WG ? 1 : 4) + sub;
+    if (row >= d.T) return;                                  // whole waves, which meet no barrier
     {
         float v[N], f[N];
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormLaunch L) {
 #pragma unroll
             for (int i = 0; i < NV; i++) m.load(f + 8 * i, i, norm_row(d.f, row, d.ldf, d.f_type), d.f_type);
             double mean = 0.0, inv = 1.0;
-            if constexpr (ROW == ROW_POST) norm_stats<NT>(d.post, f, m, d.post_eps, rows, red, mean, inv);
+            if constexpr (ROW == ROW_POST) norm_stats<WG>(d.post, f, m, d.post_eps, rows, red, mean, inv);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 float *const vi = v + 8 * i;
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormLaunch L) {
         if (!d.y && !d.yq) return;
         if (d.kind != BGL_NORM_NONE) {
             double mean, inv;
-            norm_stats<NT>(d.kind, v, m, d.eps, rows, red, mean, inv);
+            norm_stats<WG>(d.kind, v, m, d.eps, rows, red, mean, inv);
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 double n[8];
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormLaunch L) {
             uint32_t mb = I8_MX0;
 #pragma unroll
             for (int k = 0; k < N; k++) mb = max(mb, __float_as_uint(v[k]) & 0x7fffffffu);
-            const I8Scale s = i8_scale(row_max<NT>(mb, red));
+            const I8Scale s = i8_scale(row_max<WG>(mb, red));
             if (m.lt == 0) d.yscale[row] = s.sc;
             int8_t *q = d.yq + (size_t)row * d.ldq;
             const int H16 = (d.H + 15) & ~15;              // the bytes up to the row's next multiple of 16 are zeroed
@@ -356,14 +357,14 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
             if (d.post == BGL_NORM_LAYER) {
                 double s = 0.0;
                 for (int h = tid; h < d.H; h += 1024) s += (double)i8_ld(d.f, d.f_type, (size_t)row * d.ldf + h);
-                fmean = row_sum<1024>(s, red) / d.H;
+                fmean = row_sum<true>(s, red) / d.H;
             }
             double q = 0.0;
             for (int h = tid; h < d.H; h += 1024) {
                 const double t = (double)i8_ld(d.f, d.f_type, (size_t)row * d.ldf + h) - fmean;
                 q = fma(t, t, q);
             }
-            finv = 1.0 / sqrt(row_sum<1024>(q, red) / d.H + (double)d.post_eps);
+            finv = 1.0 / sqrt(row_sum<true>(q, red) / d.H + (double)d.post_eps);
         }
         auto fresh = [&](int h) -> float {               // the new residual value
             float v = i8_ld(d.x, d.x_type, (size_t)row * d.ldx + h);
@@ -387,7 +388,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
         if (d.kind == BGL_NORM_LAYER) {
             double s = 0.0;
             for (int h = tid; h < d.H; h += 1024) s += (double)value(h);
-            mean = row_sum<1024>(s, red) / d.H;
+            mean = row_sum<true>(s, red) / d.H;
         }
         if (d.kind != BGL_NORM_NONE) {
             double q = 0.0;
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
                 const double t = (double)value(h) - mean;
                 q = fma(t, t, q);
             }
-            inv = 1.0 / sqrt(row_sum<1024>(q, red) / d.H + (double)d.eps);
+            inv = 1.0 / sqrt(row_sum<true>(q, red) / d.H + (double)d.eps);
         }
         auto out = [&](int h) -> float {
             const float v = value(h);
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormLaunch L) {
             mb = max(mb, __float_as_uint(v) & 0x7fffffffu);
         }
         if (!d.yq) return;
-        const I8Scale s = i8_scale(row_max<1024>(mb, red));
+        const I8Scale s = i8_scale(row_max<true>(mb, red));
         if (tid == 0) d.yscale[row] = s.sc;
         int8_t *q = d.yq + (size_t)row * d.ldq;
         for (int h = tid; h < ((d.H + 15) & ~15); h += 1024) q[h] = (int8_t)(h < d.H ? i8_code(out(h), s) : 0);
@@ -428,13 +429,14 @@ static void norm_go(const NormLaunch &L, hipStream_t st) {
     // (4096 bf16 rows of 4096 with 16 values a thread 31.2 us, with 8 33.1; 2048 normed-twice rows of 8192 36.8 and 42.7; few
     // rows wait for one row's passes: 1 of 4096 4.1 and 3.5, 300 5.9 and 5.6, 1024 9.0 and 9.4)
     const int H = L.d.H;
-    if (H < 8) go(k_norm_wide, 1024, 1);
-    else if (H <= 512) go(k_norm<64, 1, ROW>, 256, 4);
-    else if (H <= 2048) go(k_norm<256, 1, ROW>, 256, 1);
-    else if (H <= 4096 && L.d.T <= 512) go(k_norm<512, 1, ROW>, 512, 1);
-    else if (H <= 4096) go(k_norm<256, 2, ROW>, 256, 1);
-    else if (H <= 8192) go(k_norm<512, 2, ROW>, 512, 1);
-    else if (H <= 16384) go(k_norm<1024, 2, ROW>, 1024, 1);
+    if (H < 8) return go(k_norm_wide, 1024, 1);
+    if constexpr (ROW != ROW_GLU)                            // (an MLP that narrow takes a workgroup a row)
+        if (H <= 512) return go(k_norm<64, 1, ROW>, 256, 4);
+    if (H <= 2048) go(k_norm<0, 1, ROW>, 256, 1);
+    else if (H <= 4096 && L.d.T <= 512) go(k_norm<0, 1, ROW>, 512, 1);
+    else if (H <= 4096) go(k_norm<0, 2, ROW>, 256, 1);
+    else if (H <= 8192) go(k_norm<0, 2, ROW>, 512, 1);
+    else if (H <= 16384) go(k_norm<0, 2, ROW>, 1024, 1);
     else go(k_norm_wide, 1024, 1);
 }
 
