@@ -76,11 +76,25 @@ def _vec(t, n):
     return t.data_ptr()
 
 
+def _need(ok, what):
+    """Refuses a call as the library does, for what its entries cannot see behind a pointer."""
+    if not ok:
+        raise BglError(what, E_ARG)
+
+
 class Tensor:
     """A weight tensor bound on the device (bgl_tensor*)."""
 
     def __init__(self, handle):
         self.h = C.c_void_p(handle) if not isinstance(handle, C.c_void_p) else handle
+        self._shape = None
+
+    def shape(self):
+        """(out, in), asked of the library once."""
+        if self._shape is None:
+            i = self.info()
+            self._shape = i["out"], i["inn"]
+        return self._shape
 
     def info(self):
         k, b, o, i = C.c_int(), C.c_int(), C.c_int(), C.c_int()
@@ -230,17 +244,27 @@ class Context:
         fp16 or bf16 tensors [M][out] of one type, whose rows may be apart.  A single tensor, y and bias need no lists."""
         if isinstance(ts, Tensor):
             ts, ys, biases = [ts], [ys], [biases]
-        n, M = len(ts), xq_dev.shape[0]
-        kind, bias = _type(ys[0]), biases or [None] * n
-        assert xq_dev.dtype == _dtypes()[3] and xq_dev.stride(-1) == 1 and len(ys) == n == len(bias)
-        for t, y in zip(ts, ys):
-            assert _type(y) == kind and y.stride(-1) == 1 and y.shape[0] == M
+        n, bias = len(ts), biases or [None] * len(ts)
+        _need(0 < n == len(ys) == len(bias) and xq_dev.dim() == 2, "matmul_i8: one y (and bias) a tensor, codes [M][>= in]")
+        M, kind, inn = xq_dev.shape[0], ys[0].dtype, ts[0].shape()[1]
+        _need(xq_dev.dtype == _dtypes()[3] and xq_dev.stride(1) == 1 and xq_dev.shape[1] >= inn, f"matmul_i8: codes are dense int8 rows of at least in={inn}")
+        # the kernels read the row's bytes up to the next multiple of 16
+        _need(xq_dev.shape[1] >= (inn + 15) // 16 * 16 or
+              xq_dev.storage_offset() + (M - 1) * xq_dev.stride(0) + (inn + 15) // 16 * 16 <= xq_dev.untyped_storage().nbytes(),
+              "matmul_i8: the last row of codes ends before a multiple of 16 bytes")
+        _need(ascale_dev.dtype == _dtypes()[0] and ascale_dev.shape == (M,) and ascale_dev.is_contiguous(), f"matmul_i8: scales are fp32 [{M}]")
+        for t, y, b in zip(ts, ys, bias):
+            out = t.shape()[0]
+            _need(y.dtype == kind and kind in _dtypes()[:3] and y.shape == (M, out) and (y.stride(1) == 1 or out == 1),
+                  f"matmul_i8: y is [{M}][{out}] of one type (fp32, fp16, bf16) with dense rows")
+            _need(b is None or (b.dtype == _dtypes()[0] and b.shape == (out,) and b.is_contiguous()), f"matmul_i8: a bias is fp32 [{out}]")
+        _need(all(v is None or v.get_device() == self.device for v in (xq_dev, ascale_dev, *ys, *bias)), f"matmul_i8: tensors lie on device {self.device}")
         W = (C.c_void_p * n)(*[t.h.value for t in ts])
         Y = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
         B = (C.c_void_p * n)(*[(b.data_ptr() if b is not None else None) for b in bias])
         S = (C.c_long * n)(*[y.stride(0) if M > 1 else y.shape[1] for y in ys])
         _check(lib().bgl_matmul_i8_dev(self.h, n, W, C.c_void_p(xq_dev.data_ptr()), xq_dev.stride(0) if M > 1 else xq_dev.shape[1],
-                                       _p(ascale_dev), B, Y, kind, S, M), "bgl_matmul_i8_dev")
+                                       _p(ascale_dev), B, Y, _type(ys[0]), S, M), "bgl_matmul_i8_dev")
 
     def norm(self, x, y=None, *, yq=None, yscale=None, kind=NORM_RMS, w=None, b=None, eps=1e-6, w_add=0.0, x_out=None, branch=None,
              branch_kind=NORM_NONE, branch_w=None, branch_b=None, branch_eps=1e-6, gate=None, alpha=1.0):
