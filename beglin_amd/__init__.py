@@ -252,12 +252,12 @@ class Context:
         _need(xq_dev.shape[1] >= (inn + 15) // 16 * 16 or
               xq_dev.storage_offset() + (M - 1) * xq_dev.stride(0) + (inn + 15) // 16 * 16 <= xq_dev.untyped_storage().nbytes(),
               "matmul_i8: the last row of codes ends before a multiple of 16 bytes")
-        _need(ascale_dev.dtype == _dtypes()[0] and ascale_dev.shape == (M,) and ascale_dev.is_contiguous(), f"matmul_i8: scales are fp32 [{M}]")
+        _need(ascale_dev.dtype == _dtypes()[0] and ascale_dev.numel() == M and ascale_dev.is_contiguous(), f"matmul_i8: scales are fp32 [{M}]")
         for t, y, b in zip(ts, ys, bias):
             out = t.shape()[0]
             _need(y.dtype == kind and kind in _dtypes()[:3] and y.shape == (M, out) and (y.stride(1) == 1 or out == 1),
                   f"matmul_i8: y is [{M}][{out}] of one type (fp32, fp16, bf16) with dense rows")
-            _need(b is None or (b.dtype == _dtypes()[0] and b.shape == (out,) and b.is_contiguous()), f"matmul_i8: a bias is fp32 [{out}]")
+            _need(b is None or (b.dtype == _dtypes()[0] and b.numel() == out and b.is_contiguous()), f"matmul_i8: a bias is fp32 [{out}]")
         _need(all(v is None or v.get_device() == self.device for v in (xq_dev, ascale_dev, *ys, *bias)), f"matmul_i8: tensors lie on device {self.device}")
         W = (C.c_void_p * n)(*[t.h.value for t in ts])
         Y = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
@@ -286,8 +286,11 @@ class Context:
         if y is not None:
             d.y, d.ldy, d.y_type = y.data_ptr(), _rows(y, T, H), _type(y)
         if yq is not None:
-            assert yq.dtype == _dtypes()[3] and yq.shape[0] == T and yq.stride(-1) == 1 and yscale.numel() == T
+            _need(yq.dtype == _dtypes()[3] and yq.dim() == 2 and yq.shape[0] == T and yq.shape[1] >= (H + 15) // 16 * 16 and yq.stride(1) == 1 and
+                  yscale is not None and yscale.numel() == T, f"norm: yq is int8 [{T}][H={H} up to a multiple of 16] with dense rows, yscale [{T}]")
             d.yq, d.ldq, d.yscale = yq.data_ptr(), yq.stride(0) if T > 1 else yq.shape[1], _vec(yscale, T)
+        _need(all(v is None or v.get_device() == self.device for v in (x, y, yq, yscale, w, b, x_out, branch, branch_w, branch_b, gate)),
+              f"norm: tensors lie on device {self.device}")
         _check(lib().bgl_norm_dev(self.h, C.byref(d)), "bgl_norm_dev")
 
     # ---- MoE ----

@@ -1,5 +1,6 @@
-"""Context.matmul_i8's own checks, on the CPU: what the library's entry cannot see behind a pointer is refused before the call.
-The context has no handle, so a call that reaches the library is refused there, with another message."""
+"""The checks of Context.matmul_i8 and Context.norm, on the CPU: what the library's entries cannot see behind a pointer is
+refused before the call.  The context has no handle, so a call that reaches the library is refused there, with another
+message."""
 import pytest
 import torch
 
@@ -65,9 +66,44 @@ def test_groups():
         ctx.matmul_i8(**call)
 
 
-@pytest.mark.parametrize("ok", [dict(), dict(biases=None), dict(ys=torch.zeros((M, 64))[:, 3:3 + N]), dict(ys=torch.zeros((M, N), dtype=torch.bfloat16)),
+@pytest.mark.parametrize("ok", [dict(), dict(biases=None), dict(ascale_dev=torch.zeros((M, 1)), biases=torch.zeros((1, N))), dict(ys=torch.zeros((M, 64))[:, 3:3 + N]), dict(ys=torch.zeros((M, N), dtype=torch.bfloat16)),
                                 dict(xq_dev=torch.zeros((M, 112), dtype=torch.int8)[:, :K])])
 def test_allowed_calls_reach_the_library(ok):
     ctx, call = setting()
     with pytest.raises(B.BglError, match="bgl_matmul_i8_dev: bad argument"):
         ctx.matmul_i8(**{**call, **ok})
+
+
+T, H = 3, 40
+
+
+def norm_call(**change):
+    ctx, _ = setting()
+    ctx.device = change.pop("device", -1)
+    x = change.pop("x", torch.zeros((T, H)))
+    ctx.norm(x, **{**dict(yq=torch.zeros((T, 48), dtype=torch.int8), yscale=torch.zeros(T)), **change})
+
+
+NORM_BAD = {
+    "a view that ends inside 16 codes": dict(yq=torch.zeros((T, 64), dtype=torch.int8)[:, :47]),
+    "a view of the last columns": dict(yq=torch.zeros((T, 64), dtype=torch.int8)[:, 48:]),
+    "rows of H codes": dict(yq=torch.zeros((T, H), dtype=torch.int8)),
+    "fewer rows": dict(yq=torch.zeros((T - 1, 48), dtype=torch.int8)),
+    "codes of another type": dict(yq=torch.zeros((T, 48), dtype=torch.uint8)),
+    "rows that are not dense": dict(yq=torch.zeros((T, 96), dtype=torch.int8)[:, ::2]),
+    "one dimension": dict(yq=torch.zeros(T * 48, dtype=torch.int8)),
+    "few scales": dict(yscale=torch.zeros(T - 1)), "no scales": dict(yscale=None), "another device": dict(device=0),
+}
+
+
+@pytest.mark.parametrize("change", NORM_BAD.values(), ids=list(NORM_BAD))
+def test_norm_refused(change):
+    with pytest.raises(B.BglError, match="norm: ") as e:
+        norm_call(**dict(change))
+    assert e.value.code == B.E_ARG
+
+
+def test_norm_calls_reach_the_library():
+    for ok in (dict(), dict(yq=torch.zeros((T, 96), dtype=torch.int8)[:, 16:64]), dict(yq=None, yscale=None, y=torch.zeros((T, H)))):
+        with pytest.raises(B.BglError, match="bgl_norm_dev: NULL"):
+            norm_call(**ok)
