@@ -11,10 +11,11 @@ typedef float i8_f4 __attribute__((ext_vector_type(4)));
 static inline size_t i8_elem(int type) { return type == BGL_T_F32 ? 4 : 2; }
 
 // ------------------------------------------------------------------ element types
-// One value of a row in fp32, fp16 or bf16 (every one of them is an fp32 value exactly).
+// One value of a row in fp32, fp16 or bf16 (every one of them is an fp32 value exactly).  fp16 is read as the integer that
+// i8_st stores: a thread may read back what it wrote, and accesses of two types may change places.
 __device__ __forceinline__ float i8_ld(const void *p, int type, size_t i) {
     if (type == BGL_T_F32) return ((const float *)p)[i];
-    if (type == BGL_T_F16) return (float)((const _Float16 *)p)[i];
+    if (type == BGL_T_F16) return (float)__builtin_bit_cast(_Float16, ((const uint16_t *)p)[i]);
     return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
 }
 // fp32 to the type, to nearest, ties to even; the bf16 cast keeps NaN a NaN.

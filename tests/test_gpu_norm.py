@@ -129,6 +129,30 @@ def test_in_place_and_single_outputs(ctx, torch_dev):
         assert np.array_equal(host(x), v)
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("T,H", [(3, 5), (2, 17000), (2, 33333)])
+def test_16_bit_residual_rows_are_read_back(ctx, torch_dev, kind, T, H):
+    """Rows that the kernel reads again for each pass (wider than 16384, narrower than 8): the new residual row is stored in 16
+    bits and the norm, whose RMS waits at no barrier between the two, reads it back; beside x and in its place."""
+    import beglin_amd as B
+    torch = torch_dev
+    rng = np.random.default_rng([T, H])
+    x, f = rows(torch, rng, T, H, kind, 3.0), rows(torch, rng, T, H, kind, 0.5)
+    v = (host(x).astype(np.float64) + host(f)).astype(np.float32)
+    v = host(torch.from_numpy(v).to(x.dtype))               # the residual row as stored
+    for pre in (B.NORM_RMS, B.NORM_NONE, B.NORM_LAYER):
+        for src, place in ((x, torch.zeros_like(x)), (xc := x.clone(), xc)):
+            y, yq, ys = torch.empty((T, H), device="cuda"), torch.zeros((T, (H + 15) // 16 * 16), dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+            torch.cuda.synchronize()
+            ctx.norm(src, branch=f, x_out=place, y=y, yq=yq, yscale=ys, kind=pre)
+            ctx.sync()
+            assert np.array_equal(host(place), v)
+            want = I.normed(pre, v)
+            near(y, want, "y")
+            q, s = I.quantize(want.astype(np.float32))
+            assert np.array_equal(yq[:, :H].cpu().numpy(), q) and np.array_equal(ys.cpu().numpy(), s)
+
+
 @pytest.mark.parametrize("H", [48, 1536, 4096, 14336, 20000, 131056])
 def test_quantizer_is_the_norm_of_kind_none(ctx, torch_dev, H):
     import beglin_amd as B
