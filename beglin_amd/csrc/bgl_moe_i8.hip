@@ -209,6 +209,10 @@ __device__ __forceinline__ void i8_pre(const MoeI8Launch &L, int b, int gen, uin
     float sel_w;
     int sel_i;
     route_topk_wave(sc, L.E, L.K, L.renorm, lane, sel_i, sel_w, lbuf);
+    if (lane < L.K && sel_i >= L.E) {                          // scores of which one is NaN or +Inf pick nothing: the sum is NaN
+        sel_i = lane;
+        sel_w = __uint_as_float(0x7fc00000u);
+    }
     if (lane < L.K) {
         i8_put_now(L.sync->idx + t * L.K + lane, gen, (uint32_t)sel_i);
         i8_put_now(L.sync->w + t * L.K + lane, gen, __float_as_uint(sel_w));

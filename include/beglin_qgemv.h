@@ -308,7 +308,10 @@ int bgl_moe_ffn_dev(bgl_ctx *ctx, const bgl_tensor *gate, const bgl_tensor *up, 
 int bgl_moe_route_dev(bgl_ctx *ctx, const float *router_w_dev, const float *router_b_dev, int E, int in,
                       const float *x_dev, int T, int K, int renorm, int32_t *topk_idx_dev, float *topk_w_dev);
 /* The whole routed FFN step on the device (moe_ffn_batched, qwen_infer.c:5238-5350): bgl_moe_route_dev
- * then bgl_moe_ffn_dev, with the routing kept in the context's scratch.  E = the experts in gate. */
+ * then bgl_moe_ffn_dev, with the routing kept in the context's scratch.  E = the experts in gate.  A token
+ * whose scores have no softmax (one is NaN or +Inf, or all are -Inf) picks no expert (bgl_moe_route_dev
+ * writes ids outside the stack): through K_Q8C stacks its row comes out as NaN, as the softmax is; with
+ * the other kinds its experts add nothing. */
 int bgl_moe_layer_dev(bgl_ctx *ctx, const float *router_w_dev, const float *router_b_dev, int renorm,
                       const bgl_tensor *gate, const bgl_tensor *up, const bgl_tensor *down,
                       const bgl_tensor *shared_gate, const bgl_tensor *shared_up, const bgl_tensor *shared_down,

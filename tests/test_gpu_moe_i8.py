@@ -141,6 +141,52 @@ def test_rows_at_the_ends_of_fp32(ctx, torch_dev):
     lay.free()
 
 
+@pytest.mark.parametrize("T", [1, 4, 40, 70])
+@pytest.mark.parametrize("Wsh", [0, 64])
+def test_scores_without_a_softmax(ctx, torch_dev, T, Wsh):
+    """A token with NaN or an infinity, or whose scores are not finite for the router's own values, comes out as NaN, with and
+    without shared experts and renorm; the other tokens keep their bits."""
+    torch = torch_dev
+    E, K, H, W = 12, 3, 128, 64
+    lay = Layer(ctx, [9, Wsh], E, H, W, Wsh)
+    x, rw = lay.rng.standard_normal((T, H)).astype(np.float32), (lay.rng.standard_normal((E, H)) / H ** 0.5).astype(np.float32)
+    bias = lay.rng.standard_normal(E).astype(np.float32)
+    idx, w, out = torch.empty((T, K), dtype=torch.int32, device="cuda"), torch.empty((T, K), device="cuda"), torch.empty((T, H), device="cuda")
+    xd, rwd, bd = (torch.from_numpy(v).cuda() for v in (x, rw, bias))
+    torch.cuda.synchronize()
+    for renorm in (False, True):
+        ctx.moe_route(rwd, xd, K, idx, w, router_b=bd, renorm=renorm)
+        ctx.sync()
+        want = lay.want(x, idx.cpu().numpy(), w.cpu().numpy())
+        for token, place, value in ((0, H - 1, np.nan), (T // 2, 0, np.inf), (T - 1, 7, -np.inf)):
+            bad = x.copy()
+            bad[token, place] = value
+            xb = torch.from_numpy(bad).cuda()
+            out.zero_()
+            torch.cuda.synchronize()
+            ctx.moe_layer(rwd, *lay.stacks, lay.sh, xb, K, out, router_b=bd, renorm=renorm)
+            ctx.check()
+            wb = want.copy()
+            wb[token] = np.nan
+            same(out, wb)
+        for value in (np.nan, np.inf):                      # of the router itself: every token's
+            bb = torch.from_numpy(np.where(np.arange(E) == 5, np.float32(value), bias)).cuda()
+            out.zero_()
+            torch.cuda.synchronize()
+            ctx.moe_layer(rwd, *lay.stacks, lay.sh, xd, K, out, router_b=bb, renorm=renorm)
+            ctx.check()
+            assert torch.isnan(out).all()
+        # one expert that no token can pick (-Inf) leaves the softmax of the others
+        bb = torch.from_numpy(np.where(np.arange(E) == 5, np.float32(-np.inf), bias)).cuda()
+        torch.cuda.synchronize()
+        ctx.moe_route(rwd, xd, K, idx, w, router_b=bb, renorm=renorm)
+        ctx.moe_layer(rwd, *lay.stacks, lay.sh, xd, K, out, router_b=bb, renorm=renorm)
+        ctx.check()
+        assert not (idx == 5).any()
+        same(out, lay.want(x, idx.cpu().numpy(), w.cpu().numpy()))
+    lay.free()
+
+
 @pytest.mark.parametrize("T", [1, 5, 20, 70])
 def test_captured_layer(torch_dev, T):
     """Captured after one eager run and replayed on new tokens, twice into each of two graphs of one context, with eager
