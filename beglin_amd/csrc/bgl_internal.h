@@ -110,8 +110,6 @@ bool mfma_takes(const bgl_ctx *c, int n, const BglDevTensor *Ts, int M);
 // into glu_h [M][N] (k_swiglu's arithmetic), so the caller needs no SwiGLU launch.
 int run_gemm_mfma(bgl_ctx *c, int n, const BglDevTensor *Ts, const float *x_dev, int M, const float *const *bias,
                   float *const *y, const int *ystride, float *glu_h = nullptr);
-int moe_i8_recount(bgl_ctx *c);              // bgl_ctx_check, after a wait in a layer of K_Q8C experts gave up (bgl_moe_i8.hip)
-
 // The dense MLP block at one W4A8 column in one launch (bgl_mlp_q.hip): the formats it takes, and the call.
 int run_down_swiglu_w4a8(bgl_ctx *c, const BglDevTensor &down, const float *g, const float *u, float *h, int M, float *y);
 // W4A8 products of more than 16 columns (bgl_gemm_q.hip): the calls it takes, and the call.

@@ -450,10 +450,9 @@ extern "C" int bgl_ctx_check(bgl_ctx *c) {
         HIPCHK(check(0));
     }
     HIPCHK(check(1));
-    if (gave_up[1] && moe_i8_recount(c)) return bgl_last_code();
     if (gave_up[0])
         return bgl_fail(BGL_E_TIMEOUT, "a single-launch MLP block stopped waiting for its gate+up workgroups: its outputs are invalid");
     if (gave_up[1])
-        return bgl_fail(BGL_E_TIMEOUT, "a single-launch MoE layer stopped waiting for some of its workgroups: its outputs and later layers' are invalid");
+        return bgl_fail(BGL_E_TIMEOUT, "a single-launch MoE layer stopped waiting for some of its workgroups: its outputs are invalid");
     return 0;
 }

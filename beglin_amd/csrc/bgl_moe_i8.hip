@@ -58,7 +58,9 @@ struct MoeI8Sync {
     int shared[MOE_I8_GU_WGS];           // a gate+up workgroup's share of the shared experts is done
     int gu[MOE_I8_GU_WGS];               // all it does
     int sq[MOE_I8_SQ_WGS];               // codes of the shared experts' h are there
-    int blocks[MOE_I8_PAIRS];            // 16-row blocks of a slot that are done; 0 between launches
+    // 16-row blocks of a slot that are done, in the half of the launch's number; each launch zeroes the next one's half, so
+    // that counts which waits that gave up left wrong are nobody's
+    int blocks[2][MOE_I8_PAIRS];
     int gen[MOE_I8_WGS];                 // launches so far: the same in every element between launches
     // values that carry the number of their launch in the upper half
     uint64_t score[MOE_I8_TOK * ROUTE_MAXE], idx[MOE_I8_PAIRS], w[MOE_I8_PAIRS];
@@ -70,7 +72,7 @@ struct MoeI8Launch {
     int shared, E, K, T, P, H, I, Ish, nslots, piece;   // nslots: the most slots; piece: units a down wave takes
     int hp, ip, ishp;                    // bytes of a row of codes: a multiple of 128, so that no two share a line
     int npre, ngu, nsq;                  // workgroups of each role; the rest is down's
-    int never, spin;                     // a test's launch whose waits give up; polls before a wait does
+    int never, spin;                     // a test's launch, in whose odd workgroups waits give up; polls before a wait does
     MoeI8Sync *sync;
     const float *x, *rw, *rb;            // token rows; router
     int renorm;
@@ -92,12 +94,14 @@ __device__ __forceinline__ i8_f4 i8_get4(const float *p) {
     const uint64_t a = i8_get((const uint64_t *)p), b = i8_get((const uint64_t *)p + 1);
     return i8_f4{__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))};
 }
+// what a wait waits for
+__device__ __forceinline__ int i8_expect(const MoeI8Launch &L, int gen) { return gen + (L.never & (int)blockIdx.x); }
 // A value and the number of its launch in one store; and the wait for it, by one lane.
 __device__ __forceinline__ void i8_put_now(uint64_t *p, int gen, uint32_t v) { i8_put(p, (uint64_t)(uint32_t)gen << 32 | v); }
 __device__ __forceinline__ uint32_t i8_get_now(const MoeI8Launch &L, const uint64_t *p, int gen) {
     for (int s = 0;;) {
         const uint64_t v = i8_get(p);
-        if ((int)(v >> 32) == gen + L.never) return (uint32_t)v;
+        if ((int)(v >> 32) == i8_expect(L, gen)) return (uint32_t)v;
         if (++s >= L.spin) break;
         __builtin_amdgcn_s_sleep(1);
     }
@@ -123,7 +127,7 @@ __device__ __forceinline__ void i8_wait(const MoeI8Launch &L, const int *flag, i
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[j] = i8_get(flag + min(i + 64 * j, n - 1));
 #pragma unroll
-                for (int j = 0; j < 4; j++) ok &= v[j] == gen + L.never;
+                for (int j = 0; j < 4; j++) ok &= v[j] == i8_expect(L, gen);
             }
             if (__builtin_amdgcn_ballot_w64(!ok) == 0) break;
             if (++s >= L.spin) {
@@ -431,10 +435,8 @@ __device__ __forceinline__ void i8_gate_up(const MoeI8Launch &L, int b, int gen,
     if (threadIdx.x < 64) {
         const int s = begin / per + (int)threadIdx.x, n = min(end, (s + 1) * per) - max(begin, s * per);
         bool last = false;
-        if (n > 0 && begin < end) {
-            last = __hip_atomic_fetch_add(L.sync->blocks + s, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + n == per;
-            if (last) i8_put(L.sync->blocks + s, 0);           // for the next launch
-        }
+        if (n > 0 && begin < end)
+            last = __hip_atomic_fetch_add(L.sync->blocks[gen & 1] + s, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + n == per;
         const uint64_t m = __builtin_amdgcn_ballot_w64(last);
         if (threadIdx.x == 0) *whole = m;
     }
@@ -570,7 +572,8 @@ __global__ __launch_bounds__(MOE_I8_NT, 4) void k_moe_i8(MoeI8Launch L) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ MoeI8Route R;
     const int b = blockIdx.x, gu = b - L.npre, sq = gu - L.ngu, rb = sq - L.nsq;
-    const int gen = max(1u, (uint32_t)L.sync->gen[b] + 1u);    // 0: what was never set
+    const uint32_t next = (uint32_t)L.sync->gen[b] + 1u;
+    const int gen = next ? next : 2;                           // 0: what was never set; 2: the halves of blocks keep their turns
     if (gu < 0) i8_pre(L, b, gen, lds);
     else if (sq < 0) i8_gate_up(L, gu, gen, R, lds);
     else if (rb < 0) i8_shared_codes(L, sq, gen, lds);
@@ -578,6 +581,8 @@ __global__ __launch_bounds__(MOE_I8_NT, 4) void k_moe_i8(MoeI8Launch L) {
     // the number of this launch, for all workgroups of the next, of which there may be more
     __syncthreads();
     for (int i = b + threadIdx.x * gridDim.x; i < MOE_I8_WGS; i += MOE_I8_NT * gridDim.x) L.sync->gen[i] = gen;
+    if (b == 0)
+        for (int i = threadIdx.x; i < MOE_I8_PAIRS; i += MOE_I8_NT) L.sync->blocks[~gen & 1][i] = 0;
 }
 
 // dynamic LDS of every role: gate+up's two buffers of sums
@@ -618,7 +623,7 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
         L.out = out + (size_t)t0 * L.H;
         L.idx = rw ? nullptr : idx + (size_t)t0 * K;
         L.w = rw ? nullptr : w + (size_t)t0 * K;
-        L.never = c->mlp_test_timeout > 0 ? 1 : 0;                  // a test's launch whose waits must give up
+        L.never = c->mlp_test_timeout > 0 ? 1 : 0;                  // a test's launch, in which waits must give up
         if (c->mlp_test_timeout > 0) c->mlp_test_timeout--;
         L.npre = L.T + (rw ? L.T * ((L.E + MOE_I8_NW - 1) / MOE_I8_NW) : 0);
         L.ngu = std::min(MOE_I8_GU_WGS, (L.shared ? L.Ish / 16 : 0) + L.nslots * (L.I / 16));
@@ -630,12 +635,5 @@ int run_moe_i8(bgl_ctx *c, const bgl_tensor *gate, const bgl_tensor *up, const b
         prof_end(c, tok);
         HIPCHK(hipGetLastError());
     }
-    return 0;
-}
-
-// After a wait gave up, workgroups may have counted blocks by different routings: the counts begin at 0 again (the stream is idle).
-int moe_i8_recount(bgl_ctx *c) {
-    MoeI8Sync *s = (MoeI8Sync *)c->moe_sync.p;
-    HIPCHK(hipMemset(s->blocks, 0, sizeof s->blocks));
     return 0;
 }

@@ -76,8 +76,7 @@ int  bgl_ctx_create(int device, void *hip_stream, bgl_ctx **out);   /* q4pool_in
 void bgl_ctx_destroy(bgl_ctx *ctx);                         /* q4pool_destroy (q4gemv.h:623-637) */
 int  bgl_synchronize(bgl_ctx *ctx);                         /* mlx_gpu_synchronize (mlx_moe.h:29) */
 /* Synchronize the context's stream, then report (and clear) a bounded in-kernel wait that gave up
- * since the last check: BGL_E_TIMEOUT means the outputs of that call are invalid, and for a layer of
- * K_Q8C experts those of later such layers before the check too.  No counterpart in
+ * since the last check: BGL_E_TIMEOUT means the outputs of that call are invalid.  No counterpart in
  * the reference (its CPU kernels never wait on each other); the single-launch MLP block of
  * bgl_mlp_dev and the K_Q8C layers of bgl_moe_ffn_dev and bgl_moe_layer_dev are the calls that wait. */
 int  bgl_ctx_check(bgl_ctx *ctx);

@@ -372,6 +372,41 @@ def test_bounded_waits_give_up(torch_dev, monkeypatch, T):
     c.close()
 
 
+@pytest.mark.parametrize("T", [1, 20, 70])
+def test_a_layer_after_one_that_gave_up(torch_dev, monkeypatch, T):
+    """The layers after one in whose odd workgroups the waits gave up (so that they saw another routing than the even ones, and
+    counted other blocks) are right without a check between."""
+    import beglin_amd as B
+    torch = torch_dev
+    print("[case] after a wait that gave up", T, flush=True)
+    monkeypatch.setenv("BGL_MLP_TEST_TIMEOUT", "1")
+    monkeypatch.setenv("BGL_MLP_SPIN", "2048")             # polls of the good layers too: some ms, of which they need one hundredth
+    c = B.Context(0)
+    monkeypatch.delenv("BGL_MLP_TEST_TIMEOUT")
+    monkeypatch.delenv("BGL_MLP_SPIN")
+    E, K, H, W = 16, 4, 256, 128
+    lay = Layer(c, 42, E, H, W, 64)
+    rw = torch.from_numpy((lay.rng.standard_normal((E, H)) / H ** 0.5).astype(np.float32)).cuda()
+    xs = [lay.rng.standard_normal((T, H)).astype(np.float32) for _ in range(3)]
+    outs = [torch.full((T, H), float("nan"), device="cuda") for _ in xs]
+    xd = [torch.from_numpy(x).cuda() for x in xs]
+    idx, w = torch.empty((T, K), dtype=torch.int32, device="cuda"), torch.empty((T, K), device="cuda")
+    torch.cuda.synchronize()
+    c.moe_layer(rw, *lay.stacks, lay.sh, xd[0], K, outs[0])       # (its first 64 tokens give up)
+    for x, o in zip(xd[1:], outs[1:]):
+        c.moe_layer(rw, *lay.stacks, lay.sh, x, K, o)
+    c.sync()
+    for i in (1, 2):
+        c.moe_route(rw, xd[i], K, idx, w)
+        c.sync()
+        same(outs[i], lay.want(xs[i], idx.cpu().numpy(), w.cpu().numpy()))
+    with pytest.raises(B.BglError) as e:
+        c.check()
+    assert e.value.code == B.E_TIMEOUT
+    lay.free()
+    c.close()
+
+
 def test_refusals(ctx, torch_dev):
     import beglin_amd as B
     torch = torch_dev
