@@ -275,8 +275,13 @@ __device__ __forceinline__ void i8_copy(i8_rsrc rs, uint32_t voff, uint32_t soff
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff)
                  : "memory");
 }
-// every copy of this wave has landed and every LDS read of it has returned
-__device__ __forceinline__ void i8_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// Every copy of each wave has landed and every LDS read of it has returned.  (The barrier alone is no access to memory for
+// the compiler: the empty asm behind it keeps later reads from moving before it.)
+__device__ __forceinline__ void i8_wait() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // Workgroup b of nt: each XCD (workgroups go round the 8 of them) takes a run of neighbouring tiles, and
 // within it 8 tiles of tokens share the weights that they read from its L2.
@@ -361,7 +366,6 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
 #pragma unroll
     for (int q = 0; q < WI + XI; q++) copy(q, s0, lds0);
     i8_wait();
-    __builtin_amdgcn_s_barrier();
     if (s0 + 1 < ns) {
 #pragma unroll
         for (int q = 0; q < WI + XI; q++) copy(q, s0 + 1, lds0 + SB);
@@ -375,7 +379,6 @@ __global__ __launch_bounds__(NWM *NWN * 64, 2) void k_i8_l(I8Launch L, int ntm, 
         half(0, sm + cur, false, 0, 0);
         // every wave has read the whole stage, and the next one has landed: it is read while this one's place is filled
         i8_wait();
-        __builtin_amdgcn_s_barrier();
         half(1, sm + (SB - cur), s + 2 < ns, s + 2, lds0 + cur);              // (the last stage reads what lies there)
         cur = SB - cur;
     }
@@ -531,7 +534,11 @@ static int run_l(bgl_ctx *c, I8Launch &L, int ks) {
 //   k_i8_s with 64 x 64 outputs / 128 x 128 tiles / 256 x 256: 512 x 1536 x 1536 9.3 / 12.8 / 31.8, 2048 x 2048 x 2048
 //     34.8 / 16.4 / 33.3, 2048 x 14336 x 4096 369 / 153 / 126
 //   128 x 192 tiles / 128 x 128, where the last round of the latter leaves most CUs idle: 512 x 17920 x 1536 24.6 / 29.4,
-//     1500 x 6144 x 4096 45.5 / 59.0, 2048 x 8960 x 1536 38.1 / 44.6; where it does not: 512 x 14336 x 4096 50.8 / 41.7
+//     1500 x 6144 x 4096 45.5 / 59.0, 2048 x 8960 x 1536 38.1 / 44.6; where it does not: 512 x 14336 x 4096 50.8 / 41.7.
+//     Up to 512 tiles of 128 x 192 (80 KB of LDS, 114 registers) are all there at once, two on a CU, and a step of K takes
+//     1.3 to 1.8 us for both; more follow one another at 0.8 to 1.0 a round.  us a step at K = 4096 by rounds of 256 tiles:
+//     0.5 0.73, 1 1.02, 1.2 1.4, 1.5 1.3 to 1.5, 2 1.8, 2.5 2.7, 3 2.8 to 2.9, 4 3.6, 6 5.2, 9 7.6, 12 10.3.  Over 36 shapes of
+//     512 and 1500 columns, 6144 to 49152 channels, K of 1536 and 4096 the choice is the fastest of the three tiles each time
 //   128 x 128 tiles with K in 1 / 4 slices: 1024 x 1536 x 8960 48.7 / 31.1, 128 x 8960 x 1536 14.0 / 19.9
 static int run_any(bgl_ctx *c, I8Launch &L) {
     const int K = L.t[0].T.K, M = L.M;
@@ -562,7 +569,7 @@ static int run_any(bgl_ctx *c, I8Launch &L) {
     const double c256 = 6.0 + 1.9 * ns * up(t256);
     const double c64 = 3.0 + (t64 <= I8_CUS ? 0.4 : 0.62 * up(t64)) * ns;
     const double u192 = up(l_tiles(L, 128, 192));
-    const double c192 = 6.0 + (u192 == 2.0 ? 1.44 : 0.85 * u192) * ns;
+    const double c192 = 6.0 + (u192 == 2.0 ? 1.44 : 0.85 * u192) * ns;      // 2: both tiles of a CU at once
     if (c64 <= c128 && c64 <= c192 && c64 <= c256 && (M + 63) / 64 <= 65535) return run_s(c, L, 4, 1);
     if (c192 < c128 && c192 <= c256) return run_l<4, 3, 2, 4>(c, L, 1);
     if (c128 <= c256) return run_l<4, 2, 2, 4>(c, L, ks);
