@@ -76,10 +76,26 @@ def _vec(t, n):
     return t.data_ptr()
 
 
+def _w(t):
+    """Address of a weight buffer to bind: a numpy array, or a torch tensor in host or device memory; None passes through."""
+    return None if t is None else t.data_ptr() if hasattr(t, "data_ptr") else t.ctypes.data
+
+
 def _need(ok, what):
     """Refuses a call as the library does, for what its entries cannot see behind a pointer."""
     if not ok:
         raise BglError(what, E_ARG)
+
+
+def _weights(kind, out, inn, packed, scales, sub):
+    """What a bind reads of torch tensors: dense ones, scales of the kind's type, and K_Q8C's buffers whole."""
+    for t in (packed, scales, sub):
+        _need(not hasattr(t, "data_ptr") or t.is_contiguous(), "bind: torch tensors have to be dense")
+    if hasattr(scales, "data_ptr"):
+        _need(scales.element_size() == 2 if kind == K_Q4G32H else scales.dtype == _dtypes()[0], "bind: scales of another type")
+        _need(kind != K_Q8C or scales.numel() == out, f"bind: K_Q8C takes scales [out={out}]")
+    if hasattr(packed, "data_ptr"):
+        _need(kind != K_Q8C or (packed.dtype == _dtypes()[3] and packed.numel() == out * inn), f"bind: K_Q8C takes int8 codes [{out}][{inn}]")
 
 
 class Tensor:
@@ -152,11 +168,12 @@ class Context:
 
     # ---- binding ----
     def bind(self, kind, packed, scales, out, inn, bits=0, sub=None):
-        """Bind host (numpy) buffers in the reference layout (sub: g256sf sub-codes or Q4G64A biases;
-        scales None for the dense kinds and MXFP4, whose blocks carry their exponents)."""
+        """Bind buffers in the reference layout (sub: g256sf sub-codes or Q4G64A biases; scales None for the dense
+        kinds and MXFP4, whose blocks carry their exponents): numpy arrays, or dense torch tensors in host memory or on
+        the device, where the context's stream has to see them written."""
+        _weights(kind, out, inn, packed, scales, sub)
         w = capi.bgl_wt(kind, bits if kind == K_QNG64 else (8 if kind in (K_Q8G64, K_Q8C) else 4), out, inn,
-                        packed.ctypes.data, scales.ctypes.data if scales is not None else None,
-                        sub.ctypes.data if sub is not None else None)
+                        _w(packed), _w(scales), _w(sub))
         h = C.c_void_p()
         _check(lib().bgl_bind(self.h, C.byref(w), C.byref(h)), "bgl_bind")
         return Tensor(h)
@@ -295,7 +312,7 @@ class Context:
 
     # ---- MoE ----
     def bind_experts(self, descs):
-        """descs: list of (kind, bits, packed, scales[, bias]) numpy tuples, one per expert; packed is
+        """descs: list of (kind, bits, packed, scales[, bias]) tuples, one per expert, of what bind takes; packed is
         2-D [out][row bytes or elements]; scales None for the dense kinds."""
         E = len(descs)
         arr = (capi.bgl_wt * E)()
@@ -312,8 +329,8 @@ class Context:
             else:
                 inn = sc.shape[1] * (32 if kind == K_Q4G32H else 64)
             b = bits if kind == K_QNG64 else (8 if kind in (K_Q8G64, K_Q8C) else 4)
-            arr[e] = capi.bgl_wt(kind, b, out, inn, pk.ctypes.data, sc.ctypes.data if sc is not None else None,
-                                 bi.ctypes.data if bi is not None else None)
+            _weights(kind, out, inn, pk, sc, bi)
+            arr[e] = capi.bgl_wt(kind, b, out, inn, _w(pk), _w(sc), _w(bi))
         h = C.c_void_p()
         _check(lib().bgl_bind_experts(self.h, E, arr, C.byref(h)), "bgl_bind_experts")
         return Tensor(h)

@@ -480,19 +480,40 @@ __global__ void k_split_mxfp4(const uint8_t *__restrict__ blk, int out, int in, 
     ex[i] = (uint32_t)b[0] | ((uint32_t)b[17] << 8);
 }
 
+// A caller's weights where the device reads them: in place if they lie on the context's device, aligned as the repack
+// kernels read, else a copy, which is freed with the object (a free waits for the work before it).
+struct Staged {
+    const void *p = nullptr;
+    void *own = nullptr;
+    ~Staged() { if (own) (void)hipFree(own); }
+    int take(bgl_ctx *c, const void *src, size_t bytes) {
+        if (!bytes) return 0;
+        hipPointerAttribute_t a;
+        const bool dev = hipPointerGetAttributes(&a, src) == hipSuccess && a.type == hipMemoryTypeDevice;
+        (void)hipGetLastError();                             // host memory that HIP does not know is no error
+        if (dev && a.device == c->device && (uintptr_t)src % 16 == 0) { p = src; return 0; }
+        HIPCHK(hipMalloc(&own, bytes));
+        p = own;
+        HIPCHK(hipMemcpyAsync(own, src, bytes, dev ? hipMemcpyDefault : hipMemcpyHostToDevice, c->stream));
+        return 0;
+    }
+};
+
 static int bind_mxfp4(bgl_ctx *c, const bgl_wt *w, bgl_tensor **out) {
     HIPCHK(hipSetDevice(c->device));
     const size_t pb = ref_packed_bytes(BGL_MXFP4, 4, w->out, w->in), nu = (size_t)w->out * (w->in / 64);
-    void *dblk = nullptr, *dcodes = nullptr, *dex = nullptr;
-    HIPCHK(hipMalloc(&dblk, pb));
+    Staged blk;
+    void *dcodes = nullptr, *dex = nullptr;
     HIPCHK(hipMalloc(&dcodes, nu * 32));
     HIPCHK(hipMalloc(&dex, nu * 4));
-    HIPCHK(hipMemcpyAsync(dblk, w->packed, pb, hipMemcpyHostToDevice, c->stream));
-    hipLaunchKernelGGL(k_split_mxfp4, dim3(nblk((long)nu)), dim3(256), 0, c->stream, (const uint8_t *)dblk, w->out, w->in,
-                       (uint8_t *)dcodes, (uint32_t *)dex);
-    int rc = repack_into(c, BGL_MXFP4, 4, w->out, w->in, dcodes, dex, nullptr, out);
+    int rc = blk.take(c, w->packed, pb);
+    if (!rc) {
+        hipLaunchKernelGGL(k_split_mxfp4, dim3(nblk((long)nu)), dim3(256), 0, c->stream, (const uint8_t *)blk.p, w->out, w->in,
+                           (uint8_t *)dcodes, (uint32_t *)dex);
+        rc = repack_into(c, BGL_MXFP4, 4, w->out, w->in, dcodes, dex, nullptr, out);
+    }
     hipError_t e = hipStreamSynchronize(c->stream);
-    (void)hipFree(dblk); (void)hipFree(dcodes); (void)hipFree(dex);
+    (void)hipFree(dcodes); (void)hipFree(dex);
     if (rc) return rc;
     if (e != hipSuccess) return bgl_fail(BGL_E_HIP, "bind sync: %s", hipGetErrorString(e));
     return 0;
@@ -504,16 +525,15 @@ static int bind_g256plain(bgl_ctx *c, const bgl_wt *w, bgl_tensor **out) {
     if (!w->scales) return bgl_fail(BGL_E_ARG, "bgl_bind: plain g256 needs scales");
     HIPCHK(hipSetDevice(c->device));
     const size_t pb = (size_t)w->out * w->in / 2, sb = (size_t)w->out * (w->in / 256) * 4, nsub = (size_t)w->out * (w->in / 64);
-    void *dpk = nullptr, *dsc = nullptr, *dsub = nullptr;
-    HIPCHK(hipMalloc(&dpk, pb));
-    HIPCHK(hipMalloc(&dsc, sb));
+    Staged pk, sc;
+    void *dsub = nullptr;
     HIPCHK(hipMalloc(&dsub, nsub));
-    HIPCHK(hipMemcpyAsync(dpk, w->packed, pb, hipMemcpyHostToDevice, c->stream));
-    HIPCHK(hipMemcpyAsync(dsc, w->scales, sb, hipMemcpyHostToDevice, c->stream));
     HIPCHK(hipMemsetAsync(dsub, 1, nsub, c->stream));
-    int rc = repack_into(c, BGL_Q4G256SF, 4, w->out, w->in, dpk, dsc, (const uint8_t *)dsub, out);
+    int rc = pk.take(c, w->packed, pb);
+    if (!rc) rc = sc.take(c, w->scales, sb);
+    if (!rc) rc = repack_into(c, BGL_Q4G256SF, 4, w->out, w->in, pk.p, sc.p, (const uint8_t *)dsub, out);
     hipError_t e = hipStreamSynchronize(c->stream);
-    (void)hipFree(dpk); (void)hipFree(dsc); (void)hipFree(dsub);
+    (void)hipFree(dsub);
     if (rc) return rc;
     if (e != hipSuccess) return bgl_fail(BGL_E_HIP, "bind sync: %s", hipGetErrorString(e));
     (*out)->T.gmul = 1.0f;
@@ -534,17 +554,12 @@ extern "C" int bgl_bind(bgl_ctx *c, const bgl_wt *w, bgl_tensor **out) {
     size_t pb = ref_packed_bytes(w->kind, w->bits, w->out, w->in), sb = ref_scale_bytes(w->kind, w->out, w->in);
     size_t subb = w->kind == BGL_Q4G256SF ? (size_t)w->out * (w->in / 64)
                 : w->kind == BGL_Q4G64A ? (size_t)w->out * (w->in / 64) * 4 : 0;
-    void *dpk = nullptr, *dsc = nullptr, *dsub = nullptr;
-    HIPCHK(hipMalloc(&dpk, pb));
-    if (sb) HIPCHK(hipMalloc(&dsc, sb));
-    if (subb) HIPCHK(hipMalloc(&dsub, subb));
-    HIPCHK(hipMemcpyAsync(dpk, w->packed, pb, hipMemcpyHostToDevice, c->stream));
-    if (sb) HIPCHK(hipMemcpyAsync(dsc, w->scales, sb, hipMemcpyHostToDevice, c->stream));
-    if (subb) HIPCHK(hipMemcpyAsync(dsub, w->sub, subb, hipMemcpyHostToDevice, c->stream));
-    rc = repack_into(c, w->kind, w->bits, w->out, w->in, dpk, dsc, (const uint8_t *)dsub, out);
+    Staged pk, sc, sub;
+    rc = pk.take(c, w->packed, pb);
+    if (!rc) rc = sc.take(c, w->scales, sb);
+    if (!rc) rc = sub.take(c, w->sub, subb);
+    if (!rc) rc = repack_into(c, w->kind, w->bits, w->out, w->in, pk.p, sc.p, (const uint8_t *)sub.p, out);
     hipError_t e = hipStreamSynchronize(c->stream);
-    (void)hipFree(dpk); (void)hipFree(dsc);
-    if (dsub) (void)hipFree(dsub);
     if (rc) return rc;
     if (e != hipSuccess) return bgl_fail(BGL_E_HIP, "bind sync: %s", hipGetErrorString(e));
     return 0;

@@ -90,8 +90,10 @@ int  bgl_prof_enable(bgl_ctx *ctx, int on);
 int  bgl_prof_read(bgl_ctx *ctx, double *ms_by_phase, int *launches_by_phase, int nphase);
 
 /* ---------------- weight binding: upload + repack into the tiled device layout ----------------
- * mlx_gpu_bind_af (mlx_moe.h:48-50) / kai_repack_one_lazy (qwen_infer.c:473-487).  Host buffers
- * are read once; the device copy is owned by the returned tensor. */
+ * mlx_gpu_bind_af (mlx_moe.h:48-50) / kai_repack_one_lazy (qwen_infer.c:473-487).  The buffers
+ * are read once, before the call returns; the device copy is owned by the returned tensor.  Each of
+ * them may lie in host memory or on a device: on the context's own (16-byte aligned) it is read in
+ * place, in the order of the context's stream, which has to see it written. */
 int  bgl_bind(bgl_ctx *ctx, const bgl_wt *w, bgl_tensor **out);
 /* Mixed per-cell qNg64 (MixedQNg64Tensor, mlx_moe.cpp:87-93): one width n = bits[cell] (2..15) per
  * (row, 64-group) cell, n bit-planes of 8 bytes at planes + offsets[cell] (the qng64_dense.c plane

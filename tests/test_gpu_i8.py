@@ -275,6 +275,66 @@ def test_bind_decode_and_quantize(ctx, torch_dev, out, inn):
     t.free()
 
 
+@pytest.mark.parametrize("kind,bits", [("K_Q8C", 8), ("K_Q4G64", 4), ("K_Q8G64", 8), ("K_QNG64", 5), ("K_Q4G32H", 4), ("K_Q4G256SF", 4)])
+def test_bind_from_the_device(ctx, torch_dev, kind, bits):
+    """Weights that are on the device are bound from there, aligned or not, to the same tensor as from the host; the buffers are
+    the caller's again when the call returns."""
+    import beglin_amd as B
+    torch = torch_dev
+    kind = getattr(B, kind)
+    for out, inn in ((77, 100), (130, 1411), (64, 512)) if kind == B.K_Q8C else ((70, 512),):
+        dense = torch.from_numpy(np.random.default_rng([out, inn]).standard_normal((out, inn)).astype(np.float32)).cuda()
+        torch.cuda.synchronize()
+        t0, ref = ctx.quantize(kind, dense, bits=bits, want_ref=True)
+        t0.free()
+        got = []
+        for off in (None, 0, 1, 8):                          # from the host; on the device, codes at any address
+            bufs = list(ref)
+            if off is not None:
+                for i, v in enumerate(ref):
+                    if v is not None:
+                        dt = torch.int8 if i != 1 else torch.float16 if kind == B.K_Q4G32H else torch.float32
+                        at = off if i == 0 else 16
+                        raw = torch.zeros(v.nbytes + 64, dtype=torch.uint8, device="cuda")[at:at + v.nbytes]
+                        raw.copy_(torch.from_numpy(np.frombuffer(v.tobytes(), np.uint8).copy()))
+                        bufs[i] = raw.view(dt)
+            torch.cuda.synchronize()
+            t = ctx.bind(kind, bufs[0], bufs[1], out, inn, bits=bits, sub=bufs[2])
+            if off is not None:
+                for v in bufs:
+                    if v is not None:
+                        v.zero_()
+                torch.cuda.synchronize()
+            d = torch.full((out, inn), float("nan"), device="cuda")
+            torch.cuda.synchronize()
+            ctx.dequant(t, 0, out, d)
+            ctx.sync()
+            got.append(d.cpu().numpy())
+            t.free()
+        assert np.isfinite(got[0]).all()
+        for g in got[1:]:
+            assert np.array_equal(g.view(np.uint32), got[0].view(np.uint32))
+
+
+def test_experts_from_the_device(ctx, torch_dev):
+    import beglin_amd as B
+    torch = torch_dev
+    rng = np.random.default_rng(12)
+    E, K, H, W, T = 5, 2, 64, 128, 6
+    parts = [[I.weights(rng, o, k) for _ in range(E)] for o, k in ((W, H), (W, H), (H, W))]
+    on = [[tuple(torch.from_numpy(v).cuda() for v in w) for w in p] for p in parts]
+    torch.cuda.synchronize()
+    stacks = [ctx.bind_experts([(B.K_Q8C, 8, *w) for w in p]) for p in on]
+    x, idx, w = rng.standard_normal((T, H)).astype(np.float32), rng.integers(0, E, (T, K)).astype(np.int32), rng.uniform(0, 1, (T, K)).astype(np.float32)
+    out, xd, idd, wd = torch.empty((T, H), device="cuda"), *(torch.from_numpy(v).cuda() for v in (x, idx, w))
+    torch.cuda.synchronize()
+    ctx.moe_ffn(*stacks, None, xd, idd, wd, out)
+    ctx.check()
+    same(out, I.routed(x, idx, w, *parts))
+    for t in stacks:
+        t.free()
+
+
 @pytest.mark.parametrize("M,H,W", [(1, 256, 700), (5, 96, 130), (33, 1000, 333), (64, 512, 2048), (90, 300, 1001), (2, 64, 18000)])
 def test_mlp(ctx, torch_dev, M, H, W):
     rng = np.random.default_rng([M, H, W])

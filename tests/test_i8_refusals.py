@@ -1,4 +1,4 @@
-"""The checks of Context.matmul_i8 and Context.norm, on the CPU: what the library's entries cannot see behind a pointer is
+"""The checks of Context.matmul_i8, Context.norm and Context.bind, on the CPU: what the library's entries cannot see behind a pointer is
 refused before the call.  The context has no handle, so a call that reaches the library is refused there, with another
 message."""
 import pytest
@@ -107,3 +107,22 @@ def test_norm_calls_reach_the_library():
     for ok in (dict(), dict(yq=torch.zeros((T, 96), dtype=torch.int8)[:, 16:64]), dict(yq=None, yscale=None, y=torch.zeros((T, H)))):
         with pytest.raises(B.BglError, match="bgl_norm_dev: NULL"):
             norm_call(**ok)
+
+
+@pytest.mark.parametrize("codes,scales", [
+    (torch.zeros((4, 8), dtype=torch.int8), torch.zeros(3)), (torch.zeros((4, 8), dtype=torch.int8), torch.zeros(4, dtype=torch.float16)),
+    (torch.zeros((4, 7), dtype=torch.int8), torch.zeros(4)), (torch.zeros((4, 8)), torch.zeros(4)),
+    (torch.zeros((4, 16), dtype=torch.int8)[:, ::2], torch.zeros(4))],
+    ids=["few scales", "scales of 16 bits", "few codes", "codes of another type", "codes with gaps"])
+def test_bind_refused(codes, scales):
+    ctx, _ = setting()
+    with pytest.raises(B.BglError, match="bind:") as e:
+        ctx.bind(B.K_Q8C, codes, scales, 4, 8)
+    assert e.value.code == B.E_ARG
+
+
+def test_bind_of_torch_tensors_reaches_the_library():
+    ctx, _ = setting()
+    for codes, scales in ((torch.zeros((4, 8), dtype=torch.int8), torch.zeros(4)), (torch.zeros((4, 8), dtype=torch.int8).numpy(), torch.zeros(4).numpy())):
+        with pytest.raises(B.BglError, match="bgl_bind: NULL"):
+            ctx.bind(B.K_Q8C, codes, scales, 4, 8)
