@@ -62,17 +62,23 @@ def _type(t):
     return _dtypes().index(t.dtype, 0, 3)
 
 
-def _rows(t, T, H):
-    """Elements between the rows of a [T][H] tensor whose rows are dense."""
-    assert t.shape == (T, H) and (t.stride(1) == 1 or H == 1), "rows must be dense, [T][H]"
-    return t.stride(0) if T > 1 else H
+def _rows(t, T, H, dev):
+    """Pointer and distance in elements of the dense rows of a [T][H] tensor on device dev."""
+    assert t.shape == (T, H), "rows must be [T][H]"
+    ld, one = t.stride()
+    assert one == 1 or H == 1, "rows must be dense"
+    if t.get_device() != dev:
+        _refuse(f"norm: tensors lie on device {dev}")
+    return t.data_ptr(), ld if T > 1 else H
 
 
-def _vec(t, n):
-    """Pointer of an fp32 vector of n values, None passes through."""
+def _vec(t, n, dev):
+    """Pointer of an fp32 vector of n values on device dev, None passes through."""
     if t is None:
         return None
-    assert t.dtype == _dtypes()[0] and t.numel() == n and t.is_contiguous(), "fp32 vector expected"
+    assert t.dtype is _dtypes()[0] and t.numel() == n and t.is_contiguous(), "fp32 vector expected"
+    if t.get_device() != dev:
+        _refuse(f"norm: tensors lie on device {dev}")
     return t.data_ptr()
 
 
@@ -81,21 +87,35 @@ def _w(t):
     return None if t is None else t.data_ptr() if hasattr(t, "data_ptr") else t.ctypes.data
 
 
-def _need(ok, what):
-    """Refuses a call as the library does, for what its entries cannot see behind a pointer."""
-    if not ok:
-        raise BglError(what, E_ARG)
+def _refuse(what):
+    """Refuses a call as the library does, for what its entries cannot see behind a pointer.  (The checks of the calls of a
+    step are written to take no more than the rest of a call: a small product takes 8 us, and so does its host side.)"""
+    raise BglError(what, E_ARG)
+
+
+_ARRAYS = {}
+
+
+def _arrays(n):
+    """Arrays for n tensors, outputs, biases (all NULL) and row strides."""
+    if n not in _ARRAYS:
+        _ARRAYS[n] = C.c_void_p * n, C.c_long * n
+    p, l = _ARRAYS[n]
+    return p(), p(), p(), l()
 
 
 def _weights(kind, out, inn, packed, scales, sub):
     """What a bind reads of torch tensors: dense ones, scales of the kind's type, and K_Q8C's buffers whole."""
     for t in (packed, scales, sub):
-        _need(not hasattr(t, "data_ptr") or t.is_contiguous(), "bind: torch tensors have to be dense")
+        if hasattr(t, "data_ptr") and not t.is_contiguous():
+            _refuse("bind: torch tensors have to be dense")
     if hasattr(scales, "data_ptr"):
-        _need(scales.element_size() == 2 if kind == K_Q4G32H else scales.dtype == _dtypes()[0], "bind: scales of another type")
-        _need(kind != K_Q8C or scales.numel() == out, f"bind: K_Q8C takes scales [out={out}]")
-    if hasattr(packed, "data_ptr"):
-        _need(kind != K_Q8C or (packed.dtype == _dtypes()[3] and packed.numel() == out * inn), f"bind: K_Q8C takes int8 codes [{out}][{inn}]")
+        if not (scales.element_size() == 2 if kind == K_Q4G32H else scales.dtype is _dtypes()[0]):
+            _refuse("bind: scales of another type")
+        if kind == K_Q8C and scales.numel() != out:
+            _refuse(f"bind: K_Q8C takes scales [out={out}]")
+    if kind == K_Q8C and hasattr(packed, "data_ptr") and not (packed.dtype is _dtypes()[3] and packed.numel() == out * inn):
+        _refuse(f"bind: K_Q8C takes int8 codes [{out}][{inn}]")
 
 
 class Tensor:
@@ -260,54 +280,83 @@ class Context:
         """ys[i] = (codes xq [M][>= in] times the K_Q8C tensor ts[i]) * scales + biases[i] (bgl_matmul_i8_dev); ys are fp32,
         fp16 or bf16 tensors [M][out] of one type, whose rows may be apart.  A single tensor, y and bias need no lists."""
         if isinstance(ts, Tensor):
-            ts, ys, biases = [ts], [ys], [biases]
-        n, bias = len(ts), biases or [None] * len(ts)
-        _need(0 < n == len(ys) == len(bias) and xq_dev.dim() == 2, "matmul_i8: one y (and bias) a tensor, codes [M][>= in]")
-        M, kind, inn = xq_dev.shape[0], ys[0].dtype, ts[0].shape()[1]
-        _need(xq_dev.dtype == _dtypes()[3] and xq_dev.stride(1) == 1 and xq_dev.shape[1] >= inn, f"matmul_i8: codes are dense int8 rows of at least in={inn}")
+            ts, ys, biases = (ts,), (ys,), (biases,)
+        f32, f16, bf16, i8 = _dtypes()
+        n, dev = len(ts), self.device
+        if not biases:
+            biases = (None,) * n
+        if not (0 < n == len(ys) == len(biases) and xq_dev.ndim == 2):
+            _refuse("matmul_i8: one y (and bias) a tensor, codes [M][>= in]")
+        M, width = xq_dev.shape
+        ldq, dense = xq_dev.stride()
+        inn, kind = ts[0].shape()[1], ys[0].dtype
+        if xq_dev.dtype is not i8 or dense != 1 or width < inn:
+            _refuse(f"matmul_i8: codes are dense int8 rows of at least in={inn}")
         # the kernels read the row's bytes up to the next multiple of 16
-        _need(xq_dev.shape[1] >= (inn + 15) // 16 * 16 or
-              xq_dev.storage_offset() + (M - 1) * xq_dev.stride(0) + (inn + 15) // 16 * 16 <= xq_dev.untyped_storage().nbytes(),
-              "matmul_i8: the last row of codes ends before a multiple of 16 bytes")
-        _need(ascale_dev.dtype == _dtypes()[0] and ascale_dev.numel() == M and ascale_dev.is_contiguous(), f"matmul_i8: scales are fp32 [{M}]")
-        for t, y, b in zip(ts, ys, bias):
+        if width < inn + 15 & -16 and xq_dev.storage_offset() + (M - 1) * ldq + (inn + 15 & -16) > xq_dev.untyped_storage().nbytes():
+            _refuse("matmul_i8: the last row of codes ends before a multiple of 16 bytes")
+        if ascale_dev.dtype is not f32 or ascale_dev.numel() != M or not ascale_dev.is_contiguous():
+            _refuse(f"matmul_i8: scales are fp32 [{M}]")
+        here = xq_dev.get_device() == dev == ascale_dev.get_device()
+        W, Y, B, S = _arrays(n)
+        for i in range(n):
+            t, y, b = ts[i], ys[i], biases[i]
             out = t.shape()[0]
-            _need(y.dtype == kind and kind in _dtypes()[:3] and y.shape == (M, out) and (y.stride(1) == 1 or out == 1),
-                  f"matmul_i8: y is [{M}][{out}] of one type (fp32, fp16, bf16) with dense rows")
-            _need(b is None or (b.dtype == _dtypes()[0] and b.numel() == out and b.is_contiguous()), f"matmul_i8: a bias is fp32 [{out}]")
-        _need(all(v is None or v.get_device() == self.device for v in (xq_dev, ascale_dev, *ys, *bias)), f"matmul_i8: tensors lie on device {self.device}")
-        W = (C.c_void_p * n)(*[t.h.value for t in ts])
-        Y = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-        B = (C.c_void_p * n)(*[(b.data_ptr() if b is not None else None) for b in bias])
-        S = (C.c_long * n)(*[y.stride(0) if M > 1 else y.shape[1] for y in ys])
-        _check(lib().bgl_matmul_i8_dev(self.h, n, W, C.c_void_p(xq_dev.data_ptr()), xq_dev.stride(0) if M > 1 else xq_dev.shape[1],
-                                       _p(ascale_dev), B, Y, _type(ys[0]), S, M), "bgl_matmul_i8_dev")
+            if y.dtype is not kind or y.shape != (M, out):
+                _refuse(f"matmul_i8: y is [{M}][{out}] of one type")
+            ld, dense = y.stride()
+            if dense != 1 and out > 1:
+                _refuse("matmul_i8: rows of y are dense")
+            here = here and y.get_device() == dev
+            if b is not None:
+                if b.dtype is not f32 or b.numel() != out or not b.is_contiguous():
+                    _refuse(f"matmul_i8: a bias is fp32 [{out}]")
+                here = here and b.get_device() == dev
+                B[i] = b.data_ptr()
+            W[i], Y[i], S[i] = t.h.value, y.data_ptr(), ld if M > 1 else out
+        type_ = T_F32 if kind is f32 else T_F16 if kind is f16 else T_BF16 if kind is bf16 else _refuse("matmul_i8: y is fp32, fp16 or bf16")
+        if not here:
+            _refuse(f"matmul_i8: tensors lie on device {dev}")
+        _check(lib().bgl_matmul_i8_dev(self.h, n, W, xq_dev.data_ptr(), ldq if M > 1 else width, ascale_dev.data_ptr(), B, Y, type_, S, M),
+               "bgl_matmul_i8_dev")
 
     def norm(self, x, y=None, *, yq=None, yscale=None, kind=NORM_RMS, w=None, b=None, eps=1e-6, w_add=0.0, x_out=None, branch=None,
              branch_kind=NORM_NONE, branch_w=None, branch_b=None, branch_eps=1e-6, gate=None, alpha=1.0):
         """x_out = x + alpha * gate * branch_kind(branch), and y / (yq, yscale) = kind(x_out) (bgl_norm_dev) over [T][H] rows.
         gate: of the branch's type, [1][H], [T][1] or [T][H].  yq: int8 [T][H up to a multiple of 16], yscale: fp32 [T]."""
         T, H = x.shape
-        d = capi.bgl_norm(T=T, H=H, x=x.data_ptr(), ldx=_rows(x, T, H), x_type=_type(x), alpha=alpha, w_add=w_add, kind=kind,
-                          w=_vec(w, H), b=_vec(b, H), eps=eps)
+        dev = self.device
+        d = capi.bgl_norm(T, H, *_rows(x, T, H, dev), _type(x))
+        d.alpha, d.kind, d.eps = alpha, kind, eps
+        if w_add:
+            d.w_add = w_add
+        if w is not None:
+            d.w = _vec(w, H, dev)
+        if b is not None:
+            d.b = _vec(b, H, dev)
         if branch is not None:
-            d.f, d.ldf, d.f_type = branch.data_ptr(), _rows(branch, T, H), _type(branch)
-        d.post, d.post_w, d.post_b, d.post_eps = branch_kind, _vec(branch_w, H), _vec(branch_b, H), branch_eps
+            (d.f, d.ldf), d.f_type = _rows(branch, T, H, dev), _type(branch)
+        if branch_kind:
+            d.post, d.post_eps, d.post_w, d.post_b = branch_kind, branch_eps, _vec(branch_w, H, dev), _vec(branch_b, H, dev)
         if gate is not None:
             assert branch is not None and gate.dtype == branch.dtype and gate.dim() == 2
             assert gate.shape[0] in (1, T) and gate.shape[1] in (1, H) and (gate.shape[1] == 1 or gate.stride(1) == 1)
+            if gate.get_device() != dev:
+                _refuse(f"norm: tensors lie on device {dev}")
             d.gate, d.gate_t, d.gate_c = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else 0, int(gate.shape[1] > 1)
         if x_out is not None:
             assert x_out.dtype == x.dtype
-            d.x_out, d.ldo = x_out.data_ptr(), _rows(x_out, T, H)
+            d.x_out, d.ldo = _rows(x_out, T, H, dev)
         if y is not None:
-            d.y, d.ldy, d.y_type = y.data_ptr(), _rows(y, T, H), _type(y)
+            (d.y, d.ldy), d.y_type = _rows(y, T, H, dev), _type(y)
         if yq is not None:
-            _need(yq.dtype == _dtypes()[3] and yq.dim() == 2 and yq.shape[0] == T and yq.shape[1] >= (H + 15) // 16 * 16 and yq.stride(1) == 1 and
-                  yscale is not None and yscale.numel() == T, f"norm: yq is int8 [{T}][H={H} up to a multiple of 16] with dense rows, yscale [{T}]")
-            d.yq, d.ldq, d.yscale = yq.data_ptr(), yq.stride(0) if T > 1 else yq.shape[1], _vec(yscale, T)
-        _need(all(v is None or v.get_device() == self.device for v in (x, y, yq, yscale, w, b, x_out, branch, branch_w, branch_b, gate)),
-              f"norm: tensors lie on device {self.device}")
+            rows, width = yq.shape if yq.ndim == 2 else (0, 0)
+            ld, one = yq.stride() if rows == T else (0, 0)
+            if one != 1 or width < H + 15 & -16 or yq.dtype is not _dtypes()[3] or yscale is None or yscale.numel() != T:
+                _refuse(f"norm: yq is int8 [{T}][H={H} up to a multiple of 16] with dense rows, yscale [{T}]")
+            if yq.get_device() != dev:
+                _refuse(f"norm: tensors lie on device {dev}")
+            d.yq, d.ldq, d.yscale = yq.data_ptr(), ld if T > 1 else width, _vec(yscale, T, dev)
         _check(lib().bgl_norm_dev(self.h, C.byref(d)), "bgl_norm_dev")
 
     # ---- MoE ----

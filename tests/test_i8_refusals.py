@@ -104,7 +104,8 @@ def test_norm_refused(change):
 
 
 def test_norm_calls_reach_the_library():
-    for ok in (dict(), dict(yq=torch.zeros((T, 96), dtype=torch.int8)[:, 16:64]), dict(yq=None, yscale=None, y=torch.zeros((T, H)))):
+    for ok in (dict(), dict(w=torch.zeros(H), b=torch.zeros((1, H)), branch=torch.zeros((T, 64))[:, :H], branch_kind=B.NORM_RMS, branch_w=torch.zeros(H),
+                            gate=torch.zeros((1, H)), x_out=torch.zeros((T, H))), dict(yq=torch.zeros((T, 96), dtype=torch.int8)[:, 16:64]), dict(yq=None, yscale=None, y=torch.zeros((T, H)))):
         with pytest.raises(B.BglError, match="bgl_norm_dev: NULL"):
             norm_call(**ok)
 
