@@ -181,7 +181,7 @@ def _bind(s):
     bound = []
 
     def one(codes, scales):
-        t = s.ctx.bind(B.K_Q8C, codes.cpu().numpy(), scales.cpu().numpy(), *codes.shape)
+        t = s.ctx.bind(B.K_Q8C, codes, scales, *codes.shape)         # from where they lie, on the device
         bound.append(t)
         return t
 
