@@ -22,8 +22,9 @@
 // Workgroups wait only for ones with lower ids, and find their expert and its pairs from the routing themselves.  1024
 // threads with up to 128 registers fill a CU, so that equal shares take equal times (with 512 threads a CU often had two
 // workgroups of down and its neighbour none: 173 us for 32 tokens, and 161 as four launches).
-// 64 experts of 2048 x 1408, 6 a token, a shared 2816: 1 token 31 us (four launches 41), 8 tokens 76 (96), 32 tokens 129
-// (161), 64 tokens 153 (204).  32 tokens' gate and up move 4.9 TB/s, a large copy 5.1; what is above the bytes' time is the
+// 64 experts of 2048 x 1408, 6 a token, a shared 2816, three layers' weights and seven sets of tokens in turn in a graph:
+// 1 token 31 us (four launches 41), 8 tokens 77 (96), 32 tokens 130 (161), 64 tokens 155 (204), 128 as two launches 309.
+// (With the same token's experts in the last-level cache 1 token takes 28.6.)  32 tokens' gate and up move 4.9 TB/s, a large copy 5.1; what is above the bytes' time is the
 // routing (9 us at one token from the first load to the last workgroup's list, of which 2.4 the top-K), the codes between
 // the last h and down's products (6) and the slowest CU's share.
 #include <string.h>

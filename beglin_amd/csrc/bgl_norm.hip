@@ -12,8 +12,11 @@
 // Every value is computed in double and rounded once to fp32 (and from there to a 16-bit type): a code
 // of the int8 output changes by one where a value lies within rounding of a border between codes, and
 // with the values right to fp32's last bit the codes are those of the formula.  gfx950 issues double
-// multiply-adds at the rate of single ones, and the launch is bound by memory: 4096 rows of 4096 in bf16
-// (residual add, RMS norm) take 31 us, 4.3 TB/s of what they read and write, where a large copy moves 5.1.
+// multiply-adds at the rate of single ones.  Rows normed once are bound by memory: 4096 rows of 4096 in bf16
+// (residual add, RMS norm) take 31 us, 4.4 TB/s of what they read and write, where a large copy moves 5.1, and the
+// vector units issue for 11 of them.  Rows normed twice are not: 777 of 2883 with two layer norms and a gate take 15.3 us,
+// of which 7 to 9 are issue (77 instructions a value's place), 6 the bytes, and the waves wait 58% of the time, for loads
+// and at the barriers of four sums.
 //
 // The row stays in registers between its passes (statistics, then the output): a wave to a row up to H = 512, then
 // workgroups of 256, 512 or 1024 threads with 8 or 16 values each.  Wider

@@ -178,8 +178,10 @@ int  bgl_quant_act_i8_dev(bgl_ctx *ctx, const float *x_dev, int M, int in, int g
  * y_type (BGL_T_*).  xq: rows ldq bytes apart, ldq % 16 == 0, ldq >= in, 16-byte aligned; the bytes
  * between in and the row's next multiple of 16 may hold anything.  ascale [M].  bias_dev, or an entry
  * of it, may be NULL.  y[i]: rows ldy[i] values apart (ldy NULL: dense), so a group may fill the parts of
- * one wider row.  A product whose K is split over workgroups keeps its sums in the context's scratch,
- * which a capture must not have to grow; no counterpart in the reference.  bgl_matmul_dev, bgl_matmul_group_dev, bgl_mlp_dev,
+ * one wider row.  A product whose K is split over workgroups keeps its sums in the context's scratch
+ * (40 MB, reserved by the first product with in > 896), which a capture must not have to grow and
+ * which graphs captured from one context share: replay them one after the other.  No counterpart in
+ * the reference.  bgl_matmul_dev, bgl_matmul_group_dev, bgl_mlp_dev,
  * bgl_prep_act_dev / bgl_matmul_prepped_dev, bgl_quantize_dev (largest |w| of a row = 127) and
  * bgl_dequant_dev take K_Q8C as any kind; bgl_moe_ffn_dev and bgl_moe_layer_dev take stacks of it. */
 int  bgl_matmul_i8_dev(bgl_ctx *ctx, int n, const bgl_tensor *const *w, const int8_t *xq_dev, long ldq, const float *ascale_dev,
