@@ -489,8 +489,8 @@ struct Staged {
     int take(bgl_ctx *c, const void *src, size_t bytes) {
         if (!bytes) return 0;
         hipPointerAttribute_t a;
-        const bool dev = hipPointerGetAttributes(&a, src) == hipSuccess && a.type == hipMemoryTypeDevice;
-        (void)hipGetLastError();                             // host memory that HIP does not know is no error
+        const bool known = hipPointerGetAttributes(&a, src) == hipSuccess, dev = known && a.type == hipMemoryTypeDevice;
+        if (!known) (void)hipGetLastError();                 // host memory that HIP does not know is no error
         if (dev && a.device == c->device && (uintptr_t)src % 16 == 0) { p = src; return 0; }
         HIPCHK(hipMalloc(&own, bytes));
         p = own;
