@@ -14,6 +14,7 @@ K_Q4G64, K_Q8G64, K_Q4G256SF, K_QNG64, K_Q4G32H = 1, 2, 3, 4, 5
 K_Q4G64A, K_F16, K_F32, K_MXFP4, K_Q4G256P, K_Q8C = 6, 7, 8, 9, 10, 11
 T_F32, T_F16, T_BF16 = 0, 1, 2
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+ROT_NONE, ROT_HALF, ROT_PAIRS = 0, 1, 2
 ACT_F32, ACT_W4A8 = 0, 1
 
 _P = C.c_void_p
@@ -32,6 +33,24 @@ class bgl_norm(C.Structure):
                 ("gate", _P), ("gate_t", _L), ("gate_c", _L), ("alpha", C.c_float), ("w_add", C.c_float),
                 ("x_out", _P), ("ldo", _L), ("kind", _I), ("w", _P), ("b", _P), ("eps", C.c_float),
                 ("y", _P), ("ldy", _L), ("y_type", _I), ("yq", _P), ("ldq", _L), ("yscale", _P)]
+
+
+class bgl_heads(C.Structure):
+    _fields_ = [("T", _I), ("D", _I), ("nq", _I), ("nk", _I), ("q", _P), ("k", _P), ("v", _P),
+                ("ldq", _L), ("hdq", _L), ("ldk", _L), ("hdk", _L), ("ldv", _L), ("hdv", _L), ("type", _I),
+                ("norm", _I), ("q_w", _P), ("k_w", _P), ("eps", C.c_float), ("w_add", C.c_float),
+                ("rot_kind", _I), ("rot", _I), ("rope", _P), ("n_pos", _I), ("pos", _P),
+                ("q_out", _P), ("k_out", _P), ("ldqo", _L), ("hdqo", _L), ("ldko", _L), ("hdko", _L), ("out_type", _I)]
+
+
+class bgl_kv(C.Structure):
+    _fields_ = [("data", _P), ("pages", _I), ("page", _I), ("heads", _I), ("D", _I)]
+
+
+class bgl_attn(C.Structure):
+    _fields_ = [("S", _I), ("T", _I), ("nq", _I), ("q", _P), ("ldq", _L), ("hdq", _L), ("out", _P), ("ldo", _L), ("hdo", _L),
+                ("type", _I), ("start", _P), ("len", _P), ("table", _P), ("ldt", _I),
+                ("scale", C.c_float), ("causal", _I), ("window", _I), ("sink", _P), ("max_rows", _I), ("max_len", _I)]
 
 
 # (name, restype, argtypes) for every entry point declared in include/beglin_qgemv.h
@@ -60,6 +79,11 @@ SIGNATURES = [
     ("bgl_quant_act_i8_dev", _I, [_P, _P, _I, _I, _I, _P, _P]),
     ("bgl_matmul_i8_dev", _I, [_P, _I, C.POINTER(_P), _P, _L, _P, C.POINTER(_P), C.POINTER(_P), _I, C.POINTER(_L), _I]),
     ("bgl_norm_dev", _I, [_P, C.POINTER(bgl_norm)]),
+    ("bgl_heads_dev", _I, [_P, C.POINTER(bgl_heads)]),
+    ("bgl_kv_bytes", C.c_size_t, [_I, _I, _I, _I]),
+    ("bgl_kv_append_dev", _I, [_P, C.POINTER(bgl_kv), C.POINTER(bgl_heads), _P]),
+    ("bgl_kv_read_dev", _I, [_P, C.POINTER(bgl_kv), _P, _I, _P, _L, _L, _P, _L, _L, _I]),
+    ("bgl_attn_dev", _I, [_P, C.POINTER(bgl_kv), C.POINTER(bgl_attn)]),
     ("bgl_gemv_q4g64_mt", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),
     ("bgl_gemv_q4g64_mt_fused", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),
     ("bgl_gemv_q4g64_sdot_mt", _I, [_P, _P, _P, _P, _P, _P, _I, _I]),

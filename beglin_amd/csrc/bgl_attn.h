@@ -1,0 +1,88 @@
+// bgl_attn.h -- what the kernels of attention over the 4-bit cache share: the launch, which rows and keys belong
+// together, the cache's codes as matrix-core operands, and the end of a row.
+#pragma once
+#include "bgl_kv.h"
+
+typedef unsigned int at_u4 __attribute__((ext_vector_type(4)));
+
+struct AttnLaunch {
+    bgl_kv c;
+    bgl_attn a;
+    int g;                       // heads of q for one of the cache
+    int ppt, ppt_shift;          // 16-token tiles a page; log2 of it, or -1
+    int limit;                   // sequences with more than this many rows times g are another launch's
+    float scale2;                // |scale| * log2(e); a negative scale turns q's sign
+    float *part;                 // bgl_attn.hip's partial sums: [2 * workgroups] pieces
+    int *sync;                   // pieces written, for each workgroup that began one
+};
+
+// Weights are 2^14 exp(..): the largest is 2^14, so that fp16 keeps 11 bits of what is 2^28 times smaller.
+#define AT_P2 14.0f
+
+// A sequence: its rows (begin, n), its keys, and the range [lo, len) that one of its rows may see.
+struct AttnSeq {
+    int begin, n, len, lo;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnLaunch &L, int s) {
+    AttnSeq q;
+    const int b = L.a.start[s], e = L.a.start[s + 1], len = L.a.len[s];
+    q.begin = min(max(b, 0), L.a.T);
+    q.n = max(0, min(e, L.a.T) - q.begin);
+    q.len = (int)min((long)max(len, 0), (long)L.a.ldt * L.c.page);
+    q.lo = L.a.window ? (int)max(0l, (long)q.len - q.n - L.a.window + 1) : 0;
+    q.lo = min(q.lo, q.len);
+    return q;
+}
+// The keys [lo, hi] that row i of n sees (none: hi < lo).
+__device__ __forceinline__ void attn_keys(const AttnLaunch &L, const AttnSeq &q, int i, int &lo, int &hi) {
+    const int pos = q.len - q.n + i;
+    hi = L.a.causal ? min(pos, q.len - 1) : q.len - 1;
+    lo = L.a.window ? (int)max(0l, (long)pos - L.a.window + 1) : 0;
+}
+
+// ------------------------------------------------------------------ the cache's codes as operands
+// fp16 pairs of the codes at bits 0 or 4 of each half of w (see bgl_kv.h), times s plus m, rounded once
+__device__ __forceinline__ kv_h2 at_lo(uint32_t w, kv_h2 s, kv_h2 m) {
+    const kv_h2 c = __builtin_bit_cast(kv_h2, (w & 0x000f000fu) | 0x64006400u) - kv_h2{(_Float16)1024.0f, (_Float16)1024.0f};
+    return __builtin_elementwise_fma(c, s, m);
+}
+__device__ __forceinline__ kv_h2 at_hi(uint32_t w, kv_h2 s, kv_h2 m) {
+    const kv_h2 c = __builtin_bit_cast(kv_h2, (w & 0x00f000f0u) | 0x54005400u) - kv_h2{(_Float16)64.0f, (_Float16)64.0f};
+    return __builtin_elementwise_fma(c, s, m);
+}
+__device__ __forceinline__ kv_h8 at_join(kv_h2 a, kv_h2 b, kv_h2 c, kv_h2 d) {
+    return kv_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// 8 neighbouring values of a key from their dword and the group's (s, m)
+__device__ __forceinline__ kv_h8 at_key(uint32_t w, uint32_t sm) {
+    const kv_h2 p = __builtin_bit_cast(kv_h2, sm), s = {p[0], p[0]}, m = {p[1], p[1]};
+    return at_join(at_lo(w, s, m), at_hi(w, s, m), at_lo(w >> 8, s, m), at_hi(w >> 8, s, m));
+}
+
+__device__ __forceinline__ kv_f4 at_mfma(kv_h8 a, kv_h8 b, kv_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Maxima and sums over the four lanes of a wave that hold the same row (l, l ^ 16, l ^ 32, l ^ 48), in every one of them.
+__device__ __forceinline__ float at_max4(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float at_sum4(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// ------------------------------------------------------------------ a row's end
+// What the sum of values (weights 2^14 exp2(s - M)) is multiplied by: 1 / (their sum + the sink's weight); 0 for a row without a key.
+__device__ __forceinline__ float attn_factor(float M, float sum, bool sink, float sink2) {
+    if (!sink) return M == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float top = fmaxf(M, sink2);
+    if (top == -INFINITY && sum == 0.0f) return 0.0f;
+    const float f = M == -INFINITY ? 0.0f : at_exp2(M - top);
+    return f / (sum * f + at_exp2(sink2 - top + AT_P2));
+}
+

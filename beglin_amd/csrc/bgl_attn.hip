@@ -1,0 +1,536 @@
+// bgl_attn.hip -- attention of a few rows a sequence (single tokens, drafted ones) over the paged cache in 4 bits:
+//
+//   s_j = scale q . k_j;   out = sum_j exp(s_j - M) v_j / sum_j exp(s_j - M)      one pass: M, both sums and out run along
+//
+// The rows are bound by the cache's bytes, 1.25 D for a key and head, read once for all of a head's group of query rows.  Those
+// rows (g heads of q times the tokens) are the 16 columns of the matrix instruction, keys its rows:
+//   scores   S^T = K Q^T: a lane has 4 keys of one query row from each 16-key tile
+//   output   O^T = V^T P^T: what a lane has of S^T is, as weights, its part of P^T's operand: nothing is moved between lanes
+// but the row maxima; a row's statistics lie in the lanes that hold its sums.
+//
+// Work: 128 keys of one head and row block are a unit, 32 for each wave.  The units of all sequences lie in one line that
+// is cut into equal runs, one a workgroup, so a batch of very different lengths leaves no workgroup behind.  A head whose
+// keys end up in several runs is joined by whichever of them finishes last, in the order of its keys: the same bits every time.
+#include <string.h>
+
+#include <algorithm>
+
+#include "../../include/beglin_qgemv.h"
+#include "bgl_i8.h"
+#include "bgl_attn.h"
+
+#define HIPCHK(expr)                                                                             \
+    do {                                                                                         \
+        hipError_t e_ = (expr);                                                                  \
+        if (e_ != hipSuccess) return bgl_fail(BGL_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+    } while (0)
+
+#define AT_UNIT 128              // keys a unit
+#define AT_WG 768                // workgroups at most
+
+// What a wave has loaded of 32 keys: two tiles.
+template <int G>
+struct AttnRaw {
+    static constexpr bool K2 = G % 3 == 0 || G > 4, V2 = G % 3 == 0;      // a lane's values lie in one group of 32, or in two
+    uint32_t kc[2][G], vc[2][G], ks[2][K2 ? 2 : 1];
+    at_u4 vs[2][V2 ? 2 : 1];
+};
+
+// Dwords i .. of G at any 4-byte place.
+template <int G>
+__device__ __forceinline__ void at_dwords(uint32_t (&w)[G], const uint8_t *p) {
+    typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef unsigned int u2 __attribute__((ext_vector_type(2), aligned(4)));
+#pragma unroll
+    for (int i = 0; i + 4 <= G; i += 4) {
+        const u4 v = *(const u4 *)(p + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[i + j] = v[j];
+    }
+    constexpr int at = G / 4 * 4;
+    if constexpr (G % 4 >= 2) {
+        const u2 v = *(const u2 *)(p + 4 * at);
+        w[at] = v[0];
+        w[at + 1] = v[1];
+    }
+    if constexpr (G % 2) w[G - 1] = *(const uint32_t *)(p + 4 * (G - 1));
+}
+
+template <int G, int NT, int PARTS>
+struct AttnWave {
+    static constexpr int D = 32 * G, RB = 16 * NT;
+    const AttnLaunch &L;
+    const int lane, col, b;                              // col: the lane's query row of each 16, key of a K tile, unit of a V tile
+    AttnSeq q;
+    int head;
+    ucint table;
+    kv_h8 qf[NT][PARTS][G];
+    float fac[NT], zero[NT];                             // zero: where scores begin; NaN for a query with a NaN or an infinity
+    int lo[NT], hi[NT], lo_max, hi_min;
+    kv_f4 o[NT][2 * G];
+    float m[NT], l[NT];
+
+    __device__ AttnWave(const AttnLaunch &l_) : L(l_), lane(threadIdx.x & 63), col(threadIdx.x & 15), b((threadIdx.x >> 4) & 3) {}
+
+    // Rows rb * RB .. of the sequence's n * g (row r: token r / g, head r % g of the group), scaled by a power of two that puts a
+    // row's largest value in [2^14, 2^15): exact in fp16 down to 2^-28 of it (two parts for fp32 rows, 2^-22).
+    __device__ void begin(int s, int head_, int rb) {
+        head = head_;
+        table = uni(L.a.table + (size_t)s * L.a.ldt);
+        lo_max = 0;
+        hi_min = INT32_MAX;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int rows = q.n * L.g, r = rb * RB + 16 * t + col, rr = min(r, rows - 1), i = rr / L.g;
+            const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
+            attn_keys(L, q, i, lo[t], hi[t]);
+            lo_max = max(lo_max, lo[t]);
+            hi_min = min(hi_min, hi[t]);
+            float x[G][8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                kv_load8(x[j], L.a.q, L.a.type, at + 8 * j);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[j][e]) & 0x7fffffffu);
+            }
+            top = __float_as_uint(at_max4(__uint_as_float(min(top, 0x7f800000u))));        // NaN counts as an infinity
+            const bool bad = top >= 0x7f800000u;
+            const int ex = bad || top == 0 ? 14 : max((int)(top >> 23), 1) - 127;
+            const float turn = L.a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float y = bad ? 0.0f : ldexpf(x[j][e], 14 - ex) * turn;
+                    const _Float16 h = (_Float16)y;
+                    qf[t][0][j][e] = h;
+                    if constexpr (PARTS == 2) qf[t][1][j][e] = (_Float16)(y - (float)h);
+                }
+            }
+            // (a factor of 0 would make NaN of masked scores)
+            fac[t] = fmaxf(ldexpf(L.scale2, ex - 14), 1e-30f);
+            zero[t] = bad ? NAN : 0.0f;
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) o[t][j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+            lo_max = max(lo_max, __shfl_xor(lo_max, x));
+            hi_min = min(hi_min, __shfl_xor(hi_min, x));
+        }
+        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+        hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    }
+
+    // The page of the tile at a key (a multiple of 16), or -1: past the keys, or no page.
+    __device__ __forceinline__ int page(int key) const {
+        if (key >= q.len) return -1;
+        const int t = key >> 4, pg = table[L.ppt_shift >= 0 ? t >> L.ppt_shift : t / L.ppt];
+        return pg >= 0 && pg < L.c.pages ? pg : -1;
+    }
+    __device__ __forceinline__ void load(AttnRaw<G> &w, int key, const int (&pg)[2]) const {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int t = (key >> 4) + h, in = L.ppt_shift >= 0 ? t & (L.ppt - 1) : t % L.ppt;
+            // a tile without a page loads the first record, and none of it counts
+            const size_t rec = pg[h] < 0 ? 0 : ((size_t)pg[h] * L.c.heads + head) * L.ppt + in;
+            const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
+            at_dwords<G>(w.kc[h], p + lane * (4 * G));
+            at_dwords<G>(w.vc[h], p + 10 * D + lane * (4 * G));
+            const uint32_t *ks = (const uint32_t *)(p + 8 * D);
+            const at_u4 *vs = (const at_u4 *)(p + 18 * D);
+            w.ks[h][0] = ks[(G * b >> 2) * 16 + col];
+            w.vs[h][0] = vs[(G * col >> 4) * 4 + b];
+            if constexpr (AttnRaw<G>::K2) w.ks[h][1] = ks[((G * b + G - 1) >> 2) * 16 + col];
+            if constexpr (AttnRaw<G>::V2) w.vs[h][1] = vs[((G * col + G - 1) >> 4) * 4 + b];
+        }
+    }
+
+    // Keys key .. key + 31 into m, l and o.
+    __device__ __forceinline__ void step(AttnRaw<G> &w, int key, const int (&pg)[2]) {
+        constexpr bool K2 = AttnRaw<G>::K2, V2 = AttnRaw<G>::V2;
+        kv_f4 s[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = kv_f4{zero[t], zero[t], zero[t], zero[t]};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                const uint32_t sm = K2 && (G * b + j) >> 2 != G * b >> 2 ? w.ks[h][K2] : w.ks[h][0];
+                const kv_h8 k = at_key(w.kc[h][j], sm);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) s[t][h] = at_mfma(k, qf[t][p][j], s[t][h]);
+                }
+            }
+        }
+        // Some of the keys may be hidden from some rows: at the last key, along the rows' diagonal, at the window's edge.
+        const bool some = pg[0] < 0 || pg[1] < 0 || key < lo_max || key + 31 > hi_min;
+        bool poison = false;
+        kv_h8 bad[V2 ? 2 : 1], seen[NT];
+        if (some) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k0 = key + 16 * h + 4 * b;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const bool see = pg[h] >= 0 && k0 + r >= lo[t] && k0 + r <= hi[t];
+                        s[t][h][r] = see ? s[t][h][r] : -INFINITY;
+                        seen[t][4 * h + (r & 1) * 2 + (r >> 1)] = see ? (_Float16)1.0f : (_Float16)0.0f;
+                    }
+                }
+                // Memory behind the last key holds anything: 0 there, which a weight of 0 leaves 0.
+                const int left = pg[h] < 0 ? 0 : q.len - k0;
+                const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
+                const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int x = 0; x < (V2 ? 2 : 1); x++) {
+                    w.vs[h][x] &= at_u4{e, f, e, f};
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const uint32_t v = w.vs[h][x][2 + (y >> 1)] >> (16 * (y & 1));
+                        const bool nan = (v & 0x7c00u) == 0x7c00u;
+                        bad[x][4 * h + y] = nan ? (_Float16)1.0f : (_Float16)0.0f;
+                        poison |= nan;
+                    }
+                }
+            }
+            poison = __any(poison);
+            if (poison) {                                // NaN among them: it reaches the rows that see it, below
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int x = 0; x < (V2 ? 2 : 1); x++)
+#pragma unroll
+                        for (int y = 0; y < 4; y++)
+                            if (bad[x][4 * h + y] != (_Float16)0.0f) w.vs[h][x][2 + (y >> 1)] &= y & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+        }
+        kv_h8 pf[NT][PARTS];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float top = s[t][0][0];
+#pragma unroll
+            for (int x = 1; x < 8; x++) top = fmaxf(top, s[t][x >> 2][x & 3]);
+            top = at_max4(top) * fac[t];
+            if (__any(top > m[t])) {
+                const float to = fmaxf(m[t], top), f = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
+                m[t] = to;
+                l[t] *= f;
+#pragma unroll
+                for (int j = 0; j < 2 * G; j++) o[t][j] *= f;
+            }
+            const float off = AT_P2 - (m[t] == -INFINITY ? 0.0f : m[t]);
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const int h = x >> 2, r = x & 3;
+                const float p = at_exp2(fmaf(s[t][h][r], fac[t], off));
+                l[t] += p;
+                const int at = 4 * h + (r & 1) * 2 + (r >> 1);      // tokens 0, 2, 1, 3: the order of V's pairs
+                pf[t][0][at] = (_Float16)p;
+                if constexpr (PARTS == 2) pf[t][1][at] = (_Float16)(p - (float)pf[t][0][at]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            kv_h2 v[2][4];                               // values 2 j (pairs 0, 2 and 1, 3 of each tile) and 2 j + 1
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const at_u4 z = V2 && (G * col + j) >> 4 != G * col >> 4 ? w.vs[h][V2] : w.vs[h][0];
+                const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
+                const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
+                const uint32_t c = w.vc[h][j], d = c >> 8;
+                v[0][2 * h] = at_lo(c, s0, m0);
+                v[0][2 * h + 1] = at_lo(d, s1, m1);
+                v[1][2 * h] = at_hi(c, s0, m0);
+                v[1][2 * h + 1] = at_hi(d, s1, m1);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const kv_h8 a = at_join(v[e][0], v[e][1], v[e][2], v[e][3]);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) o[t][2 * j + e] = at_mfma(a, pf[t][p], o[t][2 * j + e]);
+                }
+            }
+        }
+        if (poison) {
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                const kv_h8 a = V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const kv_f4 n = at_mfma(a, seen[t], kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (n[i] > 0.0f) o[t][2 * j][i] = o[t][2 * j + 1][i] = NAN;
+                }
+            }
+        }
+    }
+};
+
+template <int G, int NT>
+struct AttnShared {
+    static constexpr int D = 32 * G, RB = 16 * NT, ROW = D + 4;
+    long before[257];                                    // units before thread i's sequences
+    long wave_sum[4];
+    float m[4][RB], l[4][RB];
+    int last;
+    float o[4][RB][ROW];
+};
+
+// The line of units.
+struct AttnLine {
+    int per;                                             // sequences a thread has counted
+    long total;
+    int wgs;
+};
+template <int RB>
+__device__ __forceinline__ void attn_units(const AttnLaunch &L, const AttnSeq &q, int &blocks, int &chunks) {
+    blocks = q.n > 0 && (long)q.n * L.g <= L.limit ? (q.n * L.g + RB - 1) / RB : 0;
+    chunks = max(1, (q.len - (q.lo & ~15) + AT_UNIT - 1) / AT_UNIT);
+}
+
+template <int G, int NT, int PARTS>
+__global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
+    using Wave = AttnWave<G, NT, PARTS>;
+    constexpr int D = 32 * G, RB = 16 * NT;
+    __shared__ AttnShared<G, NT> sh;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), heads = L.c.heads, S = L.a.S;
+    const int per = (S + 255) / 256;
+    long mine = 0;
+    for (int s = tid * per; s < min(S, (tid + 1) * per); s++) {
+        int blocks, chunks;
+        attn_units<RB>(L, attn_seq(L, s), blocks, chunks);
+        mine += (long)blocks * heads * chunks;
+    }
+    long upto = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const long v = __shfl_up(upto, x);
+        if ((tid & 63) >= x) upto += v;
+    }
+    if ((tid & 63) == 63) sh.wave_sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) upto += sh.wave_sum[w];
+    sh.before[tid] = upto - mine;
+    if (tid == 255) sh.before[256] = upto;
+    __syncthreads();
+    const long total = sh.before[256], wgs = min((long)gridDim.x, total);
+    const long w = blockIdx.x;
+    if (w >= wgs) return;
+    const long end = total * (w + 1) / wgs;
+    long u = total * w / wgs;
+    // the sequence of unit u: the last thread whose sequences begin at or before it, then that thread's sequences in turn
+    int th = 0;
+#pragma unroll
+    for (int x = 128; x; x >>= 1)
+        if (sh.before[th + x] <= u) th += x;
+    int s = th * per;
+    long base = sh.before[th];                           // units before sequence s
+    Wave W(L);
+    int blocks, chunks;
+    auto seek = [&] {                                    // to the sequence of unit u
+        while (true) {
+            W.q = attn_seq(L, s);
+            W.q.begin = __builtin_amdgcn_readfirstlane(W.q.begin);
+            W.q.n = __builtin_amdgcn_readfirstlane(W.q.n);
+            W.q.len = __builtin_amdgcn_readfirstlane(W.q.len);
+            W.q.lo = __builtin_amdgcn_readfirstlane(W.q.lo);
+            attn_units<RB>(L, W.q, blocks, chunks);
+            const long n = (long)blocks * heads * chunks;
+            if (u < base + n) break;
+            base += n;
+            s++;
+        }
+    };
+    while (u < end) {
+        seek();
+        const long item = (u - base) / chunks;           // head * blocks + row block
+        const int head = __builtin_amdgcn_readfirstlane((int)(item / blocks)), rb = __builtin_amdgcn_readfirstlane((int)(item % blocks));
+        const int c0 = __builtin_amdgcn_readfirstlane((int)(u - base - item * chunks));
+        const int c1 = __builtin_amdgcn_readfirstlane((int)min((long)chunks, c0 + (end - u)));
+        W.begin(s, head, rb);
+        const int key0 = (W.q.lo & ~15) + wave * 32;
+        AttnRaw<G> ra, rn;
+        int pa[2], pb[2];
+        int left = 0, key = key0 + c0 * AT_UNIT;         // units in which the wave has keys
+        if (key < W.q.len) left = min(c1 - c0, (W.q.len - key + AT_UNIT - 1) / AT_UNIT);
+        auto fetch = [&](AttnRaw<G> &r, int (&p)[2], int k) {
+            p[0] = W.page(k);
+            p[1] = W.page(k + 16);
+            W.load(r, k, p);
+        };
+        if (left) fetch(ra, pa, key);
+        while (left) {                                   // the next unit is on its way while one is worked on
+            if (left > 1) fetch(rn, pb, key + AT_UNIT);
+            W.step(ra, key, pa);
+            key += AT_UNIT;
+            if (--left == 0) break;
+            if (left > 1) fetch(ra, pa, key + AT_UNIT);
+            W.step(rn, key, pb);
+            key += AT_UNIT;
+            --left;
+        }
+        // the four waves' sums
+        __syncthreads();                                 // the segment before this one has read them
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float sum = at_sum4(W.l[t]);
+            if (W.b == 0) { sh.m[wave][16 * t + W.col] = W.m[t]; sh.l[wave][16 * t + W.col] = sum; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int r = 16 * t + W.col;
+            const float M = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
+            const float f = W.m[t] == -INFINITY ? 0.0f : at_exp2(W.m[t] - M);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float *to = &sh.o[wave][r][2 * G * (4 * W.b + i)];
+#pragma unroll
+                for (int j = 0; j < 2 * G; j += 2) {
+                    // (a wave without keys has sums of 0, whatever its factor)
+                    to[j] = W.o[t][j][i] * f;
+                    to[j + 1] = W.o[t][j + 1][i] * f;
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = c0 == 0 && c1 == chunks;
+        const int rows = min(RB, W.q.n * L.g - rb * RB);
+        const long first = u - c0, last = first + chunks - 1;                        // the item's units
+        const long wA = ((first + 1) * wgs - 1) / total, wB = ((last + 1) * wgs - 1) / total;
+        float *const piece = L.part + (2 * w + (c0 == 0)) * (RB * (D + 2));
+        auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out
+            const int i = (rb * RB + r) / L.g, h = head * L.g + (rb * RB + r) % L.g;
+            const size_t at = (size_t)((long)(W.q.begin + i) * L.a.ldo + (long)h * L.a.hdo + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) i8_st(L.a.out, L.a.type, at + e, v[e]);
+        };
+        auto sink2 = [&](int r) { return L.a.sink ? L.a.sink[head * L.g + (rb * RB + r) % L.g] * 1.44269504088896340736f : 0.0f; };
+        for (int x = tid; x < rows * (D / 4); x += 256) {
+            const int r = x / (D / 4), d = x % (D / 4) * 4;
+            const float M = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
+            kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v += *(const kv_f4 *)&sh.o[k][r][d];
+                sum += sh.l[k][r] * (sh.m[k][r] == -INFINITY ? 0.0f : at_exp2(sh.m[k][r] - M));
+            }
+            if (whole) {
+                put(r, d, v * attn_factor(M, sum, L.a.sink != nullptr, sink2(r)));
+            } else {
+                *(kv_f4 *)(piece + r * D + d) = v;
+                if (d == 0) { piece[RB * D + r] = M; piece[RB * D + RB + r] = sum; }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const int n = atomicAdd(L.sync + wA, 1) + 1;
+                sh.last = n == (int)(wB - wA + 1);
+                if (sh.last) atomicExch(L.sync + wA, 0);
+            }
+            __syncthreads();
+            if (sh.last) {                               // every piece of the item is written
+                __threadfence();
+                auto at = [&](long k) { return L.part + (2 * k + (k == wA)) * (RB * (D + 2)); };
+                for (int x = tid; x < rows * (D / 4); x += 256) {
+                    const int r = x / (D / 4), d = x % (D / 4) * 4;
+                    float M = -INFINITY;
+                    for (long k = wA; k <= wB; k++) M = fmaxf(M, at(k)[RB * D + r]);
+                    kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float sum = 0.0f;
+                    for (long k = wA; k <= wB; k++) {
+                        const float mk = at(k)[RB * D + r], f = mk == -INFINITY ? 0.0f : at_exp2(mk - M);
+                        v += *(const kv_f4 *)(at(k) + r * D + d) * f;
+                        sum += at(k)[RB * D + RB + r] * f;
+                    }
+                    put(r, d, v * attn_factor(M, sum, L.a.sink != nullptr, sink2(r)));
+                }
+            }
+        }
+        u += c1 - c0;
+    }
+}
+
+// ================================================================================== host side
+template <int G, int NT, int PARTS>
+static void attn_go(bgl_ctx *c, const AttnLaunch &L, unsigned wgs) {
+    hipLaunchKernelGGL((k_attn<G, NT, PARTS>), dim3(wgs), dim3(256), 0, c->stream, L);
+}
+template <int G>
+static void attn_pick(bgl_ctx *c, const AttnLaunch &L, int nt, unsigned wgs) {
+    if constexpr (G <= 4) {
+        if (nt == 2) {
+            if (L.a.type == BGL_T_F32) attn_go<G, 2, 2>(c, L, wgs);
+            else attn_go<G, 2, 1>(c, L, wgs);
+            return;
+        }
+    }
+    if (L.a.type == BGL_T_F32) attn_go<G, 1, 2>(c, L, wgs);
+    else attn_go<G, 1, 1>(c, L, wgs);
+}
+
+static bool rows_ok(long ld, long hd, long n, long heads, long D) {
+    if (ld < 0 || hd < 0) return false;
+    if (n == 1) return heads == 1 || hd >= D;
+    if (heads == 1) return ld >= D;
+    return (hd >= D && ld >= (heads - 1) * hd + D) || (ld >= D && hd >= (n - 1) * ld + D);
+}
+
+extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
+    if (!c || !a || !a->q || !a->out || !a->start || !a->len || !a->table) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: NULL argument");
+    if (const int rc = kv_check("bgl_attn_dev", kv)) return rc;
+    if (a->S < 1 || a->T < 1 || a->ldt < 1) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: S=%d T=%d ldt=%d", a->S, a->T, a->ldt);
+    if (a->nq < 1 || a->nq > 65535 || a->nq % kv->heads)
+        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: nq=%d heads over a cache of %d", a->nq, kv->heads);
+    if (a->type != BGL_T_F32 && a->type != BGL_T_F16 && a->type != BGL_T_BF16) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: unknown element type");
+    if (!rows_ok(a->ldq, a->hdq, a->T, a->nq, kv->D) || !rows_ok(a->ldo, a->hdo, a->T, a->nq, kv->D))
+        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: rows of D=%d values overlap at these strides", kv->D);
+    if (a->window < 0 || (a->window && !a->causal)) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: window=%d (at least 0, and with causal)", a->window);
+    if (a->max_rows < 0 || a->max_len < 0) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: max_rows=%d max_len=%d", a->max_rows, a->max_len);
+    if (!(a->scale == a->scale) || a->scale - a->scale != 0.0f) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: scale is not finite");
+    if (a->q == a->out) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: out is q");
+    if ((long)a->T * (a->nq / kv->heads) > INT32_MAX / 2) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of %d heads", a->T, a->nq);
+    HIPCHK(hipSetDevice(c->device));
+    AttnLaunch L;
+    memset(&L, 0, sizeof L);
+    L.c = *kv;
+    L.a = *a;
+    L.g = a->nq / kv->heads;
+    L.ppt = kv->page / KV_TILE;
+    L.ppt_shift = (L.ppt & (L.ppt - 1)) == 0 ? __builtin_ctz(L.ppt) : -1;
+    L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
+    L.limit = INT32_MAX;
+    const int rows = std::min(std::max(1, a->max_rows), a->T) * L.g, G = kv->D / 32;
+    const int nt = rows > 16 && G <= 4 ? 2 : 1, RB = 16 * nt;
+    if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)2 * AT_WG * 32 * (128 + 2) * 4, false)) return rc;
+    if (const int rc = dbuf_reserve(c, c->attn_sync, AT_WG * sizeof(int), true)) return rc;
+    L.part = (float *)c->attn_part.p;
+    L.sync = (int *)c->attn_sync.p;
+    const long units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * (((long)std::max(1, a->max_len) + AT_UNIT - 1) / AT_UNIT);
+    const unsigned wgs = (unsigned)std::min<long>(AT_WG, std::max<long>(1, units));
+    const int tok = prof_begin(c, 1);
+    switch (G) {
+    case 2: attn_pick<2>(c, L, nt, wgs); break;
+    case 3: attn_pick<3>(c, L, nt, wgs); break;
+    case 4: attn_pick<4>(c, L, nt, wgs); break;
+    case 6: attn_pick<6>(c, L, nt, wgs); break;
+    default: attn_pick<8>(c, L, nt, wgs); break;
+    }
+    prof_end(c, tok);
+    HIPCHK(hipGetLastError());
+    return 0;
+}

@@ -1,0 +1,409 @@
+// bgl_heads.hip -- queries, keys and values on their way from the q/k/v products to attention: a norm over each head,
+// the rotation by the token's position, and the keys and values as 4-bit codes in the pages of a cache.
+//
+//   n = x | x / sqrt(mean(x^2) + eps) w | (x - mean) / sqrt(var + eps) w         over the D values of a head
+//   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i                            for the pairs (i, j) that are rotated
+//   groups of 32: m = fp16(min), s = fp16((max - m) / 15), c = rint((x - m) / s), value fp16(c s + m)
+//
+// A code changes by one where a value lies within rounding of a border between codes.  So y is computed in double and rounded
+// once to fp32, and from there each step is one fp32 operation: the codes are the formula's.  (gfx950 issues double
+// multiply-adds at the rate of single ones.)
+#include <string.h>
+
+#include <algorithm>
+
+#include "../../include/beglin_qgemv.h"
+#include "bgl_i8.h"
+#include "bgl_kv.h"
+
+#define HIPCHK(expr)                                                                             \
+    do {                                                                                         \
+        hipError_t e_ = (expr);                                                                  \
+        if (e_ != hipSuccess) return bgl_fail(BGL_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+    } while (0)
+
+struct HeadsLaunch {
+    bgl_heads d;
+    bgl_kv c;
+    const int32_t *slots;        // of the d.T tokens of this launch; null: no cache
+    int before, after;           // tokens of the call before and behind this launch's (slots reach that far)
+    int nq, nk, nv;              // heads to do of each
+};
+
+// Sums over the GL lanes of a head, in every one of them.
+template <int GL>
+__device__ __forceinline__ double hd_sum(double v) {
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    if (GL > 8) v += dpp_d<0x140>(v);
+    if (GL > 16) v += __shfl_xor(v, 16);
+    if (GL > 32) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// What a lane needs of the rotation for its 8 values d0 .. d0 + 7: their cosines and sines (half: one each; pairs: one each
+// two values), and for half where the other value of each pair lies.
+struct HdTurn {
+    float c[8], s[8];
+    int other;                   // first of the 8 partners; 0 distance: not rotated
+};
+__device__ __forceinline__ HdTurn hd_turn(const bgl_heads &d, const float *rope, int d0) {
+    HdTurn t;
+    t.other = d0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) { t.c[j] = 1.0f; t.s[j] = 0.0f; }
+    if (d.rot_kind == BGL_ROT_NONE || d0 >= d.rot) return t;
+    const int h = d.rot / 2;
+    if (d.rot_kind == BGL_ROT_HALF) {
+        t.other = d0 < h ? d0 + h : d0 - h;
+        const int i = d0 < h ? d0 : t.other;
+        kv_load8(t.c, rope, BGL_T_F32, i);
+        kv_load8(t.s, rope, BGL_T_F32, h + i);
+    } else {
+        const kv_mf4 c = *(const kv_mf4 *)(rope + d0 / 2), s = *(const kv_mf4 *)(rope + h + d0 / 2);
+#pragma unroll
+        for (int j = 0; j < 4; j++) { t.c[2 * j] = t.c[2 * j + 1] = c[j]; t.s[2 * j] = t.s[2 * j + 1] = s[j]; }
+    }
+    return t;
+}
+
+// y of a lane's 8 values of the head at p (values past D: 0).
+template <int GL>
+__device__ __forceinline__ void hd_row(float (&y)[8], const bgl_heads &d, const void *p, long at, const float *w, const HdTurn &t, int d0, bool in) {
+    float x[8], px[8];
+    kv_load8(x, p, d.type, at + (in ? d0 : 0));
+    const bool half = d.rot_kind == BGL_ROT_HALF && t.other != d0;
+    if (d.rot_kind == BGL_ROT_HALF) kv_load8(px, p, d.type, at + (in ? t.other : 0));
+    double n[8], pn[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) n[j] = in ? (double)x[j] : 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) pn[j] = half ? (double)px[j] : 0.0;
+    if (d.norm != BGL_NORM_NONE) {
+        double mean = 0.0, q = 0.0;
+        if (d.norm == BGL_NORM_LAYER) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) mean += n[j];
+            mean = hd_sum<GL>(mean) / d.D;
+#pragma unroll
+            for (int j = 0; j < 8; j++) { n[j] = in ? n[j] - mean : 0.0; pn[j] -= mean; }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) q = fma(n[j], n[j], q);
+        const double inv = 1.0 / sqrt(hd_sum<GL>(q) / d.D + (double)d.eps);
+#pragma unroll
+        for (int j = 0; j < 8; j++) { n[j] *= inv; pn[j] *= inv; }
+        if (w) {
+            float g[8], pg[8];
+            kv_load8(g, w, BGL_T_F32, in ? d0 : 0);
+            if (d.rot_kind == BGL_ROT_HALF) kv_load8(pg, w, BGL_T_F32, in ? t.other : 0);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                n[j] *= (double)g[j] + (double)d.w_add;
+                if (d.rot_kind == BGL_ROT_HALF) pn[j] *= (double)pg[j] + (double)d.w_add;
+            }
+        }
+    }
+    if (d.rot_kind == BGL_ROT_NONE || d0 >= d.rot) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = (float)n[j];
+    } else if (d.rot_kind == BGL_ROT_HALF) {
+        const bool first = t.other > d0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = (float)fma(n[j], (double)t.c[j], first ? -(pn[j] * (double)t.s[j]) : pn[j] * (double)t.s[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            y[j] = (float)fma(n[j], (double)t.c[j], -(n[j + 1] * (double)t.s[j]));
+            y[j + 1] = (float)fma(n[j + 1], (double)t.c[j], n[j] * (double)t.s[j]);
+        }
+    }
+}
+
+// The codes of a lane's 8 values, whose group is those of the lane's quad, and the group's step and floor (s | m << 16).
+__device__ __forceinline__ uint32_t hd_codes(uint32_t (&c)[8], const float (&x)[8]) {
+    float lo = INFINITY, hi = -INFINITY, t[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+        t[j] = fminf(fmaxf(x[j], -32768.0f), 32768.0f);
+        lo = fminf(lo, t[j]);
+        hi = fmaxf(hi, t[j]);
+    }
+    lo = fminf(lo, dpp_f<0xB1>(lo)); lo = fminf(lo, dpp_f<0x4E>(lo));
+    hi = fmaxf(hi, dpp_f<0xB1>(hi)); hi = fmaxf(hi, dpp_f<0x4E>(hi));
+    top = max(top, (uint32_t)dpp_i<0xB1>((int)top)); top = max(top, (uint32_t)dpp_i<0x4E>((int)top));
+    const _Float16 m = (_Float16)lo;
+    const float fm = (float)m;
+    const _Float16 s = (_Float16)fmaxf(0.0f, __fdiv_rn(__fsub_rn(hi, fm), 15.0f));
+    const float r = __fdiv_rn(1.0f, (float)s);
+    const bool none = !((float)s > 0.0f) || top >= 0x7f800000u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float q = none ? 0.0f : rintf(__fmul_rn(__fsub_rn(t[j], fm), r));
+        c[j] = (uint32_t)(int)fminf(fmaxf(q, 0.0f), 15.0f);
+    }
+    if (top >= 0x7f800000u) return 0x7e000000u;                    // NaN, step 0
+    return (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
+}
+
+__device__ __forceinline__ void hd_put_k(uint8_t *rec, int D, int tok, int li, const float (&x)[8]) {
+    uint32_t c[8];
+    const uint32_t sm = hd_codes(c, x);
+    const int G = D / 32, b = li / G, j = li - b * G;
+    // values 1, 3 lie 16 bits above 0, 2, and 4 .. 7 8 bits above 0 .. 3
+    const uint32_t w = c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12 | c[1] << 16 | c[3] << 20 | c[5] << 24 | c[7] << 28;
+    ((uint32_t *)rec)[(b * KV_TILE + tok) * G + j] = w;
+    if ((li & 3) == 0) ((uint32_t *)(rec + kv_k_steps(D)))[(li >> 2) * KV_TILE + tok] = sm;
+}
+__device__ __forceinline__ void hd_put_v(uint8_t *rec, int D, int tok, int li, const float (&x)[8]) {
+    uint32_t c[8];
+    const uint32_t sm = hd_codes(c, x);
+    const int b = tok >> 2, r = tok & 3;
+    uint8_t *p = rec + kv_v_codes(D) + (b * (D / 2) + 4 * li) * 4 + r;
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[4 * j] = (uint8_t)(c[2 * j] | c[2 * j + 1] << 4);
+    if ((li & 3) == 0) {
+        uint16_t *q = (uint16_t *)(rec + kv_v_steps(D)) + ((li >> 2) * 4 + b) * 8 + (r & 1) * 2 + (r >> 1);
+        q[0] = (uint16_t)sm;
+        q[4] = (uint16_t)(sm >> 16);
+    }
+}
+
+// A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other.
+template <int GL>
+__global__ __launch_bounds__(256) void k_heads(HeadsLaunch L) {
+    const bgl_heads &d = L.d;
+    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), d0 = 8 * li;
+    const bool in = d0 < d.D;
+    const float *rope = nullptr;
+    if (d.rot_kind != BGL_ROT_NONE) {
+        const int p = d.pos[t];
+        if (p < 0 || p >= d.n_pos) return;
+        rope = d.rope + (size_t)p * d.rot;
+    }
+    const HdTurn turn = hd_turn(d, rope, in ? d0 : 0);
+    const int slot = L.slots ? L.slots[t] : -1;
+    const bool kept = slot >= 0 && slot < (long)L.c.pages * L.c.page;
+    const int n = L.nq + L.nk + L.nv, step = (int)gridDim.y * (256 / GL);
+    for (int i = (int)blockIdx.y * (256 / GL) + (int)threadIdx.x / GL; i < n; i += step) {
+        float y[8];
+        if (i < L.nq) {
+            hd_row<GL>(y, d, d.q, t * d.ldq + i * d.hdq, d.q_w, turn, d0, in);
+            if (in) kv_store8(d.q_out, d.out_type, t * d.ldqo + i * d.hdqo + d0, y);
+        } else if (i < L.nq + L.nk) {
+            const int h = i - L.nq;
+            hd_row<GL>(y, d, d.k, t * d.ldk + h * d.hdk, d.k_w, turn, d0, in);
+            if (d.k_out) {
+                if (in) kv_store8(d.k_out, d.out_type, t * d.ldko + h * d.hdko + d0, y);
+            } else if (kept && in) {
+                hd_put_k(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
+            }
+        } else {
+            const int h = i - L.nq - L.nk;
+            if (kept && in) {
+                kv_load8(y, d.v, d.type, t * d.ldv + h * d.hdv + d0);
+                hd_put_v(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
+            }
+        }
+    }
+}
+
+struct KvReadLaunch {
+    bgl_kv c;
+    const int32_t *slots;
+    int n, type;
+    void *k, *v;
+    long ldk, hdk, ldv, hdv;
+};
+__device__ __forceinline__ float kv_value(uint32_t c, uint32_t s, uint32_t m) {
+    const _Float16 a = (_Float16)(float)c, b = __builtin_bit_cast(_Float16, (uint16_t)s), e = __builtin_bit_cast(_Float16, (uint16_t)m);
+    return (float)__builtin_fmaf16(a, b, e);
+}
+template <int GL>
+__global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
+    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), d0 = 8 * li, D = L.c.D, G = D / 32;
+    const int slot = L.slots[t];
+    if (slot < 0 || slot >= (long)L.c.pages * L.c.page || d0 >= D) return;
+    const int tok = slot % L.c.page % KV_TILE, step = (int)gridDim.y * (256 / GL);
+    for (int i = (int)blockIdx.y * (256 / GL) + (int)threadIdx.x / GL; i < 2 * L.c.heads; i += step) {
+        const int h = i % L.c.heads;
+        const uint8_t *rec = kv_at(L.c, slot, h);
+        float y[8];
+        if (i < L.c.heads) {
+            if (!L.k) continue;
+            const int b = li / G, j = li - b * G;
+            const uint32_t w = ((const uint32_t *)rec)[(b * KV_TILE + tok) * G + j];
+            const uint32_t sm = ((const uint32_t *)(rec + kv_k_steps(D)))[(li >> 2) * KV_TILE + tok];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = kv_value(w >> ((e & 1) * 16 + (e >> 2) * 8 + (e >> 1 & 1) * 4) & 15u, sm, sm >> 16);
+            kv_store8(L.k, L.type, t * L.ldk + h * L.hdk + d0, y);
+        } else {
+            if (!L.v) continue;
+            const int b = tok >> 2, r = tok & 3;
+            const uint8_t *p = rec + kv_v_codes(D) + (b * (D / 2) + 4 * li) * 4 + r;
+            const uint16_t *q = (const uint16_t *)(rec + kv_v_steps(D)) + ((li >> 2) * 4 + b) * 8 + (r & 1) * 2 + (r >> 1);
+            const uint32_t s = q[0], m = q[4];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = kv_value(p[4 * (e >> 1)] >> (4 * (e & 1)) & 15u, s, m);
+            kv_store8(L.v, L.type, t * L.ldv + h * L.hdv + d0, y);
+        }
+    }
+}
+
+// ================================================================================== host side
+// A launch has less than 2^32 threads, 256 of them a token and up to 16 workgroups of few tokens.
+#define HD_TOKENS (1 << 20)
+
+// Workgroups a token: as many as it takes to do every head at once, while the launch leaves units idle.
+static unsigned hd_parts(int T, int items, int per) {
+    const int all = (items + per - 1) / per;
+    return (unsigned)std::max(1, std::min(all, 1024 / std::max(1, T)));
+}
+template <typename F>
+static void hd_lanes(int D, F go) {
+    if (D <= 64) go(std::integral_constant<int, 8>{});
+    else if (D <= 128) go(std::integral_constant<int, 16>{});
+    else if (D <= 256) go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, 64>{});
+}
+
+static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
+    const bgl_heads &a = all.d;
+    const int tok = prof_begin(c, 2);
+    for (long t = 0; t < a.T; t += HD_TOKENS) {
+        HeadsLaunch L = all;
+        bgl_heads &d = L.d;
+        d.T = (int)std::min<long>(HD_TOKENS, a.T - t);
+        L.before = (int)t;
+        L.after = (int)(a.T - t - d.T);
+        auto at = [&](const void *p, long ld, int type) { return p ? (char *)p + t * ld * (long)i8_elem(type) : nullptr; };
+        d.q = at(a.q, a.ldq, a.type); d.k = at(a.k, a.ldk, a.type); d.v = at(a.v, a.ldv, a.type);
+        d.q_out = at(a.q_out, a.ldqo, a.out_type); d.k_out = at(a.k_out, a.ldko, a.out_type);
+        if (a.pos) d.pos = a.pos + t;
+        if (all.slots) L.slots = all.slots + t;
+        hd_lanes(d.D, [&](auto gl) {
+            constexpr int GL = decltype(gl)::value;
+            hipLaunchKernelGGL((k_heads<GL>), dim3((unsigned)d.T, hd_parts(d.T, L.nq + L.nk + L.nv, 256 / GL)), dim3(256), 0, c->stream, L);
+        });
+    }
+    prof_end(c, tok);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+// Rows [n][heads][D] at a pointer: tokens ld apart and heads hd, both at least one row of what they step over, in either order.
+static bool rows_ok(long ld, long hd, long n, long heads, long D) {
+    if (ld < 0 || hd < 0) return false;
+    if (n == 1) return heads == 1 || hd >= D;
+    if (heads == 1) return ld >= D;
+    return (hd >= D && ld >= (heads - 1) * hd + D) || (ld >= D && hd >= (n - 1) * ld + D);
+}
+static bool type_ok(int t) { return t == BGL_T_F32 || t == BGL_T_F16 || t == BGL_T_BF16; }
+
+int kv_check(const char *who, const bgl_kv *kv) {
+    if (!kv || !kv->data) return bgl_fail(BGL_E_ARG, "%s: NULL cache", who);
+    if (!bgl_kv_bytes(kv->pages, kv->page, kv->heads, kv->D))
+        return bgl_fail(BGL_E_ARG, "%s: no cache of %d pages of %d tokens (a multiple of 16), %d heads of %d values (64, 96, 128, 192, 256)", who,
+                        kv->pages, kv->page, kv->heads, kv->D);
+    if ((uintptr_t)kv->data % 16) return bgl_fail(BGL_E_ARG, "%s: the cache is not 16-byte aligned", who);
+    return 0;
+}
+
+extern "C" size_t bgl_kv_bytes(int pages, int page, int heads, int D) {
+    if (pages < 1 || page < KV_TILE || page % KV_TILE || heads < 1 || heads > 65535 || !kv_dim_ok(D)) return 0;
+    if ((long)pages * page > INT32_MAX) return 0;                  // slots are 32-bit
+    return (size_t)pages * heads * (page / KV_TILE) * kv_record(D);
+}
+
+// What bgl_heads_dev and bgl_kv_append_dev ask of q, k and the rotation.
+static int heads_check(const char *who, const bgl_heads *d) {
+    if (d->T < 1 || d->D < 8 || d->D > 512 || d->D % 8) return bgl_fail(BGL_E_ARG, "%s: T=%d D=%d (a multiple of 8 up to 512)", who, d->T, d->D);
+    if (!type_ok(d->type) || ((d->q_out || d->k_out) && !type_ok(d->out_type))) return bgl_fail(BGL_E_ARG, "%s: unknown element type", who);
+    if (d->norm != BGL_NORM_NONE && d->norm != BGL_NORM_RMS && d->norm != BGL_NORM_LAYER) return bgl_fail(BGL_E_ARG, "%s: unknown norm kind", who);
+    if (d->rot_kind != BGL_ROT_NONE && d->rot_kind != BGL_ROT_HALF && d->rot_kind != BGL_ROT_PAIRS)
+        return bgl_fail(BGL_E_ARG, "%s: unknown rotation", who);
+    if (d->rot_kind != BGL_ROT_NONE) {
+        if (!d->rope || !d->pos || d->n_pos < 1) return bgl_fail(BGL_E_ARG, "%s: a rotation needs rope, pos and n_pos", who);
+        if (d->rot < 8 || d->rot > d->D || d->rot % (d->rot_kind == BGL_ROT_HALF ? 16 : 8))
+            return bgl_fail(BGL_E_ARG, "%s: rot=%d of %d values (a multiple of 16, or 8 for pairs)", who, d->rot, d->D);
+    }
+    if ((d->q != nullptr) != (d->q_out != nullptr)) return bgl_fail(BGL_E_ARG, "%s: q and q_out go together", who);
+    if (d->q && (d->nq < 1 || d->nq > 65535)) return bgl_fail(BGL_E_ARG, "%s: nq=%d", who, d->nq);
+    if (d->k && (d->nk < 1 || d->nk > 65535)) return bgl_fail(BGL_E_ARG, "%s: nk=%d", who, d->nk);
+    if ((d->q && (!rows_ok(d->ldq, d->hdq, d->T, d->nq, d->D) || !rows_ok(d->ldqo, d->hdqo, d->T, d->nq, d->D))) ||
+        (d->k && !rows_ok(d->ldk, d->hdk, d->T, d->nk, d->D)) || (d->k_out && !rows_ok(d->ldko, d->hdko, d->T, d->nk, d->D)) ||
+        (d->v && !rows_ok(d->ldv, d->hdv, d->T, d->nk, d->D)))
+        return bgl_fail(BGL_E_ARG, "%s: rows of D=%d values overlap at these strides", who, d->D);
+    if (d->q && d->q == d->q_out && (d->type != d->out_type || d->ldq != d->ldqo || d->hdq != d->hdqo))
+        return bgl_fail(BGL_E_ARG, "%s: q_out is q with another type or stride", who);
+    if (d->k_out && d->k == d->k_out && (d->type != d->out_type || d->ldk != d->ldko || d->hdk != d->hdko))
+        return bgl_fail(BGL_E_ARG, "%s: k_out is k with another type or stride", who);
+    if ((d->q_out && (d->q_out == d->k || d->q_out == d->v || d->q_out == d->k_out)) || (d->k_out && (d->k_out == d->q || d->k_out == d->v)))
+        return bgl_fail(BGL_E_ARG, "%s: an output is one of the other rows", who);
+    return 0;
+}
+
+extern "C" int bgl_heads_dev(bgl_ctx *c, const bgl_heads *d) {
+    if (!c || !d) return bgl_fail(BGL_E_ARG, "bgl_heads_dev: NULL argument");
+    if (!d->q && !d->k) return bgl_fail(BGL_E_ARG, "bgl_heads_dev: neither q nor k");
+    if (d->v) return bgl_fail(BGL_E_ARG, "bgl_heads_dev: v is not used");
+    if ((d->k != nullptr) != (d->k_out != nullptr)) return bgl_fail(BGL_E_ARG, "bgl_heads_dev: k and k_out go together");
+    if (const int rc = heads_check("bgl_heads_dev", d)) return rc;
+    HIPCHK(hipSetDevice(c->device));
+    HeadsLaunch L;
+    memset(&L, 0, sizeof L);
+    L.d = *d;
+    L.nq = d->q ? d->nq : 0;
+    L.nk = d->k ? d->nk : 0;
+    return heads_launch(c, L);
+}
+
+extern "C" int bgl_kv_append_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_heads *d, const int32_t *slots) {
+    if (!c || !d || !slots || !d->k || !d->v) return bgl_fail(BGL_E_ARG, "bgl_kv_append_dev: NULL argument");
+    if (const int rc = kv_check("bgl_kv_append_dev", kv)) return rc;
+    if (d->k_out) return bgl_fail(BGL_E_ARG, "bgl_kv_append_dev: k_out has to be NULL");
+    if (const int rc = heads_check("bgl_kv_append_dev", d)) return rc;
+    if (d->nk != kv->heads || d->D != kv->D)
+        return bgl_fail(BGL_E_ARG, "bgl_kv_append_dev: %d heads of %d values into a cache of %d of %d", d->nk, d->D, kv->heads, kv->D);
+    HIPCHK(hipSetDevice(c->device));
+    HeadsLaunch L;
+    memset(&L, 0, sizeof L);
+    L.d = *d;
+    L.c = *kv;
+    L.slots = slots;
+    L.nq = d->q ? d->nq : 0;
+    L.nk = L.nv = d->nk;
+    return heads_launch(c, L);
+}
+
+extern "C" int bgl_kv_read_dev(bgl_ctx *c, const bgl_kv *kv, const int32_t *slots, int n, void *k, long ldk, long hdk, void *v, long ldv,
+                               long hdv, int type) {
+    if (!c || !slots || (!k && !v)) return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: NULL argument");
+    if (const int rc = kv_check("bgl_kv_read_dev", kv)) return rc;
+    if (n < 1) return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: n=%d", n);
+    if (!type_ok(type)) return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: unknown element type");
+    if ((k && !rows_ok(ldk, hdk, n, kv->heads, kv->D)) || (v && !rows_ok(ldv, hdv, n, kv->heads, kv->D)) || k == v)
+        return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: rows of D=%d values overlap", kv->D);
+    HIPCHK(hipSetDevice(c->device));
+    const int tok = prof_begin(c, 2);
+    for (long t = 0; t < n; t += HD_TOKENS) {
+        KvReadLaunch L;
+        memset(&L, 0, sizeof L);
+        L.c = *kv;
+        L.slots = slots + t;
+        L.n = (int)std::min<long>(HD_TOKENS, n - t);
+        L.type = type;
+        L.k = k ? (char *)k + t * ldk * (long)i8_elem(type) : nullptr; L.ldk = ldk; L.hdk = hdk;
+        L.v = v ? (char *)v + t * ldv * (long)i8_elem(type) : nullptr; L.ldv = ldv; L.hdv = hdv;
+        hd_lanes(kv->D, [&](auto gl) {
+            constexpr int GL = decltype(gl)::value;
+            hipLaunchKernelGGL((k_kv_read<GL>), dim3((unsigned)L.n, hd_parts(L.n, 2 * kv->heads, 256 / GL)), dim3(256), 0, c->stream, L);
+        });
+    }
+    prof_end(c, tok);
+    HIPCHK(hipGetLastError());
+    return 0;
+}

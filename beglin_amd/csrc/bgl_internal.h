@@ -52,6 +52,7 @@ struct bgl_ctx {
     DevBuf moe_scores;                    // router scores [T][E]
     DevBuf moe_sync;                      // K_Q8C experts: what the workgroups of a launch tell each other (MoeI8Sync)
     DevBuf mlp;                           // bgl_mlp_dev: gate and up outputs [M][I] each, then h [M][I]
+    DevBuf attn_part, attn_sync;          // bgl_attn_dev: partial sums of rows whose keys several workgroups share, and their counters
     std::unordered_map<uint64_t, DevBuf> mlp_sync;   // single-launch MLP, per shape (in << 32 | down workgroups): counters, generations, flag
     bool no_qmfma = false;                // BGL_NO_QMFMA=1: W4A8 at 2..16 columns through the dot4 kernel (k_gemv_q)
     int qm_rb = 0, qm_s = 0;              // BGL_QM_RB / BGL_QM_S: k_gemv_qm row blocks / unit slices per workgroup (tuning; 0 by shape)

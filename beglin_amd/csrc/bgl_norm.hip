@@ -175,11 +175,6 @@ __device__ __forceinline__ void norm_chunk(double (&n)[8], const Map &m, int i, 
 }
 
 // Sums over a wave through DPP and readlane (a shuffle would go through the LDS, twice for a double).
-template <int CTRL>
-__device__ __forceinline__ double dpp_d(double v) {
-    const int2 p = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(dpp_i<CTRL>(p.x), dpp_i<CTRL>(p.y)));
-}
 __device__ __forceinline__ double rlane_d(double v, int l) {
     const int2 p = __builtin_bit_cast(int2, v);
     return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(p.x, l), __builtin_amdgcn_readlane(p.y, l)));

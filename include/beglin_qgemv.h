@@ -45,6 +45,7 @@ enum { BGL_K_Q4G64 = 1, BGL_K_Q8G64 = 2, BGL_K_Q4G256SF = 3, BGL_K_QNG64 = 4, BG
        BGL_K_Q4G64A = 6, BGL_K_F16 = 7, BGL_K_F32 = 8, BGL_K_MXFP4 = 9, BGL_K_Q4G256P = 10, BGL_K_Q8C = 11 };
 enum { BGL_T_F32 = 0, BGL_T_F16 = 1, BGL_T_BF16 = 2 };          /* element types of rows in device memory */
 enum { BGL_NORM_NONE = 0, BGL_NORM_RMS = 1, BGL_NORM_LAYER = 2 };
+enum { BGL_ROT_NONE = 0, BGL_ROT_HALF = 1, BGL_ROT_PAIRS = 2 }; /* which two values of a head a rotation turns */
 enum { BGL_ACT_F32 = 0, BGL_ACT_W4A8 = 1 };
 enum { BGL_OK = 0, BGL_E_ARG = -1, BGL_E_UNSUPPORTED = -2, BGL_E_HIP = -3, BGL_E_NODEV = -4, BGL_E_NOMEM = -5,
        BGL_E_CAPTURE = -6 /* per-call scratch would have to grow inside a stream capture */,
@@ -216,6 +217,86 @@ typedef struct {
     int8_t *yq; long ldq; float *yscale;
 } bgl_norm;
 int  bgl_norm_dev(bgl_ctx *ctx, const bgl_norm *d);
+
+/* ---------------- attention: heads, a paged cache in 4 bits, the rows that attend ----------------
+ * What lies between a layer's q/k/v products and its output product.  No counterpart in the reference's
+ * GEMV files (its CPU attention is part of forward_token, qwen_infer.c:1435-1585, over an fp32 cache). */
+/* Norms of queries and keys for each head, with the position rotation in the same pass, over T tokens:
+ * nq heads of q, nk of k, D values each.
+ *     n = norm(x): BGL_NORM_NONE x
+ *                  BGL_NORM_RMS   x / sqrt(mean(x^2) + eps) * (w + w_add)
+ *                  BGL_NORM_LAYER (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) * (w + w_add)
+ *     with c_i = rope[pos[t]][i], s_i = rope[pos[t]][rot / 2 + i], i < rot / 2:
+ *     BGL_ROT_HALF   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i   for j = i + rot / 2
+ *     BGL_ROT_PAIRS  the same for values 2 i and 2 i + 1
+ *     y_d = n_d for d >= rot, and everywhere with BGL_ROT_NONE (rope and pos unused)
+ * Values are computed in double and rounded to fp32, then to out_type.  q_w, k_w: fp32 [D], NULL: no factor.  rope: fp32 rows of
+ * rot values, n_pos of them; a token whose pos lies outside [0, n_pos) is skipped: nothing is written for it.  Value
+ * d of head h of token t lies ld * t + hd * h + d values behind the pointer.  D is a multiple of 8 up to 512, rot of 16
+ * (HALF) or 8 (PAIRS).  q_out may be q, and k_out k, with the same type and strides; apart from that what is written
+ * overlaps nothing that is read.  bgl_heads_dev: q with q_out, k with k_out, or both; v is not used. */
+typedef struct {
+    int T, D, nq, nk;
+    const void *q, *k, *v;
+    long ldq, hdq, ldk, hdk, ldv, hdv;
+    int type;                                      /* BGL_T_* of q, k and v */
+    int norm; const float *q_w, *k_w; float eps, w_add;
+    int rot_kind, rot; const float *rope; int n_pos; const int32_t *pos;
+    void *q_out, *k_out;
+    long ldqo, hdqo, ldko, hdko;
+    int out_type;                                  /* of q_out and k_out */
+} bgl_heads;
+int  bgl_heads_dev(bgl_ctx *ctx, const bgl_heads *d);
+/* A cache of keys and values in pages of `page` tokens (a multiple of 16), `heads` heads of D = 64, 96, 128, 192 or 256
+ * values.  Each 32 values of a head are held as codes c of 4 bits with a step s and a floor m in fp16, from fp32 values x:
+ *     x held to +-32768;  m = fp16(min x);  s = fp16(max(0, (max x - m) / 15))
+ *     c = rint((x - m) * (1 / s)) held to 0 .. 15, 0 where s = 0      (every step one fp32 operation)
+ * and stand for fp16(c * s + m), rounded once.  32 values with a NaN or an infinity among them are kept as NaN.
+ * data: bgl_kv_bytes bytes of device memory, 16-byte aligned, [pages][heads][page / 16] records of 20 D bytes for 16
+ * tokens each.  With G = D / 32 a record holds
+ *     K codes  [4 b][16 tokens][G j] dwords: values 8 (G b + j) + 0 .. 7 of the token, nibbles 0 4 1 5 2 6 3 7
+ *              (value 1 in the low half of byte 2, value 2 in the high half of byte 0)
+ *     K steps  [G][16 tokens] (s, m)
+ *     V codes  [4 b][D / 2 p][4 r] bytes: values 2 p (low half) and 2 p + 1 of token 4 b + r
+ *     V steps  [G][4 b] (s of tokens 4 b + 0, 2, 1, 3, then m of the same)
+ * Nothing has to be cleared: what no token was written to is read by nobody who keeps to the lengths. */
+typedef struct {
+    void *data;
+    int pages, page, heads, D;
+} bgl_kv;
+size_t bgl_kv_bytes(int pages, int page, int heads, int D);               /* 0: no such cache */
+/* Keys and values of d's T tokens into the cache, k normed and rotated as bgl_heads_dev does, v as it is; token t goes to
+ * slot slots[t] = page id * page + place in the page.  Slots outside the cache: the token's keys and values are not
+ * written.  The slots of one call are distinct.  With q and q_out the queries are normed and rotated in the same launch.
+ * d->nk and d->D are the cache's; k_out has to be NULL. */
+int  bgl_kv_append_dev(bgl_ctx *ctx, const bgl_kv *kv, const bgl_heads *d, const int32_t *slots);
+/* The values of n slots, [n][heads] rows of D in `type`, as strided rows (see bgl_heads); k or v may be NULL.  Rows of
+ * slots outside the cache are left as they are. */
+int  bgl_kv_read_dev(bgl_ctx *ctx, const bgl_kv *kv, const int32_t *slots, int n, void *k, long ldk, long hdk, void *v, long ldv, long hdv,
+                     int type);
+/* Attention of S sequences over the cache.  Rows start[s] .. start[s + 1] - 1 of q and out belong to sequence s, which
+ * has len[s] keys, its rows' own among them; key j lies in page table[s * ldt + j / page].  Row i of n rows sees
+ * the keys j < len[s] for which
+ *     causal == 0 or j <= len[s] - n + i;   window == 0 or j > len[s] - n + i - window;   the key's page id is in [0, pages)
+ *     out = sum_j exp(scale q.k_j) v_j / (sum_j exp(scale q.k_j) + exp(sink[h]))
+ * for head h of nq, which reads head h / (nq / heads) of the cache; sink NULL: without that term.  A row that sees no key
+ * becomes 0; rows of no sequence are left as they are.  Sums, maxima and products' accumulators are fp32; with fp16 and
+ * bf16 rows the weights exp(..) are rounded to fp16 before they multiply v (queries and cached values are exact as
+ * operands), with fp32 rows they and the queries are held as two fp16 parts each, 22 bits.  The keys j >= ldt * page do not exist.
+ * max_rows and max_len: the most rows and keys of a sequence as far as the caller knows; launch shapes go by them, no
+ * result needs them to be right.  Rows of one sequence are summed in an order that its lengths and the batch's give:
+ * the same call gives the same bits.  The first call reserves the context's scratch for partial sums, which graphs captured from
+ * one context share: replay them one after the other. */
+typedef struct {
+    int S, T, nq;                                  /* sequences; rows of q and out; heads of q, a multiple of the cache's */
+    const void *q; long ldq, hdq;
+    void *out; long ldo, hdo;
+    int type;                                      /* BGL_T_* of q and out */
+    const int32_t *start, *len, *table; int ldt;   /* [S + 1], [S], [S][ldt] */
+    float scale; int causal, window; const float *sink;
+    int max_rows, max_len;
+} bgl_attn;
+int  bgl_attn_dev(bgl_ctx *ctx, const bgl_kv *kv, const bgl_attn *a);
 
 /* ---------------- host-pointer drop-ins with the reference's argument lists ----------------
  * The q4pool* argument becomes the context.  The weight pointer identifies the tensor: the first

@@ -1,0 +1,380 @@
+"""bgl_attn_dev against attention in 64 bits over the values that the cache stands for.
+
+How far a value may be off, from the kernel's roundings (all relative):
+  scores   q is exact as an operand (two parts of it hold 2^-22 for fp32 rows), D products are summed in fp32, and the sum is scaled
+           and shifted: A (2 D + 32) 2^-24 + A 2^-22 (fp32 rows), A the largest sum |q_i k_i| scale that the row sees; both the weight and the
+           sum of weights follow it: twice that.  A merge of partial sums shifts by the maximum once more, which the 32 holds.
+  weights  fp16: 2^-11, two parts: 2^-22; exp2 itself 2^-22.  A weight below 2^-28 of the largest is off by at most 2^-39 of it.
+  sums     32 products in a matrix instruction and L / 32 instructions and joins, each at most 2^-23.
+  output   half a step of its type.
+All but the last multiply sum p |v|."""
+import numpy as np
+import pytest
+
+import kv_forms as F
+
+pytestmark = pytest.mark.gpu
+KINDS = {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}
+
+
+@pytest.fixture(scope="module")
+def torch_dev():
+    import torch
+    assert torch.cuda.is_available(), "gpu tests need a GPU"
+    return torch
+
+
+@pytest.fixture(scope="module")
+def ctx(torch_dev):
+    import beglin_amd
+    c = beglin_amd.Context(0)
+    yield c
+    c.sync()
+    c.close()
+
+
+def host(t):
+    return t.float().cpu().numpy()
+
+
+class Batch:
+    """Sequences of (rows, keys) over a cache whose other places, and whose table's other entries, hold anything."""
+
+    def __init__(self, torch, ctx, seqs, nq, nk, D, kind, page, seed=0, poison=(), gone=(), scale_q=1.0, scale_k=1.0, layout="dense"):
+        import beglin_amd
+        rng = np.random.default_rng(seed)
+        self.torch, self.seqs, self.nq, self.nk, self.D, self.page = torch, seqs, nq, nk, D, page
+        need = [(n + page - 1) // page for _, n in seqs]
+        pages = sum(need) + 3
+        self.cache = beglin_amd.KVCache(pages, page, nk, D)
+        self.cache.data.fill_(0xFF)                                                # NaN everywhere
+        order = rng.permutation(pages).astype(np.int32)
+        wide = max(need + [1]) + 1
+        table = rng.choice(np.array([-1, 2 ** 31 - 1, -2 ** 31, pages, pages + 7, order[-1]]), (len(seqs), wide)).astype(np.int32)
+        self.k, self.v, at = [], [], 0
+        for s, (_, n) in enumerate(seqs):
+            table[s, :need[s]] = order[at:at + need[s]]
+            at += need[s]
+            if not n:
+                self.k.append(np.zeros((0, nk, D))), self.v.append(np.zeros((0, nk, D)))
+                continue
+            k = (rng.standard_normal((n, nk, D)) * scale_k).astype(np.float32)
+            k[:, :, :3] *= 5
+            v = (rng.standard_normal((n, nk, D)) + 0.3).astype(np.float32)
+            for (t, j, h, d, which) in poison:
+                if t == s:
+                    (k if which == "k" else v)[j, h, d] = np.nan if d % 2 else np.inf
+            j = np.arange(n)
+            slots = torch.from_numpy((table[s, j // page] * page + j % page).astype(np.int32)).cuda()
+            ctx.kv_append(self.cache, slots, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+            gk, gv = (torch.empty((n, nk, D), dtype=torch.float16, device="cuda") for _ in range(2))
+            ctx.kv_read(self.cache, slots, gk, gv)
+            torch.cuda.synchronize()
+            self.k.append(gk.cpu().numpy()), self.v.append(gv.cpu().numpy())
+        self.gone = gone                                                           # (sequence, page) whose entry names no page
+        for s, p in gone:
+            table[s, p] = -1 if p % 2 else pages
+        self.start = np.concatenate([[0], np.cumsum([r for r, _ in seqs])]).astype(np.int32)
+        self.T = int(self.start[-1])
+        self.extra = 2                                                             # rows behind the last sequence
+        q = (rng.standard_normal((self.T + self.extra, nq, D)) * scale_q).astype(np.float32)
+        dt = getattr(torch, KINDS[kind])
+        q = torch.from_numpy(q).to(dt).cuda()
+        if layout == "heads":
+            q = q.transpose(0, 1).contiguous().transpose(0, 1)
+        elif layout == "part":
+            w = torch.zeros((q.shape[0], nq + 2 * nk, D), dtype=dt, device="cuda")
+            w[:, :nq] = q
+            q = w[:, :nq]
+        elif layout == "odd":
+            w = torch.zeros((q.shape[0], nq * (D + 1) + 1), dtype=dt, device="cuda")[:, 1:].unflatten(1, (nq, D + 1))[:, :, :D]
+            w.copy_(q)
+            q = w
+        self.q = q
+        self.out = torch.full_like(q, 7.0)
+        self.sink = rng.standard_normal(nq).astype(np.float32) * 2
+        dev = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+        self.start_d, self.lens_d, self.table_d = dev(self.start), dev(np.array([n for _, n in seqs], np.int32)), dev(table)
+
+    def run(self, ctx, sink=False, **how):
+        ctx.attention(self.cache, self.q, self.out, self.start_d, self.lens_d, self.table_d,
+                      sink=self.torch.from_numpy(self.sink).cuda() if sink else None, **how)
+        self.torch.cuda.synchronize()
+        return host(self.out)
+
+    def seen(self, s, causal, window):
+        r, n = self.seqs[s]
+        pos, key = np.arange(n - r, n)[:, None], np.arange(n)[None]
+        see = (key <= pos) if causal else np.ones((r, n), bool)
+        if window:
+            see = see & (key > pos - window)
+        for t, p in self.gone:
+            if t == s:
+                see = see & (key // self.page != p)
+        return see
+
+    def check(self, got, causal=True, window=0, sink=False, scale=None, only=None):
+        D, q = self.D, host(self.q).astype(np.float64)
+        kind = str(self.q.dtype).split(".")[1]
+        scale = D ** -0.5 if scale is None else scale
+        parts = kind == "float32"
+        g = self.nq // self.nk
+        for s, (r, n) in enumerate(self.seqs):
+            if only is not None and s not in only:
+                continue
+            see = self.seen(s, causal, window)
+            for h in range(self.nq):
+                x = q[self.start[s]:self.start[s] + r, h]
+                k, v = self.k[s][:, h // g].astype(np.float64), self.v[s][:, h // g].astype(np.float64)
+                out = got[self.start[s]:self.start[s] + r, h].astype(np.float64)
+                bad = ~np.isfinite(k).all(-1)                                      # keys whose score is NaN
+                lost = (see & bad[None]).any(-1) | (~np.isfinite(x).all(-1) & see.any(-1))
+                nan = lost[:, None] | ((see[:, :, None] & ~np.isfinite(v)[None]).any(1) if not np.isfinite(v).all() else False)
+                assert np.array_equal(np.isnan(out), np.broadcast_to(nan, out.shape)), (s, h, "NaN")
+                fine = ~lost
+                kk, vv = np.where(np.isfinite(k), k, 0), np.where(np.isfinite(v), v, 0)
+                x = np.where(np.isfinite(x), x, 0)
+                want, weight, _ = F.attention(x, kk, vv, scale, see, self.sink[h] if sink else None)
+                A = np.where(see, np.abs(x) @ np.abs(kk).T, 0).max(-1, initial=0) * abs(scale)
+                if sink:
+                    A = np.maximum(A, abs(float(self.sink[h])))
+                ds = A * ((2 * D + 32) * 2.0 ** -24 + (2.0 ** -22 if parts else 0))
+                rel = (2.0 ** -22 if parts else 2.0 ** -11) + 2.0 ** -21 + 2 * ds + (32 + n / 32 + 800) * 2.0 ** -23
+                tol = rel[:, None] * weight + n * 2.0 ** -38 * np.abs(vv).max(initial=0)
+                tol = tol * (1 + F.HALF[kind]) + F.HALF[kind] * np.abs(want) + F.LEAST[kind] + 1e-30
+                off = np.where(nan, 0, np.abs(out - want) - tol)[fine]
+                worst = off.max(initial=-1.0)
+                assert worst <= 0, (s, h, worst, np.argwhere(off > 0)[:3])
+        assert (got[self.T:] == 7).all(), "rows of no sequence"
+
+
+DECODE = [  # sequences (rows, keys), nq, nk, D, type, page, layout
+    ([(1, 1)], 1, 1, 64, "f32", 16, "dense"),
+    ([(1, 2), (1, 0), (0, 5), (1, 16), (1, 17)], 2, 1, 128, "f16", 16, "dense"),
+    ([(1, 31), (1, 32), (1, 33), (1, 127), (1, 128), (1, 129)], 12, 2, 128, "f32", 16, "part"),
+    ([(1, 300)], 12, 2, 128, "bf16", 48, "heads"),
+    ([(1, 700), (1, 3), (1, 1500)], 8, 8, 64, "bf16", 64, "odd"),
+    ([(1, 257), (1, 96)], 16, 1, 96, "f16", 32, "odd"),
+    ([(1, 513), (1, 65)], 6, 3, 96, "f32", 48, "part"),
+    ([(1, 400)], 10, 2, 192, "bf16", 16, "heads"),
+    ([(1, 333), (1, 40)], 3, 1, 192, "f32", 64, "dense"),
+    ([(1, 640), (1, 100)], 16, 2, 256, "f16", 128, "dense"),
+    ([(1, 200), (1, 90)], 4, 4, 256, "f32", 16, "odd"),
+    ([(3, 200), (1, 77), (2, 2), (4, 500)], 8, 2, 128, "bf16", 32, "part"),
+    ([(5, 100), (8, 8), (7, 300)], 8, 2, 64, "f32", 16, "dense"),                  # up to 32 rows of a head
+    ([(3, 130), (2, 259)], 20, 2, 128, "f32", 32, "heads"),
+    ([(5, 70)], 7, 1, 96, "f16", 16, "dense"),
+    ([(3, 90), (9, 60)], 14, 2, 256, "bf16", 16, "dense"),                         # several blocks of rows
+    ([(5, 3), (9, 4), (3, 1)], 4, 1, 64, "f16", 16, "dense"),                      # more rows than keys
+    ([(1, 20000)], 4, 1, 128, "bf16", 128, "dense"),
+    ([(1, 9000), (2, 1), (1, 3000)], 4, 2, 64, "f32", 16, "dense"),
+]
+
+
+@pytest.mark.parametrize("case", DECODE, ids=[str(i) for i in range(len(DECODE))])
+def test_few_rows(torch_dev, ctx, case):
+    seqs, nq, nk, D, kind, page, layout = case
+    b = Batch(torch_dev, ctx, seqs, nq, nk, D, kind, page, layout=layout)
+    b.check(b.run(ctx))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, sink=True, causal=False, scale=0.3), causal=False, sink=True, scale=0.3)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=21, scale=-0.05, max_rows=1, max_len=1), window=21, scale=-0.05)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=200, sink=True, max_rows=1000, max_len=10 ** 6), window=200, sink=True)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_pages_that_are_gone(torch_dev, ctx, kind, D):
+    """Table entries that name no page hide their keys; a row may be left without any."""
+    b = Batch(torch_dev, ctx, [(2, 150), (1, 20), (1, 33)], 4, 2, D, kind, 16, gone=[(0, 0), (0, 1), (0, 5), (1, 0), (1, 1), (2, 2)])
+    got = b.run(ctx)
+    b.check(got)
+    assert (got[2] == 0).all()
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, sink=True, window=40), sink=True, window=40)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("window", [0, 9])
+def test_nan_reaches_the_rows_that_see_it(torch_dev, ctx, kind, D, window):
+    """NaN and infinities among keys (a row that sees one is NaN) and values (its 32 values are), on both sides of the rows' diagonal
+    and of the window's edge."""
+    last = D - 1
+    poison = [(0, 95, 0, 3, "k"), (0, 93, 1, 40, "v"), (1, 60, 1, last, "v"), (1, 51, 0, 1, "v"), (2, 5, 0, last, "k"), (3, 2, 1, 2, "v")]
+    b = Batch(torch_dev, ctx, [(6, 97), (8, 63), (1, 6), (4, 4), (2, 50)], 4, 2, D, kind, 16, poison=poison)
+    b.q[-4, 1, 5] = float("inf")                                                   # a query as well (of the last sequence)
+    b.q[-3, 0, 0] = float("nan")
+    b.check(b.run(ctx, window=window), window=window)
+
+
+def test_queries_of_any_size(torch_dev, ctx):
+    """Rows whose values lie far apart or far from 1: a row is scaled by its largest value."""
+    torch = torch_dev
+    for kind, sizes in (("f32", (1e-30, 1e-3, 1.0, 50.0)), ("bf16", (1e-30, 1.0, 300.0)), ("f16", (1e-6, 1.0, 30.0))):
+        b = Batch(torch, ctx, [(len(sizes), 70)], 2, 1, 128, kind, 16)
+        for i, z in enumerate(sizes):
+            b.q[i] *= z
+        b.q[0, 0] = 0
+        b.check(b.run(ctx))
+
+
+def test_scores_far_apart(torch_dev, ctx):
+    """Scores in the hundreds: one key takes all, in one part of the keys or another."""
+    for kind in ("f32", "f16", "bf16"):
+        b = Batch(torch_dev, ctx, [(1, 900), (2, 450)], 4, 1, 128, kind, 32, scale_q=8.0, scale_k=6.0)
+        b.check(b.run(ctx))
+
+
+def test_same_bits_every_time(torch_dev, ctx):
+    torch = torch_dev
+    b = Batch(torch, ctx, [(1, n) for n in (4000, 17, 900, 2500, 1, 333)], 8, 2, 128, "bf16", 64)
+    first = b.run(ctx).copy()
+    for _ in range(5):
+        b.out.fill_(3.0)
+        assert np.array_equal(b.run(ctx)[:b.T], first[:b.T])
+
+
+def test_many_sequences(torch_dev, ctx):
+    """More sequences than a workgroup has threads, some without rows or keys."""
+    rng = np.random.default_rng(2)
+    seqs = [(int(rng.integers(0, 3)), int(rng.integers(0, 70))) for _ in range(700)]
+    seqs = [(min(r, max(n, 1)), n) for r, n in seqs]
+    b = Batch(torch_dev, ctx, seqs[:300], 2, 1, 64, "f16", 16)
+    b.check(b.run(ctx))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=5, sink=True), window=5, sink=True)
+
+
+def test_bad_starts_and_lengths_stay_in_bounds(torch_dev, ctx):
+    """start and len are read on the device: rows outside [0, T) and keys outside the table do not exist."""
+    torch = torch_dev
+    b = Batch(torch, ctx, [(1, 40), (1, 50), (1, 30)], 2, 1, 64, "f32", 16)
+    want = b.run(ctx).copy()
+    b.lens_d[0] = -7
+    b.lens_d[2] = 2 ** 31 - 1                                                      # its table's entries past the pages name none, or NaN
+    b.start_d[0] = -2 ** 31
+    b.start_d[3] = 2 ** 31 - 1
+    b.out.fill_(7.0)
+    got = b.run(ctx)
+    assert np.array_equal(got[1], want[1])
+
+
+def test_cache_past_4_gib(torch_dev, ctx):
+    """Pages whose records lie further than 2^32 bytes behind the first, and q rows that do."""
+    import beglin_amd
+    torch = torch_dev
+    page, nk, D = 256, 8, 128
+    per = page // 16 * nk * 20 * D
+    pages = (5 << 30) // per
+    cache = beglin_amd.KVCache(pages, page, nk, D)
+    small = beglin_amd.KVCache(3, page, nk, D)
+    n = 600
+    rng = np.random.default_rng(4)
+    k, v = (torch.from_numpy(rng.standard_normal((n, nk, D)).astype(np.float32)).cuda() for _ in range(2))
+    tables = []
+    for c, ids in ((cache, [pages - 1, 3, pages - 2]), (small, [0, 1, 2])):
+        ids = np.array(ids, np.int32)
+        at = np.arange(n)
+        slots = torch.from_numpy((ids[at // page].astype(np.int64) * page + at % page).astype(np.int32)).cuda()
+        ctx.kv_append(c, slots, k, v)
+        tables.append(torch.from_numpy(ids[None]).cuda())
+        a, e = torch.empty((n, nk, D), device="cuda"), torch.empty((n, nk, D), device="cuda")
+        ctx.kv_read(c, slots, a, e)
+        torch.cuda.synchronize()
+        assert np.array_equal(a.cpu().numpy(), F.kept(k.cpu().numpy()).astype(np.float32))
+    q = torch.from_numpy(rng.standard_normal((2, 16, D)).astype(np.float32)).cuda()
+    start, lens = torch.tensor([0, 2], dtype=torch.int32, device="cuda"), torch.tensor([n], dtype=torch.int32, device="cuda")
+    outs = []
+    for c, t in zip((cache, small), tables):
+        out = torch.empty_like(q)
+        ctx.attention(c, q, out, start, lens, t)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
+    del cache
+    torch.cuda.empty_cache()
+
+
+def test_captured_decode_steps(torch_dev):
+    """append and attention of a step as one graph, replayed as the sequences grow, beside eager calls of the same context on other buffers."""
+    import beglin_amd as B
+    torch = torch_dev
+    rng = np.random.default_rng(9)
+    st = torch.cuda.Stream()
+    c = B.Context(0, st.cuda_stream)
+    S, nq, nk, D, page, wide = 3, 8, 2, 128, 16, 6
+    dt = torch.bfloat16
+    kv = [B.KVCache(S * wide, page, nk, D) for _ in range(2)]
+    for x in kv:
+        x.data.fill_(0xFF)
+    table = torch.from_numpy(rng.permutation(S * wide).astype(np.int32).reshape(S, wide)).cuda()
+    start = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros((S, nq + 2 * nk, D), dtype=dt, device="cuda")
+    q, k, v = qkv[:, :nq], qkv[:, nq:nq + nk], qkv[:, nq + nk:]
+    lens, slots, pos = (torch.zeros(S, dtype=torch.int32, device="cuda") for _ in range(3))
+    a = np.arange(512)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    rope = torch.from_numpy(np.concatenate([np.cos(a), np.sin(a)], 1).astype(np.float32)).cuda()
+    outs = [(torch.empty((S, nq, D), dtype=dt, device="cuda"), torch.empty((S, nq, D), dtype=dt, device="cuda")) for _ in range(2)]
+
+    def step(i):
+        c.kv_append(kv[i], slots, k, v, q=q, q_out=outs[i][0], norm=B.NORM_RMS, rope=rope, pos=pos)
+        c.attention(kv[i], outs[i][0], outs[i][1], start, lens, table, max_rows=1, max_len=wide * page)
+
+    def inputs(n):
+        ls = [n + 1 + 7 * s for s in range(S)]
+        qkv.copy_(torch.from_numpy(rng.standard_normal(tuple(qkv.shape)).astype(np.float32)))
+        lens.copy_(torch.tensor(ls, dtype=torch.int32))
+        pos.copy_(torch.tensor([x - 1 for x in ls], dtype=torch.int32))
+        slots.copy_(torch.tensor([int(table[s, (x - 1) // page]) * page + (x - 1) % page for s, x in enumerate(ls)], dtype=torch.int32))
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        for n in range(-14, 0):                                                    # sequences 1 and 2 are longer: their first keys
+            ls = [n + 1 + 7 * s for s in range(S)]
+            if max(ls) < 1:
+                continue
+            inputs(n)
+            slots.copy_(torch.where(lens > 0, slots, -1))
+            lens.clamp_(min=0)
+            pos.clamp_(min=0)
+            step(0), step(1)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            step(0)
+        for n in range(20):
+            inputs(n)
+            g.replay()
+            step(1)
+            st.synchronize()
+            assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1]), n
+            assert torch.isfinite(outs[0][1].float()).all()
+    assert torch.equal(kv[0].data, kv[1].data)
+    c.close()
+
+
+def test_first_call_inside_a_capture_is_refused(torch_dev):
+    import beglin_amd as B
+    torch = torch_dev
+    st = torch.cuda.Stream()
+    c = B.Context(0, st.cuda_stream)
+    kv = B.KVCache(2, 16, 1, 64)
+    kv.data.zero_()
+    q = torch.zeros((1, 1, 64), device="cuda")
+    out = torch.zeros_like(q)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    start, lens, table = i(0, 1), i(5), i(0, 1).reshape(1, 2)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            with pytest.raises(B.BglError) as e:
+                c.attention(kv, q, out, start, lens, table)
+            assert e.value.code == B.E_CAPTURE
+            q.zero_()
+        st.synchronize()
+    c.attention(kv, q, out, start, lens, table)
+    c.close()
