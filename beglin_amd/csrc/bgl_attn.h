@@ -13,7 +13,7 @@ struct AttnLaunch {
     int limit;                   // sequences with more than this many rows times g are another launch's
     float scale2;                // |scale| * log2(e); a negative scale turns q's sign
     float *part;                 // bgl_attn.hip's partial sums: [2 * workgroups] pieces
-    int *sync;                   // pieces written, for each workgroup that began one
+    int *sync;                   // for each workgroup that began a group of pieces, or an item: how many are written
 };
 
 // Weights are 2^14 exp(..): the largest is 2^14, so that fp16 keeps 11 bits of what is 2^28 times smaller.

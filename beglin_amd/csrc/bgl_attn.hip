@@ -27,6 +27,7 @@
 
 #define AT_UNIT 128              // keys a unit
 #define AT_WG 768                // workgroups at most
+#define AT_SC1 16                // the cache-policy bit of a buffer access of device scope
 
 // What a wave has loaded of 32 keys: two tiles.
 template <int G>
@@ -74,9 +75,7 @@ struct AttnWave {
 
     // Rows rb * RB .. of the sequence's n * g (row r: token r / g, head r % g of the group), scaled by a power of two that puts a
     // row's largest value in [2^14, 2^15): exact in fp16 down to 2^-28 of it (two parts for fp32 rows, 2^-22).
-    __device__ void begin(int s, int head_, int rb) {
-        head = head_;
-        table = uni(L.a.table + (size_t)s * L.a.ldt);
+    __device__ __forceinline__ void begin(int rb) {
         lo_max = 0;
         hi_min = INT32_MAX;
 #pragma unroll
@@ -277,45 +276,58 @@ struct AttnWave {
     }
 };
 
+#define AT_JOIN 32               // pieces that are joined at once, at most
 template <int G, int NT>
 struct AttnShared {
     static constexpr int D = 32 * G, RB = 16 * NT, ROW = D + 4;
-    long before[257];                                    // units before thread i's sequences
-    long wave_sum[4];
-    float m[4][RB], l[4][RB];
+    uint32_t before[257];                                // units before thread i's sequences
+    uint32_t wave_sum[4];
+    float m[4][RB], l[4][RB], M[RB], sum[RB];
     int last;
-    float o[4][RB][ROW];
+    union {
+        float o[4][RB][ROW];
+        struct { float m[AT_JOIN][RB], l[AT_JOIN][RB]; } j;
+    };
 };
 
-// The line of units.
-struct AttnLine {
-    int per;                                             // sequences a thread has counted
-    long total;
-    int wgs;
-};
 template <int RB>
 __device__ __forceinline__ void attn_units(const AttnLaunch &L, const AttnSeq &q, int &blocks, int &chunks) {
     blocks = q.n > 0 && (long)q.n * L.g <= L.limit ? (q.n * L.g + RB - 1) / RB : 0;
     chunks = max(1, (q.len - (q.lo & ~15) + AT_UNIT - 1) / AT_UNIT);
 }
 
+// The line of units in runs: the first `more` workgroups have one unit more than the others' `each`.
+struct AttnRuns {
+    uint32_t each, more, wgs;
+    __device__ AttnRuns(uint32_t total, uint32_t grid) {
+        wgs = min(grid, total);
+        each = wgs ? total / wgs : 0;
+        more = total - each * wgs;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * each + min(w, more); }
+    __device__ __forceinline__ uint32_t owner(uint32_t u) const {
+        const uint32_t head = more * (each + 1);
+        return u < head ? u / (each + 1) : more + (u - head) / each;
+    }
+};
+
 template <int G, int NT, int PARTS>
 __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
     using Wave = AttnWave<G, NT, PARTS>;
-    constexpr int D = 32 * G, RB = 16 * NT;
+    constexpr int D = 32 * G, RB = 16 * NT, PIECE = RB * (D + 2);
     __shared__ AttnShared<G, NT> sh;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), heads = L.c.heads, S = L.a.S;
     const int per = (S + 255) / 256;
-    long mine = 0;
+    uint32_t mine = 0;
     for (int s = tid * per; s < min(S, (tid + 1) * per); s++) {
         int blocks, chunks;
         attn_units<RB>(L, attn_seq(L, s), blocks, chunks);
-        mine += (long)blocks * heads * chunks;
+        mine += (uint32_t)(blocks * heads * chunks);
     }
-    long upto = mine;
+    uint32_t upto = mine;
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) {
-        const long v = __shfl_up(upto, x);
+        const uint32_t v = __shfl_up(upto, x);
         if ((tid & 63) >= x) upto += v;
     }
     if ((tid & 63) == 63) sh.wave_sum[wave] = upto;
@@ -324,45 +336,43 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
     sh.before[tid] = upto - mine;
     if (tid == 255) sh.before[256] = upto;
     __syncthreads();
-    const long total = sh.before[256], wgs = min((long)gridDim.x, total);
-    const long w = blockIdx.x;
-    if (w >= wgs) return;
-    const long end = total * (w + 1) / wgs;
-    long u = total * w / wgs;
+    const __amdgpu_buffer_rsrc_t pieces = __builtin_amdgcn_make_buffer_rsrc(L.part, (short)0, AT_WG * 2 * PIECE * 4, 0x00020000);
+    const AttnRuns runs((uint32_t)__builtin_amdgcn_readfirstlane((int)sh.before[256]), gridDim.x);
+    const uint32_t w = blockIdx.x;
+    if (w >= runs.wgs) return;
+    const uint32_t end = runs.begin(w + 1);
+    uint32_t u = runs.begin(w);
     // the sequence of unit u: the last thread whose sequences begin at or before it, then that thread's sequences in turn
     int th = 0;
 #pragma unroll
     for (int x = 128; x; x >>= 1)
         if (sh.before[th + x] <= u) th += x;
+    th = __builtin_amdgcn_readfirstlane(th);
     int s = th * per;
-    long base = sh.before[th];                           // units before sequence s
+    uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.before[th]);       // units before sequence s
     Wave W(L);
     int blocks, chunks;
-    auto seek = [&] {                                    // to the sequence of unit u
-        while (true) {
+    while (u < end) {
+        while (true) {                                   // to the sequence of unit u
             W.q = attn_seq(L, s);
             W.q.begin = __builtin_amdgcn_readfirstlane(W.q.begin);
             W.q.n = __builtin_amdgcn_readfirstlane(W.q.n);
             W.q.len = __builtin_amdgcn_readfirstlane(W.q.len);
             W.q.lo = __builtin_amdgcn_readfirstlane(W.q.lo);
             attn_units<RB>(L, W.q, blocks, chunks);
-            const long n = (long)blocks * heads * chunks;
+            const uint32_t n = (uint32_t)(blocks * heads * chunks);
             if (u < base + n) break;
             base += n;
             s++;
         }
-    };
-    while (u < end) {
-        seek();
-        const long item = (u - base) / chunks;           // head * blocks + row block
-        const int head = __builtin_amdgcn_readfirstlane((int)(item / blocks)), rb = __builtin_amdgcn_readfirstlane((int)(item % blocks));
-        const int c0 = __builtin_amdgcn_readfirstlane((int)(u - base - item * chunks));
-        const int c1 = __builtin_amdgcn_readfirstlane((int)min((long)chunks, c0 + (end - u)));
-        W.begin(s, head, rb);
-        const int key0 = (W.q.lo & ~15) + wave * 32;
+        const int item = (int)((u - base) / (uint32_t)chunks);                       // head * blocks + row block
+        const int head = item / blocks, rb = item - head * blocks;
+        const int c0 = (int)(u - base) - item * chunks, c1 = min(chunks, c0 + (int)(end - u));
+        W.head = head;
+        W.table = uni(L.a.table + (size_t)s * L.a.ldt);
         AttnRaw<G> ra, rn;
         int pa[2], pb[2];
-        int left = 0, key = key0 + c0 * AT_UNIT;         // units in which the wave has keys
+        int left = 0, key = (W.q.lo & ~15) + wave * 32 + c0 * AT_UNIT;                 // left: units in which the wave has keys
         if (key < W.q.len) left = min(c1 - c0, (W.q.len - key + AT_UNIT - 1) / AT_UNIT);
         auto fetch = [&](AttnRaw<G> &r, int (&p)[2], int k) {
             p[0] = W.page(k);
@@ -370,6 +380,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
             W.load(r, k, p);
         };
         if (left) fetch(ra, pa, key);
+        W.begin(rb);
         while (left) {                                   // the next unit is on its way while one is worked on
             if (left > 1) fetch(rn, pb, key + AT_UNIT);
             W.step(ra, key, pa);
@@ -380,6 +391,12 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
             key += AT_UNIT;
             --left;
         }
+        const int rows = min(RB, W.q.n * L.g - rb * RB);
+        auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out, over the row's sum of weights
+            const int i = (rb * RB + r) / L.g, h = (rb * RB + r) - i * L.g;
+            v *= attn_factor(sh.M[r], sh.sum[r], L.a.sink != nullptr, L.a.sink ? L.a.sink[head * L.g + h] * 1.44269504088896340736f : 0.0f);
+            kv_store4(L.a.out, L.a.type, (long)(W.q.begin + i) * L.a.ldo + (long)(head * L.g + h) * L.a.hdo + d, v);
+        };
         // the four waves' sums
         __syncthreads();                                 // the segment before this one has read them
 #pragma unroll
@@ -392,73 +409,110 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
         for (int t = 0; t < NT; t++) {
             const int r = 16 * t + W.col;
             const float M = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
-            const float f = W.m[t] == -INFINITY ? 0.0f : at_exp2(W.m[t] - M);
+            const float f = W.m[t] == -INFINITY ? 0.0f : at_exp2(W.m[t] - M);          // (a wave without keys has sums of 0 or NaN)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float *to = &sh.o[wave][r][2 * G * (4 * W.b + i)];
 #pragma unroll
-                for (int j = 0; j < 2 * G; j += 2) {
-                    // (a wave without keys has sums of 0, whatever its factor)
-                    to[j] = W.o[t][j][i] * f;
-                    to[j + 1] = W.o[t][j + 1][i] * f;
-                }
+                for (int j = 0; j < 2 * G; j++) to[j] = W.o[t][j][i] * f;
             }
+        }
+        if (tid < RB) {
+            float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) M = fmaxf(M, sh.m[k][tid]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) sum += sh.l[k][tid] * (sh.m[k][tid] == -INFINITY ? 0.0f : at_exp2(sh.m[k][tid] - M));
+            sh.M[tid] = M;
+            sh.sum[tid] = sum;
         }
         __syncthreads();
         const bool whole = c0 == 0 && c1 == chunks;
-        const int rows = min(RB, W.q.n * L.g - rb * RB);
-        const long first = u - c0, last = first + chunks - 1;                        // the item's units
-        const long wA = ((first + 1) * wgs - 1) / total, wB = ((last + 1) * wgs - 1) / total;
-        float *const piece = L.part + (2 * w + (c0 == 0)) * (RB * (D + 2));
-        auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out
-            const int i = (rb * RB + r) / L.g, h = head * L.g + (rb * RB + r) % L.g;
-            const size_t at = (size_t)((long)(W.q.begin + i) * L.a.ldo + (long)h * L.a.hdo + d);
-#pragma unroll
-            for (int e = 0; e < 4; e++) i8_st(L.a.out, L.a.type, at + e, v[e]);
-        };
-        auto sink2 = [&](int r) { return L.a.sink ? L.a.sink[head * L.g + (rb * RB + r) % L.g] * 1.44269504088896340736f : 0.0f; };
+        // Pieces go through accesses of device scope (sc1), which no XCD's L2 holds back or stale: no cache is written back or
+        // emptied (a fence of that scope in each of 768 workgroups took 200 us).
+        auto piece = [&](uint32_t k, uint32_t first) { return (2 * k + (k == first)) * (uint32_t)(PIECE * 4); };
+        auto get4 = [&](uint32_t at) { return __builtin_bit_cast(kv_f4, __builtin_amdgcn_raw_buffer_load_b128(pieces, at, 0, AT_SC1)); };
+        auto get = [&](uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pieces, at, 0, AT_SC1)); };
+        auto set4 = [&](uint32_t at, kv_f4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(at_u4, v), pieces, at, 0, AT_SC1); };
+        auto set = [&](uint32_t at, float v) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), pieces, at, 0, AT_SC1); };
+        const uint32_t wA = whole ? w : runs.owner(u - c0), wB = whole ? w : runs.owner(u - c0 + chunks - 1);
+        const uint32_t mine_at = piece(w, wA);
         for (int x = tid; x < rows * (D / 4); x += 256) {
             const int r = x / (D / 4), d = x % (D / 4) * 4;
-            const float M = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
-            kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            float sum = 0.0f;
+            kv_f4 v = *(const kv_f4 *)&sh.o[0][r][d];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v += *(const kv_f4 *)&sh.o[k][r][d];
-                sum += sh.l[k][r] * (sh.m[k][r] == -INFINITY ? 0.0f : at_exp2(sh.m[k][r] - M));
-            }
-            if (whole) {
-                put(r, d, v * attn_factor(M, sum, L.a.sink != nullptr, sink2(r)));
-            } else {
-                *(kv_f4 *)(piece + r * D + d) = v;
-                if (d == 0) { piece[RB * D + r] = M; piece[RB * D + RB + r] = sum; }
-            }
+            for (int k = 1; k < 4; k++) v += *(const kv_f4 *)&sh.o[k][r][d];
+            if (whole) put(r, d, v);
+            else set4(mine_at + (r * D + d) * 4, v);
         }
         if (!whole) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const int n = atomicAdd(L.sync + wA, 1) + 1;
-                sh.last = n == (int)(wB - wA + 1);
-                if (sh.last) atomicExch(L.sync + wA, 0);
+            if (tid < rows) {
+                set(mine_at + (RB * D + tid) * 4, sh.M[tid]);
+                set(mine_at + (RB * D + RB + tid) * 4, sh.sum[tid]);
             }
-            __syncthreads();
-            if (sh.last) {                               // every piece of the item is written
-                __threadfence();
-                auto at = [&](long k) { return L.part + (2 * k + (k == wA)) * (RB * (D + 2)); };
+            // Pieces wA .. wB are joined in groups of `size`, then the groups' sums: whoever comes last joins.
+            const uint32_t n = wB - wA + 1;
+            uint32_t size = n;
+            if (n > AT_JOIN / 2) {
+                size = (uint32_t)ceilf(sqrtf((float)n));                             // <= 28 of 768
+            }
+            const uint32_t groups = (n + size - 1) / size;
+            auto last = [&](int *count, uint32_t of) {   // whether the others have all written theirs
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                       // they are in memory
+                __syncthreads();
+                if (tid == 0) {
+                    sh.last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == (int)of;
+                    if (sh.last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                return sh.last != 0;
+            };
+            // pieces first, first + step, .. (count of them) into out, or into the first of them
+            auto join = [&](uint32_t first, uint32_t step, int count, bool end_) {
+                for (int x = tid; x < count * rows; x += 256) {
+                    const int k = x / rows, r = x - k * rows;
+                    const uint32_t at = piece(first + k * step, wA) + (RB * D + r) * 4;
+                    sh.j.m[k][r] = get(at);
+                    sh.j.l[k][r] = get(at + RB * 4);
+                }
+                __syncthreads();
+                if (tid < rows) {
+                    float M = -INFINITY, sum = 0.0f;
+                    for (int k = 0; k < count; k++) M = fmaxf(M, sh.j.m[k][tid]);
+                    for (int k = 0; k < count; k++) {
+                        const float f = sh.j.m[k][tid] == -INFINITY ? 0.0f : at_exp2(sh.j.m[k][tid] - M);
+                        sum += sh.j.l[k][tid] * f;
+                        sh.j.m[k][tid] = f;
+                    }
+                    sh.M[tid] = M;
+                    sh.sum[tid] = sum;
+                }
+                __syncthreads();
                 for (int x = tid; x < rows * (D / 4); x += 256) {
                     const int r = x / (D / 4), d = x % (D / 4) * 4;
-                    float M = -INFINITY;
-                    for (long k = wA; k <= wB; k++) M = fmaxf(M, at(k)[RB * D + r]);
                     kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                    float sum = 0.0f;
-                    for (long k = wA; k <= wB; k++) {
-                        const float mk = at(k)[RB * D + r], f = mk == -INFINITY ? 0.0f : at_exp2(mk - M);
-                        v += *(const kv_f4 *)(at(k) + r * D + d) * f;
-                        sum += at(k)[RB * D + RB + r] * f;
+                    for (int k0 = 0; k0 < count; k0 += 8) {                          // eight loads on their way at once
+                        kv_f4 y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) y[k] = get4(piece(first + min(k0 + k, count - 1) * step, wA) + (r * D + d) * 4);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (k0 + k < count) v += y[k] * sh.j.m[k0 + k][r];
                     }
-                    put(r, d, v * attn_factor(M, sum, L.a.sink != nullptr, sink2(r)));
+                    if (end_) put(r, d, v);
+                    else set4(piece(first, wA) + (r * D + d) * 4, v);
                 }
+                if (!end_ && tid < rows) {
+                    const uint32_t to = piece(first, wA) + (RB * D + tid) * 4;
+                    set(to, sh.M[tid]);
+                    set(to + RB * 4, sh.sum[tid]);
+                }
+            };
+            const uint32_t group = (w - wA) / size, at = wA + group * size;
+            const uint32_t in = min(size, wB + 1 - at);
+            if (last(L.sync + 3 * at + (at == wA), in)) {    // (an item may end where the next begins)
+                if (in > 1 || groups == 1) join(at, 1, (int)in, groups == 1);
+                if (groups > 1 && last(L.sync + 3 * wA + 2, groups)) join(wA, size, (int)groups, true);
             }
         }
         u += c1 - c0;
@@ -504,6 +558,9 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (!(a->scale == a->scale) || a->scale - a->scale != 0.0f) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: scale is not finite");
     if (a->q == a->out) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: out is q");
     if ((long)a->T * (a->nq / kv->heads) > INT32_MAX / 2) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of %d heads", a->T, a->nq);
+    // units are counted in 32 bits
+    if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_UNIT + 2) > 2e9)
+        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows over %d pages of %d tokens", a->T, a->ldt, kv->page);
     HIPCHK(hipSetDevice(c->device));
     AttnLaunch L;
     memset(&L, 0, sizeof L);
@@ -517,7 +574,7 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     const int rows = std::min(std::max(1, a->max_rows), a->T) * L.g, G = kv->D / 32;
     const int nt = rows > 16 && G <= 4 ? 2 : 1, RB = 16 * nt;
     if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)2 * AT_WG * 32 * (128 + 2) * 4, false)) return rc;
-    if (const int rc = dbuf_reserve(c, c->attn_sync, AT_WG * sizeof(int), true)) return rc;
+    if (const int rc = dbuf_reserve(c, c->attn_sync, 3 * AT_WG * sizeof(int), true)) return rc;
     L.part = (float *)c->attn_part.p;
     L.sync = (int *)c->attn_sync.p;
     const long units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * (((long)std::max(1, a->max_len) + AT_UNIT - 1) / AT_UNIT);

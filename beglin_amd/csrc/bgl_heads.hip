@@ -3,7 +3,7 @@
 //
 //   n = x | x / sqrt(mean(x^2) + eps) w | (x - mean) / sqrt(var + eps) w         over the D values of a head
 //   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i                            for the pairs (i, j) that are rotated
-//   groups of 32: m = fp16(min), s = fp16((max - m) / 15), c = rint((x - m) / s), value fp16(c s + m)
+//   groups of 32: m = fp16(min), s = fp16((max - m) (1/15)), c = rint((x - m) / s), value fp16(c s + m)
 //
 // A code changes by one where a value lies within rounding of a border between codes.  So y is computed in double and rounded
 // once to fp32, and from there each step is one fp32 operation: the codes are the formula's.  (gfx950 issues double
@@ -137,7 +137,7 @@ __device__ __forceinline__ uint32_t hd_codes(uint32_t (&c)[8], const float (&x)[
     top = max(top, (uint32_t)dpp_i<0xB1>((int)top)); top = max(top, (uint32_t)dpp_i<0x4E>((int)top));
     const _Float16 m = (_Float16)lo;
     const float fm = (float)m;
-    const _Float16 s = (_Float16)fmaxf(0.0f, __fdiv_rn(__fsub_rn(hi, fm), 15.0f));
+    const _Float16 s = (_Float16)fmaxf(0.0f, __fmul_rn(__fsub_rn(hi, fm), 1.0f / 15.0f));
     const float r = __fdiv_rn(1.0f, (float)s);
     const bool none = !((float)s > 0.0f) || top >= 0x7f800000u;
 #pragma unroll

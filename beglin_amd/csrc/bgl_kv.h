@@ -68,5 +68,12 @@ __device__ __forceinline__ void kv_store8(void *p, int type, long at, const floa
     *(kv_mu4 *)((uint16_t *)p + at) = u;
 }
 
+// 4 values
+__device__ __forceinline__ void kv_store4(void *p, int type, long at, kv_f4 q) {
+    typedef unsigned int u2 __attribute__((ext_vector_type(2), aligned(2)));
+    if (type == BGL_T_F32) *(kv_mf4 *)((float *)p + at) = q;
+    else *(u2 *)((uint16_t *)p + at) = u2{(uint32_t)i8_h16(q[0], type) | (uint32_t)i8_h16(q[1], type) << 16,
+                                          (uint32_t)i8_h16(q[2], type) | (uint32_t)i8_h16(q[3], type) << 16};
+}
 // The descriptor's checks (bgl_heads.hip); 0 or an error code.
 int kv_check(const char *who, const bgl_kv *kv);

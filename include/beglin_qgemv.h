@@ -249,7 +249,7 @@ typedef struct {
 int  bgl_heads_dev(bgl_ctx *ctx, const bgl_heads *d);
 /* A cache of keys and values in pages of `page` tokens (a multiple of 16), `heads` heads of D = 64, 96, 128, 192 or 256
  * values.  Each 32 values of a head are held as codes c of 4 bits with a step s and a floor m in fp16, from fp32 values x:
- *     x held to +-32768;  m = fp16(min x);  s = fp16(max(0, (max x - m) / 15))
+ *     x held to +-32768;  m = fp16(min x);  s = fp16(max(0, (max x - m) * fp32(1 / 15)))
  *     c = rint((x - m) * (1 / s)) held to 0 .. 15, 0 where s = 0      (every step one fp32 operation)
  * and stand for fp16(c * s + m), rounded once.  32 values with a NaN or an infinity among them are kept as NaN.
  * data: bgl_kv_bytes bytes of device memory, 16-byte aligned, [pages][heads][page / 16] records of 20 D bytes for 16

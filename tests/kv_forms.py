@@ -40,7 +40,7 @@ def kept(x):
     g = np.clip(np.where(bad, 0, g), np.float32(-32768), np.float32(32768)).astype(np.float32)
     m = g.min(-1, keepdims=True).astype(np.float16)
     fm = m.astype(np.float32)
-    s = np.maximum(np.float32(0), (g.max(-1, keepdims=True) - fm) / np.float32(15)).astype(np.float16)
+    s = np.maximum(np.float32(0), (g.max(-1, keepdims=True) - fm) * (np.float32(1) / np.float32(15))).astype(np.float16)
     fs = s.astype(np.float32)
     r = np.float32(1) / np.where(fs > 0, fs, np.float32(1))
     c = np.where(fs > 0, np.clip(np.rint((g - fm) * r), 0, 15), 0)
@@ -81,7 +81,7 @@ def pack(k, v):
     for half, x in enumerate((k, v)):
         g = x.reshape(n, 16, G, 32).astype(np.float32)
         m = g.min(-1).astype(np.float16)
-        s = np.maximum(np.float32(0), (g.max(-1) - m.astype(np.float32)) / np.float32(15)).astype(np.float16)
+        s = np.maximum(np.float32(0), (g.max(-1) - m.astype(np.float32)) * (np.float32(1) / np.float32(15))).astype(np.float16)
         fs = s.astype(np.float32)[..., None]
         r = np.float32(1) / np.where(fs > 0, fs, np.float32(1))
         c = np.where(fs > 0, np.clip(np.rint((g - m.astype(np.float32)[..., None]) * r), 0, 15), 0).astype(np.uint8)
