@@ -9,7 +9,8 @@ struct AttnLaunch {
     bgl_kv c;
     bgl_attn a;
     int g;                       // heads of q for one of the cache
-    int ppt, ppt_shift;          // 16-token tiles a page; log2 of it, or -1
+    int ppt;                     // 16-token tiles a page
+    uint32_t div_mul, div_shift; // t / ppt = (mulhi(t, div_mul) + t) >> div_shift for t < 2^31
     int limit;                   // sequences with more than this many rows times g are another launch's
     float scale2;                // |scale| * log2(e); a negative scale turns q's sign
     float *part;                 // bgl_attn.hip's partial sums: [2 * workgroups] pieces
@@ -41,22 +42,32 @@ __device__ __forceinline__ void attn_keys(const AttnLaunch &L, const AttnSeq &q,
 }
 
 // ------------------------------------------------------------------ the cache's codes as operands
-// fp16 pairs of the codes at bits 0 or 4 of each half of w (see bgl_kv.h), times s plus m, rounded once
-__device__ __forceinline__ kv_h2 at_lo(uint32_t w, kv_h2 s, kv_h2 m) {
-    const kv_h2 c = __builtin_bit_cast(kv_h2, (w & 0x000f000fu) | 0x64006400u) - kv_h2{(_Float16)1024.0f, (_Float16)1024.0f};
+// fp16 pairs of the codes at bits 0 or 4 of each half of w (see bgl_kv.h), times s plus m, rounded once.  (The compiler takes two
+// instructions for and + or with two constants, which cannot both be scalar operands.)
+struct AtMagic {
+    uint32_t lo, hi;                                     // in vector registers
+    __device__ AtMagic() : lo(0x64006400u), hi(0x54005400u) { asm volatile("" : "+v"(lo), "+v"(hi)); }
+};
+__device__ __forceinline__ uint32_t at_and_or(uint32_t w, uint32_t mask, uint32_t with) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(with));
+    return r;
+}
+__device__ __forceinline__ kv_h2 at_lo(const AtMagic &g, uint32_t w, kv_h2 s, kv_h2 m) {
+    const kv_h2 c = __builtin_bit_cast(kv_h2, at_and_or(w, 0x000f000fu, g.lo)) - kv_h2{(_Float16)1024.0f, (_Float16)1024.0f};
     return __builtin_elementwise_fma(c, s, m);
 }
-__device__ __forceinline__ kv_h2 at_hi(uint32_t w, kv_h2 s, kv_h2 m) {
-    const kv_h2 c = __builtin_bit_cast(kv_h2, (w & 0x00f000f0u) | 0x54005400u) - kv_h2{(_Float16)64.0f, (_Float16)64.0f};
+__device__ __forceinline__ kv_h2 at_hi(const AtMagic &g, uint32_t w, kv_h2 s, kv_h2 m) {
+    const kv_h2 c = __builtin_bit_cast(kv_h2, at_and_or(w, 0x00f000f0u, g.hi)) - kv_h2{(_Float16)64.0f, (_Float16)64.0f};
     return __builtin_elementwise_fma(c, s, m);
 }
 __device__ __forceinline__ kv_h8 at_join(kv_h2 a, kv_h2 b, kv_h2 c, kv_h2 d) {
     return kv_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 // 8 neighbouring values of a key from their dword and the group's (s, m)
-__device__ __forceinline__ kv_h8 at_key(uint32_t w, uint32_t sm) {
+__device__ __forceinline__ kv_h8 at_key(const AtMagic &g, uint32_t w, uint32_t sm) {
     const kv_h2 p = __builtin_bit_cast(kv_h2, sm), s = {p[0], p[0]}, m = {p[1], p[1]};
-    return at_join(at_lo(w, s, m), at_hi(w, s, m), at_lo(w >> 8, s, m), at_hi(w >> 8, s, m));
+    return at_join(at_lo(g, w, s, m), at_hi(g, w, s, m), at_lo(g, w >> 8, s, m), at_hi(g, w >> 8, s, m));
 }
 
 __device__ __forceinline__ kv_f4 at_mfma(kv_h8 a, kv_h8 b, kv_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }

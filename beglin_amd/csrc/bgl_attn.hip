@@ -57,6 +57,9 @@ __device__ __forceinline__ void at_dwords(uint32_t (&w)[G], const uint8_t *p) {
     if constexpr (G % 2) w[G - 1] = *(const uint32_t *)(p + 4 * (G - 1));
 }
 
+// Where token r of four stands in an operand of weights: 0, 2, 1, 3 is the order of V's pairs.
+__device__ __forceinline__ constexpr int at_place(int r) { return (r & 1) * 2 + (r >> 1); }
+
 template <int G, int NT, int PARTS>
 struct AttnWave {
     static constexpr int D = 32 * G, RB = 16 * NT;
@@ -65,6 +68,7 @@ struct AttnWave {
     AttnSeq q;
     int head;
     ucint table;
+    const AtMagic magic;
     kv_h8 qf[NT][PARTS][G];
     float fac[NT], zero[NT];                             // zero: where scores begin; NaN for a query with a NaN or an infinity
     int lo[NT], hi[NT], lo_max, hi_min;
@@ -95,20 +99,20 @@ struct AttnWave {
             }
             top = __float_as_uint(at_max4(__uint_as_float(min(top, 0x7f800000u))));        // NaN counts as an infinity
             const bool bad = top >= 0x7f800000u;
-            const int ex = bad || top == 0 ? 14 : max((int)(top >> 23), 1) - 127;
-            const float turn = L.a.scale < 0.0f ? -1.0f : 1.0f;
+            const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
+            const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
 #pragma unroll
             for (int j = 0; j < G; j++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float y = bad ? 0.0f : ldexpf(x[j][e], 14 - ex) * turn;
-                    const _Float16 h = (_Float16)y;
-                    qf[t][0][j][e] = h;
-                    if constexpr (PARTS == 2) qf[t][1][j][e] = (_Float16)(y - (float)h);
+                for (int y = 0; y < 8; y++) {
+                    const float v = x[j][y] * up;
+                    const _Float16 h = (_Float16)v;
+                    qf[t][0][j][y] = h;
+                    if constexpr (PARTS == 2) qf[t][1][j][y] = (_Float16)(v - (float)h);
                 }
             }
             // (a factor of 0 would make NaN of masked scores)
-            fac[t] = fmaxf(ldexpf(L.scale2, ex - 14), 1e-30f);
+            fac[t] = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
             zero[t] = bad ? NAN : 0.0f;
             m[t] = -INFINITY;
             l[t] = 0.0f;
@@ -124,32 +128,34 @@ struct AttnWave {
         hi_min = __builtin_amdgcn_readfirstlane(hi_min);
     }
 
-    // The page of the tile at a key (a multiple of 16), or -1: past the keys, or no page.
-    __device__ __forceinline__ int page(int key) const {
-        if (key >= q.len) return -1;
-        const int t = key >> 4, pg = table[L.ppt_shift >= 0 ? t >> L.ppt_shift : t / L.ppt];
-        return pg >= 0 && pg < L.c.pages ? pg : -1;
+    // The page of a 16-token tile.
+    __device__ __forceinline__ int page_at(int t) const { return (int)(__umulhi((uint32_t)t, L.div_mul) + (uint32_t)t) >> L.div_shift; }
+    // The table's entry for the tile at a key (a multiple of 16); -1 past the keys.  It may name no page.
+    __device__ __forceinline__ int entry(int key) const { return key < q.len ? table[page_at(key >> 4)] : -1; }
+    // The record of the tile at a key, in the page of the table's entry; a tile without a page loads the first record, and none of
+    // it counts.
+    __device__ __forceinline__ const uint8_t *record(int key, int pg) const {
+        const int t = key >> 4;
+        const size_t rec = none(pg) ? 0 : ((size_t)pg * L.c.heads + head) * L.ppt + (t - page_at(t) * L.ppt);
+        return (const uint8_t *)L.c.data + rec * (20 * D);
     }
-    __device__ __forceinline__ void load(AttnRaw<G> &w, int key, const int (&pg)[2]) const {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int t = (key >> 4) + h, in = L.ppt_shift >= 0 ? t & (L.ppt - 1) : t % L.ppt;
-            // a tile without a page loads the first record, and none of it counts
-            const size_t rec = pg[h] < 0 ? 0 : ((size_t)pg[h] * L.c.heads + head) * L.ppt + in;
-            const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
-            at_dwords<G>(w.kc[h], p + lane * (4 * G));
-            at_dwords<G>(w.vc[h], p + 10 * D + lane * (4 * G));
-            const uint32_t *ks = (const uint32_t *)(p + 8 * D);
-            const at_u4 *vs = (const at_u4 *)(p + 18 * D);
-            w.ks[h][0] = ks[(G * b >> 2) * 16 + col];
-            w.vs[h][0] = vs[(G * col >> 4) * 4 + b];
-            if constexpr (AttnRaw<G>::K2) w.ks[h][1] = ks[((G * b + G - 1) >> 2) * 16 + col];
-            if constexpr (AttnRaw<G>::V2) w.vs[h][1] = vs[((G * col + G - 1) >> 4) * 4 + b];
-        }
+    __device__ __forceinline__ void load_k(AttnRaw<G> &w, int h, const uint8_t *p) const {
+        at_dwords<G>(w.kc[h], p + lane * (4 * G));
+        const uint32_t *ks = (const uint32_t *)(p + 8 * D);
+        w.ks[h][0] = ks[(G * b >> 2) * 16 + col];
+        if constexpr (AttnRaw<G>::K2) w.ks[h][1] = ks[((G * b + G - 1) >> 2) * 16 + col];
     }
+    __device__ __forceinline__ void load_v(AttnRaw<G> &w, int h, const uint8_t *p) const {
+        at_dwords<G>(w.vc[h], p + 10 * D + lane * (4 * G));
+        const at_u4 *vs = (const at_u4 *)(p + 18 * D);
+        w.vs[h][0] = vs[(G * col >> 4) * 4 + b];
+        if constexpr (AttnRaw<G>::V2) w.vs[h][1] = vs[((G * col + G - 1) >> 4) * 4 + b];
+    }
+    __device__ __forceinline__ bool none(int pg) const { return (uint32_t)pg >= (uint32_t)L.c.pages; }
 
-    // Keys key .. key + 31 into m, l and o.
-    __device__ __forceinline__ void step(AttnRaw<G> &w, int key, const int (&pg)[2]) {
+    // Keys key .. key + 31 into m, l and o.  next: the records of the wave's next 32 keys, or null; they are loaded into the registers
+    // that this step has used up.
+    __device__ __forceinline__ void step(AttnRaw<G> &w, int key, const int (&pg)[2], const uint8_t *const (&next)[2]) {
         constexpr bool K2 = AttnRaw<G>::K2, V2 = AttnRaw<G>::V2;
         kv_f4 s[NT][2];
 #pragma unroll
@@ -159,7 +165,7 @@ struct AttnWave {
 #pragma unroll
             for (int j = 0; j < G; j++) {
                 const uint32_t sm = K2 && (G * b + j) >> 2 != G * b >> 2 ? w.ks[h][K2] : w.ks[h][0];
-                const kv_h8 k = at_key(w.kc[h][j], sm);
+                const kv_h8 k = at_key(magic, w.kc[h][j], sm);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -167,11 +173,20 @@ struct AttnWave {
                 }
             }
         }
-        // Some of the keys may be hidden from some rows: at the last key, along the rows' diagonal, at the window's edge.
-        const bool some = pg[0] < 0 || pg[1] < 0 || key < lo_max || key + 31 > hi_min;
+        if (next[0]) {
+            load_k(w, 0, next[0]);
+            load_k(w, 1, next[1]);
+        }
+        // Some of the keys may be hidden from some rows: at the last key, along the rows' diagonal, at the window's edge.  (The empty
+        // asm keeps the compiler from doing this for every unit, with selects.)
+        uint32_t hidden[NT], bad[V2 ? 2 : 1];                                        // bit x: token x / 4 tile, as P has them
         bool poison = false;
-        kv_h8 bad[V2 ? 2 : 1], seen[NT];
-        if (some) {
+        if (none(pg[0]) || none(pg[1]) || key < lo_max || key + 31 > hi_min) {
+            asm volatile("");
+#pragma unroll
+            for (int t = 0; t < NT; t++) hidden[t] = 0;
+#pragma unroll
+            for (int x = 0; x < (V2 ? 2 : 1); x++) bad[x] = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int k0 = key + 16 * h + 4 * b;
@@ -179,36 +194,30 @@ struct AttnWave {
                 for (int r = 0; r < 4; r++) {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        const bool see = pg[h] >= 0 && k0 + r >= lo[t] && k0 + r <= hi[t];
-                        s[t][h][r] = see ? s[t][h][r] : -INFINITY;
-                        seen[t][4 * h + (r & 1) * 2 + (r >> 1)] = see ? (_Float16)1.0f : (_Float16)0.0f;
+                        const bool hide = none(pg[h]) || k0 + r < lo[t] || k0 + r > hi[t];
+                        s[t][h][r] = hide ? -INFINITY : s[t][h][r];
+                        hidden[t] |= hide ? 1u << (4 * h + at_place(r)) : 0u;
                     }
                 }
                 // Memory behind the last key holds anything: 0 there, which a weight of 0 leaves 0.
-                const int left = pg[h] < 0 ? 0 : q.len - k0;
+                const int left = none(pg[h]) ? 0 : q.len - k0;
                 const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
                 const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
 #pragma unroll
                 for (int x = 0; x < (V2 ? 2 : 1); x++) {
                     w.vs[h][x] &= at_u4{e, f, e, f};
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        const uint32_t v = w.vs[h][x][2 + (y >> 1)] >> (16 * (y & 1));
-                        const bool nan = (v & 0x7c00u) == 0x7c00u;
-                        bad[x][4 * h + y] = nan ? (_Float16)1.0f : (_Float16)0.0f;
-                        poison |= nan;
-                    }
+                    for (int y = 0; y < 4; y++)
+                        if ((w.vs[h][x][2 + (y >> 1)] >> (16 * (y & 1)) & 0x7c00u) == 0x7c00u) bad[x] |= 1u << (4 * h + y);
                 }
             }
-            poison = __any(poison);
+            poison = __any((bad[0] | bad[V2]) != 0);
             if (poison) {                                // NaN among them: it reaches the rows that see it, below
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int x = 0; x < (V2 ? 2 : 1); x++)
 #pragma unroll
-                    for (int x = 0; x < (V2 ? 2 : 1); x++)
-#pragma unroll
-                        for (int y = 0; y < 4; y++)
-                            if (bad[x][4 * h + y] != (_Float16)0.0f) w.vs[h][x][2 + (y >> 1)] &= y & 1 ? 0x0000ffffu : 0xffff0000u;
+                    for (int y = 0; y < 8; y++)
+                        if (bad[x] >> y & 1) w.vs[y >> 2][x][2 + (y >> 1 & 1)] &= y & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
         kv_h8 pf[NT][PARTS];
@@ -231,7 +240,7 @@ struct AttnWave {
                 const int h = x >> 2, r = x & 3;
                 const float p = at_exp2(fmaf(s[t][h][r], fac[t], off));
                 l[t] += p;
-                const int at = 4 * h + (r & 1) * 2 + (r >> 1);      // tokens 0, 2, 1, 3: the order of V's pairs
+                const int at = 4 * h + at_place(r);
                 pf[t][0][at] = (_Float16)p;
                 if constexpr (PARTS == 2) pf[t][1][at] = (_Float16)(p - (float)pf[t][0][at]);
             }
@@ -245,10 +254,10 @@ struct AttnWave {
                 const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
                 const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
                 const uint32_t c = w.vc[h][j], d = c >> 8;
-                v[0][2 * h] = at_lo(c, s0, m0);
-                v[0][2 * h + 1] = at_lo(d, s1, m1);
-                v[1][2 * h] = at_hi(c, s0, m0);
-                v[1][2 * h + 1] = at_hi(d, s1, m1);
+                v[0][2 * h] = at_lo(magic, c, s0, m0);
+                v[0][2 * h + 1] = at_lo(magic, d, s1, m1);
+                v[1][2 * h] = at_hi(magic, c, s0, m0);
+                v[1][2 * h + 1] = at_hi(magic, d, s1, m1);
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -260,13 +269,24 @@ struct AttnWave {
                 }
             }
         }
-        if (poison) {
+        if (next[0]) {
+            load_v(w, 0, next[0]);
+            load_v(w, 1, next[1]);
+        }
+        if (poison) {                                    // how many NaN a row sees, for each of its values
+            asm volatile("");
+            auto ones = [](uint32_t bits) {
+                kv_h8 v;
+#pragma unroll
+                for (int y = 0; y < 8; y++) v[y] = bits >> y & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+                return v;
+            };
 #pragma unroll
             for (int j = 0; j < G; j++) {
-                const kv_h8 a = V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0];
+                const kv_h8 a = ones(V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0]);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const kv_f4 n = at_mfma(a, seen[t], kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
+                    const kv_f4 n = at_mfma(a, ones(~hidden[t]), kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         if (n[i] > 0.0f) o[t][2 * j][i] = o[t][2 * j + 1][i] = NAN;
@@ -280,8 +300,6 @@ struct AttnWave {
 template <int G, int NT>
 struct AttnShared {
     static constexpr int D = 32 * G, RB = 16 * NT, ROW = D + 4;
-    uint32_t before[257];                                // units before thread i's sequences
-    uint32_t wave_sum[4];
     float m[4][RB], l[4][RB], M[RB], sum[RB];
     int last;
     union {
@@ -294,6 +312,16 @@ template <int RB>
 __device__ __forceinline__ void attn_units(const AttnLaunch &L, const AttnSeq &q, int &blocks, int &chunks) {
     blocks = q.n > 0 && (long)q.n * L.g <= L.limit ? (q.n * L.g + RB - 1) / RB : 0;
     chunks = max(1, (q.len - (q.lo & ~15) + AT_UNIT - 1) / AT_UNIT);
+}
+
+// Sums of lanes 0 .. l.
+__device__ __forceinline__ int at_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);                  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);                  // lane 15 of rows 0 and 2 to rows 1 and 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);            // lane 31 to rows 2 and 3
 }
 
 // The line of units in runs: the first `more` workgroups have one unit more than the others' `each`.
@@ -317,79 +345,80 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
     constexpr int D = 32 * G, RB = 16 * NT, PIECE = RB * (D + 2);
     __shared__ AttnShared<G, NT> sh;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), heads = L.c.heads, S = L.a.S;
-    const int per = (S + 255) / 256;
-    uint32_t mine = 0;
-    for (int s = tid * per; s < min(S, (tid + 1) * per); s++) {
+    // Every wave counts all units by itself, lane by lane, each lane `per` sequences.
+    const int per = (S + 63) / 64, lane = tid & 63;
+    AttnSeq mine_q;
+    mine_q.begin = mine_q.n = mine_q.len = mine_q.lo = 0;
+    int mine = 0;
+    for (int s = lane * per; s < min(S, (lane + 1) * per); s++) {
         int blocks, chunks;
-        attn_units<RB>(L, attn_seq(L, s), blocks, chunks);
-        mine += (uint32_t)(blocks * heads * chunks);
+        mine_q = attn_seq(L, s);
+        attn_units<RB>(L, mine_q, blocks, chunks);
+        mine += blocks * heads * chunks;
     }
-    uint32_t upto = mine;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const uint32_t v = __shfl_up(upto, x);
-        if ((tid & 63) >= x) upto += v;
-    }
-    if ((tid & 63) == 63) sh.wave_sum[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) upto += sh.wave_sum[w];
-    sh.before[tid] = upto - mine;
-    if (tid == 255) sh.before[256] = upto;
-    __syncthreads();
+    const int upto = at_scan(mine);                      // units before the next lane's sequences
     const __amdgpu_buffer_rsrc_t pieces = __builtin_amdgcn_make_buffer_rsrc(L.part, (short)0, AT_WG * 2 * PIECE * 4, 0x00020000);
-    const AttnRuns runs((uint32_t)__builtin_amdgcn_readfirstlane((int)sh.before[256]), gridDim.x);
+    const AttnRuns runs((uint32_t)__builtin_amdgcn_readlane(upto, 63), gridDim.x);
     const uint32_t w = blockIdx.x;
     if (w >= runs.wgs) return;
     const uint32_t end = runs.begin(w + 1);
     uint32_t u = runs.begin(w);
-    // the sequence of unit u: the last thread whose sequences begin at or before it, then that thread's sequences in turn
-    int th = 0;
-#pragma unroll
-    for (int x = 128; x; x >>= 1)
-        if (sh.before[th + x] <= u) th += x;
-    th = __builtin_amdgcn_readfirstlane(th);
-    int s = th * per;
-    uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.before[th]);       // units before sequence s
     Wave W(L);
     int blocks, chunks;
     while (u < end) {
-        while (true) {                                   // to the sequence of unit u
-            W.q = attn_seq(L, s);
-            W.q.begin = __builtin_amdgcn_readfirstlane(W.q.begin);
-            W.q.n = __builtin_amdgcn_readfirstlane(W.q.n);
-            W.q.len = __builtin_amdgcn_readfirstlane(W.q.len);
-            W.q.lo = __builtin_amdgcn_readfirstlane(W.q.lo);
-            attn_units<RB>(L, W.q, blocks, chunks);
-            const uint32_t n = (uint32_t)(blocks * heads * chunks);
-            if (u < base + n) break;
-            base += n;
-            s++;
+        // the sequence of unit u: the first lane whose sequences end behind it, then that lane's sequences in turn
+        const int at_lane = __popcll(__ballot((uint32_t)upto <= u));
+        uint32_t base = (uint32_t)__builtin_amdgcn_readlane(upto - mine, at_lane);     // units before sequence s
+        int s = at_lane * per;
+        W.q.begin = __builtin_amdgcn_readlane(mine_q.begin, at_lane);
+        W.q.n = __builtin_amdgcn_readlane(mine_q.n, at_lane);
+        W.q.len = __builtin_amdgcn_readlane(mine_q.len, at_lane);
+        W.q.lo = __builtin_amdgcn_readlane(mine_q.lo, at_lane);
+        attn_units<RB>(L, W.q, blocks, chunks);
+        if (per > 1) {
+            while (true) {
+                W.q = attn_seq(L, s);
+                W.q.begin = __builtin_amdgcn_readfirstlane(W.q.begin);
+                W.q.n = __builtin_amdgcn_readfirstlane(W.q.n);
+                W.q.len = __builtin_amdgcn_readfirstlane(W.q.len);
+                W.q.lo = __builtin_amdgcn_readfirstlane(W.q.lo);
+                attn_units<RB>(L, W.q, blocks, chunks);
+                const uint32_t n = (uint32_t)(blocks * heads * chunks);
+                if (u < base + n) break;
+                base += n;
+                s++;
+            }
         }
         const int item = (int)((u - base) / (uint32_t)chunks);                       // head * blocks + row block
         const int head = item / blocks, rb = item - head * blocks;
         const int c0 = (int)(u - base) - item * chunks, c1 = min(chunks, c0 + (int)(end - u));
         W.head = head;
         W.table = uni(L.a.table + (size_t)s * L.a.ldt);
-        AttnRaw<G> ra, rn;
-        int pa[2], pb[2];
+        AttnRaw<G> raw;
         int left = 0, key = (W.q.lo & ~15) + wave * 32 + c0 * AT_UNIT;                 // left: units in which the wave has keys
         if (key < W.q.len) left = min(c1 - c0, (W.q.len - key + AT_UNIT - 1) / AT_UNIT);
-        auto fetch = [&](AttnRaw<G> &r, int (&p)[2], int k) {
-            p[0] = W.page(k);
-            p[1] = W.page(k + 16);
-            W.load(r, k, p);
-        };
-        if (left) fetch(ra, pa, key);
+        int pg[2] = {W.entry(key), W.entry(key + 16)};
+        int pn[2] = {W.entry(key + AT_UNIT), W.entry(key + AT_UNIT + 16)};             // the table's entries, a unit ahead of its loads
+        if (left) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t *p = W.record(key + 16 * h, pg[h]);
+                W.load_k(raw, h, p);
+                W.load_v(raw, h, p);
+            }
+        }
         W.begin(rb);
-        while (left) {                                   // the next unit is on its way while one is worked on
-            if (left > 1) fetch(rn, pb, key + AT_UNIT);
-            W.step(ra, key, pa);
-            key += AT_UNIT;
-            if (--left == 0) break;
-            if (left > 1) fetch(ra, pa, key + AT_UNIT);
-            W.step(rn, key, pb);
-            key += AT_UNIT;
-            --left;
+#pragma clang loop unroll(disable)
+        for (; left; left--, key += AT_UNIT) {           // the next unit is on its way while one is worked on
+            const uint8_t *next[2] = {nullptr, nullptr};
+            if (left > 1) {
+                next[0] = W.record(key + AT_UNIT, pn[0]);
+                next[1] = W.record(key + AT_UNIT + 16, pn[1]);
+            }
+            const int p2[2] = {W.entry(key + 2 * AT_UNIT), W.entry(key + 2 * AT_UNIT + 16)};
+            W.step(raw, key, pg, next);
+#pragma unroll
+            for (int h = 0; h < 2; h++) { pg[h] = pn[h]; pn[h] = p2[h]; }
         }
         const int rows = min(RB, W.q.n * L.g - rb * RB);
         auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out, over the row's sum of weights
@@ -453,9 +482,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
             // Pieces wA .. wB are joined in groups of `size`, then the groups' sums: whoever comes last joins.
             const uint32_t n = wB - wA + 1;
             uint32_t size = n;
-            if (n > AT_JOIN / 2) {
-                size = (uint32_t)ceilf(sqrtf((float)n));                             // <= 28 of 768
-            }
+            if (n > AT_JOIN) size = (uint32_t)ceilf(sqrtf((float)n));                  // 28 of 768
             const uint32_t groups = (n + size - 1) / size;
             auto last = [&](int *count, uint32_t of) {   // whether the others have all written theirs
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                       // they are in memory
@@ -467,13 +494,24 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
                 __syncthreads();
                 return sh.last != 0;
             };
-            // pieces first, first + step, .. (count of them) into out, or into the first of them
+            // Pieces first, first + step, .. (count of them, AT_JOIN at most) into out, or into the first of them.  `split`
+            // neighbouring lanes share 4 values of a row, and load their pieces 16 at a time, the first before the factors are known.
             auto join = [&](uint32_t first, uint32_t step, int count, bool end_) {
+                const int n4 = rows * (D / 4), lg = n4 <= 32 ? 3 : n4 <= 64 ? 2 : n4 <= 128 ? 1 : 0, split = 1 << lg, sub = tid & (split - 1);
+                auto from = [&](int k) { return piece(first + k * step, wA); };
+                kv_f4 y[16];
+                auto load = [&](int x, int k0) {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const int at = k0 + k * split + sub;
+                        if (k0 + k * split < count) y[k] = get4(from(min(at, count - 1)) + min(x, n4 - 1) * 16);
+                    }
+                };
+                load(tid >> lg, 0);
                 for (int x = tid; x < count * rows; x += 256) {
                     const int k = x / rows, r = x - k * rows;
-                    const uint32_t at = piece(first + k * step, wA) + (RB * D + r) * 4;
-                    sh.j.m[k][r] = get(at);
-                    sh.j.l[k][r] = get(at + RB * 4);
+                    sh.j.m[k][r] = get(from(k) + (RB * D + r) * 4);
+                    sh.j.l[k][r] = get(from(k) + (RB * D + RB + r) * 4);
                 }
                 __syncthreads();
                 if (tid < rows) {
@@ -488,24 +526,27 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
                     sh.sum[tid] = sum;
                 }
                 __syncthreads();
-                for (int x = tid; x < rows * (D / 4); x += 256) {
+                for (int x = tid >> lg; x < n4; x += 256 >> lg) {
                     const int r = x / (D / 4), d = x % (D / 4) * 4;
                     kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int k0 = 0; k0 < count; k0 += 8) {                          // eight loads on their way at once
-                        kv_f4 y[8];
+                    for (int k0 = 0; k0 < count; k0 += 16 * split) {
+                        if (k0 > 0 || x != tid >> lg) load(x, k0);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) y[k] = get4(piece(first + min(k0 + k, count - 1) * step, wA) + (r * D + d) * 4);
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (k0 + k < count) v += y[k] * sh.j.m[k0 + k][r];
+                        for (int k = 0; k < 16; k++)
+                            if (k0 + k * split + sub < count) v += y[k] * sh.j.m[k0 + k * split + sub][r];
                     }
-                    if (end_) put(r, d, v);
-                    else set4(piece(first, wA) + (r * D + d) * 4, v);
+                    for (int i = 1; i < split; i <<= 1) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], i);
+                    }
+                    if (sub == 0) {
+                        if (end_) put(r, d, v);
+                        else set4(from(0) + x * 16, v);
+                    }
                 }
                 if (!end_ && tid < rows) {
-                    const uint32_t to = piece(first, wA) + (RB * D + tid) * 4;
-                    set(to, sh.M[tid]);
-                    set(to + RB * 4, sh.sum[tid]);
+                    set(from(0) + (RB * D + tid) * 4, sh.M[tid]);
+                    set(from(0) + (RB * D + RB + tid) * 4, sh.sum[tid]);
                 }
             };
             const uint32_t group = (w - wA) / size, at = wA + group * size;
@@ -522,7 +563,13 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
 // ================================================================================== host side
 template <int G, int NT, int PARTS>
 static void attn_go(bgl_ctx *c, const AttnLaunch &L, unsigned wgs) {
-    hipLaunchKernelGGL((k_attn<G, NT, PARTS>), dim3(wgs), dim3(256), 0, c->stream, L);
+    // no more workgroups than run at once: the runs are equal
+    static const unsigned at_once = [] {
+        int n = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn<G, NT, PARTS>, 256, 0) != hipSuccess) n = 2;
+        return (unsigned)std::max(1, n) * 256u;
+    }();
+    hipLaunchKernelGGL((k_attn<G, NT, PARTS>), dim3(std::min(wgs, at_once)), dim3(256), 0, c->stream, L);
 }
 template <int G>
 static void attn_pick(bgl_ctx *c, const AttnLaunch &L, int nt, unsigned wgs) {
@@ -568,7 +615,8 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.a = *a;
     L.g = a->nq / kv->heads;
     L.ppt = kv->page / KV_TILE;
-    L.ppt_shift = (L.ppt & (L.ppt - 1)) == 0 ? __builtin_ctz(L.ppt) : -1;
+    while ((1 << L.div_shift) < L.ppt) L.div_shift++;
+    L.div_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << L.div_shift) - (uint32_t)L.ppt)) / L.ppt + 1);
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
     const int rows = std::min(std::max(1, a->max_rows), a->T) * L.g, G = kv->D / 32;
