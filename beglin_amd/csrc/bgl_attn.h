@@ -17,8 +17,10 @@ struct AttnLaunch {
     int *sync;                   // for each workgroup that began a group of pieces, or an item: how many are written
 };
 
-// Weights are 2^14 exp(..): the largest is 2^14, so that fp16 keeps 11 bits of what is 2^28 times smaller.
-#define AT_P2 14.0f
+// Weights are 2^8 exp2(s - m), where m is a row's largest score so far or up to 7 below it: m moves, and what was summed with it,
+// only when a score passes it by more.  So weights stay below 2^15, and fp16 keeps 11 bits of all that are 2^-22 of the largest.
+#define AT_P2 8.0f
+#define AT_SLACK 7.0f
 
 // A sequence: its rows (begin, n), its keys, and the range [lo, len) that one of its rows may see.
 struct AttnSeq {
@@ -87,6 +89,84 @@ __device__ __forceinline__ float at_sum4(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Dwords i .. of G at any 4-byte place.
+template <int G>
+__device__ __forceinline__ void at_dwords(uint32_t (&w)[G], const uint8_t *p) {
+    typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef unsigned int u2 __attribute__((ext_vector_type(2), aligned(4)));
+#pragma unroll
+    for (int i = 0; i + 4 <= G; i += 4) {
+        const u4 v = *(const u4 *)(p + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[i + j] = v[j];
+    }
+    constexpr int at = G / 4 * 4;
+    if constexpr (G % 4 >= 2) {
+        const u2 v = *(const u2 *)(p + 4 * at);
+        w[at] = v[0];
+        w[at + 1] = v[1];
+    }
+    if constexpr (G % 2) w[G - 1] = *(const uint32_t *)(p + 4 * (G - 1));
+}
+
+// Where token r of four stands in an operand of weights: 0, 2, 1, 3 is the order of V's pairs.
+__device__ __forceinline__ constexpr int at_place(int r) { return (r & 1) * 2 + (r >> 1); }
+
+// The smallest of a value over the 16 lanes of a row, as a scalar.
+__device__ __forceinline__ int at_min16(int v) {
+    v = min(v, dpp_i<0xB1>(v));
+    v = min(v, dpp_i<0x4E>(v));
+    v = min(v, dpp_i<0x141>(v));
+    v = min(v, dpp_i<0x140>(v));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+// The page of the 16-token tile t of a sequence.
+__device__ __forceinline__ int at_page(const AttnLaunch &L, int t) { return (int)(__umulhi((uint32_t)t, L.div_mul) + (uint32_t)t) >> L.div_shift; }
+
+// A row of queries as operands: row r of the sequence's n * g (token r / g, head r % g of the group; past the last: the last), values 8 G b ..
+// for lane block b, scaled by a power of two that puts the row's largest value in [2^14, 2^15): exact in fp16 down to
+// 2^-28 of it (two parts for fp32 rows: 2^-22).  fac turns the products into scores of base 2, zero is where they begin (NaN for a
+// row with a NaN or an infinity), [lo, hi] are the keys that it sees.
+template <int G, int PARTS>
+__device__ __forceinline__ void at_query(const AttnLaunch &L, const AttnSeq &q, int head, int r, int b, kv_h8 (&qf)[PARTS][G], float &fac, float &zero,
+                                         int &lo, int &hi) {
+    const int rr = min(r, q.n * L.g - 1), i = rr / L.g;
+    const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
+    attn_keys(L, q, i, lo, hi);
+    float x[G][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+        kv_load8(x[j], L.a.q, L.a.type, at + 8 * j);
+#pragma unroll
+        for (int y = 0; y < 8; y++) top = max(top, __float_as_uint(x[j][y]) & 0x7fffffffu);
+    }
+    top = __float_as_uint(at_max4(__uint_as_float(min(top, 0x7f800000u))));                // NaN counts as an infinity
+    const bool bad = top >= 0x7f800000u;
+    const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
+    const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+#pragma unroll
+        for (int y = 0; y < 8; y++) {
+            const float v = x[j][y] * up;
+            const _Float16 h = (_Float16)v;
+            qf[0][j][y] = h;
+            if constexpr (PARTS == 2) qf[1][j][y] = (_Float16)(v - (float)h);
+        }
+    }
+    // (a factor of 0 would make NaN of masked scores)
+    fac = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
+    zero = bad ? NAN : 0.0f;
+}
+// fp16 ones where a bit of the eight is set
+__device__ __forceinline__ kv_h8 at_ones(uint32_t bits) {
+    kv_h8 v;
+#pragma unroll
+    for (int y = 0; y < 8; y++) v[y] = bits >> y & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+    return v;
+}
+
 // ------------------------------------------------------------------ a row's end
 // What the sum of values (weights 2^14 exp2(s - M)) is multiplied by: 1 / (their sum + the sink's weight); 0 for a row without a key.
 __device__ __forceinline__ float attn_factor(float M, float sum, bool sink, float sink2) {
@@ -97,3 +177,7 @@ __device__ __forceinline__ float attn_factor(float M, float sum, bool sink, floa
     return f / (sum * f + at_exp2(sink2 - top + AT_P2));
 }
 
+
+// The prompt kernel (bgl_attn_p.hip): the call's sequences with more than L.limit rows times g, L.limit < INT32_MAX; max_rows and
+// max_len as the caller gave them.
+int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L);

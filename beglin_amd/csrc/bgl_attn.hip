@@ -27,6 +27,7 @@
 
 #define AT_UNIT 128              // keys a unit
 #define AT_WG 768                // workgroups at most
+#define AT_FEW 32                // rows of a head's group that a sequence of few rows has, at most
 #define AT_SC1 16                // the cache-policy bit of a buffer access of device scope
 
 // What a wave has loaded of 32 keys: two tiles.
@@ -36,29 +37,6 @@ struct AttnRaw {
     uint32_t kc[2][G], vc[2][G], ks[2][K2 ? 2 : 1];
     at_u4 vs[2][V2 ? 2 : 1];
 };
-
-// Dwords i .. of G at any 4-byte place.
-template <int G>
-__device__ __forceinline__ void at_dwords(uint32_t (&w)[G], const uint8_t *p) {
-    typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
-    typedef unsigned int u2 __attribute__((ext_vector_type(2), aligned(4)));
-#pragma unroll
-    for (int i = 0; i + 4 <= G; i += 4) {
-        const u4 v = *(const u4 *)(p + 4 * i);
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[i + j] = v[j];
-    }
-    constexpr int at = G / 4 * 4;
-    if constexpr (G % 4 >= 2) {
-        const u2 v = *(const u2 *)(p + 4 * at);
-        w[at] = v[0];
-        w[at + 1] = v[1];
-    }
-    if constexpr (G % 2) w[G - 1] = *(const uint32_t *)(p + 4 * (G - 1));
-}
-
-// Where token r of four stands in an operand of weights: 0, 2, 1, 3 is the order of V's pairs.
-__device__ __forceinline__ constexpr int at_place(int r) { return (r & 1) * 2 + (r >> 1); }
 
 template <int G, int NT, int PARTS>
 struct AttnWave {
@@ -77,66 +55,31 @@ struct AttnWave {
 
     __device__ AttnWave(const AttnLaunch &l_) : L(l_), lane(threadIdx.x & 63), col(threadIdx.x & 15), b((threadIdx.x >> 4) & 3) {}
 
-    // Rows rb * RB .. of the sequence's n * g (row r: token r / g, head r % g of the group), scaled by a power of two that puts a
-    // row's largest value in [2^14, 2^15): exact in fp16 down to 2^-28 of it (two parts for fp32 rows, 2^-22).
+    // Rows rb * RB .. of the sequence's n * g.
     __device__ __forceinline__ void begin(int rb) {
         lo_max = 0;
         hi_min = INT32_MAX;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const int rows = q.n * L.g, r = rb * RB + 16 * t + col, rr = min(r, rows - 1), i = rr / L.g;
-            const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
-            attn_keys(L, q, i, lo[t], hi[t]);
+            at_query<G, PARTS>(L, q, head, rb * RB + 16 * t + col, b, qf[t], fac[t], zero[t], lo[t], hi[t]);
             lo_max = max(lo_max, lo[t]);
             hi_min = min(hi_min, hi[t]);
-            float x[G][8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < G; j++) {
-                kv_load8(x[j], L.a.q, L.a.type, at + 8 * j);
-#pragma unroll
-                for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[j][e]) & 0x7fffffffu);
-            }
-            top = __float_as_uint(at_max4(__uint_as_float(min(top, 0x7f800000u))));        // NaN counts as an infinity
-            const bool bad = top >= 0x7f800000u;
-            const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
-            const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
-#pragma unroll
-            for (int j = 0; j < G; j++) {
-#pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const float v = x[j][y] * up;
-                    const _Float16 h = (_Float16)v;
-                    qf[t][0][j][y] = h;
-                    if constexpr (PARTS == 2) qf[t][1][j][y] = (_Float16)(v - (float)h);
-                }
-            }
-            // (a factor of 0 would make NaN of masked scores)
-            fac[t] = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
-            zero[t] = bad ? NAN : 0.0f;
             m[t] = -INFINITY;
             l[t] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2 * G; j++) o[t][j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) {
-            lo_max = max(lo_max, __shfl_xor(lo_max, x));
-            hi_min = min(hi_min, __shfl_xor(hi_min, x));
-        }
-        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-        hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+        lo_max = -at_min16(-lo_max);
+        hi_min = at_min16(hi_min);
     }
 
-    // The page of a 16-token tile.
-    __device__ __forceinline__ int page_at(int t) const { return (int)(__umulhi((uint32_t)t, L.div_mul) + (uint32_t)t) >> L.div_shift; }
     // The table's entry for the tile at a key (a multiple of 16); -1 past the keys.  It may name no page.
-    __device__ __forceinline__ int entry(int key) const { return key < q.len ? table[page_at(key >> 4)] : -1; }
+    __device__ __forceinline__ int entry(int key) const { return key < q.len ? table[at_page(L, key >> 4)] : -1; }
     // The record of the tile at a key, in the page of the table's entry; a tile without a page loads the first record, and none of
     // it counts.
     __device__ __forceinline__ const uint8_t *record(int key, int pg) const {
         const int t = key >> 4;
-        const size_t rec = none(pg) ? 0 : ((size_t)pg * L.c.heads + head) * L.ppt + (t - page_at(t) * L.ppt);
+        const size_t rec = none(pg) ? 0 : ((size_t)pg * L.c.heads + head) * L.ppt + (t - at_page(L, t) * L.ppt);
         return (const uint8_t *)L.c.data + rec * (20 * D);
     }
     __device__ __forceinline__ void load_k(AttnRaw<G> &w, int h, const uint8_t *p) const {
@@ -226,9 +169,9 @@ struct AttnWave {
             float top = s[t][0][0];
 #pragma unroll
             for (int x = 1; x < 8; x++) top = fmaxf(top, s[t][x >> 2][x & 3]);
-            top = at_max4(top) * fac[t];
-            if (__any(top > m[t])) {
-                const float to = fmaxf(m[t], top), f = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
+            top *= fac[t];
+            if (__any(top > m[t] + AT_SLACK)) {
+                const float to = fmaxf(m[t], at_max4(top)), f = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
                 m[t] = to;
                 l[t] *= f;
 #pragma unroll
@@ -275,18 +218,12 @@ struct AttnWave {
         }
         if (poison) {                                    // how many NaN a row sees, for each of its values
             asm volatile("");
-            auto ones = [](uint32_t bits) {
-                kv_h8 v;
-#pragma unroll
-                for (int y = 0; y < 8; y++) v[y] = bits >> y & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-                return v;
-            };
 #pragma unroll
             for (int j = 0; j < G; j++) {
-                const kv_h8 a = ones(V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0]);
+                const kv_h8 a = at_ones(V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0]);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const kv_f4 n = at_mfma(a, ones(~hidden[t]), kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
+                    const kv_f4 n = at_mfma(a, at_ones(~hidden[t]), kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         if (n[i] > 0.0f) o[t][2 * j][i] = o[t][2 * j + 1][i] = NAN;
@@ -619,7 +556,20 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.div_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << L.div_shift) - (uint32_t)L.ppt)) / L.ppt + 1);
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
-    const int rows = std::min(std::max(1, a->max_rows), a->T) * L.g, G = kv->D / 32;
+    const int G = kv->D / 32;
+    int rows = (int)std::min<long>((long)std::min(std::max(1, a->max_rows), a->T) * L.g, INT32_MAX);
+    // Many rows of a head at once are the prompt kernel's, where they are told of; beside them sequences of few rows stay here.
+    const bool prompt = rows > AT_FEW;
+    if (prompt) {
+        L.limit = a->S > 1 ? AT_FEW : 0;
+        const int tok = prof_begin(c, 1);
+        const int rc = run_attn_prompt(c, L);
+        prof_end(c, tok);
+        if (rc) return rc;
+        HIPCHK(hipGetLastError());
+        if (a->S == 1) return 0;
+        rows = AT_FEW;
+    }
     const int nt = rows > 16 && G <= 4 ? 2 : 1, RB = 16 * nt;
     if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)2 * AT_WG * 32 * (128 + 2) * 4, false)) return rc;
     if (const int rc = dbuf_reserve(c, c->attn_sync, 3 * AT_WG * sizeof(int), true)) return rc;

@@ -4,7 +4,8 @@ How far a value may be off, from the kernel's roundings (all relative):
   scores   q is exact as an operand (two parts of it hold 2^-22 for fp32 rows), D products are summed in fp32, and the sum is scaled
            and shifted: A (2 D + 32) 2^-24 + A 2^-22 (fp32 rows), A the largest sum |q_i k_i| scale that the row sees; both the weight and the
            sum of weights follow it: twice that.  A merge of partial sums shifts by the maximum once more, which the 32 holds.
-  weights  fp16: 2^-11, two parts: 2^-22; exp2 itself 2^-22.  A weight below 2^-28 of the largest is off by at most 2^-39 of it.
+  weights  fp16: 2^-11, two parts: 2^-22; exp2 itself 2^-22.  A weight below 2^-22 of the largest is off by at
+           most 2^-33 of it (weights are 2^8 exp2(s - m) with m at most 7 below the largest score, and fp16 errs by 2^-25 below 2^-14).
   sums     32 products in a matrix instruction and L / 32 instructions and joins, each at most 2^-23.
   output   half a step of its type.
 All but the last multiply sum p |v|."""
@@ -140,7 +141,7 @@ class Batch:
                     A = np.maximum(A, abs(float(self.sink[h])))
                 ds = A * ((2 * D + 32) * 2.0 ** -24 + (2.0 ** -22 if parts else 0))
                 rel = (2.0 ** -22 if parts else 2.0 ** -11) + 2.0 ** -21 + 2 * ds + (32 + n / 32 + 800) * 2.0 ** -23
-                tol = rel[:, None] * weight + n * 2.0 ** -38 * np.abs(vv).max(initial=0)
+                tol = rel[:, None] * weight + n * 2.0 ** -33 * np.abs(vv).max(initial=0)
                 tol = tol * (1 + F.HALF[kind]) + F.HALF[kind] * np.abs(want) + F.LEAST[kind] + 1e-30
                 off = np.where(nan, 0, np.abs(out - want) - tol)[fine]
                 worst = off.max(initial=-1.0)
@@ -182,6 +183,53 @@ def test_few_rows(torch_dev, ctx, case):
     b.check(b.run(ctx, window=21, scale=-0.05, max_rows=1, max_len=1), window=21, scale=-0.05)
     b.out.fill_(7.0)
     b.check(b.run(ctx, window=200, sink=True, max_rows=1000, max_len=10 ** 6), window=200, sink=True)
+
+
+PROMPTS = [  # sequences (rows, keys), nq, nk, D, type, page, layout
+    ([(33, 33)], 1, 1, 64, "f32", 16, "dense"),
+    ([(300, 300)], 4, 1, 128, "bf16", 32, "part"),
+    ([(130, 700)], 6, 2, 128, "f32", 48, "heads"),
+    ([(64, 1000), (1, 500), (70, 70), (0, 40), (2, 300)], 8, 2, 64, "f16", 16, "odd"),
+    ([(40, 90), (257, 300)], 6, 6, 96, "f16", 32, "dense"),
+    ([(100, 130)], 2, 1, 96, "f32", 16, "odd"),
+    ([(77, 200), (5, 64), (129, 129)], 4, 2, 192, "bf16", 64, "part"),
+    ([(90, 90)], 3, 1, 192, "f32", 16, "dense"),
+    ([(50, 333), (1, 1)], 16, 2, 256, "bf16", 16, "dense"),
+    ([(60, 61)], 2, 2, 256, "f32", 48, "heads"),
+    ([(45, 12), (70, 65)], 2, 1, 128, "bf16", 16, "dense"),                        # more rows than keys
+    ([(40, 6000)], 1, 1, 128, "f16", 128, "dense"),                                # few rows, many keys: in parts
+    ([(200, 4000)], 4, 2, 64, "f32", 64, "dense"),
+]
+
+
+@pytest.mark.parametrize("case", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
+def test_many_rows(torch_dev, ctx, case):
+    seqs, nq, nk, D, kind, page, layout = case
+    b = Batch(torch_dev, ctx, seqs, nq, nk, D, kind, page, layout=layout)
+    most, longest = max(r for r, _ in seqs), max(n for _, n in seqs)
+    b.check(b.run(ctx))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, sink=True, causal=False, scale=0.3, max_rows=most, max_len=longest), causal=False, sink=True, scale=0.3)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=21, scale=-0.05, max_rows=33, max_len=1), window=21, scale=-0.05)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=100, sink=True, max_rows=40, max_len=10 ** 6), window=100, sink=True)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, max_rows=1, max_len=longest))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("window", [0, 30])
+def test_nan_and_pages_that_are_gone_among_many_rows(torch_dev, ctx, kind, D, window):
+    last = D - 1
+    poison = [(0, 95, 0, 3, "k"), (0, 80, 1, 40, "v"), (1, 60, 1, last, "v"), (1, 51, 0, 1, "v"), (2, 5, 0, last, "k"), (3, 2, 1, 2, "v"), (3, 17, 0, 33, "v")]
+    b = Batch(torch_dev, ctx, [(40, 97), (34, 63), (1, 6), (36, 36), (50, 50)], 4, 2, D, kind, 16, poison=poison, gone=[(0, 2), (4, 0), (4, 2), (1, 3)])
+    b.q[-4, 1, 5] = float("inf")
+    b.q[-3, 0, 0] = float("nan")
+    b.check(b.run(ctx, window=window), window=window)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=window, sink=True, max_rows=50, max_len=97), window=window, sink=True)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
@@ -230,11 +278,12 @@ def test_scores_far_apart(torch_dev, ctx):
 
 def test_same_bits_every_time(torch_dev, ctx):
     torch = torch_dev
-    b = Batch(torch, ctx, [(1, n) for n in (4000, 17, 900, 2500, 1, 333)], 8, 2, 128, "bf16", 64)
-    first = b.run(ctx).copy()
-    for _ in range(5):
-        b.out.fill_(3.0)
-        assert np.array_equal(b.run(ctx)[:b.T], first[:b.T])
+    for seqs in ([(1, n) for n in (4000, 17, 900, 2500, 1, 333)], [(40, 3000), (90, 200), (1, 50)]):
+        b = Batch(torch, ctx, seqs, 8, 2, 128, "bf16", 64)
+        first = b.run(ctx).copy()
+        for _ in range(5):
+            b.out.fill_(3.0)
+            assert np.array_equal(b.run(ctx)[:b.T], first[:b.T])
 
 
 def test_many_sequences(torch_dev, ctx):
