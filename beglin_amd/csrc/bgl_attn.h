@@ -159,12 +159,78 @@ __device__ __forceinline__ void at_query(const AttnLaunch &L, const AttnSeq &q, 
     fac = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
     zero = bad ? NAN : 0.0f;
 }
+// Keys e = 0, 1, .. behind a lane's first, of which a row sees those in [lo, hi]: the score, or -infinity.  (Integer operations on
+// vector registers: comparisons would hold a scalar mask for each key.)
+__device__ __forceinline__ int at_hides(int e, int lo, int hi) { return ((hi - e) | (e - lo)) >> 31; }
+__device__ __forceinline__ float at_hide(float s, int hides) {
+    return __uint_as_float((__float_as_uint(s) & ~(uint32_t)hides) | (0xff800000u & (uint32_t)hides));
+}
+// The same keys as a bit each, in the order of a weights' operand: those of two tiles that are seen.
+__device__ __forceinline__ uint32_t at_seen(int lo, int hi, int tile) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int x = 0; x < 8; x++) bits |= (uint32_t)(1 + at_hides(16 * (tile + (x >> 2)) + (x & 3), lo, hi)) << (4 * (x >> 2) + at_place(x & 3));
+    return bits;
+}
+// [lo, hi] of a row, counted from a lane's first key; difference of any two ints held to where at_hides is right
+__device__ __forceinline__ int at_from(int edge, int key) { return (int)min(max((long)edge - key, -(1l << 20)), 1l << 20); }
 // fp16 ones where a bit of the eight is set
 __device__ __forceinline__ kv_h8 at_ones(uint32_t bits) {
     kv_h8 v;
 #pragma unroll
     for (int y = 0; y < 8; y++) v[y] = bits >> y & 1 ? (_Float16)1.0f : (_Float16)0.0f;
     return v;
+}
+
+// ------------------------------------------------------------------ NaN among the values
+// A NaN times a weight of 0 is NaN: where rows of a product see different keys, V's NaN (a floor that is one) are multiplied as 0, and the
+// rows that see them get theirs once the sums are done, in one more pass over the floors.
+// Whether one of a lane's floors is NaN; it and its step's codes then count as 0.
+__device__ __forceinline__ bool at_clean(at_u4 &z) {
+    bool nan = false;
+#pragma unroll
+    for (int y = 2; y < 4; y++) {
+        const uint32_t lo = (z[y] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u, hi = (z[y] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+        nan |= (lo | hi) != 0;
+        z[y] &= ~(lo | hi);                              // (a NaN's step is 0)
+    }
+    return nan;
+}
+// Keys key .. key + 31: NaN into the sums of the rows that see one of V's.
+template <int G, int NT>
+__device__ __forceinline__ void at_nan(const AttnLaunch &L, const AttnSeq &q, int head, ucint table, int key, int lane, const int (&lo)[NT], const int (&hi)[NT],
+                                       kv_f4 (&o)[NT][2 * G]) {
+    const int col = lane & 15, b = lane >> 4;
+    uint32_t bits[2] = {0, 0};                           // of the lane's first and last group
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int t = (key >> 4) + h, pg = 16 * t < q.len ? table[at_page(L, t)] : -1;
+        if ((uint32_t)pg >= (uint32_t)L.c.pages) continue;
+        const uint8_t *p = (const uint8_t *)L.c.data + (((size_t)pg * L.c.heads + head) * L.ppt + (t - at_page(L, t) * L.ppt)) * (20 * 32 * G);
+        const at_u4 *vs = (const at_u4 *)(p + 18 * 32 * G);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const at_u4 z = vs[((G * col + (x ? G - 1 : 0)) >> 4) * 4 + b];
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+                if ((z[2 + (y >> 1)] >> (16 * (y & 1)) & 0x7c00u) == 0x7c00u && 16 * t + 4 * b + at_place(y) < q.len) bits[x] |= 1u << (4 * h + y);
+        }
+    }
+    if (!__any((bits[0] | bits[1]) != 0)) return;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const kv_h8 seen = at_ones(at_seen(at_from(lo[t], key + 4 * b), at_from(hi[t], key + 4 * b), 0));
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const kv_f4 n = at_mfma(at_ones((G * col + j) >> 4 != G * col >> 4 ? bits[1] : bits[0]), seen, kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const float add = n[y] > 0.0f ? NAN : 0.0f;
+                o[t][2 * j][y] += add;
+                o[t][2 * j + 1][y] += add;
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------ a row's end

@@ -52,6 +52,7 @@ struct AttnWave {
     int lo[NT], hi[NT], lo_max, hi_min;
     kv_f4 o[NT][2 * G];
     float m[NT], l[NT];
+    bool nan;                                            // V has had one, in a lane's keys
 
     __device__ AttnWave(const AttnLaunch &l_) : L(l_), lane(threadIdx.x & 63), col(threadIdx.x & 15), b((threadIdx.x >> 4) & 3) {}
 
@@ -59,6 +60,7 @@ struct AttnWave {
     __device__ __forceinline__ void begin(int rb) {
         lo_max = 0;
         hi_min = INT32_MAX;
+        nan = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             at_query<G, PARTS>(L, q, head, rb * RB + 16 * t + col, b, qf[t], fac[t], zero[t], lo[t], hi[t]);
@@ -122,25 +124,16 @@ struct AttnWave {
         }
         // Some of the keys may be hidden from some rows: at the last key, along the rows' diagonal, at the window's edge.  (The empty
         // asm keeps the compiler from doing this for every unit, with selects.)
-        uint32_t hidden[NT], bad[V2 ? 2 : 1];                                        // bit x: token x / 4 tile, as P has them
-        bool poison = false;
         if (none(pg[0]) || none(pg[1]) || key < lo_max || key + 31 > hi_min) {
             asm volatile("");
-#pragma unroll
-            for (int t = 0; t < NT; t++) hidden[t] = 0;
-#pragma unroll
-            for (int x = 0; x < (V2 ? 2 : 1); x++) bad[x] = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int k0 = key + 16 * h + 4 * b;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
+                for (int t = 0; t < NT; t++) {
+                    const int from = at_from(lo[t], k0), to = none(pg[h]) ? -1 : at_from(hi[t], k0);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const bool hide = none(pg[h]) || k0 + r < lo[t] || k0 + r > hi[t];
-                        s[t][h][r] = hide ? -INFINITY : s[t][h][r];
-                        hidden[t] |= hide ? 1u << (4 * h + at_place(r)) : 0u;
-                    }
+                    for (int r = 0; r < 4; r++) s[t][h][r] = at_hide(s[t][h][r], at_hides(r, from, to));
                 }
                 // Memory behind the last key holds anything: 0 there, which a weight of 0 leaves 0.
                 const int left = none(pg[h]) ? 0 : q.len - k0;
@@ -149,18 +142,8 @@ struct AttnWave {
 #pragma unroll
                 for (int x = 0; x < (V2 ? 2 : 1); x++) {
                     w.vs[h][x] &= at_u4{e, f, e, f};
-#pragma unroll
-                    for (int y = 0; y < 4; y++)
-                        if ((w.vs[h][x][2 + (y >> 1)] >> (16 * (y & 1)) & 0x7c00u) == 0x7c00u) bad[x] |= 1u << (4 * h + y);
+                    nan |= at_clean(w.vs[h][x]);
                 }
-            }
-            poison = __any((bad[0] | bad[V2]) != 0);
-            if (poison) {                                // NaN among them: it reaches the rows that see it, below
-#pragma unroll
-                for (int x = 0; x < (V2 ? 2 : 1); x++)
-#pragma unroll
-                    for (int y = 0; y < 8; y++)
-                        if (bad[x] >> y & 1) w.vs[y >> 2][x][2 + (y >> 1 & 1)] &= y & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
         kv_h8 pf[NT][PARTS];
@@ -215,20 +198,6 @@ struct AttnWave {
         if (next[0]) {
             load_v(w, 0, next[0]);
             load_v(w, 1, next[1]);
-        }
-        if (poison) {                                    // how many NaN a row sees, for each of its values
-            asm volatile("");
-#pragma unroll
-            for (int j = 0; j < G; j++) {
-                const kv_h8 a = at_ones(V2 && (G * col + j) >> 4 != G * col >> 4 ? bad[V2] : bad[0]);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const kv_f4 n = at_mfma(a, at_ones(~hidden[t]), kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (n[i] > 0.0f) o[t][2 * j][i] = o[t][2 * j + 1][i] = NAN;
-                }
-            }
         }
     }
 };
@@ -357,6 +326,8 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
 #pragma unroll
             for (int h = 0; h < 2; h++) { pg[h] = pn[h]; pn[h] = p2[h]; }
         }
+        if (__any(W.nan))
+            for (int k = (W.q.lo & ~15) + wave * 32 + c0 * AT_UNIT; k < key; k += AT_UNIT) at_nan<G, NT>(L, W.q, head, W.table, k, lane, W.lo, W.hi, W.o);
         const int rows = min(RB, W.q.n * L.g - rb * RB);
         auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out, over the row's sum of weights
             const int i = (rb * RB + r) / L.g, h = (rb * RB + r) - i * L.g;

@@ -45,20 +45,19 @@ struct PromptItem {
     }
 };
 
-template <int G, int WAVES, int NT, int PARTS>
+template <int G, int NT, int PARTS>
 struct Prompt {
-    static constexpr int D = 32 * G, RB = 16 * NT * WAVES, THREADS = 64 * WAVES, ST = 64;
+    static constexpr int D = 32 * G, WAVES = 8, RB = 16 * NT * WAVES, ST = 64;
     static constexpr bool K2 = G % 3 == 0 || G > 4, V2 = G % 3 == 0;                  // as in AttnRaw
     struct Shared {
         kv_h8 k[2][4][G][64], v[2][2][2 * G][64];
-        uint32_t flag[2][4];                             // a tile: 1 some value of V is NaN, 2 it has no page
-        uint32_t nan[2][4][G];                           // which of the 16 keys, for each group
+        at_u4 flag[2];                                   // a tile each: 1 some value of V is NaN, 2 it has no page
     };
 };
 
-template <int G, int WAVES, int NT, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(PromptLaunch P) {
-    using T = Prompt<G, WAVES, NT, PARTS>;
+template <int G, int NT, int PARTS>
+__global__ __launch_bounds__(512, 2) void k_attn_prompt(PromptLaunch P) {
+    using T = Prompt<G, NT, PARTS>;
     constexpr int D = T::D, RB = T::RB, ST = T::ST;
     constexpr bool K2 = T::K2, V2 = T::V2;
     const AttnLaunch &L = P.A;
@@ -73,107 +72,86 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, b = lane >> 4;
     const ucint table = uni(L.a.table + (size_t)it.s * L.a.ldt);
     const AtMagic magic;
-    auto none = [&](int pg) { return (uint32_t)pg >= (uint32_t)L.c.pages; };
-    auto entry = [&](int key) { return key < q.len ? table[at_page(L, key >> 4)] : -1; };
+    // In the loop over keys the table is read by vector loads: a scalar load on its way makes every wait for the LDS a wait for all of it.
+    const int *vtable = L.a.table + (size_t)it.s * L.a.ldt;
+    int zero_lane = 0;
+    asm volatile("" : "+v"(zero_lane));
+    const int last_page = at_page(L, max(0, q.len - 1) >> 4);
+    // A wave converts, of each stage's four tiles, K or V of one.
+    const int tile = wave >> 1;
+    const bool of_v = wave & 1;
+    const int codes_at = (of_v ? 10 * D : 0) + lane * (4 * G);
+    const int steps_at = of_v ? 18 * D + ((G * col >> 4) * 4 + b) * 16 : 8 * D + ((G * b >> 2) * 16 + col) * 4;
+    const int steps_at2 = of_v ? 18 * D + (((G * col + G - 1) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + G - 1) >> 2) * 16 + col) * 4;
     for (int block = it.block; block * RB < rows; block += P.blocks) {
         // the keys of the block's rows, this part's stages of 64 among them
         int lo_first, lo_last, hi_first, hi_last;
         attn_keys(L, q, block * RB / L.g, lo_first, hi_first);
-        attn_keys(L, q, min(block * RB + RB, rows) / L.g - (min(block * RB + RB, rows) % L.g == 0), lo_last, hi_last);
+        attn_keys(L, q, (min(block * RB + RB, rows) - 1) / L.g, lo_last, hi_last);
         const int key0 = lo_first & ~15, stages = max(0, (hi_last + 1 - key0 + ST - 1) / ST);
         const int parts = block < P.blocks ? P.parts : 1;          // blocks that max_rows did not tell of have no room for pieces
         if (it.part >= parts) break;
-        int st = __builtin_amdgcn_readfirstlane((int)((long)stages * it.part / parts));
+        const int st0 = __builtin_amdgcn_readfirstlane((int)((long)stages * it.part / parts));
         const int st1 = __builtin_amdgcn_readfirstlane((int)((long)stages * (it.part + 1) / parts));
 
-        // A wave's share of a stage's conversion: one of the four tiles, both of it (4 waves) or K or V of it (8).
-        const int tile = WAVES == 8 ? wave >> 1 : wave;
-        const bool do_k = WAVES == 4 || !(wave & 1), do_v = WAVES == 4 || (wave & 1);
-        uint32_t kc[G], ks[K2 ? 2 : 1], vc[G];
-        at_u4 vs[V2 ? 2 : 1];
         auto key_of = [&](int stage) { return key0 + stage * ST + 16 * tile; };
-        auto load = [&](int key, int pg) {
-            const int t = key >> 4;
-            const size_t rec = none(pg) ? 0 : ((size_t)pg * L.c.heads + it.head) * L.ppt + (t - at_page(L, t) * L.ppt);
-            const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
-            if (do_k) {
-                at_dwords<G>(kc, p + lane * (4 * G));
-                const uint32_t *s = (const uint32_t *)(p + 8 * D);
-                ks[0] = s[(G * b >> 2) * 16 + col];
-                if constexpr (K2) ks[1] = s[((G * b + G - 1) >> 2) * 16 + col];
-            }
-            if (do_v) {
-                at_dwords<G>(vc, p + 10 * D + lane * (4 * G));
-                const at_u4 *s = (const at_u4 *)(p + 18 * D);
-                vs[0] = s[(G * col >> 4) * 4 + b];
-                if constexpr (V2) vs[1] = s[((G * col + G - 1) >> 4) * 4 + b];
-            }
+        auto entry = [&](int stage) { return vtable[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
+        auto page = [&](int stage, int e) {              // the page, or -1: past the keys, or none
+            e = __builtin_amdgcn_readfirstlane(e);
+            return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
         };
-        auto convert = [&](int buf, int key, int pg) {
-            if (do_k) {
+        uint32_t codes[G];
+        typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
+        at_u4 steps, steps2;
+        // (a tile without a page loads the first record, and none of it counts)
+        auto load = [&](int stage, int pg) {
+            const int t = key_of(stage) >> 4;
+            const size_t rec = pg < 0 ? 0 : ((size_t)pg * L.c.heads + it.head) * L.ppt + (t - at_page(L, t) * L.ppt);
+            const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
+            at_dwords<G>(codes, p + codes_at);
+            steps = *(const u4 *)(p + steps_at);
+            if constexpr (K2 || V2) steps2 = *(const u4 *)(p + steps_at2);
+        };
+        auto convert = [&](int buf, int stage, int pg) {
+            if (!of_v) {
 #pragma unroll
-                for (int j = 0; j < G; j++) sh.k[buf][tile][j][lane] = at_key(magic, kc[j], K2 && (G * b + j) >> 2 != G * b >> 2 ? ks[K2] : ks[0]);
+                for (int j = 0; j < G; j++)
+                    sh.k[buf][tile][j][lane] = at_key(magic, codes[j], K2 && (G * b + j) >> 2 != G * b >> 2 ? steps2[0] : steps[0]);
+                return;
             }
-            if (do_v) {
-                uint32_t flag = none(pg) ? 2 : 0;
-                const int left = none(pg) ? 0 : q.len - key - 4 * b;                   // of the lane's four keys
-                if (none(pg) || key + 16 > q.len) {      // what lies behind the last key may be anything: 0
-                    asm volatile("");
-                    const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
-                    const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int x = 0; x < (V2 ? 2 : 1); x++) vs[x] &= at_u4{e, f, e, f};
-                }
-                bool nan = false;
-#pragma unroll
-                for (int x = 0; x < (V2 ? 2 : 1); x++)
-#pragma unroll
-                    for (int y = 2; y < 4; y++) nan |= (vs[x][y] & 0x7c00u) == 0x7c00u || (vs[x][y] & 0x7c000000u) == 0x7c000000u;
-                if (__any(nan)) {                        // they reach the rows that see them, in the products' end
-                    asm volatile("");
-                    flag |= 1;
-                    uint32_t bits[V2 ? 2 : 1];
-#pragma unroll
-                    for (int x = 0; x < (V2 ? 2 : 1); x++) {
-                        bits[x] = 0;
-#pragma unroll
-                        for (int y = 0; y < 4; y++)
-                            if ((vs[x][2 + (y >> 1)] >> (16 * (y & 1)) & 0x7c00u) == 0x7c00u) {
-                                bits[x] |= 1u << y;
-                                vs[x][2 + (y >> 1)] &= y & 1 ? 0x0000ffffu : 0xffff0000u;
-                            }
-                    }
-                    // bit 4 b + y of group g; every lane of (b, g) says the same
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        uint32_t mine = (G * col >> 4) == g ? bits[0] << (4 * b) : 0u;
-                        if constexpr (V2) mine |= ((G * col + G - 1) >> 4) == g ? bits[1] << (4 * b) : 0u;
-#pragma unroll
-                        for (int x = 1; x < 64; x <<= 1) mine |= (uint32_t)__shfl_xor((int)mine, x);
-                        if (lane == 0) sh.nan[buf][tile][g] = mine;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < G; j++) {
-                    const at_u4 z = V2 && (G * col + j) >> 4 != G * col >> 4 ? vs[V2] : vs[0];
-                    const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
-                    const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
-                    const uint32_t c = vc[j], d = c >> 8;
-                    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        u2 w;
-                        w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
-                        w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
-                        ((u2 *)&sh.v[buf][tile >> 1][2 * j + e][lane])[tile & 1] = w;
-                    }
-                }
-                if (lane == 0) sh.flag[buf][tile] = flag;
+            uint32_t flag = pg < 0 ? 2 : 0;
+            if (pg < 0 || key_of(stage) + 16 > q.len) {  // what lies behind the last key may be anything: 0
+                asm volatile("");
+                const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;           // of the lane's four keys
+                const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
+                const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+                steps &= at_u4{e, f, e, f};
+                if constexpr (V2) steps2 &= at_u4{e, f, e, f};
             }
+            bool nan = at_clean(steps);
+            if constexpr (V2) nan |= at_clean(steps2);
+            if (__any(nan)) flag |= 1;
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                const at_u4 z = V2 && (G * col + j) >> 4 != G * col >> 4 ? steps2 : steps;
+                const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
+                const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
+                const uint32_t c = codes[j], d = c >> 8;
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    u2 w;
+                    w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
+                    w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
+                    ((u2 *)&sh.v[buf][tile >> 1][2 * j + e][lane])[tile & 1] = w;
+                }
+            }
+            if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
         };
 
-        int pg = entry(key_of(st)), pn = entry(key_of(st + 1));
-        if (st < st1) load(key_of(st), pg);
+        int pg = page(st0, entry(st0));
+        load(st0, pg);
+        int next = entry(st0 + 1);
         // the wave's rows
         kv_h8 qf[NT][PARTS][G];
         float fac[NT], zero[NT], m[NT];
@@ -198,41 +176,42 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         hi_max = row0 < rows ? -at_min16(-hi_max) : -1;  // (a wave without rows has nothing to do)
         const kv_h8 ones = at_ones(0xff);
 
-        auto work = [&](int buf, int blk, int key) {     // keys key .. key + 31
-            const uint32_t f0 = sh.flag[buf][2 * blk], f1 = sh.flag[buf][2 * blk + 1];
-            const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(f0 | f1 << 2));
-            kv_f4 s[NT][2];
+        bool nan = false;                                // V has had one
+        // A stage's operands in runs of G, each read from the LDS while the run before it is multiplied: K of tiles 0 .. 3, then V of
+        // both halves, values 0 .. G - 1 and G .. 2 G - 1.
+        kv_h8 f[2][G];
+        auto read = [&](int buf, int run) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = kv_f4{zero[t], zero[t], zero[t], zero[t]};
+            for (int j = 0; j < G; j++) f[run & 1][j] = run < 4 ? sh.k[buf][run][j][lane] : sh.v[buf][(run - 4) >> 1][((run & 1) ? G : 0) + j][lane];
+        };
+        auto work = [&](int buf, int key) {
+            const at_u4 fl = sh.flag[buf];
+            kv_f4 s[NT][4];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 4; h++) {
+                read(buf, h + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < G; j++) {
-                    const kv_h8 k = sh.k[buf][2 * blk + h][j][lane];
+                for (int j = 0; j < G; j++)
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                    for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                        for (int p = 0; p < PARTS; p++) s[t][h] = at_mfma(k, qf[t][p][j], s[t][h]);
-                }
-            uint32_t hidden[NT];
-            if ((flags & 10) || key < lo_max || key + 31 > hi_min) {
+                        for (int t = 0; t < NT; t++)
+                            s[t][h] = at_mfma(f[h & 1][j], qf[t][p][j], j + p ? s[t][h] : kv_f4{zero[t], zero[t], zero[t], zero[t]});
+            }
+            const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
+            if ((flags & 0xaa) || key < lo_max || key + ST - 1 > hi_min) {
                 asm volatile("");
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    hidden[t] = 0;
+                    const int from = at_from(lo[t], key + 4 * b), to = at_from(hi[t], key + 4 * b);
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 4; h++) {
+                        const int last = flags >> (2 * h) & 2 ? -1 : to;               // no page
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int k = key + 16 * h + 4 * b + r;
-                            const bool hide = (flags >> (2 * h) & 2) || k < lo[t] || k > hi[t];
-                            s[t][h][r] = hide ? -INFINITY : s[t][h][r];
-                            hidden[t] |= hide ? 1u << (4 * h + at_place(r)) : 0u;
-                        }
+                        for (int r = 0; r < 4; r++) s[t][h][r] = at_hide(s[t][h][r], at_hides(16 * h + r, from, last));
+                    }
                 }
-            } else if (flags) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) hidden[t] = 0;
             }
             float top[NT];
             bool more = false;
@@ -240,88 +219,77 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
             for (int t = 0; t < NT; t++) {
                 top[t] = s[t][0][0];
 #pragma unroll
-                for (int x = 1; x < 8; x++) top[t] = fmaxf(top[t], s[t][x >> 2][x & 3]);
+                for (int x = 1; x < 16; x++) top[t] = fmaxf(top[t], s[t][x >> 2][x & 3]);
                 top[t] *= fac[t];
                 more |= top[t] > m[t] + AT_SLACK;
             }
             if (__any(more)) {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const float to = fmaxf(m[t], at_max4(top[t])), f = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
+                    const float to = fmaxf(m[t], at_max4(top[t])), g = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
                     m[t] = to;
-                    l[t] *= f;
+                    l[t] *= g;
 #pragma unroll
-                    for (int j = 0; j < 2 * G; j++) o[t][j] *= f;
+                    for (int j = 0; j < 2 * G; j++) o[t][j] *= g;
                 }
             }
-            kv_h8 pf[NT][PARTS];
+            kv_h8 pf[2][NT][PARTS];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const float off = AT_P2 - (m[t] == -INFINITY ? 0.0f : m[t]);
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const int h = x >> 2, r = x & 3, at = 4 * h + at_place(r);
+                for (int x = 0; x < 16; x++) {
+                    const int h = x >> 2, r = x & 3, at = 4 * (h & 1) + at_place(r);
                     const float p = at_exp2(fmaf(s[t][h][r], fac[t], off));
-                    pf[t][0][at] = (_Float16)p;
-                    if constexpr (PARTS == 2) pf[t][1][at] = (_Float16)(p - (float)pf[t][0][at]);
+                    pf[h >> 1][t][0][at] = (_Float16)p;
+                    if constexpr (PARTS == 2) pf[h >> 1][t][1][at] = (_Float16)(p - (float)pf[h >> 1][t][0][at]);
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 2 * G; j++) {
-                const kv_h8 a = sh.v[buf][blk][j][lane];
+            for (int run = 4; run < 8; run++) {
+                const int i = (run - 4) >> 1;
+                if (run < 7) read(buf, run + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int j = 0; j < G; j++)
 #pragma unroll
-                    for (int p = 0; p < PARTS; p++) o[t][j] = at_mfma(a, pf[t][p], o[t][j]);
-            }
+                    for (int p = 0; p < PARTS; p++)
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+                        for (int t = 0; t < NT; t++) o[t][(run & 1) * G + j] = at_mfma(f[run & 1][j], pf[i][t][p], o[t][(run & 1) * G + j]);
+                if (run & 1) {
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) l[t] = at_mfma(ones, pf[t][p], l[t]);
-            if (flags & 5) {                             // how many NaN a row sees, for each of its values
-                asm volatile("");
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int j = 0; j < 2 * G; j++) {
-                    const int g = (2 * G * col + j) >> 5;
-                    uint32_t bits = 0;
-                    if (flags & 1) bits |= sh.nan[buf][2 * blk][g] >> (4 * b) & 15;
-                    if (flags & 4) bits |= (sh.nan[buf][2 * blk + 1][g] >> (4 * b) & 15) << 4;
-                    const kv_h8 a = at_ones(bits);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const kv_f4 n = at_mfma(a, at_ones(~hidden[t]), kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (n[i] > 0.0f) o[t][j][i] = NAN;
-                    }
+                        for (int p = 0; p < PARTS; p++) l[t] = at_mfma(ones, pf[i][t][p], l[t]);
                 }
             }
+            if (flags & 0x55) nan = true;
         };
 
         __syncthreads();                                 // the block before this one has been read
-        int buf = 0;
-        if (st < st1) {
-            convert(0, key_of(st), pg);
-            pg = pn;
-            pn = entry(key_of(st + 2));
-            if (st + 1 < st1) load(key_of(st + 1), pg);
-        }
+        convert(0, st0, pg);                             // (without a stage: of a tile past the keys, or one that nothing reads)
+        int pn = page(st0 + 1, next);
+        load(st0 + 1, pn);
+        next = entry(st0 + 2);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        int buf = 0;
 #pragma clang loop unroll(disable)
-        for (; st < st1; st++, buf ^= 1) {
-            if (st + 1 < st1) {
-                convert(buf ^ 1, key_of(st + 1), pg);
-                pg = pn;
-                pn = entry(key_of(st + 3));
-                if (st + 2 < st1) load(key_of(st + 2), pg);
-            }
+        for (int st = st0; st < st1; st++, buf ^= 1) {
             const int key = key0 + st * ST;
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++)
-                if (key + 32 * blk <= hi_max && key + 32 * blk + 31 >= lo_min) work(buf, blk, key + 32 * blk);
+            const bool mine = key <= hi_max && key + ST - 1 >= lo_min;
+            if (mine) read(buf, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            convert(buf ^ 1, st + 1, pn);
+            pn = page(st + 2, next);
+            load(st + 2, pn);
+            next = entry(st + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            if (mine) work(buf, key);
             // LDS writes are done; loads that are on their way end in registers, which their uses wait for
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
+        if (nan)
+            for (int key = key0 + st0 * ST; key < key0 + st1 * ST; key += 32) at_nan<G, NT>(L, q, it.head, table, key, lane, lo, hi, o);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int r = row0 + 16 * t + col;
@@ -391,9 +359,9 @@ __global__ __launch_bounds__(256) void k_attn_join(PromptLaunch P) {
 }
 
 // ================================================================================== host side
-template <int G, int WAVES, int NT, int PARTS>
+template <int G, int NT, int PARTS>
 static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
-    constexpr int RB = 16 * NT * WAVES, D = 32 * G;
+    constexpr int RB = Prompt<G, NT, PARTS>::RB, D = 32 * G;
     PromptLaunch P;
     memset(&P, 0, sizeof P);
     P.A = L;
@@ -401,14 +369,14 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
     P.blocks = (int)((rows + RB - 1) / RB);
     const long items = (long)P.blocks * L.a.S * L.c.heads;
     // few blocks: their keys in parts, of 256 keys at least
-    const int at_once = WAVES == 8 ? 256 : 512;
+    const int at_once = 256;
     P.parts = (int)std::max<long>(1, std::min<long>({16, at_once / std::max(1l, items), ((long)std::max(1, L.a.max_len) + 255) / 256}));
     if (items * P.parts > INT32_MAX / 4) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d sequences of up to %d rows", L.a.S, L.a.max_rows);
     if (P.parts > 1) {
         if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)items * P.parts * RB * (D + 2) * 4, false)) return rc;
         P.A.part = (float *)c->attn_part.p;
     }
-    hipLaunchKernelGGL((k_attn_prompt<G, WAVES, NT, PARTS>), dim3((unsigned)(items * P.parts)), dim3(64 * WAVES), 0, c->stream, P);
+    hipLaunchKernelGGL((k_attn_prompt<G, NT, PARTS>), dim3((unsigned)(items * P.parts)), dim3(512), 0, c->stream, P);
     if (P.parts > 1) {
         constexpr int per = 256 / (D / 4);
         hipLaunchKernelGGL((k_attn_join<D, RB>), dim3((unsigned)items, (RB + per - 1) / per), dim3(256), 0, c->stream, P);
@@ -417,8 +385,8 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
 }
 template <int G>
 static int prompt_pick(bgl_ctx *c, const AttnLaunch &L) {
-    if (L.a.type == BGL_T_F32) return prompt_go<G, 8, G <= 4 ? 2 : 1, 2>(c, L);
-    return prompt_go<G, 8, G <= 6 ? 2 : 1, 1>(c, L);
+    if (L.a.type == BGL_T_F32) return prompt_go<G, G <= 4 ? 2 : 1, 2>(c, L);
+    return prompt_go<G, G <= 4 ? 2 : 1, 1>(c, L);
 }
 
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L) {
