@@ -120,41 +120,60 @@ __device__ __forceinline__ int at_min16(int v) {
     v = min(v, dpp_i<0x140>(v));
     return __builtin_amdgcn_readfirstlane(v);
 }
+// The same over the 32 lanes of either half.
+__device__ __forceinline__ int pr_min32(int v) {
+    v = min(v, dpp_i<0xB1>(v));
+    v = min(v, dpp_i<0x4E>(v));
+    v = min(v, dpp_i<0x141>(v));
+    v = min(v, dpp_i<0x140>(v));
+    return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+}
 // The page of the 16-token tile t of a sequence.
 __device__ __forceinline__ int at_page(const AttnLaunch &L, int t) { return (int)(__umulhi((uint32_t)t, L.div_mul) + (uint32_t)t) >> L.div_shift; }
 
-// A row of queries as operands: row r of the sequence's n * g (token r / g, head r % g of the group; past the last: the last), values 8 G b ..
-// for lane block b, scaled by a power of two that puts the row's largest value in [2^14, 2^15): exact in fp16 down to
-// 2^-28 of it (two parts for fp32 rows: 2^-22).  fac turns the products into scores of base 2, zero is where they begin (NaN for a
-// row with a NaN or an infinity), [lo, hi] are the keys that it sees.
-template <int G, int PARTS>
-__device__ __forceinline__ void at_query(const AttnLaunch &L, const AttnSeq &q, int head, int r, int b, kv_h8 (&qf)[PARTS][G], float &fac, float &zero,
-                                         int &lo, int &hi) {
+// A row of queries as operands: row r of the sequence's n * g (token r / g, head r % g of the group; past the last: the last), scaled by a power of
+// two that puts the row's largest value in [2^14, 2^15): exact in fp16 down to 2^-28 of it (two parts for fp32 rows:
+// 2^-22).  Values 8 G b .. + 8 G - 1 for a lane of block b of four (columns of 16), or with WIDE those of blocks b and 2 + b for a lane of half b
+// (columns of 32).  fac turns the products into scores of base 2, zero is where they begin (NaN for a row with a NaN or an
+// infinity), [lo, hi] are the keys that the row sees.
+template <int G, int PARTS, bool WIDE = false>
+__device__ __forceinline__ void at_query(const AttnLaunch &L, const AttnSeq &q, int head, int r, int b, kv_h8 (&qf)[WIDE ? 2 : 1][PARTS][G], float &fac,
+                                         float &zero, int &lo, int &hi) {
+    constexpr int N = WIDE ? 2 : 1;
     const int rr = min(r, q.n * L.g - 1), i = rr / L.g;
     const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
     attn_keys(L, q, i, lo, hi);
-    float x[G][8];
+    float x[N][G][8];
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < G; j++) {
-        kv_load8(x[j], L.a.q, L.a.type, at + 8 * j);
+    for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int y = 0; y < 8; y++) top = max(top, __float_as_uint(x[j][y]) & 0x7fffffffu);
+        for (int j = 0; j < G; j++) {
+            kv_load8(x[n][j], L.a.q, L.a.type, at + 16 * G * n + 8 * j);
+#pragma unroll
+            for (int y = 0; y < 8; y++) top = max(top, __float_as_uint(x[n][j][y]) & 0x7fffffffu);
+        }
+    top = min(top, 0x7f800000u);                                                       // NaN counts as an infinity
+    if constexpr (WIDE) {
+        auto a = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        top = max((uint32_t)a[0], (uint32_t)a[1]);
+    } else {
+        top = __float_as_uint(at_max4(__uint_as_float(top)));
     }
-    top = __float_as_uint(at_max4(__uint_as_float(min(top, 0x7f800000u))));                // NaN counts as an infinity
     const bool bad = top >= 0x7f800000u;
     const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
     const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
 #pragma unroll
-    for (int j = 0; j < G; j++) {
+    for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int y = 0; y < 8; y++) {
-            const float v = x[j][y] * up;
-            const _Float16 h = (_Float16)v;
-            qf[0][j][y] = h;
-            if constexpr (PARTS == 2) qf[1][j][y] = (_Float16)(v - (float)h);
-        }
-    }
+        for (int j = 0; j < G; j++)
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const float v = x[n][j][y] * up;
+                const _Float16 h = (_Float16)v;
+                qf[n][0][j][y] = h;
+                if constexpr (PARTS == 2) qf[n][1][j][y] = (_Float16)(v - (float)h);
+            }
     // (a factor of 0 would make NaN of masked scores)
     fac = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
     zero = bad ? NAN : 0.0f;

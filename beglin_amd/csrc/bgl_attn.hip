@@ -47,7 +47,7 @@ struct AttnWave {
     int head;
     ucint table;
     const AtMagic magic;
-    kv_h8 qf[NT][PARTS][G];
+    kv_h8 qf[NT][1][PARTS][G];
     float fac[NT], zero[NT];                             // zero: where scores begin; NaN for a query with a NaN or an infinity
     int lo[NT], hi[NT], lo_max, hi_min;
     kv_f4 o[NT][2 * G];
@@ -114,7 +114,7 @@ struct AttnWave {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
-                    for (int p = 0; p < PARTS; p++) s[t][h] = at_mfma(k, qf[t][p][j], s[t][h]);
+                    for (int p = 0; p < PARTS; p++) s[t][h] = at_mfma(k, qf[t][0][p][j], s[t][h]);
                 }
             }
         }

@@ -45,21 +45,63 @@ struct PromptItem {
     }
 };
 
-template <int G, int NT, int PARTS>
+// v_mfma_f32_32x32x16_f16: lane l has 8 values of the sum for row or column l % 32, those of its half h = l / 32; results i = 0 .. 15 are
+// rows 8 (i / 4) + 4 h + i % 4 of column l % 32.
+typedef float pr_f16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ pr_f16 pr_mfma(kv_h8 a, kv_h8 b, pr_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ pr_f16 pr_all(float v) { return pr_f16{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
+// the larger value, and the sum, of a lane and the other lane of its row (l ^ 32)
+__device__ __forceinline__ float pr_max2(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// WAVES 8: two a SIMD.  4: one, with all of its registers, for wide heads and two parts.
+template <int G, int WAVES, int PARTS>
 struct Prompt {
-    static constexpr int D = 32 * G, WAVES = 8, RB = 16 * NT * WAVES, ST = 64;
-    static constexpr bool K2 = G % 3 == 0 || G > 4, V2 = G % 3 == 0;                  // as in AttnRaw
+    static constexpr int D = 32 * G, RB = 32 * WAVES, ST = 64;
+    static constexpr int SN = G % 3 == 0 || G > 4 ? 2 : 1;         // groups of 32 that a lane's values lie in, at most
     struct Shared {
-        kv_h8 k[2][4][G][64], v[2][2][2 * G][64];
+        kv_h8 k[2][2][2 * G][64];                        // [buffer][32 keys][of the sum over values, 16 at a time]
+        kv_h8 v[2][4][G][64];                            // [buffer][16 keys, the sum][32 values]
         at_u4 flag[2];                                   // a tile each: 1 some value of V is NaN, 2 it has no page
     };
 };
 
-template <int G, int NT, int PARTS>
-__global__ __launch_bounds__(512, 2) void k_attn_prompt(PromptLaunch P) {
-    using T = Prompt<G, NT, PARTS>;
-    constexpr int D = T::D, RB = T::RB, ST = T::ST;
-    constexpr bool K2 = T::K2, V2 = T::V2;
+// at_nan for 32 rows: keys key .. key + 15.
+template <int G>
+__device__ __forceinline__ void pr_nan(const AttnLaunch &L, const AttnSeq &q, int head, ucint table, int key, int lane, int lo, int hi, pr_f16 (&o)[G]) {
+    const int n = lane & 15, h = lane >> 5, t = key >> 4, pg = key < q.len ? table[at_page(L, t)] : -1;
+    if ((uint32_t)pg >= (uint32_t)L.c.pages) return;
+    const uint8_t *p = (const uint8_t *)L.c.data + (((size_t)pg * L.c.heads + head) * L.ppt + (t - at_page(L, t) * L.ppt)) * (20 * 32 * G);
+    const at_u4 *vs = (const at_u4 *)(p + 18 * 32 * G);
+    uint32_t bits[2] = {0, 0};                           // of the lane's first and last group
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const at_u4 z = vs[((G * n + (x ? G - 1 : 0)) >> 4) * 4 + 2 * u + h];
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+                if ((z[2 + (y >> 1)] >> (16 * (y & 1)) & 0x7c00u) == 0x7c00u && key + 8 * u + 4 * h + at_place(y) < q.len) bits[x] |= 1u << (4 * u + y);
+        }
+    if (!__any((bits[0] | bits[1]) != 0)) return;
+    const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
+    uint32_t seen = 0;
+#pragma unroll
+    for (int x = 0; x < 8; x++) seen |= (uint32_t)(1 + at_hides(8 * (x >> 2) + (x & 3), from, to)) << (4 * (x >> 2) + at_place(x & 3));
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+        const pr_f16 c = pr_mfma(at_ones((G * n + j) >> 4 != G * n >> 4 ? bits[1] : bits[0]), at_ones(seen), pr_all(0.0f));
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[j][i] += c[i] > 0.0f ? NAN : 0.0f;
+    }
+}
+
+template <int G, int WAVES, int PARTS>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(PromptLaunch P) {
+    using T = Prompt<G, WAVES, PARTS>;
+    constexpr int D = T::D, RB = T::RB, ST = T::ST, SN = T::SN, JOBS = 8 / WAVES;
     const AttnLaunch &L = P.A;
     __shared__ typename T::Shared sh;
     const PromptItem it(P, blockIdx.x);
@@ -69,20 +111,21 @@ __global__ __launch_bounds__(512, 2) void k_attn_prompt(PromptLaunch P) {
     q.len = __builtin_amdgcn_readfirstlane(q.len);
     const int rows = q.n * L.g;
     if ((long)q.n * L.g <= L.limit) return;              // another kernel's
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, b = lane >> 4;
-    const ucint table = uni(L.a.table + (size_t)it.s * L.a.ldt);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, b = lane >> 4, h = lane >> 5;
     const AtMagic magic;
     // In the loop over keys the table is read by vector loads: a scalar load on its way makes every wait for the LDS a wait for all of it.
-    const int *vtable = L.a.table + (size_t)it.s * L.a.ldt;
+    const int *table = L.a.table + (size_t)it.s * L.a.ldt;
     int zero_lane = 0;
     asm volatile("" : "+v"(zero_lane));
     const int last_page = at_page(L, max(0, q.len - 1) >> 4);
-    // A wave converts, of each stage's four tiles, K or V of one.
-    const int tile = wave >> 1;
-    const bool of_v = wave & 1;
-    const int codes_at = (of_v ? 10 * D : 0) + lane * (4 * G);
-    const int steps_at = of_v ? 18 * D + ((G * col >> 4) * 4 + b) * 16 : 8 * D + ((G * b >> 2) * 16 + col) * 4;
-    const int steps_at2 = of_v ? 18 * D + (((G * col + G - 1) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + G - 1) >> 2) * 16 + col) * 4;
+    // A wave converts, of each stage's four tiles, K or V of one (8 waves), or both.
+    const int tile = WAVES == 8 ? wave >> 1 : wave;
+    auto of_v = [&](int job) { return WAVES == 8 ? (wave & 1) != 0 : job != 0; };
+    auto codes_at = [&](int job) { return (of_v(job) ? 10 * D : 0) + lane * (4 * G); };
+    auto steps_at = [&](int job, int x) {                // of the lane's first or last group
+        return of_v(job) ? 18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4;
+    };
     for (int block = it.block; block * RB < rows; block += P.blocks) {
         // the keys of the block's rows, this part's stages of 64 among them
         int lo_first, lo_last, hi_first, hi_last;
@@ -95,174 +138,173 @@ __global__ __launch_bounds__(512, 2) void k_attn_prompt(PromptLaunch P) {
         const int st1 = __builtin_amdgcn_readfirstlane((int)((long)stages * (it.part + 1) / parts));
 
         auto key_of = [&](int stage) { return key0 + stage * ST + 16 * tile; };
-        auto entry = [&](int stage) { return vtable[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
+        auto entry = [&](int stage) { return table[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
         auto page = [&](int stage, int e) {              // the page, or -1: past the keys, or none
             e = __builtin_amdgcn_readfirstlane(e);
             return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
         };
-        uint32_t codes[G];
+        uint32_t codes[JOBS][G];
         typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
-        at_u4 steps, steps2;
+        at_u4 steps[JOBS][SN];
         // (a tile without a page loads the first record, and none of it counts)
         auto load = [&](int stage, int pg) {
             const int t = key_of(stage) >> 4;
             const size_t rec = pg < 0 ? 0 : ((size_t)pg * L.c.heads + it.head) * L.ppt + (t - at_page(L, t) * L.ppt);
             const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
-            at_dwords<G>(codes, p + codes_at);
-            steps = *(const u4 *)(p + steps_at);
-            if constexpr (K2 || V2) steps2 = *(const u4 *)(p + steps_at2);
+#pragma unroll
+            for (int job = 0; job < JOBS; job++) {
+                at_dwords<G>(codes[job], p + codes_at(job));
+#pragma unroll
+                for (int x = 0; x < SN; x++) steps[job][x] = *(const u4 *)(p + steps_at(job, x));
+            }
         };
         auto convert = [&](int buf, int stage, int pg) {
-            if (!of_v) {
 #pragma unroll
-                for (int j = 0; j < G; j++)
-                    sh.k[buf][tile][j][lane] = at_key(magic, codes[j], K2 && (G * b + j) >> 2 != G * b >> 2 ? steps2[0] : steps[0]);
-                return;
-            }
-            uint32_t flag = pg < 0 ? 2 : 0;
-            if (pg < 0 || key_of(stage) + 16 > q.len) {  // what lies behind the last key may be anything: 0
-                asm volatile("");
-                const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;           // of the lane's four keys
-                const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
-                const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
-                steps &= at_u4{e, f, e, f};
-                if constexpr (V2) steps2 &= at_u4{e, f, e, f};
-            }
-            bool nan = at_clean(steps);
-            if constexpr (V2) nan |= at_clean(steps2);
-            if (__any(nan)) flag |= 1;
+            for (int job = 0; job < JOBS; job++) {
+                if (!of_v(job)) {
 #pragma unroll
-            for (int j = 0; j < G; j++) {
-                const at_u4 z = V2 && (G * col + j) >> 4 != G * col >> 4 ? steps2 : steps;
-                const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
-                const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
-                const uint32_t c = codes[j], d = c >> 8;
-                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    u2 w;
-                    w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
-                    w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
-                    ((u2 *)&sh.v[buf][tile >> 1][2 * j + e][lane])[tile & 1] = w;
+                    for (int j = 0; j < G; j++)
+                        sh.k[buf][tile >> 1][(b >> 1) * G + j][(b & 1) * 32 + (tile & 1) * 16 + col] =
+                            at_key(magic, codes[job][j], SN == 2 && (G * b + j) >> 2 != G * b >> 2 ? steps[job][SN - 1][0] : steps[job][0][0]);
+                    continue;
                 }
+                uint32_t flag = pg < 0 ? 2 : 0;
+                if (pg < 0 || key_of(stage) + 16 > q.len) {          // what lies behind the last key may be anything: 0
+                    asm volatile("");
+                    const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;       // of the lane's four keys
+                    const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
+                    const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int x = 0; x < SN; x++) steps[job][x] &= at_u4{e, f, e, f};
+                }
+                // a floor whose exponent is all ones carries into its sign
+                uint32_t ones = 0;
+#pragma unroll
+                for (int x = 0; x < SN; x++)
+#pragma unroll
+                    for (int y = 2; y < 4; y++) ones |= (steps[job][x][y] & 0x7c007c00u) + 0x04000400u;
+                if (__any((ones & 0x80008000u) != 0)) {
+                    asm volatile("");
+                    flag |= 1;
+#pragma unroll
+                    for (int x = 0; x < SN; x++) (void)at_clean(steps[job][x]);
+                }
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    const at_u4 z = SN == 2 && G % 3 == 0 && (G * col + j) >> 4 != G * col >> 4 ? steps[job][SN - 1] : steps[job][0];
+                    const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
+                    const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
+                    const uint32_t c = codes[job][j], d = c >> 8;
+                    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        u2 w;
+                        w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
+                        w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
+                        ((u2 *)&sh.v[buf][tile][j][(b & 1) * 32 + 16 * e + col])[b >> 1] = w;
+                    }
+                }
+                if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
             }
-            if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
         };
 
         int pg = page(st0, entry(st0));
         load(st0, pg);
         int next = entry(st0 + 1);
-        // the wave's rows
-        kv_h8 qf[NT][PARTS][G];
-        float fac[NT], zero[NT], m[NT];
-        int lo[NT], hi[NT], lo_max = 0, lo_min = INT32_MAX, hi_min = INT32_MAX, hi_max = -1;
-        kv_f4 o[NT][2 * G], l[NT];
-        const int row0 = block * RB + wave * 16 * NT;
+        // the wave's rows, one a lane (and l ^ 32)
+        const int row0 = block * RB + wave * 32;
+        kv_h8 qf[PARTS][2 * G];
+        float fac, zero, m = -INFINITY;
+        int lo, hi;
+        {
+            kv_h8 part[2][PARTS][G];                     // of the lane's values 8 G (2 x + h) ..
+            at_query<G, PARTS, true>(L, q, it.head, row0 + (lane & 31), h, part, fac, zero, lo, hi);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            at_query<G, PARTS>(L, q, it.head, row0 + 16 * t + col, b, qf[t], fac[t], zero[t], lo[t], hi[t]);
-            lo_max = max(lo_max, lo[t]);
-            lo_min = min(lo_min, lo[t]);
-            hi_min = min(hi_min, hi[t]);
-            hi_max = max(hi_max, hi[t]);
-            m[t] = -INFINITY;
-            l[t] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int j = 0; j < 2 * G; j++) o[t][j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                    for (int j = 0; j < G; j++) qf[p][x * G + j] = part[x][p][j];
         }
-        lo_max = -at_min16(-lo_max);
-        lo_min = at_min16(lo_min);
-        hi_min = at_min16(hi_min);
-        hi_max = row0 < rows ? -at_min16(-hi_max) : -1;  // (a wave without rows has nothing to do)
+        pr_f16 o[G], l = pr_all(0.0f);
+#pragma unroll
+        for (int j = 0; j < G; j++) o[j] = pr_all(0.0f);
+        const int lo_max = -pr_min32(-lo), lo_min = pr_min32(lo), hi_min = pr_min32(hi);
+        const int hi_max = row0 < rows ? -pr_min32(-hi) : -1;      // (a wave without rows has nothing to do)
         const kv_h8 ones = at_ones(0xff);
 
         bool nan = false;                                // V has had one
-        // A stage's operands in runs of G, each read from the LDS while the run before it is multiplied: K of tiles 0 .. 3, then V of
-        // both halves, values 0 .. G - 1 and G .. 2 G - 1.
-        kv_h8 f[2][G];
+        // A stage's operands in runs of four, each read from the LDS while the run before it is multiplied: K of both 32 keys side by side
+        // (two sums that do not wait for each other), then V.
+        kv_h8 f[2][4];
         auto read = [&](int buf, int run) {
 #pragma unroll
-            for (int j = 0; j < G; j++) f[run & 1][j] = run < 4 ? sh.k[buf][run][j][lane] : sh.v[buf][(run - 4) >> 1][((run & 1) ? G : 0) + j][lane];
+            for (int x = 0; x < 4; x++) {
+                if (run < G) f[run & 1][x] = sh.k[buf][x & 1][2 * run + (x >> 1)][lane];
+                else f[run & 1][x] = sh.v[buf][(4 * (run - G) + x) / G][(4 * (run - G) + x) % G][lane];
+            }
         };
         auto work = [&](int buf, int key) {
             const at_u4 fl = sh.flag[buf];
-            kv_f4 s[NT][4];
+            pr_f16 s[2];
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
-                read(buf, h + 1);
+            for (int run = 0; run < G; run++) {
+                read(buf, run + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < G; j++)
+                for (int x = 0; x < 4; x++)
 #pragma unroll
                     for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-                            s[t][h] = at_mfma(f[h & 1][j], qf[t][p][j], j + p ? s[t][h] : kv_f4{zero[t], zero[t], zero[t], zero[t]});
+                        s[x & 1] = pr_mfma(f[run & 1][x], qf[p][2 * run + (x >> 1)], run + p + (x >> 1) ? s[x & 1] : pr_all(zero));
             }
             const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
             if ((flags & 0xaa) || key < lo_max || key + ST - 1 > hi_min) {
                 asm volatile("");
+                const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const int from = at_from(lo[t], key + 4 * b), to = at_from(hi[t], key + 4 * b);
+                for (int t = 0; t < 4; t++) {
+                    const int last = flags >> (2 * t) & 2 ? -1 : to;                   // no page
 #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        const int last = flags >> (2 * h) & 2 ? -1 : to;               // no page
-#pragma unroll
-                        for (int r = 0; r < 4; r++) s[t][h][r] = at_hide(s[t][h][r], at_hides(16 * h + r, from, last));
-                    }
+                    for (int i = 0; i < 8; i++)
+                        s[t >> 1][8 * (t & 1) + i] = at_hide(s[t >> 1][8 * (t & 1) + i], at_hides(16 * t + 8 * (i >> 2) + (i & 3), from, last));
                 }
             }
-            float top[NT];
-            bool more = false;
+            float top = s[0][0];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                top[t] = s[t][0][0];
+            for (int x = 1; x < 32; x++) top = fmaxf(top, s[x >> 4][x & 15]);
+            top *= fac;
+            if (__any(top > m + AT_SLACK)) {
+                const float to = fmaxf(m, pr_max2(top)), g = to == -INFINITY ? 1.0f : at_exp2(m - to);
+                m = to;
+                l *= g;
 #pragma unroll
-                for (int x = 1; x < 16; x++) top[t] = fmaxf(top[t], s[t][x >> 2][x & 3]);
-                top[t] *= fac[t];
-                more |= top[t] > m[t] + AT_SLACK;
+                for (int j = 0; j < G; j++) o[j] *= g;
             }
-            if (__any(more)) {
+            kv_h8 pf[4][PARTS];
+            const float off = AT_P2 - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const float to = fmaxf(m[t], at_max4(top[t])), g = to == -INFINITY ? 1.0f : at_exp2(m[t] - to);
-                    m[t] = to;
-                    l[t] *= g;
-#pragma unroll
-                    for (int j = 0; j < 2 * G; j++) o[t][j] *= g;
-                }
-            }
-            kv_h8 pf[2][NT][PARTS];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float off = AT_P2 - (m[t] == -INFINITY ? 0.0f : m[t]);
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const int h = x >> 2, r = x & 3, at = 4 * (h & 1) + at_place(r);
-                    const float p = at_exp2(fmaf(s[t][h][r], fac[t], off));
-                    pf[h >> 1][t][0][at] = (_Float16)p;
-                    if constexpr (PARTS == 2) pf[h >> 1][t][1][at] = (_Float16)(p - (float)pf[h >> 1][t][0][at]);
-                }
+            for (int x = 0; x < 32; x++) {
+                const int at = 4 * (x >> 2 & 1) + at_place(x & 3);
+                const float p = at_exp2(fmaf(s[x >> 4][x & 15], fac, off));
+                pf[x >> 3][0][at] = (_Float16)p;
+                if constexpr (PARTS == 2) pf[x >> 3][1][at] = (_Float16)(p - (float)pf[x >> 3][0][at]);
             }
 #pragma unroll
-            for (int run = 4; run < 8; run++) {
-                const int i = (run - 4) >> 1;
-                if (run < 7) read(buf, run + 1);
+            for (int run = G; run < 2 * G; run++) {
+                if (run + 1 < 2 * G) read(buf, run + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < G; j++)
+                for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                    for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                        for (int t = 0; t < NT; t++) o[t][(run & 1) * G + j] = at_mfma(f[run & 1][j], pf[i][t][p], o[t][(run & 1) * G + j]);
-                if (run & 1) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++) l[t] = at_mfma(ones, pf[i][t][p], l[t]);
-                }
+                    for (int x = 0; x < 4; x++) {
+                        const int c = (4 * (run - G) + x) / G, j = (4 * (run - G) + x) % G;
+                        o[j] = pr_mfma(f[run & 1][x], pf[c][p], o[j]);
+                    }
             }
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) l = pr_mfma(ones, pf[c][p], l);
             if (flags & 0x55) nan = true;
         };
 
@@ -289,48 +331,55 @@ __global__ __launch_bounds__(512, 2) void k_attn_prompt(PromptLaunch P) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         if (nan)
-            for (int key = key0 + st0 * ST; key < key0 + st1 * ST; key += 32) at_nan<G, NT>(L, q, it.head, table, key, lane, lo, hi, o);
+            for (int key = key0 + st0 * ST; key < key0 + st1 * ST; key += 16)
+                pr_nan<G>(L, q, it.head, uni(L.a.table + (size_t)it.s * L.a.ldt), key, lane, lo, hi, o);
+        const int r = row0 + (lane & 31);
+        if (r >= rows) continue;
+        const int i = r / L.g, head = it.head * L.g + r - i * L.g;
+        const float sum = l[0];
+        // unit n = 8 x + 4 h + y holds values 2 G n .. : value 2 j + e is result 8 e + 4 x + y of o[j]
+        if (parts > 1) {
+            float *const to = prompt_piece<D, RB>(P, it.item, it.part);
+            const int rr = r - block * RB;
+            if (h == 0) { to[RB * D + rr] = m; to[RB * D + RB + rr] = sum; }
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int r = row0 + 16 * t + col;
-            if (r >= rows) continue;
-            const int i = r / L.g, h = it.head * L.g + r - i * L.g;
-            const float sum = l[t][0];
-            if (parts > 1) {
-                float *const to = prompt_piece<D, RB>(P, it.item, it.part);
-                const int rr = r - block * RB;
-                if (b == 0) { to[RB * D + rr] = m[t]; to[RB * D + RB + rr] = sum; }
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+                for (int y = 0; y < 4; y++)
 #pragma unroll
-                    for (int j = 0; j < 2 * G; j += 2) {
+                    for (int j = 0; j < G; j++) {
                         typedef float f2 __attribute__((ext_vector_type(2)));
-                        *(f2 *)(to + rr * D + 2 * G * (4 * b + x) + j) = f2{o[t][j][x], o[t][j + 1][x]};
+                        *(f2 *)(to + rr * D + 2 * G * (8 * x + 4 * h + y) + 2 * j) = f2{o[j][4 * x + y], o[j][8 + 4 * x + y]};
                     }
-                continue;
-            }
-            const float f = attn_factor(m[t], sum, L.a.sink != nullptr, L.a.sink ? L.a.sink[h] * 1.44269504088896340736f : 0.0f);
-            const long at = (long)(q.begin + i) * L.a.ldo + (long)h * L.a.hdo;
+            continue;
+        }
+        const float f1 = attn_factor(m, sum, L.a.sink != nullptr, L.a.sink ? L.a.sink[head] * 1.44269504088896340736f : 0.0f);
+        const long at = (long)(q.begin + i) * L.a.ldo + (long)head * L.a.hdo;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const long d = at + 2 * G * (4 * b + x);
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const long d = at + 2 * G * (8 * x + 4 * h + y);
                 if constexpr (G % 4 == 0) {
 #pragma unroll
-                    for (int j = 0; j < 2 * G; j += 8) {
-                        float y[8];
+                    for (int j = 0; j < G; j += 4) {
+                        float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) y[e] = o[t][j + e][x] * f;
-                        kv_store8(L.a.out, L.a.type, d + j, y);
+                        for (int e = 0; e < 8; e++) v[e] = o[j + (e >> 1)][8 * (e & 1) + 4 * x + y] * f1;
+                        kv_store8(L.a.out, L.a.type, d + 2 * j, v);
                     }
                 } else if constexpr (G % 2 == 0) {
 #pragma unroll
-                    for (int j = 0; j < 2 * G; j += 4) kv_store4(L.a.out, L.a.type, d + j, kv_f4{o[t][j][x], o[t][j + 1][x], o[t][j + 2][x], o[t][j + 3][x]} * f);
+                    for (int j = 0; j < G; j += 2)
+                        kv_store4(L.a.out, L.a.type, d + 2 * j, kv_f4{o[j][4 * x + y], o[j][8 + 4 * x + y], o[j + 1][4 * x + y], o[j + 1][8 + 4 * x + y]} * f1);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 2 * G; j++) i8_st(L.a.out, L.a.type, (size_t)(d + j), o[t][j][x] * f);
+                    for (int j = 0; j < G; j++) {
+                        i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j), o[j][4 * x + y] * f1);
+                        i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j + 1), o[j][8 + 4 * x + y] * f1);
+                    }
                 }
             }
-        }
     }
 }
 
@@ -359,9 +408,9 @@ __global__ __launch_bounds__(256) void k_attn_join(PromptLaunch P) {
 }
 
 // ================================================================================== host side
-template <int G, int NT, int PARTS>
+template <int G, int WAVES, int PARTS>
 static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
-    constexpr int RB = Prompt<G, NT, PARTS>::RB, D = 32 * G;
+    constexpr int RB = Prompt<G, WAVES, PARTS>::RB, D = 32 * G;
     PromptLaunch P;
     memset(&P, 0, sizeof P);
     P.A = L;
@@ -376,7 +425,7 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
         if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)items * P.parts * RB * (D + 2) * 4, false)) return rc;
         P.A.part = (float *)c->attn_part.p;
     }
-    hipLaunchKernelGGL((k_attn_prompt<G, NT, PARTS>), dim3((unsigned)(items * P.parts)), dim3(512), 0, c->stream, P);
+    hipLaunchKernelGGL((k_attn_prompt<G, WAVES, PARTS>), dim3((unsigned)(items * P.parts)), dim3(64 * WAVES), 0, c->stream, P);
     if (P.parts > 1) {
         constexpr int per = 256 / (D / 4);
         hipLaunchKernelGGL((k_attn_join<D, RB>), dim3((unsigned)items, (RB + per - 1) / per), dim3(256), 0, c->stream, P);
@@ -385,8 +434,8 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
 }
 template <int G>
 static int prompt_pick(bgl_ctx *c, const AttnLaunch &L) {
-    if (L.a.type == BGL_T_F32) return prompt_go<G, G <= 4 ? 2 : 1, 2>(c, L);
-    return prompt_go<G, G <= 4 ? 2 : 1, 1>(c, L);
+    if (L.a.type == BGL_T_F32) return prompt_go<G, G <= 3 ? 8 : 4, 2>(c, L);
+    return prompt_go<G, G <= 4 ? 8 : 4, 1>(c, L);
 }
 
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L) {

@@ -25,8 +25,10 @@ def torch_dev():
 @pytest.fixture(scope="module")
 def ctx(torch_dev):
     import beglin_amd
-    c = beglin_amd.Context(0)
-    yield c
+    st = torch_dev.cuda.Stream()                                                   # torch's work and the library's in one order
+    c = beglin_amd.Context(0, st.cuda_stream)
+    with torch_dev.cuda.stream(st):
+        yield c
     c.sync()
     c.close()
 
