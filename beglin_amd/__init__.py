@@ -144,44 +144,42 @@ class Tensor:
             self.h = None
 
 
-def _heads(t, who, dev, shape=None, type_=None):
-    """Pointer and distances in elements between the tokens and the heads of a [T][heads][D] tensor on device dev."""
-    if t.dim() != 3 or (shape is not None and t.shape != shape):
-        _refuse(f"{who}: heads are [T][heads][D], here {tuple(shape) if shape is not None else tuple(t.shape)}")
+def _heads(t, shape, kind, dev, who):
+    """Pointer and distances in elements between the tokens and the heads of a [T][heads][D] tensor of a type on device dev."""
+    if t.shape != shape or t.dtype is not kind or t.get_device() != dev:
+        _refuse(f"{who}: heads are {kind} {tuple(shape)} on device {dev}")
     ld, hd, one = t.stride()
     if one != 1:
         _refuse(f"{who}: the values of a head are dense")
-    if type_ is not None and t.dtype is not type_:
-        _refuse(f"{who}: rows of another type")
-    if t.get_device() != dev:
-        _refuse(f"{who}: tensors lie on device {dev}")
     return t.data_ptr(), ld, hd
 
 
-def _row_type(t, who):
+def _row_type(kind, who):
     d = _dtypes()
-    k = t.dtype
-    return T_F32 if k is d[0] else T_F16 if k is d[1] else T_BF16 if k is d[2] else _refuse(f"{who}: rows are fp32, fp16 or bf16")
+    return T_F32 if kind is d[0] else T_F16 if kind is d[1] else T_BF16 if kind is d[2] else _refuse(f"{who}: rows are fp32, fp16 or bf16")
 
 
-def _ints(t, n, who, dev):
+_INT32 = None
+_NO_ROWS = None, 0, 0
+
+
+def _ints(t, n, dev, who):
     """Pointer of a dense int32 vector of n values on device dev."""
-    import torch
-    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
-        _refuse(f"{who}: int32 [{n}] expected")
-    if t.get_device() != dev:
-        _refuse(f"{who}: tensors lie on device {dev}")
+    global _INT32
+    if _INT32 is None:
+        import torch
+        _INT32 = torch.int32
+    if t.dtype is not _INT32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{who}: int32 [{n}] on device {dev} expected")
     return t.data_ptr()
 
 
-def _floats(t, n, who, dev):
+def _floats(t, n, dev, who):
     """Pointer of a dense fp32 vector of n values on device dev, None passes through."""
     if t is None:
         return None
-    if t.dtype is not _dtypes()[0] or t.numel() != n or not t.is_contiguous():
-        _refuse(f"{who}: fp32 [{n}] expected")
-    if t.get_device() != dev:
-        _refuse(f"{who}: tensors lie on device {dev}")
+    if t.dtype is not _dtypes()[0] or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{who}: fp32 [{n}] on device {dev} expected")
     return t.data_ptr()
 
 
@@ -421,42 +419,40 @@ class Context:
 
     # ---- attention: heads, the paged cache in 4 bits, the rows that attend ----
     def _heads(self, who, q, k, v, q_out, k_out, norm, q_w, k_w, eps, w_add, rope, pos, rot):
-        dev, first = self.device, q if q is not None else k
-        if first is None:
-            _refuse(f"{who}: neither q nor k")
-        if first.dim() != 3:
-            _refuse(f"{who}: heads are [T][heads][D]")
-        T, n, D = first.shape
+        dev, first = self.device, k if q is None else q
+        if first is None or first.ndim != 3 or (q is None) != (q_out is None) or (k is None and k_out is not None):
+            _refuse(f"{who}: q with q_out, or k, as [T][heads][D]")
+        T, nq, D = shape = first.shape
         kind = first.dtype
-        d = capi.bgl_heads(T, D)
-        d.type, d.norm, d.eps, d.w_add = _row_type(first, who), norm, eps, w_add
+        nk, Q, QO, K, KO, V, out = 0, _NO_ROWS, _NO_ROWS, _NO_ROWS, _NO_ROWS, _NO_ROWS, kind
         if q is not None:
-            d.nq = n
-            d.q, d.ldq, d.hdq = _heads(q, who, dev)
-            if q_out is None:
-                _refuse(f"{who}: q and q_out go together")
-            d.q_out, d.ldqo, d.hdqo = _heads(q_out, who, dev, q.shape)
-            d.out_type = _row_type(q_out, who)
-            if q_w is not None and norm:
-                d.q_w = _floats(q_w, D, who, dev)
+            out = q_out.dtype
+            Q, QO = _heads(q, shape, kind, dev, who), _heads(q_out, shape, out, dev, who)
+        else:
+            nq = 0
         if k is not None:
-            d.nk = k.shape[1] if k.dim() == 3 else 0
-            d.k, d.ldk, d.hdk = _heads(k, who, dev, (T, d.nk, D), kind)
-            if k_w is not None and norm:
-                d.k_w = _floats(k_w, D, who, dev)
-        if v is not None:
-            d.v, d.ldv, d.hdv = _heads(v, who, dev, (T, d.nk, D), kind)
-        if k_out is not None:
-            if k is None:
-                _refuse(f"{who}: k and k_out go together")
-            d.k_out, d.ldko, d.hdko = _heads(k_out, who, dev, k.shape, None if q is None else q_out.dtype)
-            d.out_type = _row_type(k_out, who)
-        if rope is not None and rot:
-            if rope.dim() != 2:
+            nk = k.shape[1] if k.ndim == 3 else 0
+            shape = (T, nk, D)
+            K = _heads(k, shape, kind, dev, who)
+            if v is not None:
+                V = _heads(v, shape, kind, dev, who)
+            if k_out is not None:
+                if q is None:
+                    out = k_out.dtype
+                KO = _heads(k_out, shape, out, dev, who)
+        n_pos = size = 0
+        table = at = qw = kw = None
+        if rope is None:
+            rot = ROT_NONE
+        elif rot:
+            if rope.ndim != 2:
                 _refuse(f"{who}: rope is fp32 [positions][rot]")
-            d.n_pos, d.rot = rope.shape
-            d.rot_kind, d.rope, d.pos = rot, _floats(rope, rope.numel(), who, dev), _ints(pos, T, who, dev)
-        return d
+            n_pos, size = rope.shape
+            table, at = _floats(rope, n_pos * size, dev, who), _ints(pos, T, dev, who)
+        if norm:
+            qw, kw = _floats(q_w, D, dev, who), _floats(k_w, D, dev, who)
+        return capi.bgl_heads(T, D, nq, nk, Q[0], K[0], V[0], Q[1], Q[2], K[1], K[2], V[1], V[2], _row_type(kind, who), norm, qw, kw, eps, w_add,
+                              rot, size, table, n_pos, at, QO[0], KO[0], QO[1], QO[2], KO[1], KO[2], _row_type(out, who))
 
     def heads(self, q, k, q_out, k_out, *, norm=NORM_NONE, q_w=None, k_w=None, eps=1e-6, w_add=0.0, rope=None, pos=None, rot=ROT_HALF):
         """q_out, k_out = rotation(norm(q)), rotation(norm(k)) head by head (bgl_heads_dev) over [T][heads][D] tensors, whose tokens and
@@ -468,53 +464,38 @@ class Context:
     def kv_append(self, cache, slots, k, v, *, q=None, q_out=None, norm=NORM_NONE, q_w=None, k_w=None, eps=1e-6, w_add=0.0, rope=None,
                   pos=None, rot=ROT_HALF):
         """Keys (normed and rotated as by heads) and values [T][heads][D] into the cache at slots int32 [T] (bgl_kv_append_dev),
-        with q and q_out the queries in the same launch."""
+        with q and q_out the queries in the same call."""
         d = self._heads("kv_append", q, k, v, q_out, None, norm, q_w, k_w, eps, w_add, rope, pos, rot)
         if cache.device != self.device:
             _refuse(f"kv_append: tensors lie on device {self.device}")
-        _check(lib().bgl_kv_append_dev(self.h, C.byref(cache.d), C.byref(d), _ints(slots, d.T, "kv_append", self.device)),
-               "bgl_kv_append_dev")
+        _check(lib().bgl_kv_append_dev(self.h, C.byref(cache.d), C.byref(d), _ints(slots, d.T, self.device, "kv_append")), "bgl_kv_append_dev")
 
     def kv_read(self, cache, slots, k=None, v=None):
         """The values of the cache at slots int32 [n] into k and v [n][heads][D] (bgl_kv_read_dev); rows of slots outside the
         cache are left as they are."""
-        one = k if k is not None else v
-        if one is None:
-            _refuse("kv_read: neither k nor v")
-        n, dev = slots.numel(), self.device
-        shape = (n, cache.heads, cache.dim)
-        K = _heads(k, "kv_read", dev, shape, one.dtype) if k is not None else (None, 0, 0)
-        V = _heads(v, "kv_read", dev, shape, one.dtype) if v is not None else (None, 0, 0)
-        if cache.device != dev:
-            _refuse(f"kv_read: tensors lie on device {dev}")
-        _check(lib().bgl_kv_read_dev(self.h, C.byref(cache.d), _ints(slots, n, "kv_read", dev), n, *K, *V, _row_type(one, "kv_read")),
+        one, n, dev = v if k is None else k, slots.numel(), self.device
+        if one is None or cache.device != dev:
+            _refuse(f"kv_read: k or v, and the cache, on device {dev}")
+        shape, kind = (n, cache.heads, cache.dim), one.dtype
+        K = _NO_ROWS if k is None else _heads(k, shape, kind, dev, "kv_read")
+        V = _NO_ROWS if v is None else _heads(v, shape, kind, dev, "kv_read")
+        _check(lib().bgl_kv_read_dev(self.h, C.byref(cache.d), _ints(slots, n, dev, "kv_read"), n, *K, *V, _row_type(kind, "kv_read")),
                "bgl_kv_read_dev")
 
     def attention(self, cache, q, out, start, lens, table, *, scale=None, causal=True, window=0, sink=None, max_rows=None, max_len=None):
         """out = attention of the rows q [T][heads][D] over the cache (bgl_attn_dev): sequence s has the rows start[s] ..
         start[s + 1] - 1 and lens[s] keys in the pages table[s]; int32 tensors [S + 1], [S], [S][pages].  scale None: 1 / sqrt(D).
         sink: fp32 [heads].  max_rows, max_len: the most rows and keys of a sequence, where the program knows them."""
-        dev = self.device
-        if table.dim() != 2:
-            _refuse("attention: table is int32 [S][pages]")
+        dev, who = self.device, "attention"
+        if table.ndim != 2 or q.ndim != 3 or q.shape[2] != cache.dim or cache.device != dev:
+            _refuse(f"attention: q [T][heads][{cache.dim}], table [S][pages], the cache on device {dev}")
         S, ldt = table.shape
-        a = capi.bgl_attn(S)
-        a.q, a.ldq, a.hdq = _heads(q, "attention", dev)
-        a.T, a.nq, D = q.shape
-        if D != cache.dim:
-            _refuse(f"attention: rows of {D} values over a cache of {cache.dim}")
-        a.out, a.ldo, a.hdo = _heads(out, "attention", dev, q.shape, q.dtype)
-        a.type = _row_type(q, "attention")
-        a.start, a.len, a.ldt = _ints(start, S + 1, "attention", dev), _ints(lens, S, "attention", dev), ldt
-        a.table = _ints(table, S * ldt, "attention", dev)
-        a.scale = D ** -0.5 if scale is None else scale
-        a.causal, a.window = int(causal), window
-        if sink is not None:
-            a.sink = _floats(sink, a.nq, "attention", dev)
-        a.max_rows = a.T if max_rows is None else max_rows
-        a.max_len = ldt * cache.page if max_len is None else max_len
-        if cache.device != dev:
-            _refuse(f"attention: tensors lie on device {dev}")
+        T, nq, D = shape = q.shape
+        kind = q.dtype
+        a = capi.bgl_attn(S, T, nq, *_heads(q, shape, kind, dev, who), *_heads(out, shape, kind, dev, who), _row_type(kind, who),
+                          _ints(start, S + 1, dev, who), _ints(lens, S, dev, who), _ints(table, S * ldt, dev, who), ldt,
+                          D ** -0.5 if scale is None else scale, causal, window, _floats(sink, nq, dev, who),
+                          T if max_rows is None else max_rows, ldt * cache.page if max_len is None else max_len)
         _check(lib().bgl_attn_dev(self.h, C.byref(cache.d), C.byref(a)), "bgl_attn_dev")
 
     # ---- MoE ----

@@ -26,11 +26,20 @@ struct HeadsLaunch {
     bgl_heads d;
     bgl_kv c;
     const int32_t *slots;        // of the d.T tokens of this launch; null: no cache
-    int before, after;           // tokens of the call before and behind this launch's (slots reach that far)
     int nq, nk, nv;              // heads to do of each
 };
 
 // Sums over the GL lanes of a head, in every one of them.
+template <int GL>
+__device__ __forceinline__ float hd_sum(float v) {
+    v += dpp_f<0xB1>(v);
+    v += dpp_f<0x4E>(v);
+    v += dpp_f<0x141>(v);
+    if (GL > 8) v += dpp_f<0x140>(v);
+    if (GL > 16) v += __shfl_xor(v, 16);
+    if (GL > 32) v += __shfl_xor(v, 32);
+    return v;
+}
 template <int GL>
 __device__ __forceinline__ double hd_sum(double v) {
     v += dpp_d<0xB1>(v);
@@ -42,83 +51,132 @@ __device__ __forceinline__ double hd_sum(double v) {
     return v;
 }
 
-// What a lane needs of the rotation for its 8 values d0 .. d0 + 7: their cosines and sines (half: one each; pairs: one each
-// two values), and for half where the other value of each pair lies.
+// What a lane needs of the rotation for its 8 values d0 .. d0 + 7: their cosines and sines (the sines of half's first values with
+// their sign), and for half where the other value of each pair lies.
 struct HdTurn {
     float c[8], s[8];
-    int other;                   // first of the 8 partners; 0 distance: not rotated
+    int other;                   // first of the 8 partners
+    bool on;                     // the values are rotated
 };
 __device__ __forceinline__ HdTurn hd_turn(const bgl_heads &d, const float *rope, int d0) {
     HdTurn t;
     t.other = d0;
+    t.on = d.rot_kind != BGL_ROT_NONE && d0 < d.rot;
 #pragma unroll
     for (int j = 0; j < 8; j++) { t.c[j] = 1.0f; t.s[j] = 0.0f; }
-    if (d.rot_kind == BGL_ROT_NONE || d0 >= d.rot) return t;
+    if (!t.on) return t;
     const int h = d.rot / 2;
     if (d.rot_kind == BGL_ROT_HALF) {
         t.other = d0 < h ? d0 + h : d0 - h;
         const int i = d0 < h ? d0 : t.other;
         kv_load8(t.c, rope, BGL_T_F32, i);
         kv_load8(t.s, rope, BGL_T_F32, h + i);
+#pragma unroll
+        for (int j = 0; j < 8; j++) t.s[j] = d0 < h ? -t.s[j] : t.s[j];
     } else {
         const kv_mf4 c = *(const kv_mf4 *)(rope + d0 / 2), s = *(const kv_mf4 *)(rope + h + d0 / 2);
 #pragma unroll
-        for (int j = 0; j < 4; j++) { t.c[2 * j] = t.c[2 * j + 1] = c[j]; t.s[2 * j] = t.s[2 * j + 1] = s[j]; }
+        for (int j = 0; j < 4; j++) {
+            t.c[2 * j] = t.c[2 * j + 1] = c[j];
+            t.s[2 * j] = -s[j];
+            t.s[2 * j + 1] = s[j];
+        }
     }
     return t;
 }
+// The norm's factors of a lane's values and of their partners.
+struct HdWeights {
+    float w[8], pw[8];
+};
+__device__ __forceinline__ HdWeights hd_weights(const bgl_heads &d, const float *w, const HdTurn &t, int d0) {
+    HdWeights g;
+#pragma unroll
+    for (int j = 0; j < 8; j++) g.w[j] = g.pw[j] = 1.0f;
+    if (d.norm == BGL_NORM_NONE || !w) return g;
+    kv_load8(g.w, w, BGL_T_F32, d0);
+    kv_load8(g.pw, w, BGL_T_F32, t.other);
+    return g;
+}
 
-// y of a lane's 8 values of the head at p (values past D: 0).
-template <int GL>
-__device__ __forceinline__ void hd_row(float (&y)[8], const bgl_heads &d, const void *p, long at, const float *w, const HdTurn &t, int d0, bool in) {
-    float x[8], px[8];
-    kv_load8(x, p, d.type, at + (in ? d0 : 0));
-    const bool half = d.rot_kind == BGL_ROT_HALF && t.other != d0;
-    if (d.rot_kind == BGL_ROT_HALF) kv_load8(px, p, d.type, at + (in ? t.other : 0));
-    double n[8], pn[8];
+// y of a lane's 8 values x of a head (0 for a lane behind D) and, for half, their partners px.  R: the arithmetic's type.
+template <typename R, int GL>
+__device__ __forceinline__ void hd_turned(float (&y)[8], const bgl_heads &d, const float (&x)[8], const float (&px)[8], const HdWeights &g, const HdTurn &t,
+                                          R mean, R inv) {
+    R n[8];
+    const R add = d.norm != BGL_NORM_NONE && d.w_add != 0.0f ? (R)d.w_add : (R)0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) n[j] = in ? (double)x[j] : 0.0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) pn[j] = half ? (double)px[j] : 0.0;
-    if (d.norm != BGL_NORM_NONE) {
-        double mean = 0.0, q = 0.0;
-        if (d.norm == BGL_NORM_LAYER) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) mean += n[j];
-            mean = hd_sum<GL>(mean) / d.D;
-#pragma unroll
-            for (int j = 0; j < 8; j++) { n[j] = in ? n[j] - mean : 0.0; pn[j] -= mean; }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) q = fma(n[j], n[j], q);
-        const double inv = 1.0 / sqrt(hd_sum<GL>(q) / d.D + (double)d.eps);
-#pragma unroll
-        for (int j = 0; j < 8; j++) { n[j] *= inv; pn[j] *= inv; }
-        if (w) {
-            float g[8], pg[8];
-            kv_load8(g, w, BGL_T_F32, in ? d0 : 0);
-            if (d.rot_kind == BGL_ROT_HALF) kv_load8(pg, w, BGL_T_F32, in ? t.other : 0);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                n[j] *= (double)g[j] + (double)d.w_add;
-                if (d.rot_kind == BGL_ROT_HALF) pn[j] *= (double)pg[j] + (double)d.w_add;
-            }
-        }
-    }
-    if (d.rot_kind == BGL_ROT_NONE || d0 >= d.rot) {
+    for (int j = 0; j < 8; j++) n[j] = ((R)x[j] - mean) * inv * ((R)g.w[j] + add);
+    if (d.rot_kind == BGL_ROT_NONE) {
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] = (float)n[j];
     } else if (d.rot_kind == BGL_ROT_HALF) {
-        const bool first = t.other > d0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = (float)fma(n[j], (double)t.c[j], first ? -(pn[j] * (double)t.s[j]) : pn[j] * (double)t.s[j]);
+        for (int j = 0; j < 8; j++) {
+            const R pn = ((R)px[j] - mean) * inv * ((R)g.pw[j] + add);
+            const R v = fma(n[j], (R)t.c[j], pn * (R)t.s[j]);
+            y[j] = (float)(t.on ? v : n[j]);
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            y[j] = (float)fma(n[j], (double)t.c[j], -(n[j + 1] * (double)t.s[j]));
-            y[j + 1] = (float)fma(n[j + 1], (double)t.c[j], n[j] * (double)t.s[j]);
+        for (int j = 0; j < 8; j++) {
+            const R v = fma(n[j], (R)t.c[j], n[j ^ 1] * (R)t.s[j]);
+            y[j] = (float)(t.on ? v : n[j]);
         }
     }
+}
+// A 16-bit output needs no double (16 additions and multiplications err by 2^-20 at most), unless a norm takes a difference from the mean
+// or hides a row of tiny values behind no eps.
+static __host__ __device__ __forceinline__ bool hd_fast(const bgl_heads &d) {
+    return d.out_type != BGL_T_F32 && (d.norm == BGL_NORM_NONE || (d.norm == BGL_NORM_RMS && d.eps >= 1e-20f));
+}
+template <int GL>
+__device__ __forceinline__ void hd_row_fast(float (&y)[8], const bgl_heads &d, float (&x)[8], float (&px)[8], const HdWeights &g, const HdTurn &t) {
+    float inv = 1.0f;
+    if (d.norm != BGL_NORM_NONE) {
+        float q = 0.0f, eps = d.eps;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q = fmaf(x[j], x[j], q);
+        q = hd_sum<GL>(q);
+        if (__any(!(q < 1e30f))) {                       // squares near fp32's end (or NaN): all of it 2^-80 as large, where eps counts no more
+            const float down = q < 1e30f ? 1.0f : 0x1p-80f;
+            eps = q < 1e30f ? eps : 0.0f;
+            q = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) { x[j] *= down; px[j] *= down; q = fmaf(x[j], x[j], q); }
+            q = hd_sum<GL>(q);
+        }
+        inv = 1.0f / sqrtf(q / d.D + eps);
+    }
+    hd_turned<float, GL>(y, d, x, px, g, t, 0.0f, inv);
+}
+// Keeps what is the same for every head in fp32 registers: as doubles, made once, it takes twice as many.
+__device__ __forceinline__ void hd_opaque(float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) asm volatile("" : "+v"(v[j]));
+}
+template <int GL>
+__device__ __forceinline__ void hd_row(float (&y)[8], const bgl_heads &d, const float (&x)[8], const float (&px)[8], HdWeights &g, HdTurn &t) {
+    hd_opaque(g.w);
+    hd_opaque(g.pw);
+    hd_opaque(t.c);
+    hd_opaque(t.s);
+    double mean = 0.0, inv = 1.0;
+    if (d.norm != BGL_NORM_NONE) {
+        double q = 0.0;
+        if (d.norm == BGL_NORM_LAYER) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) mean += (double)x[j];
+            mean = hd_sum<GL>(mean) / d.D;
+        }
+        const bool in = (int)(threadIdx.x & (GL - 1)) * 8 < d.D;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const double v = in ? (double)x[j] - mean : 0.0;
+            q = fma(v, v, q);
+        }
+        inv = rsqrt(hd_sum<GL>(q) / d.D + (double)d.eps);
+    }
+    hd_turned<double, GL>(y, d, x, px, g, t, mean, inv);
 }
 
 // The codes of a lane's 8 values, whose group is those of the lane's quad, and the group's step and floor (s | m << 16).
@@ -172,42 +230,63 @@ __device__ __forceinline__ void hd_put_v(uint8_t *rec, int D, int tok, int li, c
     }
 }
 
-// A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other.
-template <int GL>
-__global__ __launch_bounds__(256) void k_heads(HeadsLaunch L) {
+// A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other.  FAST, EXACT: which rows the launch has, those
+// of hd_row_fast, the others and the cache's, or both: few tokens are one launch, many take one each, for the others' doubles would leave the
+// fast ones half as many waves (4096 tokens of 40 heads, bf16: 49 us together).
+template <int GL, bool FAST, bool EXACT>
+__global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
     const bgl_heads &d = L.d;
-    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), d0 = 8 * li;
-    const bool in = d0 < d.D;
-    const float *rope = nullptr;
-    if (d.rot_kind != BGL_ROT_NONE) {
-        const int p = d.pos[t];
-        if (p < 0 || p >= d.n_pos) return;
-        rope = d.rope + (size_t)p * d.rot;
-    }
-    const HdTurn turn = hd_turn(d, rope, in ? d0 : 0);
+    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), per = (int)blockDim.x / GL;
+    const bool in = 8 * li < d.D;
+    const int d0 = in ? 8 * li : 0;
+    const int pos = d.rot_kind != BGL_ROT_NONE ? d.pos[t] : 0;
     const int slot = L.slots ? L.slots[t] : -1;
+    const float *const rope = d.rope + (size_t)pos * d.rot;
     const bool kept = slot >= 0 && slot < (long)L.c.pages * L.c.page;
-    const int n = L.nq + L.nk + L.nv, step = (int)gridDim.y * (256 / GL);
-    for (int i = (int)blockIdx.y * (256 / GL) + (int)threadIdx.x / GL; i < n; i += step) {
-        float y[8];
-        if (i < L.nq) {
-            hd_row<GL>(y, d, d.q, t * d.ldq + i * d.hdq, d.q_w, turn, d0, in);
-            if (in) kv_store8(d.q_out, d.out_type, t * d.ldqo + i * d.hdqo + d0, y);
-        } else if (i < L.nq + L.nk) {
-            const int h = i - L.nq;
-            hd_row<GL>(y, d, d.k, t * d.ldk + h * d.hdk, d.k_w, turn, d0, in);
-            if (d.k_out) {
-                if (in) kv_store8(d.k_out, d.out_type, t * d.ldko + h * d.hdko + d0, y);
-            } else if (kept && in) {
-                hd_put_k(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
-            }
-        } else {
-            const int h = i - L.nq - L.nk;
-            if (kept && in) {
-                kv_load8(y, d.v, d.type, t * d.ldv + h * d.hdv + d0);
-                hd_put_v(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
-            }
+    if (d.rot_kind != BGL_ROT_NONE && (uint32_t)pos >= (uint32_t)d.n_pos) return;
+    const int step = (int)gridDim.y * per, first = (int)blockIdx.y * per + (int)threadIdx.x / GL;
+    HdTurn turn = hd_turn(d, rope, d0);
+    auto load = [&](float (&x)[8], float (&px)[8], const void *p, long at) {
+        kv_load8(x, p, d.type, at + d0);
+        if (d.rot_kind == BGL_ROT_HALF) kv_load8(px, p, d.type, at + turn.other);
+        if (!in) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = 0.0f;
         }
+    };
+    int i = first;
+    if (i < L.nq) {
+        HdWeights g = hd_weights(d, d.q_w, turn, d0);
+        const bool fast = FAST && (!EXACT || hd_fast(d));
+        for (; i < L.nq; i += step) {
+            float x[8], px[8], y[8];
+            load(x, px, d.q, t * d.ldq + i * d.hdq);
+            if (fast) hd_row_fast<GL>(y, d, x, px, g, turn);
+            else if constexpr (EXACT) hd_row<GL>(y, d, x, px, g, turn);
+            if (in) kv_store8(d.q_out, d.out_type, t * d.ldqo + i * d.hdqo + d0, y);
+        }
+    }
+    if (i < L.nq + L.nk) {
+        HdWeights g = hd_weights(d, d.k_w, turn, d0);
+        const bool fast = FAST && (!EXACT || (d.k_out && hd_fast(d)));
+        for (; i < L.nq + L.nk; i += step) {
+            const int h = i - L.nq;
+            float x[8], px[8], y[8];
+            if (!d.k_out && !kept) continue;
+            load(x, px, d.k, t * d.ldk + h * d.hdk);
+            if (fast) hd_row_fast<GL>(y, d, x, px, g, turn);
+            else if constexpr (EXACT) hd_row<GL>(y, d, x, px, g, turn);
+            if (!in) continue;
+            if (d.k_out) kv_store8(d.k_out, d.out_type, t * d.ldko + h * d.hdko + d0, y);
+            else if constexpr (EXACT) hd_put_k(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
+        }
+    }
+    if (!EXACT || !kept || !in) return;
+    for (; i < L.nq + L.nk + L.nv; i += step) {
+        const int h = i - L.nq - L.nk;
+        float y[8];
+        kv_load8(y, d.v, d.type, t * d.ldv + h * d.hdv + d0);
+        hd_put_v(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
     }
 }
 
@@ -256,6 +335,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
 // ================================================================================== host side
 // A launch has less than 2^32 threads, 256 of them a token and up to 16 workgroups of few tokens.
 #define HD_TOKENS (1 << 20)
+#define HD_MANY (1 << 14)         // heads of queries that are a launch of their own beside the cache's rows
 
 // Workgroups a token: as many as it takes to do every head at once, while the launch leaves units idle.
 static unsigned hd_parts(int T, int items, int per) {
@@ -277,8 +357,6 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
         HeadsLaunch L = all;
         bgl_heads &d = L.d;
         d.T = (int)std::min<long>(HD_TOKENS, a.T - t);
-        L.before = (int)t;
-        L.after = (int)(a.T - t - d.T);
         auto at = [&](const void *p, long ld, int type) { return p ? (char *)p + t * ld * (long)i8_elem(type) : nullptr; };
         d.q = at(a.q, a.ldq, a.type); d.k = at(a.k, a.ldk, a.type); d.v = at(a.v, a.ldv, a.type);
         d.q_out = at(a.q_out, a.ldqo, a.out_type); d.k_out = at(a.k_out, a.ldko, a.out_type);
@@ -286,7 +364,18 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
         if (all.slots) L.slots = all.slots + t;
         hd_lanes(d.D, [&](auto gl) {
             constexpr int GL = decltype(gl)::value;
-            hipLaunchKernelGGL((k_heads<GL>), dim3((unsigned)d.T, hd_parts(d.T, L.nq + L.nk + L.nv, 256 / GL)), dim3(256), 0, c->stream, L);
+            auto go = [&](auto kernel, int nq, int nk, int nv) {
+                L.nq = nq; L.nk = nk; L.nv = nv;
+                hipLaunchKernelGGL(kernel, dim3((unsigned)d.T, hd_parts(d.T, nq + nk + nv, 256 / GL)), dim3(256), 0, c->stream, L);
+            };
+            const bool q_fast = all.nq && hd_fast(d), k_fast = all.nk && d.k_out && hd_fast(d), exact = all.nv || (all.nq && !q_fast) || (all.nk && !k_fast);
+            if (!exact) go(k_heads<GL, true, false>, all.nq, all.nk, 0);
+            else if (!q_fast) go(k_heads<GL, false, true>, all.nq, all.nk, all.nv);
+            else if (a.T * all.nq < HD_MANY) go(k_heads<GL, true, true>, all.nq, all.nk, all.nv);
+            else {
+                go(k_heads<GL, true, false>, all.nq, 0, 0);
+                go(k_heads<GL, false, true>, 0, all.nk, all.nv);
+            }
         });
     }
     prof_end(c, tok);

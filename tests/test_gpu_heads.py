@@ -1,8 +1,10 @@
 """bgl_heads_dev, bgl_kv_append_dev and bgl_kv_read_dev against the formulas in 64 bits.
 
-A head's values are computed in double and rounded to fp32 and then to the output's type, so a value may be off by half a
-step of each: 2^-24 and 2^-11 (fp16) or 2^-8 (bf16) more, relative; a difference of two products that nearly cancel adds what
-a double's rounding (2^-53 of the products, far below 1e-13 of the head's largest value) leaves.  The cache's values
+A head's values for an fp32 output are computed in double and rounded to fp32, so a value may be off by half a step, 2^-24 relative; a
+difference of two products that nearly cancel adds what a double's rounding (2^-53 of the products, far below 1e-13 of the
+head's largest value) leaves.  For a 16-bit output fp32 arithmetic may stand in: a sum of squares in at most 8 + 6 additions,
+halved by the root, with the division, root, products and the rotation's two roundings, (14 / 2 + 1 + 1 + 1 + 3 + 2) 2^-24 < 2^-20 of
+the two products that are added, at most twice the largest value of the head; and half a step of the type, 2^-11 or 2^-8.  The cache's values
 follow from the fp32 rows by single operations, so they are equal; where the rows pass through a norm or a rotation, a
 value within 1e-10 of a border between two fp32 values may fall to either side, and with it one code to the next: such
 codes are counted, and at most one in 10^5 may differ, by one step of its group."""
@@ -41,7 +43,8 @@ def near(got, want, name):
     kind = str(got.dtype).split(".")[1]
     rel = F.HALF["float32"] + (F.HALF[kind] if kind != "float32" else 0)
     g = host(got).astype(np.float64)
-    off = np.abs(g - want) - (rel * (1 + 1e-6) * np.abs(want) + F.LEAST[kind] + 1e-13 * np.abs(want).max(-1, keepdims=True))
+    sums = 1e-13 if kind == "float32" else 2 * 2.0 ** -20
+    off = np.abs(g - want) - (rel * (1 + 1e-6) * np.abs(want) + F.LEAST[kind] + sums * np.abs(want).max(-1, keepdims=True))
     assert np.isfinite(g).all() and off.max() <= 0, (name, off.max(), np.argwhere(off > 0)[:4])
 
 
