@@ -11,6 +11,7 @@ struct AttnLaunch {
     int g;                       // heads of q for one of the cache
     int ppt;                     // 16-token tiles a page
     uint32_t div_mul, div_shift; // t / ppt = (mulhi(t, div_mul) + t) >> div_shift for t < 2^31
+    int unit;                    // bgl_attn.hip: keys a unit, a multiple of AT_STEP
     int limit;                   // sequences with more than this many rows times g are another launch's
     float scale2;                // |scale| * log2(e); a negative scale turns q's sign
     float *part;                 // bgl_attn.hip's partial sums: [2 * workgroups] pieces
@@ -36,7 +37,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnLaunch &L, int s) {
     q.lo = min(q.lo, q.len);
     return q;
 }
-// The keys [lo, hi] that row i of n sees (none: hi < lo).
+// The keys [lo, hi] that token i of n sees (none: hi < lo).
 __device__ __forceinline__ void attn_keys(const AttnLaunch &L, const AttnSeq &q, int i, int &lo, int &hi) {
     const int pos = q.len - q.n + i;
     hi = L.a.causal ? min(pos, q.len - 1) : q.len - 1;
@@ -134,50 +135,69 @@ __device__ __forceinline__ int at_page(const AttnLaunch &L, int t) { return (int
 // A row of queries as operands: row r of the sequence's n * g (token r / g, head r % g of the group; past the last: the last), scaled by a power of
 // two that puts the row's largest value in [2^14, 2^15): exact in fp16 down to 2^-28 of it (two parts for fp32 rows:
 // 2^-22).  Values 8 G b .. + 8 G - 1 for a lane of block b of four (columns of 16), or with WIDE those of blocks b and 2 + b for a lane of half b
-// (columns of 32).  fac turns the products into scores of base 2, zero is where they begin (NaN for a row with a NaN or an
-// infinity), [lo, hi] are the keys that the row sees.
+// (columns of 32).  PARTS is 2 for fp32 rows and 1 for the others.
 template <int G, int PARTS, bool WIDE = false>
-__device__ __forceinline__ void at_query(const AttnLaunch &L, const AttnSeq &q, int head, int r, int b, kv_h8 (&qf)[WIDE ? 2 : 1][PARTS][G], float &fac,
-                                         float &zero, int &lo, int &hi) {
-    constexpr int N = WIDE ? 2 : 1;
-    const int rr = min(r, q.n * L.g - 1), i = rr / L.g;
-    const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
-    attn_keys(L, q, i, lo, hi);
-    float x[N][G][8];
-    uint32_t top = 0;
+struct AtQuery {
+    static constexpr int N = WIDE ? 2 : 1;
+    kv_mu4 raw[N][G][PARTS];     // as they lie in memory: loaded early, waited for late
+
+    __device__ __forceinline__ void load(const AttnLaunch &L, const AttnSeq &q, int head, int r, int b) {
+        const int rr = min(r, q.n * L.g - 1), i = rr / L.g;
+        const long at = (long)(q.begin + i) * L.a.ldq + (long)(head * L.g + rr - i * L.g) * L.a.hdq + 8 * G * b;
 #pragma unroll
-    for (int n = 0; n < N; n++)
+        for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int j = 0; j < G; j++) {
-            kv_load8(x[n][j], L.a.q, L.a.type, at + 16 * G * n + 8 * j);
+            for (int j = 0; j < G; j++) {
+                const kv_mu4 *const p = (const kv_mu4 *)((const uint16_t *)L.a.q + PARTS * (at + 16 * G * n + 8 * j));
 #pragma unroll
-            for (int y = 0; y < 8; y++) top = max(top, __float_as_uint(x[n][j][y]) & 0x7fffffffu);
-        }
-    top = min(top, 0x7f800000u);                                                       // NaN counts as an infinity
-    if constexpr (WIDE) {
-        auto a = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        top = max((uint32_t)a[0], (uint32_t)a[1]);
-    } else {
-        top = __float_as_uint(at_max4(__uint_as_float(top)));
-    }
-    const bool bad = top >= 0x7f800000u;
-    const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
-    const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
-#pragma unroll
-    for (int n = 0; n < N; n++)
-#pragma unroll
-        for (int j = 0; j < G; j++)
-#pragma unroll
-            for (int y = 0; y < 8; y++) {
-                const float v = x[n][j][y] * up;
-                const _Float16 h = (_Float16)v;
-                qf[n][0][j][y] = h;
-                if constexpr (PARTS == 2) qf[n][1][j][y] = (_Float16)(v - (float)h);
+                for (int e = 0; e < PARTS; e++) raw[n][j][e] = p[e];
             }
-    // (a factor of 0 would make NaN of masked scores)
-    fac = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
-    zero = bad ? NAN : 0.0f;
-}
+    }
+    __device__ __forceinline__ float value(int n, int j, int y, bool f16) const {
+        if constexpr (PARTS == 2) return __uint_as_float(raw[n][j][y >> 2][y & 3]);
+        const uint32_t w = raw[n][j][0][y >> 1] >> (16 * (y & 1)) & 0xffffu;
+        return f16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)w) : __uint_as_float(w << 16);
+    }
+    // fac turns the products into scores of base 2, zero is where they begin (NaN for a row with a NaN or an infinity).
+    __device__ __forceinline__ void operands(const AttnLaunch &L, kv_h8 (&qf)[N][PARTS][G], float &fac, float &zero) const {
+        if (PARTS == 1 && L.a.type == BGL_T_F16) turn<true>(L, qf, fac, zero);
+        else turn<false>(L, qf, fac, zero);
+    }
+    template <bool F16>
+    __device__ __forceinline__ void turn(const AttnLaunch &L, kv_h8 (&qf)[N][PARTS][G], float &fac, float &zero) const {
+        uint32_t top = 0;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int j = 0; j < G; j++)
+#pragma unroll
+                for (int y = 0; y < 8; y++) top = max(top, __float_as_uint(value(n, j, y, F16)) & 0x7fffffffu);
+        top = min(top, 0x7f800000u);                                                   // NaN counts as an infinity
+        if constexpr (WIDE) {
+            auto a = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max((uint32_t)a[0], (uint32_t)a[1]);
+        } else {
+            top = __float_as_uint(at_max4(__uint_as_float(top)));
+        }
+        const bool bad = top >= 0x7f800000u;
+        const int e = bad ? 0 : min(14 - (max((int)(top >> 23), 1) - 127), 126);
+        const float up = __int_as_float((127 + e) << 23) * (L.a.scale < 0.0f ? -1.0f : 1.0f);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int j = 0; j < G; j++)
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const float v = value(n, j, y, F16) * up;
+                    const _Float16 h = (_Float16)v;
+                    qf[n][0][j][y] = h;
+                    if constexpr (PARTS == 2) qf[n][1][j][y] = (_Float16)(v - (float)h);
+                }
+        // (a factor of 0 would make NaN of masked scores)
+        fac = fmaxf(L.scale2 * __int_as_float((127 - e) << 23), 1e-30f);
+        zero = bad ? NAN : 0.0f;
+    }
+};
 // Keys e = 0, 1, .. behind a lane's first, of which a row sees those in [lo, hi]: the score, or -infinity.  (Integer operations on
 // vector registers: comparisons would hold a scalar mask for each key.)
 __device__ __forceinline__ int at_hides(int e, int lo, int hi) { return ((hi - e) | (e - lo)) >> 31; }

@@ -8,7 +8,7 @@
 //   output   O^T = V^T P^T: what a lane has of S^T is, as weights, its part of P^T's operand: nothing is moved between lanes
 // but the row maxima; a row's statistics lie in the lanes that hold its sums.
 //
-// Work: 128 keys of one head and row block are a unit, 32 for each wave.  The units of all sequences lie in one line that
+// Work: 128 keys of one head and row block are a unit, 32 for each wave (or 512, where no sequence has more).  The units of all sequences lie in one line that
 // is cut into equal runs, one a workgroup, so a batch of very different lengths leaves no workgroup behind.  A head whose
 // keys end up in several runs is joined by whichever of them finishes last, in the order of its keys: the same bits every time.
 #include <string.h>
@@ -25,7 +25,7 @@
         if (e_ != hipSuccess) return bgl_fail(BGL_E_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
     } while (0)
 
-#define AT_UNIT 128              // keys a unit
+#define AT_STEP 128              // keys that the four waves of a workgroup go over at once
 #define AT_WG 768                // workgroups at most
 #define AT_FEW 32                // rows of a head's group that a sequence of few rows has, at most
 #define AT_SC1 16                // the cache-policy bit of a buffer access of device scope
@@ -47,6 +47,7 @@ struct AttnWave {
     int head;
     ucint table;
     const AtMagic magic;
+    AtQuery<G, PARTS> query[NT];
     kv_h8 qf[NT][1][PARTS][G];
     float fac[NT], zero[NT];                             // zero: where scores begin; NaN for a query with a NaN or an infinity
     int lo[NT], hi[NT], lo_max, hi_min;
@@ -56,14 +57,19 @@ struct AttnWave {
 
     __device__ AttnWave(const AttnLaunch &l_) : L(l_), lane(threadIdx.x & 63), col(threadIdx.x & 15), b((threadIdx.x >> 4) & 3) {}
 
-    // Rows rb * RB .. of the sequence's n * g.
+    // Rows rb * RB .. of the sequence's n * g: their loads, then their operands.
+    __device__ __forceinline__ void ask(int rb) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) query[t].load(L, q, head, rb * RB + 16 * t + col, b);
+    }
     __device__ __forceinline__ void begin(int rb) {
         lo_max = 0;
         hi_min = INT32_MAX;
         nan = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            at_query<G, PARTS>(L, q, head, rb * RB + 16 * t + col, b, qf[t], fac[t], zero[t], lo[t], hi[t]);
+            query[t].operands(L, qf[t], fac[t], zero[t]);
+            attn_keys(L, q, min(rb * RB + 16 * t + col, q.n * L.g - 1) / L.g, lo[t], hi[t]);
             lo_max = max(lo_max, lo[t]);
             hi_min = min(hi_min, hi[t]);
             m[t] = -INFINITY;
@@ -217,7 +223,7 @@ struct AttnShared {
 template <int RB>
 __device__ __forceinline__ void attn_units(const AttnLaunch &L, const AttnSeq &q, int &blocks, int &chunks) {
     blocks = q.n > 0 && (long)q.n * L.g <= L.limit ? (q.n * L.g + RB - 1) / RB : 0;
-    chunks = max(1, (q.len - (q.lo & ~15) + AT_UNIT - 1) / AT_UNIT);
+    chunks = max(1, (q.len - (q.lo & ~15) + L.unit - 1) / L.unit);
 }
 
 // Sums of lanes 0 .. l.
@@ -301,11 +307,14 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
         W.head = head;
         W.table = uni(L.a.table + (size_t)s * L.a.ldt);
         AttnRaw<G> raw;
-        int left = 0, key = (W.q.lo & ~15) + wave * 32 + c0 * AT_UNIT;                 // left: units in which the wave has keys
-        if (key < W.q.len) left = min(c1 - c0, (W.q.len - key + AT_UNIT - 1) / AT_UNIT);
+        W.ask(rb);
+        // the wave's 32 keys of each step, up to the segment's end
+        const int stop = min(W.q.len, (W.q.lo & ~15) + c1 * L.unit);
+        int key = (W.q.lo & ~15) + wave * 32 + c0 * L.unit;
+        const int key_first = key;
         int pg[2] = {W.entry(key), W.entry(key + 16)};
-        int pn[2] = {W.entry(key + AT_UNIT), W.entry(key + AT_UNIT + 16)};             // the table's entries, a unit ahead of its loads
-        if (left) {
+        int pn[2] = {W.entry(key + AT_STEP), W.entry(key + AT_STEP + 16)};             // the table's entries, a step ahead of its loads
+        if (key < stop) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint8_t *p = W.record(key + 16 * h, pg[h]);
@@ -315,19 +324,19 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
         }
         W.begin(rb);
 #pragma clang loop unroll(disable)
-        for (; left; left--, key += AT_UNIT) {           // the next unit is on its way while one is worked on
+        for (; key < stop; key += AT_STEP) {             // the next step's keys are on their way while one's are worked on
             const uint8_t *next[2] = {nullptr, nullptr};
-            if (left > 1) {
-                next[0] = W.record(key + AT_UNIT, pn[0]);
-                next[1] = W.record(key + AT_UNIT + 16, pn[1]);
+            if (key + AT_STEP < stop) {
+                next[0] = W.record(key + AT_STEP, pn[0]);
+                next[1] = W.record(key + AT_STEP + 16, pn[1]);
             }
-            const int p2[2] = {W.entry(key + 2 * AT_UNIT), W.entry(key + 2 * AT_UNIT + 16)};
+            const int p2[2] = {W.entry(key + 2 * AT_STEP), W.entry(key + 2 * AT_STEP + 16)};
             W.step(raw, key, pg, next);
 #pragma unroll
             for (int h = 0; h < 2; h++) { pg[h] = pn[h]; pn[h] = p2[h]; }
         }
         if (__any(W.nan))
-            for (int k = (W.q.lo & ~15) + wave * 32 + c0 * AT_UNIT; k < key; k += AT_UNIT) at_nan<G, NT>(L, W.q, head, W.table, k, lane, W.lo, W.hi, W.o);
+            for (int k = key_first; k < key; k += AT_STEP) at_nan<G, NT>(L, W.q, head, W.table, k, lane, W.lo, W.hi, W.o);
         const int rows = min(RB, W.q.n * L.g - rb * RB);
         auto put = [&](int r, int d, kv_f4 v) {          // 4 values of a row into out, over the row's sum of weights
             const int i = (rb * RB + r) / L.g, h = (rb * RB + r) - i * L.g;
@@ -514,7 +523,7 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (a->q == a->out) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: out is q");
     if ((long)a->T * (a->nq / kv->heads) > INT32_MAX / 2) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of %d heads", a->T, a->nq);
     // units are counted in 32 bits
-    if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_UNIT + 2) > 2e9)
+    if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_STEP + 2) > 2e9)
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows over %d pages of %d tokens", a->T, a->ldt, kv->page);
     HIPCHK(hipSetDevice(c->device));
     AttnLaunch L;
@@ -546,7 +555,9 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (const int rc = dbuf_reserve(c, c->attn_sync, 3 * AT_WG * sizeof(int), true)) return rc;
     L.part = (float *)c->attn_part.p;
     L.sync = (int *)c->attn_sync.p;
-    const long units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * (((long)std::max(1, a->max_len) + AT_UNIT - 1) / AT_UNIT);
+    // Up to four steps stay together: a head whose keys are one unit needs no join (8 heads over 512 keys: 10.4 us in units of 128).
+    L.unit = a->max_len <= 4 * AT_STEP ? 4 * AT_STEP : AT_STEP;
+    const long units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * (((long)std::max(1, a->max_len) + L.unit - 1) / L.unit);
     const unsigned wgs = (unsigned)std::min<long>(AT_WG, std::max<long>(1, units));
     const int tok = prof_begin(c, 1);
     switch (G) {

@@ -217,8 +217,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         float fac, zero, m = -INFINITY;
         int lo, hi;
         {
+            AtQuery<G, PARTS, true> query;
+            query.load(L, q, it.head, row0 + (lane & 31), h);
+            attn_keys(L, q, min(row0 + (lane & 31), rows - 1) / L.g, lo, hi);
             kv_h8 part[2][PARTS][G];                     // of the lane's values 8 G (2 x + h) ..
-            at_query<G, PARTS, true>(L, q, it.head, row0 + (lane & 31), h, part, fac, zero, lo, hi);
+            query.operands(L, part, fac, zero);
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
