@@ -121,3 +121,36 @@ def attention(q, k, v, scale, seen, sink):
     p = np.where(total > 0, p / np.where(total > 0, total, 1), 0)
     v = v.astype(np.float64)
     return p @ v, p @ np.abs(v), np.where(seen, np.abs(s), 0).max(-1, initial=0)
+
+
+def attention_near(out, q, k, v, scale, seen, sink, kind, name):
+    """out [n][D] of one head, from rows q of type `kind` over the cache's values k, v [L][D], is attention within the kernel's
+    roundings (all relative):
+      scores   q is exact as an operand (two parts of it hold 2^-22 for fp32 rows), D products are summed in fp32, and the sum is scaled
+               and shifted: A (2 D + 32) 2^-24 + A 2^-22 (fp32 rows), A the largest sum |q_i k_i| scale that the row sees; both the weight and the
+               sum of weights follow it: twice that.  A merge of partial sums shifts by the maximum once more, which the 32 holds.
+      weights  fp16: 2^-11, two parts: 2^-22; exp2 itself 2^-22.  A weight below 2^-22 of the largest is off by at
+               most 2^-33 of it (weights are 2^8 exp2(s - m) with m at most 7 below the largest score, and fp16 errs by 2^-25 below 2^-14).
+      sums     32 products in a matrix instruction and L / 32 instructions and joins, each at most 2^-23.
+      output   half a step of its type.
+    All but the last multiply sum p |v|.  NaN is where the formula has it: a row that sees a NaN among its keys or in itself, and the
+    values that see one among V's."""
+    D, n = q.shape[-1], len(k)
+    out, q = out.astype(np.float64), q.astype(np.float64)
+    k, v = k.astype(np.float64), v.astype(np.float64)
+    parts = kind == "float32"
+    lost = (seen & ~np.isfinite(k).all(-1)[None]).any(-1) | (~np.isfinite(q).all(-1) & seen.any(-1))
+    nan = lost[:, None] | ((seen[:, :, None] & ~np.isfinite(v)[None]).any(1) if not np.isfinite(v).all() else False)
+    assert np.array_equal(np.isnan(out), np.broadcast_to(nan, out.shape)), (name, "NaN")
+    kk, vv, x = np.where(np.isfinite(k), k, 0), np.where(np.isfinite(v), v, 0), np.where(np.isfinite(q), q, 0)
+    want, weight, _ = attention(x, kk, vv, scale, seen, sink)
+    A = np.where(seen, np.abs(x) @ np.abs(kk).T, 0).max(-1, initial=0) * abs(scale)
+    if sink is not None:
+        A = np.maximum(A, abs(float(sink)))
+    ds = A * ((2 * D + 32) * 2.0 ** -24 + (2.0 ** -22 if parts else 0))
+    rel = (2.0 ** -22 if parts else 2.0 ** -11) + 2.0 ** -21 + 2 * ds + (32 + n / 32 + 800) * 2.0 ** -23
+    tol = rel[:, None] * weight + n * 2.0 ** -33 * np.abs(vv).max(initial=0)
+    tol = tol * (1 + HALF[kind]) + HALF[kind] * np.abs(want) + LEAST[kind] + 1e-30
+    off = np.where(nan, 0, np.abs(out - want) - tol)[~lost]
+    worst = off.max(initial=-1.0)
+    assert worst <= 0, (name, worst, np.argwhere(off > 0)[:3])

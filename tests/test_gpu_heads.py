@@ -162,6 +162,60 @@ def test_heads_of_extreme_rows(torch_dev, ctx):
     ctx.heads(x, None, torch.empty_like(x), None, norm=2, eps=1e-6)
 
 
+def test_heads_of_extreme_16_bit_rows(torch_dev, ctx):
+    """Rows whose squares leave fp32's range, beside ones that do not, through fp32 arithmetic."""
+    torch = torch_dev
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((9, 3, 128)).astype(np.float32)
+    x[1] *= 1e38
+    x[2, 1] *= 1e20
+    x[3] *= 1e-30
+    x[4] = 0
+    x[5, 0, 7] = np.inf
+    x[6, 2, 100] = np.nan
+    x[7] = 3e38
+    q = torch.from_numpy(x).cuda().bfloat16()
+    q[8] = float("-inf")
+    rope, pos = rope_table(rng, 16, 128), np.arange(9, dtype=np.int32)
+    y = torch.empty_like(q)
+    w = (1 + 0.1 * rng.standard_normal(128)).astype(np.float32)
+    ctx.heads(q, None, y, None, norm=1, q_w=torch.from_numpy(w).cuda(), eps=1e-6, rope=torch.from_numpy(rope).cuda(), pos=torch.from_numpy(pos).cuda())
+    torch.cuda.synchronize()
+    fine = np.isfinite(host(q)).all(-1)
+    with np.errstate(invalid="ignore"):
+        want = F.heads(host(q), 1, w, 1e-6, 0.0, rope, pos, 128, 1)
+    assert not np.isfinite(host(y)[~fine]).all(-1).any()
+    near(y[torch.from_numpy(fine).cuda()], want[fine], "finite rows")
+
+
+def test_more_tokens_than_a_launch_takes(torch_dev, ctx):
+    """2^20 tokens and some: launches of one call, and their slots and positions."""
+    torch = torch_dev
+    T, D, page, n = (1 << 20) + 37, 64, 256, 70
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn((T, 1, D), generator=gen, device="cuda").half() for _ in range(2))
+    rope = torch.from_numpy(rope_table(np.random.default_rng(0), 512, D)).cuda()
+    pos = (torch.arange(T, device="cuda") % 512).int()
+    pages = T // page + 2
+    slots = (torch.arange(T, device="cuda") + 3).int()
+    whole, last = cache_of(torch, pages, page, 1, D), cache_of(torch, pages, page, 1, D)
+    q, q2 = torch.empty_like(k), torch.empty_like(k)
+    ctx.kv_append(whole, slots, k, v, q=k, q_out=q, norm=1, rope=rope, pos=pos)
+    ctx.kv_append(last, slots[-n:], k[-n:], v[-n:], q=k[-n:], q_out=q2[-n:], norm=1, rope=rope, pos=pos[-n:])
+    got = [torch.empty((T, 1, D), device="cuda") for _ in range(2)]
+    ctx.kv_read(whole, slots, *got)
+    few = [torch.empty((n, 1, D), device="cuda") for _ in range(2)]
+    ctx.kv_read(last, slots[-n:], *few)
+    ctx.heads(k, None, q2, None, norm=1, rope=rope, pos=pos)
+    torch.cuda.synchronize()
+    assert torch.equal(q, q2)
+    for a, b in zip(got, few):
+        assert torch.equal(a[-n:], b)
+    assert torch.isfinite(got[0]).all() and torch.isfinite(got[1]).all()
+    for at in (0, 1 << 19, (1 << 20) - 1, 1 << 20):
+        assert np.array_equal(got[1][at].half().cpu().numpy(), F.kept(host(v[at])))
+
+
 def cache_of(torch, pages, page, heads, D, fill=0xA5):
     import beglin_amd
     c = beglin_amd.KVCache(pages, page, heads, D)
@@ -179,6 +233,8 @@ APPEND = [  # T, nq, nk, D, type, q out, norm, style, page, layout, first place
     (333, 8, 1, 256, "f16", "f16", 1, 1, 16, "odd", 9),
     (1001, 10, 5, 64, "f32", "f16", 0, 0, 256, "part", 1),
     (1200, 0, 4, 128, "f32", "f32", 0, 0, 128, "heads", 4),
+    (600, 32, 2, 128, "bf16", "bf16", 1, 1, 64, "part", 7),                        # queries enough for a launch of their own
+    (1500, 12, 3, 64, "f16", "bf16", 0, 2, 16, "odd", 1),
 ]
 
 
