@@ -273,15 +273,14 @@ __device__ __forceinline__ void at_nan(const AttnLaunch &L, const AttnSeq &q, in
 }
 
 // ------------------------------------------------------------------ a row's end
-// What the sum of values (weights 2^14 exp2(s - M)) is multiplied by: 1 / (their sum + the sink's weight); 0 for a row without a key.
+// What the sum of values (weights 2^8 exp2(s - M)) is multiplied by: 1 / (their sum + the sink's weight); 0 for a row without a key.
 __device__ __forceinline__ float attn_factor(float M, float sum, bool sink, float sink2) {
     if (!sink) return M == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
     const float top = fmaxf(M, sink2);
     if (top == -INFINITY && sum == 0.0f) return 0.0f;
     const float f = M == -INFINITY ? 0.0f : at_exp2(M - top);
-    return f / (sum * f + at_exp2(sink2 - top + AT_P2));
+    return f / (sum * f + (sink2 == INFINITY ? INFINITY : at_exp2(sink2 - top + AT_P2)));
 }
-
 
 // The prompt kernel (bgl_attn_p.hip): the call's sequences with more than L.limit rows times g, L.limit < INT32_MAX; max_rows and
 // max_len as the caller gave them.

@@ -262,12 +262,15 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
     AttnSeq mine_q;
     mine_q.begin = mine_q.n = mine_q.len = mine_q.lo = 0;
     int mine = 0;
+    bool back = false;                                   // starts go back: the units could be more than the host has checked for
     for (int s = lane * per; s < min(S, (lane + 1) * per); s++) {
         int blocks, chunks;
         mine_q = attn_seq(L, s);
         attn_units<RB>(L, mine_q, blocks, chunks);
         mine += blocks * heads * chunks;
+        back |= min(L.a.start[s + 1], L.a.T) < mine_q.begin;
     }
+    if (__any(back)) return;
     const int upto = at_scan(mine);                      // units before the next lane's sequences
     const __amdgpu_buffer_rsrc_t pieces = __builtin_amdgcn_make_buffer_rsrc(L.part, (short)0, AT_WG * 2 * PIECE * 4, 0x00020000);
     const AttnRuns runs((uint32_t)__builtin_amdgcn_readlane(upto, 63), gridDim.x);
@@ -502,13 +505,6 @@ static void attn_pick(bgl_ctx *c, const AttnLaunch &L, int nt, unsigned wgs) {
     else attn_go<G, 1, 1>(c, L, wgs);
 }
 
-static bool rows_ok(long ld, long hd, long n, long heads, long D) {
-    if (ld < 0 || hd < 0) return false;
-    if (n == 1) return heads == 1 || hd >= D;
-    if (heads == 1) return ld >= D;
-    return (hd >= D && ld >= (heads - 1) * hd + D) || (ld >= D && hd >= (n - 1) * ld + D);
-}
-
 extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (!c || !a || !a->q || !a->out || !a->start || !a->len || !a->table) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: NULL argument");
     if (const int rc = kv_check("bgl_attn_dev", kv)) return rc;
@@ -516,14 +512,15 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (a->nq < 1 || a->nq > 65535 || a->nq % kv->heads)
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: nq=%d heads over a cache of %d", a->nq, kv->heads);
     if (a->type != BGL_T_F32 && a->type != BGL_T_F16 && a->type != BGL_T_BF16) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: unknown element type");
-    if (!rows_ok(a->ldq, a->hdq, a->T, a->nq, kv->D) || !rows_ok(a->ldo, a->hdo, a->T, a->nq, kv->D))
+    if (!kv_rows_ok(a->ldq, a->hdq, a->T, a->nq, kv->D) || !kv_rows_ok(a->ldo, a->hdo, a->T, a->nq, kv->D))
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: rows of D=%d values overlap at these strides", kv->D);
     if (a->window < 0 || (a->window && !a->causal)) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: window=%d (at least 0, and with causal)", a->window);
     if (a->max_rows < 0 || a->max_len < 0) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: max_rows=%d max_len=%d", a->max_rows, a->max_len);
     if (!(a->scale == a->scale) || a->scale - a->scale != 0.0f) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: scale is not finite");
     if (a->q == a->out) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: out is q");
     if ((long)a->T * (a->nq / kv->heads) > INT32_MAX / 2) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of %d heads", a->T, a->nq);
-    // units are counted in 32 bits
+    // keys are numbered, and units counted, in 32 bits
+    if ((long)a->ldt * kv->page > 1l << 30) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d pages of %d tokens a sequence", a->ldt, kv->page);
     if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_STEP + 2) > 2e9)
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows over %d pages of %d tokens", a->T, a->ldt, kv->page);
     HIPCHK(hipSetDevice(c->device));

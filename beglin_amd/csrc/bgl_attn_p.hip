@@ -418,12 +418,13 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
     memset(&P, 0, sizeof P);
     P.A = L;
     const long rows = (long)std::min(std::max(1, L.a.max_rows), L.a.T) * L.g;
-    P.blocks = (int)((rows + RB - 1) / RB);
+    const long most = std::max(1l, (1l << 22) / ((long)L.a.S * L.c.heads));             // a launch has less than 2^32 threads
+    P.blocks = (int)std::min(most, (rows + RB - 1) / RB);
     const long items = (long)P.blocks * L.a.S * L.c.heads;
     // few blocks: their keys in parts, of 256 keys at least
     const int at_once = 256;
     P.parts = (int)std::max<long>(1, std::min<long>({16, at_once / std::max(1l, items), ((long)std::max(1, L.a.max_len) + 255) / 256}));
-    if (items * P.parts > INT32_MAX / 4) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d sequences of up to %d rows", L.a.S, L.a.max_rows);
+    if (items > 1l << 22) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: prompts of S=%d sequences over %d heads", L.a.S, L.c.heads);
     if (P.parts > 1) {
         if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)items * P.parts * RB * (D + 2) * 4, false)) return rc;
         P.A.part = (float *)c->attn_part.p;

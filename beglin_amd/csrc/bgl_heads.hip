@@ -371,7 +371,7 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
             const bool q_fast = all.nq && hd_fast(d), k_fast = all.nk && d.k_out && hd_fast(d), exact = all.nv || (all.nq && !q_fast) || (all.nk && !k_fast);
             if (!exact) go(k_heads<GL, true, false>, all.nq, all.nk, 0);
             else if (!q_fast) go(k_heads<GL, false, true>, all.nq, all.nk, all.nv);
-            else if (a.T * all.nq < HD_MANY) go(k_heads<GL, true, true>, all.nq, all.nk, all.nv);
+            else if ((long)a.T * all.nq < HD_MANY) go(k_heads<GL, true, true>, all.nq, all.nk, all.nv);
             else {
                 go(k_heads<GL, true, false>, all.nq, 0, 0);
                 go(k_heads<GL, false, true>, 0, all.nk, all.nv);
@@ -383,8 +383,7 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
     return 0;
 }
 
-// Rows [n][heads][D] at a pointer: tokens ld apart and heads hd, both at least one row of what they step over, in either order.
-static bool rows_ok(long ld, long hd, long n, long heads, long D) {
+bool kv_rows_ok(long ld, long hd, long n, long heads, long D) {
     if (ld < 0 || hd < 0) return false;
     if (n == 1) return heads == 1 || hd >= D;
     if (heads == 1) return ld >= D;
@@ -422,9 +421,9 @@ static int heads_check(const char *who, const bgl_heads *d) {
     if ((d->q != nullptr) != (d->q_out != nullptr)) return bgl_fail(BGL_E_ARG, "%s: q and q_out go together", who);
     if (d->q && (d->nq < 1 || d->nq > 65535)) return bgl_fail(BGL_E_ARG, "%s: nq=%d", who, d->nq);
     if (d->k && (d->nk < 1 || d->nk > 65535)) return bgl_fail(BGL_E_ARG, "%s: nk=%d", who, d->nk);
-    if ((d->q && (!rows_ok(d->ldq, d->hdq, d->T, d->nq, d->D) || !rows_ok(d->ldqo, d->hdqo, d->T, d->nq, d->D))) ||
-        (d->k && !rows_ok(d->ldk, d->hdk, d->T, d->nk, d->D)) || (d->k_out && !rows_ok(d->ldko, d->hdko, d->T, d->nk, d->D)) ||
-        (d->v && !rows_ok(d->ldv, d->hdv, d->T, d->nk, d->D)))
+    if ((d->q && (!kv_rows_ok(d->ldq, d->hdq, d->T, d->nq, d->D) || !kv_rows_ok(d->ldqo, d->hdqo, d->T, d->nq, d->D))) ||
+        (d->k && !kv_rows_ok(d->ldk, d->hdk, d->T, d->nk, d->D)) || (d->k_out && !kv_rows_ok(d->ldko, d->hdko, d->T, d->nk, d->D)) ||
+        (d->v && !kv_rows_ok(d->ldv, d->hdv, d->T, d->nk, d->D)))
         return bgl_fail(BGL_E_ARG, "%s: rows of D=%d values overlap at these strides", who, d->D);
     if (d->q && d->q == d->q_out && (d->type != d->out_type || d->ldq != d->ldqo || d->hdq != d->hdqo))
         return bgl_fail(BGL_E_ARG, "%s: q_out is q with another type or stride", who);
@@ -474,7 +473,7 @@ extern "C" int bgl_kv_read_dev(bgl_ctx *c, const bgl_kv *kv, const int32_t *slot
     if (const int rc = kv_check("bgl_kv_read_dev", kv)) return rc;
     if (n < 1) return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: n=%d", n);
     if (!type_ok(type)) return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: unknown element type");
-    if ((k && !rows_ok(ldk, hdk, n, kv->heads, kv->D)) || (v && !rows_ok(ldv, hdv, n, kv->heads, kv->D)) || k == v)
+    if ((k && !kv_rows_ok(ldk, hdk, n, kv->heads, kv->D)) || (v && !kv_rows_ok(ldv, hdv, n, kv->heads, kv->D)) || k == v)
         return bgl_fail(BGL_E_ARG, "bgl_kv_read_dev: rows of D=%d values overlap", kv->D);
     HIPCHK(hipSetDevice(c->device));
     const int tok = prof_begin(c, 2);

@@ -77,3 +77,5 @@ __device__ __forceinline__ void kv_store4(void *p, int type, long at, kv_f4 q) {
 }
 // The descriptor's checks (bgl_heads.hip); 0 or an error code.
 int kv_check(const char *who, const bgl_kv *kv);
+// Rows [n][heads][D] at a pointer: tokens ld apart and heads hd, both at least one row of what they step over, in either order.
+bool kv_rows_ok(long ld, long hd, long n, long heads, long D);

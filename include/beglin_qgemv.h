@@ -230,8 +230,8 @@ int  bgl_norm_dev(bgl_ctx *ctx, const bgl_norm *d);
  *     BGL_ROT_HALF   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i   for j = i + rot / 2
  *     BGL_ROT_PAIRS  the same for values 2 i and 2 i + 1
  *     y_d = n_d for d >= rot, and everywhere with BGL_ROT_NONE (rope and pos unused)
- * Values are computed in double and rounded to fp32, then to out_type; those of a 16-bit out_type may be computed in fp32.  q_w, k_w: fp32 [D], NULL: no factor.  rope: fp32 rows of
- * rot values, n_pos of them; a token whose pos lies outside [0, n_pos) is skipped: nothing is written for it.  Value
+ * Values are computed in double and rounded to fp32, then to out_type; those of a 16-bit out_type may be computed in
+ * fp32.  q_w, k_w: fp32 [D], NULL: no factor.  rope: fp32 rows of rot values, n_pos of them; a token whose pos lies outside [0, n_pos) is skipped: nothing is written for it.  Value
  * d of head h of token t lies ld * t + hd * h + d values behind the pointer.  D is a multiple of 8 up to 512, rot of 16
  * (HALF) or 8 (PAIRS).  q_out may be q, and k_out k, with the same type and strides; apart from that what is written
  * overlaps nothing that is read.  bgl_heads_dev: q with q_out, k with k_out, or both; v is not used. */
@@ -280,13 +280,15 @@ int  bgl_kv_read_dev(bgl_ctx *ctx, const bgl_kv *kv, const int32_t *slots, int n
  *     causal == 0 or j <= len[s] - n + i;   window == 0 or j > len[s] - n + i - window;   the key's page id is in [0, pages)
  *     out = sum_j exp(scale q.k_j) v_j / (sum_j exp(scale q.k_j) + exp(sink[h]))
  * for head h of nq, which reads head h / (nq / heads) of the cache; sink NULL: without that term.  A row that sees no key
- * becomes 0; rows of no sequence are left as they are.  Sums, maxima and products' accumulators are fp32; with fp16 and
- * bf16 rows the weights exp(..) are rounded to fp16 before they multiply v (queries and cached values are exact as
- * operands), with fp32 rows they and the queries are held as two fp16 parts each, 22 bits.  The keys j >= ldt * page do not exist.
+ * becomes 0; rows of no sequence are left as they are.  out overlaps nothing that is read.  Keys j >= ldt * page do not
+ * exist (ldt * page is 2^30 at most).  start never goes back: a call where it does writes some rows or none.
+ * Sums, maxima and products' accumulators are fp32.  With fp16 and bf16 rows the weights exp(..) are rounded to fp16
+ * before they multiply v (queries and cached values are exact as operands); with fp32 rows they and the queries are held
+ * as two fp16 parts each, 22 bits.
  * max_rows and max_len: the most rows and keys of a sequence as far as the caller knows; launch shapes go by them, no
  * result needs them to be right.  Rows of one sequence are summed in an order that its lengths and the batch's give:
- * the same call gives the same bits.  The first call reserves the context's scratch for partial sums, which graphs captured from
- * one context share: replay them one after the other. */
+ * the same call gives the same bits.  The first call reserves the context's scratch for partial sums (one with many rows
+ * may have to grow it), which the context's calls and the graphs captured from it share: let them run one after the other. */
 typedef struct {
     int S, T, nq;                                  /* sequences; rows of q and out; heads of q, a multiple of the cache's */
     const void *q; long ldq, hdq;

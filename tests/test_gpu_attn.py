@@ -286,6 +286,55 @@ def test_bad_starts_and_lengths_stay_in_bounds(torch_dev, ctx):
     assert np.array_equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("hint", [None, 1])
+def test_starts_that_go_back_stay_in_bounds(torch_dev, ctx, hint):
+    torch = torch_dev
+    b = Batch(torch, ctx, [(9, 40), (5, 50), (20, 300)], 4, 1, 64, "f16", 16)
+    b.start_d.copy_(torch.tensor([0, 30, 4, 34], dtype=torch.int32))
+    got = b.run(ctx, max_rows=hint)
+    assert (got[b.T:] == 7.0).all()
+    b.start_d.copy_(torch.from_numpy(b.start))
+    b.check(b.run(ctx, max_rows=hint))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_sinks_without_end(torch_dev, ctx, rows):
+    """exp(sink) of infinity leaves a row 0, of -infinity as it is without one, NaN makes NaN."""
+    b = Batch(torch_dev, ctx, [(rows, 100), (rows, 3000), (rows, 0)], 4, 2, 64, "bf16", 16)
+    want = b.run(ctx).copy()
+    b.sink[:] = np.array([np.inf, -np.inf, 3e38, np.nan], np.float32)
+    got = b.run(ctx, sink=True)[:b.T]
+    assert (got[:, 0] == 0).all() and (got[:, 2] == 0).all()
+    assert np.array_equal(got[:, 1], want[:b.T, 1])
+    assert np.isnan(got[:2 * rows, 3]).all() and (got[2 * rows:, 3] == 0).all()      # a row without a key is 0 whatever the sink
+
+
+def test_a_prompt_among_many_sequences(torch_dev, ctx):
+    """More blocks of rows than a launch takes: a workgroup goes over several."""
+    torch = torch_dev
+    import beglin_amd
+    nq, nk, D, page, n, S = 32, 8, 64, 64, 36000, 2001
+    cache = beglin_amd.KVCache(n // page + 1, page, nk, D)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn((n, nk, D), generator=gen, device="cuda") for _ in range(2))
+    ctx.kv_append(cache, torch.arange(n, dtype=torch.int32, device="cuda"), k, v)
+    q = torch.randn((n + S - 1, nq, D), generator=gen, device="cuda").half()
+    pages = torch.arange(cache.pages, dtype=torch.int32, device="cuda")
+    out, one = torch.full_like(q, 7.0), torch.full_like(q[:n], 7.0)
+    start = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    start[S] = n + S - 1
+    lens = 1 + start[1:] % 16
+    lens[S - 1] = n
+    ctx.attention(cache, q, out, start, lens, pages[None].repeat(S, 1))
+    ctx.attention(cache, q[S - 1:], one, torch.tensor([0, n], dtype=torch.int32, device="cuda"), lens[S - 1:].contiguous(), pages[None])
+    few = torch.empty_like(q[:S - 1])
+    ctx.attention(cache, q[:S - 1], few, start[:S].contiguous(), lens[:S - 1].contiguous(), pages[None, :1].repeat(S - 1, 1), max_rows=1)
+    torch.cuda.synchronize()
+    assert torch.equal(out[S - 1:], one)
+    apart = np.abs(host(out[:S - 1]) - host(few)).max()
+    assert apart <= 2 ** -9 * np.abs(host(v[:16])).max()                           # two results, each off by a rounding of weights and one of the output
+
+
 def test_cache_past_4_gib(torch_dev, ctx):
     """Pages whose records lie further than 2^32 bytes behind the first, and q rows that do."""
     import beglin_amd
