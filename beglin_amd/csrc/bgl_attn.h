@@ -129,6 +129,15 @@ __device__ __forceinline__ int pr_min32(int v) {
     v = min(v, dpp_i<0x140>(v));
     return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
+// Sums of lanes 0 .. l.
+__device__ __forceinline__ int at_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);                  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);                  // lane 15 of rows 0 and 2 to rows 1 and 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);            // lane 31 to rows 2 and 3
+}
 // The page of the 16-token tile t of a sequence.
 __device__ __forceinline__ int at_page(const AttnLaunch &L, int t) { return (int)(__umulhi((uint32_t)t, L.div_mul) + (uint32_t)t) >> L.div_shift; }
 
@@ -282,6 +291,5 @@ __device__ __forceinline__ float attn_factor(float M, float sum, bool sink, floa
     return f / (sum * f + (sink2 == INFINITY ? INFINITY : at_exp2(sink2 - top + AT_P2)));
 }
 
-// The prompt kernel (bgl_attn_p.hip): the call's sequences with more than L.limit rows times g, L.limit < INT32_MAX; max_rows and
-// max_len as the caller gave them.
+// The prompt kernel (bgl_attn_p.hip): the call's sequences with more than L.limit rows times g, L.limit < INT32_MAX.
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L);

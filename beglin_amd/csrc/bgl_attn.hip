@@ -226,16 +226,6 @@ __device__ __forceinline__ void attn_units(const AttnLaunch &L, const AttnSeq &q
     chunks = max(1, (q.len - (q.lo & ~15) + L.unit - 1) / L.unit);
 }
 
-// Sums of lanes 0 .. l.
-__device__ __forceinline__ int at_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);                  // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);                  // lane 15 of rows 0 and 2 to rows 1 and 3
-    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);            // lane 31 to rows 2 and 3
-}
-
 // The line of units in runs: the first `more` workgroups have one unit more than the others' `each`.
 struct AttnRuns {
     uint32_t each, more, wgs;
@@ -523,19 +513,22 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if ((long)a->ldt * kv->page > 1l << 30) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d pages of %d tokens a sequence", a->ldt, kv->page);
     if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_STEP + 2) > 2e9)
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows over %d pages of %d tokens", a->T, a->ldt, kv->page);
+    const int g = a->nq / kv->heads;
+    int rows = (int)std::min<long>((long)std::min(std::max(1, a->max_rows), a->T) * g, INT32_MAX);
+    if (rows > AT_FEW && ((double)a->T * g / 128 + a->S) * kv->heads > 1 << 22)        // a launch has less than 2^32 threads
+        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: prompts of T=%d rows of %d heads", a->T, a->nq);
     HIPCHK(hipSetDevice(c->device));
     AttnLaunch L;
     memset(&L, 0, sizeof L);
     L.c = *kv;
     L.a = *a;
-    L.g = a->nq / kv->heads;
+    L.g = g;
     L.ppt = kv->page / KV_TILE;
     while ((1 << L.div_shift) < L.ppt) L.div_shift++;
     L.div_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << L.div_shift) - (uint32_t)L.ppt)) / L.ppt + 1);
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
     const int G = kv->D / 32;
-    int rows = (int)std::min<long>((long)std::min(std::max(1, a->max_rows), a->T) * L.g, INT32_MAX);
     // Many rows of a head at once are the prompt kernel's, where they are told of; beside them sequences of few rows stay here.
     const bool prompt = rows > AT_FEW;
     if (prompt) {

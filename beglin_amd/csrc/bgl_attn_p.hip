@@ -23,27 +23,56 @@
 
 struct PromptLaunch {
     AttnLaunch A;
-    int blocks;                  // row blocks a sequence and head in the grid; a workgroup takes every blocks-th from its first
     int parts;                   // parts that a block's keys are split into; more than one: pieces in A.part, joined by k_attn_join
 };
-// A piece of an item (block, sequence, head) and part: out's sums [RB][D], then the rows' m and their sums of weights.
+// A piece of an item (a block of RB rows and a head) and part: out's sums [RB][D], then the rows' m and their sums of weights.
 template <int D, int RB>
-__device__ __forceinline__ float *prompt_piece(const PromptLaunch &P, long item, int part) {
-    return P.A.part + (item * P.parts + part) * (long)(RB * (D + 2));
+__device__ __forceinline__ float *prompt_piece(const PromptLaunch &P, uint32_t item, int part) {
+    return P.A.part + ((size_t)item * P.parts + part) * (RB * (D + 2));
 }
-// Workgroup -> head (neighbouring workgroups, and with 8 heads a head an XCD, whose L2 holds its keys), part, sequence, and block from the last,
-// which sees the most keys, to the first.
-struct PromptItem {
-    int head, part, s, block;
-    long item;
-    __device__ PromptItem(const PromptLaunch &P, long x) {
-        head = (int)(x % P.A.c.heads); x /= P.A.c.heads;
-        part = (int)(x % P.parts); x /= P.parts;
-        s = (int)(x % P.A.a.S); x /= P.A.a.S;
-        block = P.blocks - 1 - (int)x;
-        item = ((long)block * P.A.a.S + s) * P.A.c.heads + head;
-    }
+// The blocks of all sequences lie in one line, a sequence's from the last, which sees the most keys, to the first: block x of the line, or
+// false behind its end.  Every wave counts them by itself, lane by lane, each lane (S + 63) / 64 sequences.
+struct PromptBlock {
+    int s, block;
+    AttnSeq q;
 };
+template <int RB>
+__device__ __forceinline__ bool prompt_block(const AttnLaunch &L, uint32_t x, PromptBlock &b) {
+    const int S = L.a.S, per = (S + 63) / 64, lane = threadIdx.x & 63;
+    auto count = [&](const AttnSeq &q) { return (long)q.n * L.g > L.limit ? (q.n * L.g + RB - 1) / RB : 0; };
+    AttnSeq mine_q;
+    mine_q.begin = mine_q.n = mine_q.len = mine_q.lo = 0;
+    int mine = 0;
+    bool back = false;                                   // starts go back: the blocks could be more than 32 bits count
+    for (int s = lane * per; s < min(S, (lane + 1) * per); s++) {
+        mine_q = attn_seq(L, s);
+        mine += count(mine_q);
+        back |= min(L.a.start[s + 1], L.a.T) < mine_q.begin;
+    }
+    const int upto = at_scan(mine);
+    if (__any(back) || x >= (uint32_t)__builtin_amdgcn_readlane(upto, 63)) return false;
+    const int at_lane = __popcll(__ballot((uint32_t)upto <= x));
+    int left = (int)x - __builtin_amdgcn_readlane(upto - mine, at_lane);               // blocks between the sequence's first and x
+    b.s = at_lane * per;
+    b.q.begin = __builtin_amdgcn_readlane(mine_q.begin, at_lane);
+    b.q.n = __builtin_amdgcn_readlane(mine_q.n, at_lane);
+    b.q.len = __builtin_amdgcn_readlane(mine_q.len, at_lane);
+    b.q.lo = __builtin_amdgcn_readlane(mine_q.lo, at_lane);
+    if (per > 1) {
+        while (true) {
+            b.q = attn_seq(L, b.s);
+            b.q.begin = __builtin_amdgcn_readfirstlane(b.q.begin);
+            b.q.n = __builtin_amdgcn_readfirstlane(b.q.n);
+            b.q.len = __builtin_amdgcn_readfirstlane(b.q.len);
+            const int n = count(b.q);
+            if (left < n) break;
+            left -= n;
+            b.s++;
+        }
+    }
+    b.block = count(b.q) - 1 - left;
+    return true;
+}
 
 // v_mfma_f32_32x32x16_f16: lane l has 8 values of the sum for row or column l % 32, those of its half h = l / 32; results i = 0 .. 15 are
 // rows 8 (i / 4) + 4 h + i % 4 of column l % 32.
@@ -104,18 +133,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     constexpr int D = T::D, RB = T::RB, ST = T::ST, SN = T::SN, JOBS = 8 / WAVES;
     const AttnLaunch &L = P.A;
     __shared__ typename T::Shared sh;
-    const PromptItem it(P, blockIdx.x);
-    AttnSeq q = attn_seq(L, it.s);
-    q.begin = __builtin_amdgcn_readfirstlane(q.begin);
-    q.n = __builtin_amdgcn_readfirstlane(q.n);
-    q.len = __builtin_amdgcn_readfirstlane(q.len);
-    const int rows = q.n * L.g;
-    if ((long)q.n * L.g <= L.limit) return;              // another kernel's
+    // Workgroup -> head (neighbouring workgroups, and with 8 heads a head an XCD, whose L2 holds its keys), part, block of the line.
+    const uint32_t heads = (uint32_t)L.c.heads, rest = blockIdx.x / heads, line = rest / (uint32_t)P.parts;
+    const int head = (int)(blockIdx.x - rest * heads), part = (int)(rest - line * (uint32_t)P.parts);
+    PromptBlock at;
+    if (!prompt_block<RB>(L, line, at)) return;
+    const AttnSeq &q = at.q;
+    const int rows = q.n * L.g, block = at.block;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, b = lane >> 4, h = lane >> 5;
     const AtMagic magic;
     // In the loop over keys the table is read by vector loads: a scalar load on its way makes every wait for the LDS a wait for all of it.
-    const int *table = L.a.table + (size_t)it.s * L.a.ldt;
+    const int *table = L.a.table + (size_t)at.s * L.a.ldt;
     int zero_lane = 0;
     asm volatile("" : "+v"(zero_lane));
     const int last_page = at_page(L, max(0, q.len - 1) >> 4);
@@ -126,284 +155,281 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     auto steps_at = [&](int job, int x) {                // of the lane's first or last group
         return of_v(job) ? 18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4;
     };
-    for (int block = it.block; block * RB < rows; block += P.blocks) {
-        // the keys of the block's rows, this part's stages of 64 among them
-        int lo_first, lo_last, hi_first, hi_last;
-        attn_keys(L, q, block * RB / L.g, lo_first, hi_first);
-        attn_keys(L, q, (min(block * RB + RB, rows) - 1) / L.g, lo_last, hi_last);
-        const int key0 = lo_first & ~15, stages = max(0, (hi_last + 1 - key0 + ST - 1) / ST);
-        const int parts = block < P.blocks ? P.parts : 1;          // blocks that max_rows did not tell of have no room for pieces
-        if (it.part >= parts) break;
-        const int st0 = __builtin_amdgcn_readfirstlane((int)((long)stages * it.part / parts));
-        const int st1 = __builtin_amdgcn_readfirstlane((int)((long)stages * (it.part + 1) / parts));
+    // the keys of the block's rows, this part's stages of 64 among them
+    int lo_first, lo_last, hi_first, hi_last;
+    attn_keys(L, q, block * RB / L.g, lo_first, hi_first);
+    attn_keys(L, q, (min(block * RB + RB, rows) - 1) / L.g, lo_last, hi_last);
+    const int key0 = lo_first & ~15, stages = max(0, (hi_last + 1 - key0 + ST - 1) / ST);
+    const int st0 = __builtin_amdgcn_readfirstlane((int)((long)stages * part / P.parts));
+    const int st1 = __builtin_amdgcn_readfirstlane((int)((long)stages * (part + 1) / P.parts));
 
-        auto key_of = [&](int stage) { return key0 + stage * ST + 16 * tile; };
-        auto entry = [&](int stage) { return table[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
-        auto page = [&](int stage, int e) {              // the page, or -1: past the keys, or none
-            e = __builtin_amdgcn_readfirstlane(e);
-            return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
-        };
-        uint32_t codes[JOBS][G];
-        typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
-        at_u4 steps[JOBS][SN];
-        // (a tile without a page loads the first record, and none of it counts)
-        auto load = [&](int stage, int pg) {
-            const int t = key_of(stage) >> 4;
-            const size_t rec = pg < 0 ? 0 : ((size_t)pg * L.c.heads + it.head) * L.ppt + (t - at_page(L, t) * L.ppt);
-            const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
+    auto key_of = [&](int stage) { return key0 + stage * ST + 16 * tile; };
+    auto entry = [&](int stage) { return table[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
+    auto page = [&](int stage, int e) {              // the page, or -1: past the keys, or none
+        e = __builtin_amdgcn_readfirstlane(e);
+        return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
+    };
+    uint32_t codes[JOBS][G];
+    typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
+    at_u4 steps[JOBS][SN];
+    // (a tile without a page loads the first record, and none of it counts)
+    auto load = [&](int stage, int pg) {
+        const int t = key_of(stage) >> 4;
+        const size_t rec = pg < 0 ? 0 : ((size_t)pg * L.c.heads + head) * L.ppt + (t - at_page(L, t) * L.ppt);
+        const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
 #pragma unroll
-            for (int job = 0; job < JOBS; job++) {
-                at_dwords<G>(codes[job], p + codes_at(job));
+        for (int job = 0; job < JOBS; job++) {
+            at_dwords<G>(codes[job], p + codes_at(job));
 #pragma unroll
-                for (int x = 0; x < SN; x++) steps[job][x] = *(const u4 *)(p + steps_at(job, x));
-            }
-        };
-        auto convert = [&](int buf, int stage, int pg) {
-#pragma unroll
-            for (int job = 0; job < JOBS; job++) {
-                if (!of_v(job)) {
-#pragma unroll
-                    for (int j = 0; j < G; j++)
-                        sh.k[buf][tile >> 1][(b >> 1) * G + j][(b & 1) * 32 + (tile & 1) * 16 + col] =
-                            at_key(magic, codes[job][j], SN == 2 && (G * b + j) >> 2 != G * b >> 2 ? steps[job][SN - 1][0] : steps[job][0][0]);
-                    continue;
-                }
-                uint32_t flag = pg < 0 ? 2 : 0;
-                if (pg < 0 || key_of(stage) + 16 > q.len) {          // what lies behind the last key may be anything: 0
-                    asm volatile("");
-                    const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;       // of the lane's four keys
-                    const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
-                    const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int x = 0; x < SN; x++) steps[job][x] &= at_u4{e, f, e, f};
-                }
-                // a floor whose exponent is all ones carries into its sign
-                uint32_t ones = 0;
-#pragma unroll
-                for (int x = 0; x < SN; x++)
-#pragma unroll
-                    for (int y = 2; y < 4; y++) ones |= (steps[job][x][y] & 0x7c007c00u) + 0x04000400u;
-                if (__any((ones & 0x80008000u) != 0)) {
-                    asm volatile("");
-                    flag |= 1;
-#pragma unroll
-                    for (int x = 0; x < SN; x++) (void)at_clean(steps[job][x]);
-                }
-#pragma unroll
-                for (int j = 0; j < G; j++) {
-                    const at_u4 z = SN == 2 && G % 3 == 0 && (G * col + j) >> 4 != G * col >> 4 ? steps[job][SN - 1] : steps[job][0];
-                    const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
-                    const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
-                    const uint32_t c = codes[job][j], d = c >> 8;
-                    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        u2 w;
-                        w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
-                        w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
-                        ((u2 *)&sh.v[buf][tile][j][(b & 1) * 32 + 16 * e + col])[b >> 1] = w;
-                    }
-                }
-                if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
-            }
-        };
-
-        int pg = page(st0, entry(st0));
-        load(st0, pg);
-        int next = entry(st0 + 1);
-        // the wave's rows, one a lane (and l ^ 32)
-        const int row0 = block * RB + wave * 32;
-        kv_h8 qf[PARTS][2 * G];
-        float fac, zero, m = -INFINITY;
-        int lo, hi;
-        {
-            AtQuery<G, PARTS, true> query;
-            query.load(L, q, it.head, row0 + (lane & 31), h);
-            attn_keys(L, q, min(row0 + (lane & 31), rows - 1) / L.g, lo, hi);
-            kv_h8 part[2][PARTS][G];                     // of the lane's values 8 G (2 x + h) ..
-            query.operands(L, part, fac, zero);
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                    for (int j = 0; j < G; j++) qf[p][x * G + j] = part[x][p][j];
+            for (int x = 0; x < SN; x++) steps[job][x] = *(const u4 *)(p + steps_at(job, x));
         }
-        pr_f16 o[G], l = pr_all(0.0f);
+    };
+    auto convert = [&](int buf, int stage, int pg) {
 #pragma unroll
-        for (int j = 0; j < G; j++) o[j] = pr_all(0.0f);
-        const int lo_max = -pr_min32(-lo), lo_min = pr_min32(lo), hi_min = pr_min32(hi);
-        const int hi_max = row0 < rows ? -pr_min32(-hi) : -1;      // (a wave without rows has nothing to do)
-        const kv_h8 ones = at_ones(0xff);
-
-        bool nan = false;                                // V has had one
-        // A stage's operands in runs of four, each read from the LDS while the run before it is multiplied: K of both 32 keys side by side
-        // (two sums that do not wait for each other), then V.
-        kv_h8 f[2][4];
-        auto read = [&](int buf, int run) {
+        for (int job = 0; job < JOBS; job++) {
+            if (!of_v(job)) {
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                if (run < G) f[run & 1][x] = sh.k[buf][x & 1][2 * run + (x >> 1)][lane];
-                else f[run & 1][x] = sh.v[buf][(4 * (run - G) + x) / G][(4 * (run - G) + x) % G][lane];
+                for (int j = 0; j < G; j++)
+                    sh.k[buf][tile >> 1][(b >> 1) * G + j][(b & 1) * 32 + (tile & 1) * 16 + col] =
+                        at_key(magic, codes[job][j], SN == 2 && (G * b + j) >> 2 != G * b >> 2 ? steps[job][SN - 1][0] : steps[job][0][0]);
+                continue;
             }
-        };
-        auto work = [&](int buf, int key) {
-            const at_u4 fl = sh.flag[buf];
-            pr_f16 s[2];
-#pragma unroll
-            for (int run = 0; run < G; run++) {
-                read(buf, run + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++)
-                        s[x & 1] = pr_mfma(f[run & 1][x], qf[p][2 * run + (x >> 1)], run + p + (x >> 1) ? s[x & 1] : pr_all(zero));
-            }
-            const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
-            if ((flags & 0xaa) || key < lo_max || key + ST - 1 > hi_min) {
+            uint32_t flag = pg < 0 ? 2 : 0;
+            if (pg < 0 || key_of(stage) + 16 > q.len) {          // what lies behind the last key may be anything: 0
                 asm volatile("");
-                const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
+                const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;       // of the lane's four keys
+                const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
+                const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int last = flags >> (2 * t) & 2 ? -1 : to;                   // no page
+                for (int x = 0; x < SN; x++) steps[job][x] &= at_u4{e, f, e, f};
+            }
+            // a floor whose exponent is all ones carries into its sign
+            uint32_t ones = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        s[t >> 1][8 * (t & 1) + i] = at_hide(s[t >> 1][8 * (t & 1) + i], at_hides(16 * t + 8 * (i >> 2) + (i & 3), from, last));
+            for (int x = 0; x < SN; x++)
+#pragma unroll
+                for (int y = 2; y < 4; y++) ones |= (steps[job][x][y] & 0x7c007c00u) + 0x04000400u;
+            if (__any((ones & 0x80008000u) != 0)) {
+                asm volatile("");
+                flag |= 1;
+#pragma unroll
+                for (int x = 0; x < SN; x++) (void)at_clean(steps[job][x]);
+            }
+#pragma unroll
+            for (int j = 0; j < G; j++) {
+                const at_u4 z = SN == 2 && G % 3 == 0 && (G * col + j) >> 4 != G * col >> 4 ? steps[job][SN - 1] : steps[job][0];
+                const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
+                const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
+                const uint32_t c = codes[job][j], d = c >> 8;
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    u2 w;
+                    w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
+                    w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
+                    ((u2 *)&sh.v[buf][tile][j][(b & 1) * 32 + 16 * e + col])[b >> 1] = w;
                 }
             }
-            float top = s[0][0];
-#pragma unroll
-            for (int x = 1; x < 32; x++) top = fmaxf(top, s[x >> 4][x & 15]);
-            top *= fac;
-            if (__any(top > m + AT_SLACK)) {
-                const float to = fmaxf(m, pr_max2(top)), g = to == -INFINITY ? 1.0f : at_exp2(m - to);
-                m = to;
-                l *= g;
-#pragma unroll
-                for (int j = 0; j < G; j++) o[j] *= g;
-            }
-            kv_h8 pf[4][PARTS];
-            const float off = AT_P2 - (m == -INFINITY ? 0.0f : m);
-#pragma unroll
-            for (int x = 0; x < 32; x++) {
-                const int at = 4 * (x >> 2 & 1) + at_place(x & 3);
-                const float p = at_exp2(fmaf(s[x >> 4][x & 15], fac, off));
-                pf[x >> 3][0][at] = (_Float16)p;
-                if constexpr (PARTS == 2) pf[x >> 3][1][at] = (_Float16)(p - (float)pf[x >> 3][0][at]);
-            }
-#pragma unroll
-            for (int run = G; run < 2 * G; run++) {
-                if (run + 1 < 2 * G) read(buf, run + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int p = 0; p < PARTS; p++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const int c = (4 * (run - G) + x) / G, j = (4 * (run - G) + x) % G;
-                        o[j] = pr_mfma(f[run & 1][x], pf[c][p], o[j]);
-                    }
-            }
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-                for (int p = 0; p < PARTS; p++) l = pr_mfma(ones, pf[c][p], l);
-            if (flags & 0x55) nan = true;
-        };
+            if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
+        }
+    };
 
-        __syncthreads();                                 // the block before this one has been read
-        convert(0, st0, pg);                             // (without a stage: of a tile past the keys, or one that nothing reads)
-        int pn = page(st0 + 1, next);
-        load(st0 + 1, pn);
-        next = entry(st0 + 2);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        int buf = 0;
-#pragma clang loop unroll(disable)
-        for (int st = st0; st < st1; st++, buf ^= 1) {
-            const int key = key0 + st * ST;
-            const bool mine = key <= hi_max && key + ST - 1 >= lo_min;
-            if (mine) read(buf, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            convert(buf ^ 1, st + 1, pn);
-            pn = page(st + 2, next);
-            load(st + 2, pn);
-            next = entry(st + 3);
-            __builtin_amdgcn_sched_barrier(0);
-            if (mine) work(buf, key);
-            // LDS writes are done; loads that are on their way end in registers, which their uses wait for
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        if (nan)
-            for (int key = key0 + st0 * ST; key < key0 + st1 * ST; key += 16)
-                pr_nan<G>(L, q, it.head, uni(L.a.table + (size_t)it.s * L.a.ldt), key, lane, lo, hi, o);
-        const int r = row0 + (lane & 31);
-        if (r >= rows) continue;
-        const int i = r / L.g, head = it.head * L.g + r - i * L.g;
-        const float sum = l[0];
-        // unit n = 8 x + 4 h + y holds values 2 G n .. : value 2 j + e is result 8 e + 4 x + y of o[j]
-        if (parts > 1) {
-            float *const to = prompt_piece<D, RB>(P, it.item, it.part);
-            const int rr = r - block * RB;
-            if (h == 0) { to[RB * D + rr] = m; to[RB * D + RB + rr] = sum; }
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int y = 0; y < 4; y++)
-#pragma unroll
-                    for (int j = 0; j < G; j++) {
-                        typedef float f2 __attribute__((ext_vector_type(2)));
-                        *(f2 *)(to + rr * D + 2 * G * (8 * x + 4 * h + y) + 2 * j) = f2{o[j][4 * x + y], o[j][8 + 4 * x + y]};
-                    }
-            continue;
-        }
-        const float f1 = attn_factor(m, sum, L.a.sink != nullptr, L.a.sink ? L.a.sink[head] * 1.44269504088896340736f : 0.0f);
-        const long at = (long)(q.begin + i) * L.a.ldo + (long)head * L.a.hdo;
+    int pg = page(st0, entry(st0));
+    load(st0, pg);
+    int next = entry(st0 + 1);
+    // the wave's rows, one a lane (and l ^ 32)
+    const int row0 = block * RB + wave * 32;
+    kv_h8 qf[PARTS][2 * G];
+    float fac, zero, m = -INFINITY;
+    int lo, hi;
+    {
+        AtQuery<G, PARTS, true> query;
+        query.load(L, q, head, row0 + (lane & 31), h);
+        attn_keys(L, q, min(row0 + (lane & 31), rows - 1) / L.g, lo, hi);
+        kv_h8 half[2][PARTS][G];                     // of the lane's values 8 G (2 x + h) ..
+        query.operands(L, half, fac, zero);
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const long d = at + 2 * G * (8 * x + 4 * h + y);
-                if constexpr (G % 4 == 0) {
+            for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                    for (int j = 0; j < G; j += 4) {
-                        float v[8];
+                for (int j = 0; j < G; j++) qf[p][x * G + j] = half[x][p][j];
+    }
+    pr_f16 o[G], l = pr_all(0.0f);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = o[j + (e >> 1)][8 * (e & 1) + 4 * x + y] * f1;
-                        kv_store8(L.a.out, L.a.type, d + 2 * j, v);
-                    }
-                } else if constexpr (G % 2 == 0) {
+    for (int j = 0; j < G; j++) o[j] = pr_all(0.0f);
+    const int lo_max = -pr_min32(-lo), lo_min = pr_min32(lo), hi_min = pr_min32(hi);
+    const int hi_max = row0 < rows ? -pr_min32(-hi) : -1;      // (a wave without rows has nothing to do)
+    const kv_h8 ones = at_ones(0xff);
+
+    bool nan = false;                                // V has had one
+    // A stage's operands in runs of four, each read from the LDS while the run before it is multiplied: K of both 32 keys side by side
+    // (two sums that do not wait for each other), then V.
+    kv_h8 f[2][4];
+    auto read = [&](int buf, int run) {
 #pragma unroll
-                    for (int j = 0; j < G; j += 2)
-                        kv_store4(L.a.out, L.a.type, d + 2 * j, kv_f4{o[j][4 * x + y], o[j][8 + 4 * x + y], o[j + 1][4 * x + y], o[j + 1][8 + 4 * x + y]} * f1);
-                } else {
+        for (int x = 0; x < 4; x++) {
+            if (run < G) f[run & 1][x] = sh.k[buf][x & 1][2 * run + (x >> 1)][lane];
+            else f[run & 1][x] = sh.v[buf][(4 * (run - G) + x) / G][(4 * (run - G) + x) % G][lane];
+        }
+    };
+    auto work = [&](int buf, int key) {
+        const at_u4 fl = sh.flag[buf];
+        pr_f16 s[2];
 #pragma unroll
-                    for (int j = 0; j < G; j++) {
-                        i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j), o[j][4 * x + y] * f1);
-                        i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j + 1), o[j][8 + 4 * x + y] * f1);
-                    }
+        for (int run = 0; run < G; run++) {
+            read(buf, run + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++)
+                    s[x & 1] = pr_mfma(f[run & 1][x], qf[p][2 * run + (x >> 1)], run + p + (x >> 1) ? s[x & 1] : pr_all(zero));
+        }
+        const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
+        if ((flags & 0xaa) || key < lo_max || key + ST - 1 > hi_min) {
+            asm volatile("");
+            const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int last = flags >> (2 * t) & 2 ? -1 : to;                   // no page
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    s[t >> 1][8 * (t & 1) + i] = at_hide(s[t >> 1][8 * (t & 1) + i], at_hides(16 * t + 8 * (i >> 2) + (i & 3), from, last));
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int x = 1; x < 32; x++) top = fmaxf(top, s[x >> 4][x & 15]);
+        top *= fac;
+        if (__any(top > m + AT_SLACK)) {
+            const float to = fmaxf(m, pr_max2(top)), g = to == -INFINITY ? 1.0f : at_exp2(m - to);
+            m = to;
+            l *= g;
+#pragma unroll
+            for (int j = 0; j < G; j++) o[j] *= g;
+        }
+        kv_h8 pf[4][PARTS];
+        const float off = AT_P2 - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int x = 0; x < 32; x++) {
+            const int at = 4 * (x >> 2 & 1) + at_place(x & 3);
+            const float p = at_exp2(fmaf(s[x >> 4][x & 15], fac, off));
+            pf[x >> 3][0][at] = (_Float16)p;
+            if constexpr (PARTS == 2) pf[x >> 3][1][at] = (_Float16)(p - (float)pf[x >> 3][0][at]);
+        }
+#pragma unroll
+        for (int run = G; run < 2 * G; run++) {
+            if (run + 1 < 2 * G) read(buf, run + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int c = (4 * (run - G) + x) / G, j = (4 * (run - G) + x) % G;
+                    o[j] = pr_mfma(f[run & 1][x], pf[c][p], o[j]);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) l = pr_mfma(ones, pf[c][p], l);
+        if (flags & 0x55) nan = true;
+    };
+
+    convert(0, st0, pg);                             // (without a stage: of a tile past the keys, or one that nothing reads)
+    int pn = page(st0 + 1, next);
+    load(st0 + 1, pn);
+    next = entry(st0 + 2);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    int buf = 0;
+#pragma clang loop unroll(disable)
+    for (int st = st0; st < st1; st++, buf ^= 1) {
+        const int key = key0 + st * ST;
+        const bool mine = key <= hi_max && key + ST - 1 >= lo_min;
+        if (mine) read(buf, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        convert(buf ^ 1, st + 1, pn);
+        pn = page(st + 2, next);
+        load(st + 2, pn);
+        next = entry(st + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        if (mine) work(buf, key);
+        // LDS writes are done; loads that are on their way end in registers, which their uses wait for
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    if (nan)
+        for (int key = key0 + st0 * ST; key < key0 + st1 * ST; key += 16)
+            pr_nan<G>(L, q, head, uni(L.a.table + (size_t)at.s * L.a.ldt), key, lane, lo, hi, o);
+    const int r = row0 + (lane & 31);
+    if (r >= rows) return;
+    const int i = r / L.g, q_head = head * L.g + r - i * L.g;
+    const float sum = l[0];
+    // unit n = 8 x + 4 h + y holds values 2 G n .. : value 2 j + e is result 8 e + 4 x + y of o[j]
+    if (P.parts > 1) {
+        float *const to = prompt_piece<D, RB>(P, line * heads + head, part);
+        const int rr = r - block * RB;
+        if (h == 0) { to[RB * D + rr] = m; to[RB * D + RB + rr] = sum; }
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    typedef float f2 __attribute__((ext_vector_type(2)));
+                    *(f2 *)(to + rr * D + 2 * G * (8 * x + 4 * h + y) + 2 * j) = f2{o[j][4 * x + y], o[j][8 + 4 * x + y]};
+                }
+        return;
+    }
+    const float f1 = attn_factor(m, sum, L.a.sink != nullptr, L.a.sink ? L.a.sink[q_head] * 1.44269504088896340736f : 0.0f);
+    const long to = (long)(q.begin + i) * L.a.ldo + (long)q_head * L.a.hdo;
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            const long d = to + 2 * G * (8 * x + 4 * h + y);
+            if constexpr (G % 4 == 0) {
+#pragma unroll
+                for (int j = 0; j < G; j += 4) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = o[j + (e >> 1)][8 * (e & 1) + 4 * x + y] * f1;
+                    kv_store8(L.a.out, L.a.type, d + 2 * j, v);
+                }
+            } else if constexpr (G % 2 == 0) {
+#pragma unroll
+                for (int j = 0; j < G; j += 2)
+                    kv_store4(L.a.out, L.a.type, d + 2 * j, kv_f4{o[j][4 * x + y], o[j][8 + 4 * x + y], o[j + 1][4 * x + y], o[j + 1][8 + 4 * x + y]} * f1);
+            } else {
+#pragma unroll
+                for (int j = 0; j < G; j++) {
+                    i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j), o[j][4 * x + y] * f1);
+                    i8_st(L.a.out, L.a.type, (size_t)(d + 2 * j + 1), o[j][8 + 4 * x + y] * f1);
                 }
             }
-    }
+        }
 }
 
 // The parts of split blocks: 256 threads for 256 / (D / 4) rows of an item at a time.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void k_attn_join(PromptLaunch P) {
     const AttnLaunch &L = P.A;
-    long x = blockIdx.x;
-    const int head = (int)(x % L.c.heads), s = (int)(x / L.c.heads % L.a.S), block = (int)(x / L.c.heads / L.a.S);
-    const AttnSeq q = attn_seq(L, s);
-    if ((long)q.n * L.g <= L.limit) return;
+    const uint32_t x = blockIdx.x, line = x / (uint32_t)L.c.heads;
+    const int head = (int)(x - line * (uint32_t)L.c.heads);
+    PromptBlock at;
+    if (!prompt_block<RB>(L, line, at)) return;
+    const AttnSeq &q = at.q;
+    const int block = at.block;
     const int r = (int)blockIdx.y * (256 / (D / 4)) + (int)threadIdx.x / (D / 4), d = (int)threadIdx.x % (D / 4) * 4;
     if (r >= RB || (int)threadIdx.x >= 256 / (D / 4) * (D / 4) || block * RB + r >= q.n * L.g) return;
     float M = -INFINITY, sum = 0.0f;
     for (int p = 0; p < P.parts; p++) M = fmaxf(M, prompt_piece<D, RB>(P, x, p)[RB * D + r]);
     kv_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int p = 0; p < P.parts; p++) {
-        const float *const at = prompt_piece<D, RB>(P, x, p);
-        const float m = at[RB * D + r], f = m == -INFINITY ? 0.0f : at_exp2(m - M);
-        v += *(const kv_f4 *)(at + r * D + d) * f;
-        sum += at[RB * D + RB + r] * f;
+        const float *const from = prompt_piece<D, RB>(P, x, p);
+        const float m = from[RB * D + r], f = m == -INFINITY ? 0.0f : at_exp2(m - M);
+        v += *(const kv_f4 *)(from + r * D + d) * f;
+        sum += from[RB * D + RB + r] * f;
     }
     const int i = (block * RB + r) / L.g, h = head * L.g + (block * RB + r) - i * L.g;
     v *= attn_factor(M, sum, L.a.sink != nullptr, L.a.sink ? L.a.sink[h] * 1.44269504088896340736f : 0.0f);
@@ -417,14 +443,11 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
     PromptLaunch P;
     memset(&P, 0, sizeof P);
     P.A = L;
-    const long rows = (long)std::min(std::max(1, L.a.max_rows), L.a.T) * L.g;
-    const long most = std::max(1l, (1l << 22) / ((long)L.a.S * L.c.heads));             // a launch has less than 2^32 threads
-    P.blocks = (int)std::min(most, (rows + RB - 1) / RB);
-    const long items = (long)P.blocks * L.a.S * L.c.heads;
+    // as many blocks as the call's rows can make: a sequence has a last one that is not full
+    const long rows = (long)L.a.T * L.g, items = (rows / RB + std::min<long>(L.a.S, rows / ((long)L.limit + 1))) * L.c.heads;
     // few blocks: their keys in parts, of 256 keys at least
     const int at_once = 256;
     P.parts = (int)std::max<long>(1, std::min<long>({16, at_once / std::max(1l, items), ((long)std::max(1, L.a.max_len) + 255) / 256}));
-    if (items > 1l << 22) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: prompts of S=%d sequences over %d heads", L.a.S, L.c.heads);
     if (P.parts > 1) {
         if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)items * P.parts * RB * (D + 2) * 4, false)) return rc;
         P.A.part = (float *)c->attn_part.p;

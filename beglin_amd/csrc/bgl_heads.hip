@@ -27,6 +27,8 @@ struct HeadsLaunch {
     bgl_kv c;
     const int32_t *slots;        // of the d.T tokens of this launch; null: no cache
     int nq, nk, nv;              // heads to do of each
+    float one_over_f;            // 1 / D
+    double one_over;
 };
 
 // Sums over the GL lanes of a head, in every one of them.
@@ -98,39 +100,30 @@ __device__ __forceinline__ HdWeights hd_weights(const bgl_heads &d, const float 
     return g;
 }
 
-// y of a lane's 8 values x of a head (0 for a lane behind D) and, for half, their partners px.  R: the arithmetic's type.
-template <typename R, int GL>
-__device__ __forceinline__ void hd_turned(float (&y)[8], const bgl_heads &d, const float (&x)[8], const float (&px)[8], const HdWeights &g, const HdTurn &t,
-                                          R mean, R inv) {
-    R n[8];
-    const R add = d.norm != BGL_NORM_NONE && d.w_add != 0.0f ? (R)d.w_add : (R)0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) n[j] = ((R)x[j] - mean) * inv * ((R)g.w[j] + add);
-    if (d.rot_kind == BGL_ROT_NONE) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = (float)n[j];
-    } else if (d.rot_kind == BGL_ROT_HALF) {
+// A row of a head, of which a lane has the 8 values x (0 for a lane behind D) and, for half, their partners px (0 where nothing is rotated):
+//     y = (x w c + x' w' s) / sqrt(..)        with w' and x' the partner's
+// In fp32 what x and x' are multiplied by is the same for every head.
+struct HdFast {
+    float a[8], b[8];
+    bool on;
+    __device__ __forceinline__ HdFast(const bgl_heads &d, const HdWeights &g, const HdTurn &t) {
+        const float add = d.norm != BGL_NORM_NONE ? d.w_add : 0.0f;
+        on = t.on;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const R pn = ((R)px[j] - mean) * inv * ((R)g.pw[j] + add);
-            const R v = fma(n[j], (R)t.c[j], pn * (R)t.s[j]);
-            y[j] = (float)(t.on ? v : n[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const R v = fma(n[j], (R)t.c[j], n[j ^ 1] * (R)t.s[j]);
-            y[j] = (float)(t.on ? v : n[j]);
+            a[j] = (g.w[j] + add) * t.c[j];
+            b[j] = ((d.rot_kind == BGL_ROT_PAIRS ? g.w[j ^ 1] : g.pw[j]) + add) * t.s[j];
         }
     }
-}
+};
 // A 16-bit output needs no double (16 additions and multiplications err by 2^-20 at most), unless a norm takes a difference from the mean
 // or hides a row of tiny values behind no eps.
 static __host__ __device__ __forceinline__ bool hd_fast(const bgl_heads &d) {
     return d.out_type != BGL_T_F32 && (d.norm == BGL_NORM_NONE || (d.norm == BGL_NORM_RMS && d.eps >= 1e-20f));
 }
 template <int GL>
-__device__ __forceinline__ void hd_row_fast(float (&y)[8], const bgl_heads &d, float (&x)[8], float (&px)[8], const HdWeights &g, const HdTurn &t) {
+__device__ __forceinline__ void hd_row_fast(float (&y)[8], const HeadsLaunch &L, float (&x)[8], float (&px)[8], const HdFast &f) {
+    const bgl_heads &d = L.d;
     float inv = 1.0f;
     if (d.norm != BGL_NORM_NONE) {
         float q = 0.0f, eps = d.eps;
@@ -145,9 +138,18 @@ __device__ __forceinline__ void hd_row_fast(float (&y)[8], const bgl_heads &d, f
             for (int j = 0; j < 8; j++) { x[j] *= down; px[j] *= down; q = fmaf(x[j], x[j], q); }
             q = hd_sum<GL>(q);
         }
-        inv = 1.0f / sqrtf(q / d.D + eps);
+        inv = __builtin_amdgcn_rsqf(fmaf(q, L.one_over_f, eps));
     }
-    hd_turned<float, GL>(y, d, x, px, g, t, 0.0f, inv);
+    if (d.rot_kind == BGL_ROT_HALF) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = fmaf(x[j], f.a[j], px[j] * f.b[j]) * inv;
+    } else if (d.rot_kind == BGL_ROT_PAIRS) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = fmaf(x[j], f.a[j], (f.on ? x[j ^ 1] : 0.0f) * f.b[j]) * inv;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[j] * f.a[j] * inv;
+    }
 }
 // Keeps what is the same for every head in fp32 registers: as doubles, made once, it takes twice as many.
 __device__ __forceinline__ void hd_opaque(float (&v)[8]) {
@@ -155,74 +157,91 @@ __device__ __forceinline__ void hd_opaque(float (&v)[8]) {
     for (int j = 0; j < 8; j++) asm volatile("" : "+v"(v[j]));
 }
 template <int GL>
-__device__ __forceinline__ void hd_row(float (&y)[8], const bgl_heads &d, const float (&x)[8], const float (&px)[8], HdWeights &g, HdTurn &t) {
+__device__ __forceinline__ void hd_row(float (&y)[8], const HeadsLaunch &L, const float (&x)[8], const float (&px)[8], HdWeights &g, HdTurn &t) {
+    const bgl_heads &d = L.d;
     hd_opaque(g.w);
     hd_opaque(g.pw);
     hd_opaque(t.c);
     hd_opaque(t.s);
-    double mean = 0.0, inv = 1.0;
-    if (d.norm != BGL_NORM_NONE) {
-        double q = 0.0;
-        if (d.norm == BGL_NORM_LAYER) {
+    double v[8], pv[8], inv = 1.0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) mean += (double)x[j];
-            mean = hd_sum<GL>(mean) / d.D;
-        }
+    for (int j = 0; j < 8; j++) { v[j] = x[j]; pv[j] = px[j]; }
+    if (d.norm == BGL_NORM_LAYER) {
+        double mean = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) mean += v[j];
+        mean = hd_sum<GL>(mean) * L.one_over;
         const bool in = (int)(threadIdx.x & (GL - 1)) * 8 < d.D;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const double v = in ? (double)x[j] - mean : 0.0;
-            q = fma(v, v, q);
-        }
-        inv = rsqrt(hd_sum<GL>(q) / d.D + (double)d.eps);
+        for (int j = 0; j < 8; j++) { v[j] = in ? v[j] - mean : 0.0; pv[j] -= mean; }
     }
-    hd_turned<double, GL>(y, d, x, px, g, t, mean, inv);
-}
-
-// The codes of a lane's 8 values, whose group is those of the lane's quad, and the group's step and floor (s | m << 16).
-__device__ __forceinline__ uint32_t hd_codes(uint32_t (&c)[8], const float (&x)[8]) {
-    float lo = INFINITY, hi = -INFINITY, t[8];
-    uint32_t top = 0;
+    if (d.norm != BGL_NORM_NONE) {
+        double q = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q = fma(v[j], v[j], q);
+        inv = rsqrt(fma(hd_sum<GL>(q), L.one_over, (double)d.eps));
+    }
+    const double add = d.norm != BGL_NORM_NONE ? (double)d.w_add : 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] *= add != 0.0 ? (double)g.w[j] + add : (double)g.w[j];
+    if (d.rot_kind == BGL_ROT_NONE) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = (float)(v[j] * inv);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) pv[j] = d.rot_kind == BGL_ROT_PAIRS ? v[j ^ 1] : pv[j] * (add != 0.0 ? (double)g.pw[j] + add : (double)g.pw[j]);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-        t[j] = fminf(fmaxf(x[j], -32768.0f), 32768.0f);
-        lo = fminf(lo, t[j]);
-        hi = fmaxf(hi, t[j]);
+        const double turned = fma(v[j], (double)t.c[j], pv[j] * (double)t.s[j]);
+        y[j] = (float)((t.on ? turned : v[j]) * inv);
     }
+}
+
+// The codes, 0 .. 15, of a lane's 8 values, whose group is those of the lane's quad, and the group's step and floor (s | m << 16).
+__device__ __forceinline__ uint32_t hd_codes(float (&c)[8], const float (&x)[8]) {
+    float bad = 0.0f, t[8];                              // bad: NaN if a value has no end
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        bad = fmaf(x[j], 0.0f, bad);
+        t[j] = __builtin_amdgcn_fmed3f(x[j], -32768.0f, 32768.0f);
+    }
+    float lo = fminf(fminf(fminf(t[0], t[1]), fminf(t[2], t[3])), fminf(fminf(t[4], t[5]), fminf(t[6], t[7])));
+    float hi = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
     lo = fminf(lo, dpp_f<0xB1>(lo)); lo = fminf(lo, dpp_f<0x4E>(lo));
     hi = fmaxf(hi, dpp_f<0xB1>(hi)); hi = fmaxf(hi, dpp_f<0x4E>(hi));
-    top = max(top, (uint32_t)dpp_i<0xB1>((int)top)); top = max(top, (uint32_t)dpp_i<0x4E>((int)top));
+    bad += dpp_f<0xB1>(bad); bad += dpp_f<0x4E>(bad);
     const _Float16 m = (_Float16)lo;
     const float fm = (float)m;
     const _Float16 s = (_Float16)fmaxf(0.0f, __fmul_rn(__fsub_rn(hi, fm), 1.0f / 15.0f));
-    const float r = __fdiv_rn(1.0f, (float)s);
-    const bool none = !((float)s > 0.0f) || top >= 0x7f800000u;
+    const float fs = (float)s;
+    // 1 / s to nearest: s has 11 bits, so the remainder is exact, its correction errs by 2^-46 of 1 / s, and no quotient of such an s lies
+    // within 2^-36 of the middle between two fp32 values
+    float r = __builtin_amdgcn_rcpf(fs);
+    r = fmaf(fmaf(-fs, r, 1.0f), r, r);
+    r = fs > 0.0f && bad == 0.0f ? r : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float q = none ? 0.0f : rintf(__fmul_rn(__fsub_rn(t[j], fm), r));
-        c[j] = (uint32_t)(int)fminf(fmaxf(q, 0.0f), 15.0f);
-    }
-    if (top >= 0x7f800000u) return 0x7e000000u;                    // NaN, step 0
+    for (int j = 0; j < 8; j++) c[j] = rintf(__builtin_amdgcn_fmed3f(__fmul_rn(__fsub_rn(t[j], fm), r), 0.0f, 15.0f));
+    if (!(bad == 0.0f)) return 0x7e000000u;              // NaN, step 0
     return (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
 }
 
 __device__ __forceinline__ void hd_put_k(uint8_t *rec, int D, int tok, int li, const float (&x)[8]) {
-    uint32_t c[8];
+    float c[8];
     const uint32_t sm = hd_codes(c, x);
     const int G = D / 32, b = li / G, j = li - b * G;
     // values 1, 3 lie 16 bits above 0, 2, and 4 .. 7 8 bits above 0 .. 3
-    const uint32_t w = c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12 | c[1] << 16 | c[3] << 20 | c[5] << 24 | c[7] << 28;
-    ((uint32_t *)rec)[(b * KV_TILE + tok) * G + j] = w;
+    const float lo = fmaf(fmaf(fmaf(c[6], 16.0f, c[4]), 16.0f, c[2]), 16.0f, c[0]), hi = fmaf(fmaf(fmaf(c[7], 16.0f, c[5]), 16.0f, c[3]), 16.0f, c[1]);
+    ((uint32_t *)rec)[(b * KV_TILE + tok) * G + j] = (uint32_t)lo | (uint32_t)hi << 16;
     if ((li & 3) == 0) ((uint32_t *)(rec + kv_k_steps(D)))[(li >> 2) * KV_TILE + tok] = sm;
 }
 __device__ __forceinline__ void hd_put_v(uint8_t *rec, int D, int tok, int li, const float (&x)[8]) {
-    uint32_t c[8];
+    float c[8];
     const uint32_t sm = hd_codes(c, x);
     const int b = tok >> 2, r = tok & 3;
     uint8_t *p = rec + kv_v_codes(D) + (b * (D / 2) + 4 * li) * 4 + r;
 #pragma unroll
-    for (int j = 0; j < 4; j++) p[4 * j] = (uint8_t)(c[2 * j] | c[2 * j + 1] << 4);
+    for (int j = 0; j < 4; j++) p[4 * j] = (uint8_t)(uint32_t)fmaf(c[2 * j + 1], 16.0f, c[2 * j]);
     if ((li & 3) == 0) {
         uint16_t *q = (uint16_t *)(rec + kv_v_steps(D)) + ((li >> 2) * 4 + b) * 8 + (r & 1) * 2 + (r >> 1);
         q[0] = (uint16_t)sm;
@@ -230,25 +249,35 @@ __device__ __forceinline__ void hd_put_v(uint8_t *rec, int D, int tok, int li, c
     }
 }
 
+// The token of workgroup x of a launch over n tokens, in whole rows of 128 where there are as many: 16 neighbours, which share the cache
+// lines of a record, go to one XCD (workgroups go round the eight), whose L2 then puts their bytes together.
+static __device__ __forceinline__ int hd_token(int x, int n) { return n < 128 ? x : (x & ~127) + ((x & 7) << 4) + (x >> 3 & 15); }
+
 // A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other.  FAST, EXACT: which rows the launch has, those
 // of hd_row_fast, the others and the cache's, or both: few tokens are one launch, many take one each, for the others' doubles would leave the
 // fast ones half as many waves (4096 tokens of 40 heads, bf16: 49 us together).
 template <int GL, bool FAST, bool EXACT>
 __global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
     const bgl_heads &d = L.d;
-    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), per = (int)blockDim.x / GL;
+    const int t = hd_token(blockIdx.x, d.T), li = threadIdx.x & (GL - 1), per = (int)blockDim.x / GL;
+    if (t >= d.T) return;
     const bool in = 8 * li < d.D;
     const int d0 = in ? 8 * li : 0;
     const int pos = d.rot_kind != BGL_ROT_NONE ? d.pos[t] : 0;
     const int slot = L.slots ? L.slots[t] : -1;
-    const float *const rope = d.rope + (size_t)pos * d.rot;
     const bool kept = slot >= 0 && slot < (long)L.c.pages * L.c.page;
+    const int tok = kept ? slot % L.c.page % KV_TILE : 0;
+    const float *const rope = d.rope + (size_t)pos * d.rot;
     if (d.rot_kind != BGL_ROT_NONE && (uint32_t)pos >= (uint32_t)d.n_pos) return;
     const int step = (int)gridDim.y * per, first = (int)blockIdx.y * per + (int)threadIdx.x / GL;
     HdTurn turn = hd_turn(d, rope, d0);
     auto load = [&](float (&x)[8], float (&px)[8], const void *p, long at) {
         kv_load8(x, p, d.type, at + d0);
-        if (d.rot_kind == BGL_ROT_HALF) kv_load8(px, p, d.type, at + turn.other);
+        if (d.rot_kind == BGL_ROT_HALF && turn.on) kv_load8(px, p, d.type, at + turn.other);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) px[j] = 0.0f;
+        }
         if (!in) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = 0.0f;
@@ -257,28 +286,30 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
     int i = first;
     if (i < L.nq) {
         HdWeights g = hd_weights(d, d.q_w, turn, d0);
+        const HdFast f(d, g, turn);
         const bool fast = FAST && (!EXACT || hd_fast(d));
         for (; i < L.nq; i += step) {
             float x[8], px[8], y[8];
             load(x, px, d.q, t * d.ldq + i * d.hdq);
-            if (fast) hd_row_fast<GL>(y, d, x, px, g, turn);
-            else if constexpr (EXACT) hd_row<GL>(y, d, x, px, g, turn);
+            if (fast) hd_row_fast<GL>(y, L, x, px, f);
+            else if constexpr (EXACT) hd_row<GL>(y, L, x, px, g, turn);
             if (in) kv_store8(d.q_out, d.out_type, t * d.ldqo + i * d.hdqo + d0, y);
         }
     }
     if (i < L.nq + L.nk) {
         HdWeights g = hd_weights(d, d.k_w, turn, d0);
+        const HdFast f(d, g, turn);
         const bool fast = FAST && (!EXACT || (d.k_out && hd_fast(d)));
         for (; i < L.nq + L.nk; i += step) {
             const int h = i - L.nq;
             float x[8], px[8], y[8];
             if (!d.k_out && !kept) continue;
             load(x, px, d.k, t * d.ldk + h * d.hdk);
-            if (fast) hd_row_fast<GL>(y, d, x, px, g, turn);
-            else if constexpr (EXACT) hd_row<GL>(y, d, x, px, g, turn);
+            if (fast) hd_row_fast<GL>(y, L, x, px, f);
+            else if constexpr (EXACT) hd_row<GL>(y, L, x, px, g, turn);
             if (!in) continue;
             if (d.k_out) kv_store8(d.k_out, d.out_type, t * d.ldko + h * d.hdko + d0, y);
-            else if constexpr (EXACT) hd_put_k(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
+            else if constexpr (EXACT) hd_put_k(kv_at(L.c, slot, h), d.D, tok, li, y);
         }
     }
     if (!EXACT || !kept || !in) return;
@@ -286,7 +317,7 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
         const int h = i - L.nq - L.nk;
         float y[8];
         kv_load8(y, d.v, d.type, t * d.ldv + h * d.hdv + d0);
-        hd_put_v(kv_at(L.c, slot, h), d.D, slot % L.c.page % KV_TILE, li, y);
+        hd_put_v(kv_at(L.c, slot, h), d.D, tok, li, y);
     }
 }
 
@@ -303,7 +334,8 @@ __device__ __forceinline__ float kv_value(uint32_t c, uint32_t s, uint32_t m) {
 }
 template <int GL>
 __global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
-    const int t = blockIdx.x, li = threadIdx.x & (GL - 1), d0 = 8 * li, D = L.c.D, G = D / 32;
+    const int t = hd_token(blockIdx.x, L.n), li = threadIdx.x & (GL - 1), d0 = 8 * li, D = L.c.D, G = D / 32;
+    if (t >= L.n) return;
     const int slot = L.slots[t];
     if (slot < 0 || slot >= (long)L.c.pages * L.c.page || d0 >= D) return;
     const int tok = slot % L.c.page % KV_TILE, step = (int)gridDim.y * (256 / GL);
@@ -338,6 +370,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
 #define HD_MANY (1 << 14)         // heads of queries that are a launch of their own beside the cache's rows
 
 // Workgroups a token: as many as it takes to do every head at once, while the launch leaves units idle.
+static unsigned hd_tokens(int T) { return T < 128 ? T : (T + 127) / 128 * 128; }
 static unsigned hd_parts(int T, int items, int per) {
     const int all = (items + per - 1) / per;
     return (unsigned)std::max(1, std::min(all, 1024 / std::max(1, T)));
@@ -355,6 +388,8 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
     const int tok = prof_begin(c, 2);
     for (long t = 0; t < a.T; t += HD_TOKENS) {
         HeadsLaunch L = all;
+        L.one_over_f = 1.0f / a.D;
+        L.one_over = 1.0 / a.D;
         bgl_heads &d = L.d;
         d.T = (int)std::min<long>(HD_TOKENS, a.T - t);
         auto at = [&](const void *p, long ld, int type) { return p ? (char *)p + t * ld * (long)i8_elem(type) : nullptr; };
@@ -366,7 +401,7 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
             constexpr int GL = decltype(gl)::value;
             auto go = [&](auto kernel, int nq, int nk, int nv) {
                 L.nq = nq; L.nk = nk; L.nv = nv;
-                hipLaunchKernelGGL(kernel, dim3((unsigned)d.T, hd_parts(d.T, nq + nk + nv, 256 / GL)), dim3(256), 0, c->stream, L);
+                hipLaunchKernelGGL(kernel, dim3(hd_tokens(d.T), hd_parts(d.T, nq + nk + nv, 256 / GL)), dim3(256), 0, c->stream, L);
             };
             const bool q_fast = all.nq && hd_fast(d), k_fast = all.nk && d.k_out && hd_fast(d), exact = all.nv || (all.nq && !q_fast) || (all.nk && !k_fast);
             if (!exact) go(k_heads<GL, true, false>, all.nq, all.nk, 0);
@@ -488,7 +523,7 @@ extern "C" int bgl_kv_read_dev(bgl_ctx *c, const bgl_kv *kv, const int32_t *slot
         L.v = v ? (char *)v + t * ldv * (long)i8_elem(type) : nullptr; L.ldv = ldv; L.hdv = hdv;
         hd_lanes(kv->D, [&](auto gl) {
             constexpr int GL = decltype(gl)::value;
-            hipLaunchKernelGGL((k_kv_read<GL>), dim3((unsigned)L.n, hd_parts(L.n, 2 * kv->heads, 256 / GL)), dim3(256), 0, c->stream, L);
+            hipLaunchKernelGGL((k_kv_read<GL>), dim3(hd_tokens(L.n), hd_parts(L.n, 2 * kv->heads, 256 / GL)), dim3(256), 0, c->stream, L);
         });
     }
     prof_end(c, tok);

@@ -63,8 +63,14 @@ __device__ __forceinline__ void kv_store8(void *p, int type, long at, const floa
         return;
     }
     kv_mu4 u;
+    if (type == BGL_T_F16) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) u[j] = (uint32_t)i8_h16(q[2 * j], type) | (uint32_t)i8_h16(q[2 * j + 1], type) << 16;
+        for (int j = 0; j < 4; j++) u[j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)q[2 * j], (_Float16)q[2 * j + 1]});
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int j = 0; j < 4; j++) u[j] = __builtin_bit_cast(uint32_t, b2{(__bf16)q[2 * j], (__bf16)q[2 * j + 1]});
+    }
     *(kv_mu4 *)((uint16_t *)p + at) = u;
 }
 
