@@ -11,6 +11,7 @@ struct AttnLaunch {
     int g;                       // heads of q for one of the cache
     int ppt;                     // 16-token tiles a page
     uint32_t div_mul, div_shift; // t / ppt = (mulhi(t, div_mul) + t) >> div_shift for t < 2^31
+    size_t page_bytes;           // of all heads
     int unit;                    // bgl_attn.hip: keys a unit, a multiple of AT_STEP
     int limit;                   // sequences with more than this many rows times g are another launch's
     float scale2;                // |scale| * log2(e); a negative scale turns q's sign

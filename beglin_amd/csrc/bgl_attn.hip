@@ -524,6 +524,7 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.a = *a;
     L.g = g;
     L.ppt = kv->page / KV_TILE;
+    L.page_bytes = (size_t)kv->heads * L.ppt * kv_record(kv->D);
     while ((1 << L.div_shift) < L.ppt) L.div_shift++;
     L.div_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << L.div_shift) - (uint32_t)L.ppt)) / L.ppt + 1);
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;

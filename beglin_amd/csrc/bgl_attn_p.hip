@@ -151,9 +151,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     // A wave converts, of each stage's four tiles, K or V of one (8 waves), or both.
     const int tile = WAVES == 8 ? wave >> 1 : wave;
     auto of_v = [&](int job) { return WAVES == 8 ? (wave & 1) != 0 : job != 0; };
-    auto codes_at = [&](int job) { return (of_v(job) ? 10 * D : 0) + lane * (4 * G); };
+    auto codes_at = [&](int job) { return (uint32_t)((of_v(job) ? 10 * D : 0) + lane * (4 * G)); };
     auto steps_at = [&](int job, int x) {                // of the lane's first or last group
-        return of_v(job) ? 18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4;
+        return (uint32_t)(of_v(job) ? 18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4);
     };
     // the keys of the block's rows, this part's stages of 64 among them
     int lo_first, lo_last, hi_first, hi_last;
@@ -164,7 +164,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     const int st1 = __builtin_amdgcn_readfirstlane((int)((long)stages * (part + 1) / P.parts));
 
     auto key_of = [&](int stage) { return key0 + stage * ST + 16 * tile; };
-    auto entry = [&](int stage) { return table[min(at_page(L, key_of(stage) >> 4), last_page) + zero_lane]; };
+    // the table's entry for the wave's tile of a stage, and where the tile lies in its page
+    uint32_t in_page = 0;
+    auto entry = [&](int stage) {
+        const int t = key_of(stage) >> 4, p = at_page(L, t);
+        in_page = (uint32_t)(t - p * L.ppt) * (20 * D);
+        return table[min(p, last_page) + zero_lane];
+    };
     auto page = [&](int stage, int e) {              // the page, or -1: past the keys, or none
         e = __builtin_amdgcn_readfirstlane(e);
         return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
@@ -172,11 +178,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     uint32_t codes[JOBS][G];
     typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
     at_u4 steps[JOBS][SN];
-    // (a tile without a page loads the first record, and none of it counts)
-    auto load = [&](int stage, int pg) {
-        const int t = key_of(stage) >> 4;
-        const size_t rec = pg < 0 ? 0 : ((size_t)pg * L.c.heads + head) * L.ppt + (t - at_page(L, t) * L.ppt);
-        const uint8_t *p = (const uint8_t *)L.c.data + rec * (20 * D);
+    const uint8_t *const records = (const uint8_t *)L.c.data + (size_t)head * L.ppt * (20 * D);
+    // (a tile without a page loads one of the first page, and none of it counts)
+    auto load = [&](int pg) {
+        const uint8_t *p = records + (size_t)(uint32_t)max(pg, 0) * L.page_bytes + in_page;
 #pragma unroll
         for (int job = 0; job < JOBS; job++) {
             at_dwords<G>(codes[job], p + codes_at(job));
@@ -235,7 +240,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     };
 
     int pg = page(st0, entry(st0));
-    load(st0, pg);
+    load(pg);
     int next = entry(st0 + 1);
     // the wave's rows, one a lane (and l ^ 32)
     const int row0 = block * RB + wave * 32;
@@ -339,7 +344,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
 
     convert(0, st0, pg);                             // (without a stage: of a tile past the keys, or one that nothing reads)
     int pn = page(st0 + 1, next);
-    load(st0 + 1, pn);
+    load(pn);
     next = entry(st0 + 2);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     int buf = 0;
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         __builtin_amdgcn_sched_barrier(0);
         convert(buf ^ 1, st + 1, pn);
         pn = page(st + 2, next);
-        load(st + 2, pn);
+        load(pn);
         next = entry(st + 3);
         __builtin_amdgcn_sched_barrier(0);
         if (mine) work(buf, key);
