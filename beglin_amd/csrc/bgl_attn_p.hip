@@ -85,15 +85,15 @@ __device__ __forceinline__ float pr_max2(float v) {
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-// WAVES 8: two a SIMD.  4: one, with all of its registers, for wide heads and two parts.
+// WAVES 8: two a SIMD, stages of 128 keys, two halves.  4: one, with all of its registers, for wide heads and two parts, stages of 64.
 template <int G, int WAVES, int PARTS>
 struct Prompt {
-    static constexpr int D = 32 * G, RB = 32 * WAVES, ST = 64;
-    static constexpr int SN = G % 3 == 0 || G > 4 ? 2 : 1;         // groups of 32 that a lane's values lie in, at most
+    static constexpr int D = 32 * G, RB = 32 * WAVES, HALVES = WAVES / 4, ST = 64 * HALVES;
+    static constexpr int KN = G % 3 == 0 || G > 4 ? 2 : 1, VN = G % 3 == 0 ? 2 : 1;    // groups of 32 that a lane's values lie in, at most
     struct Shared {
-        kv_h8 k[2][2][2 * G][64];                        // [buffer][32 keys][of the sum over values, 16 at a time]
-        kv_h8 v[2][4][G][64];                            // [buffer][16 keys, the sum][32 values]
-        at_u4 flag[2];                                   // a tile each: 1 some value of V is NaN, 2 it has no page
+        kv_h8 k[2][2 * HALVES][2 * G][64];               // [buffer][32 keys][of the sum over values, 16 at a time]
+        kv_h8 v[2][4 * HALVES][G][64];                   // [buffer][16 keys, the sum][32 values]
+        at_u4 flag[2][HALVES];                           // a tile each: 1 some value of V is NaN, 2 it has no page
     };
 };
 
@@ -130,7 +130,7 @@ __device__ __forceinline__ void pr_nan(const AttnLaunch &L, const AttnSeq &q, in
 template <int G, int WAVES, int PARTS>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(PromptLaunch P) {
     using T = Prompt<G, WAVES, PARTS>;
-    constexpr int D = T::D, RB = T::RB, ST = T::ST, SN = T::SN, JOBS = 8 / WAVES;
+    constexpr int D = T::D, RB = T::RB, ST = T::ST, HALVES = T::HALVES, KN = T::KN, VN = T::VN;
     const AttnLaunch &L = P.A;
     __shared__ typename T::Shared sh;
     // Workgroup -> head (neighbouring workgroups, and with 8 heads a head an XCD, whose L2 holds its keys), part, block of the line.
@@ -148,14 +148,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     int zero_lane = 0;
     asm volatile("" : "+v"(zero_lane));
     const int last_page = at_page(L, max(0, q.len - 1) >> 4);
-    // A wave converts, of each stage's four tiles, K or V of one (8 waves), or both.
-    const int tile = WAVES == 8 ? wave >> 1 : wave;
-    auto of_v = [&](int job) { return WAVES == 8 ? (wave & 1) != 0 : job != 0; };
-    auto codes_at = [&](int job) { return (uint32_t)((of_v(job) ? 10 * D : 0) + lane * (4 * G)); };
-    auto steps_at = [&](int job, int x) {                // of the lane's first or last group
-        return (uint32_t)(of_v(job) ? 18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16 : 8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4);
-    };
-    // the keys of the block's rows, this part's stages of 64 among them
+    const int tile = wave;                               // of each stage's, whose K and V the wave converts
+    const uint32_t kc_at = lane * (4 * G), vc_at = 10 * D + kc_at;
+    auto ks_at = [&](int x) { return (uint32_t)(8 * D + (((G * b + x * (G - 1)) >> 2) * 16 + col) * 4); };       // of the first or last group
+    auto vs_at = [&](int x) { return (uint32_t)(18 * D + (((G * col + x * (G - 1)) >> 4) * 4 + b) * 16); };
+    // the keys of the block's rows, this part's stages among them
     int lo_first, lo_last, hi_first, hi_last;
     attn_keys(L, q, block * RB / L.g, lo_first, hi_first);
     attn_keys(L, q, (min(block * RB + RB, rows) - 1) / L.g, lo_last, hi_last);
@@ -175,72 +172,71 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         e = __builtin_amdgcn_readfirstlane(e);
         return key_of(stage) < q.len && (uint32_t)e < (uint32_t)L.c.pages ? e : -1;
     };
-    uint32_t codes[JOBS][G];
-    typedef unsigned int u4 __attribute__((ext_vector_type(4), aligned(4)));
-    at_u4 steps[JOBS][SN];
+    uint32_t kc[G], ks[KN], vc[G];
+    at_u4 vs[VN];
     const uint8_t *const records = (const uint8_t *)L.c.data + (size_t)head * L.ppt * (20 * D);
     // (a tile without a page loads one of the first page, and none of it counts)
-    auto load = [&](int pg) {
-        const uint8_t *p = records + (size_t)(uint32_t)max(pg, 0) * L.page_bytes + in_page;
+    auto load_k = [&](int pg, uint32_t in) {
+        const uint8_t *p = records + (size_t)(uint32_t)max(pg, 0) * L.page_bytes + in;
+        at_dwords<G>(kc, p + kc_at);
 #pragma unroll
-        for (int job = 0; job < JOBS; job++) {
-            at_dwords<G>(codes[job], p + codes_at(job));
-#pragma unroll
-            for (int x = 0; x < SN; x++) steps[job][x] = *(const u4 *)(p + steps_at(job, x));
-        }
+        for (int x = 0; x < KN; x++) ks[x] = *(const uint32_t *)(p + ks_at(x));
     };
-    auto convert = [&](int buf, int stage, int pg) {
+    auto load_v = [&](int pg, uint32_t in) {
+        const uint8_t *p = records + (size_t)(uint32_t)max(pg, 0) * L.page_bytes + in;
+        at_dwords<G>(vc, p + vc_at);
 #pragma unroll
-        for (int job = 0; job < JOBS; job++) {
-            if (!of_v(job)) {
+        for (int x = 0; x < VN; x++) vs[x] = *(const at_u4 *)(p + vs_at(x));
+    };
+    auto convert_k = [&](int buf) {
 #pragma unroll
-                for (int j = 0; j < G; j++)
-                    sh.k[buf][tile >> 1][(b >> 1) * G + j][(b & 1) * 32 + (tile & 1) * 16 + col] =
-                        at_key(magic, codes[job][j], SN == 2 && (G * b + j) >> 2 != G * b >> 2 ? steps[job][SN - 1][0] : steps[job][0][0]);
-                continue;
-            }
-            uint32_t flag = pg < 0 ? 2 : 0;
-            if (pg < 0 || key_of(stage) + 16 > q.len) {          // what lies behind the last key may be anything: 0
-                asm volatile("");
-                const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;       // of the lane's four keys
-                const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
-                const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+        for (int j = 0; j < G; j++)
+            sh.k[buf][tile >> 1][(b >> 1) * G + j][(b & 1) * 32 + (tile & 1) * 16 + col] =
+                at_key(magic, kc[j], KN == 2 && (G * b + j) >> 2 != G * b >> 2 ? ks[KN - 1] : ks[0]);
+    };
+    auto convert_v = [&](int buf, int stage, int pg) {
+        uint32_t flag = pg < 0 ? 2 : 0;
+        if (pg < 0 || key_of(stage) + 16 > q.len) {      // what lies behind the last key may be anything: 0
+            asm volatile("");
+            const int left = pg < 0 ? 0 : q.len - key_of(stage) - 4 * b;               // of the lane's four keys
+            const uint32_t e = (left > 0 ? 0x0000ffffu : 0u) | (left > 2 ? 0xffff0000u : 0u);
+            const uint32_t f = (left > 1 ? 0x0000ffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int x = 0; x < SN; x++) steps[job][x] &= at_u4{e, f, e, f};
-            }
-            // a floor whose exponent is all ones carries into its sign
-            uint32_t ones = 0;
-#pragma unroll
-            for (int x = 0; x < SN; x++)
-#pragma unroll
-                for (int y = 2; y < 4; y++) ones |= (steps[job][x][y] & 0x7c007c00u) + 0x04000400u;
-            if (__any((ones & 0x80008000u) != 0)) {
-                asm volatile("");
-                flag |= 1;
-#pragma unroll
-                for (int x = 0; x < SN; x++) (void)at_clean(steps[job][x]);
-            }
-#pragma unroll
-            for (int j = 0; j < G; j++) {
-                const at_u4 z = SN == 2 && G % 3 == 0 && (G * col + j) >> 4 != G * col >> 4 ? steps[job][SN - 1] : steps[job][0];
-                const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
-                const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
-                const uint32_t c = codes[job][j], d = c >> 8;
-                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    u2 w;
-                    w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
-                    w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
-                    ((u2 *)&sh.v[buf][tile][j][(b & 1) * 32 + 16 * e + col])[b >> 1] = w;
-                }
-            }
-            if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
+            for (int x = 0; x < VN; x++) vs[x] &= at_u4{e, f, e, f};
         }
+        // a floor whose exponent is all ones carries into its sign
+        uint32_t ones = 0;
+#pragma unroll
+        for (int x = 0; x < VN; x++)
+#pragma unroll
+            for (int y = 2; y < 4; y++) ones |= (vs[x][y] & 0x7c007c00u) + 0x04000400u;
+        if (__any((ones & 0x80008000u) != 0)) {
+            asm volatile("");
+            flag |= 1;
+#pragma unroll
+            for (int x = 0; x < VN; x++) (void)at_clean(vs[x]);
+        }
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+            const at_u4 z = VN == 2 && (G * col + j) >> 4 != G * col >> 4 ? vs[VN - 1] : vs[0];
+            const kv_h2 s0 = __builtin_bit_cast(kv_h2, (uint32_t)z[0]), s1 = __builtin_bit_cast(kv_h2, (uint32_t)z[1]);
+            const kv_h2 m0 = __builtin_bit_cast(kv_h2, (uint32_t)z[2]), m1 = __builtin_bit_cast(kv_h2, (uint32_t)z[3]);
+            const uint32_t c = vc[j], d = c >> 8;
+            typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                u2 w;
+                w[0] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, c, s0, m0) : at_lo(magic, c, s0, m0));
+                w[1] = __builtin_bit_cast(uint32_t, e ? at_hi(magic, d, s1, m1) : at_lo(magic, d, s1, m1));
+                ((u2 *)&sh.v[buf][tile][j][(b & 1) * 32 + 16 * e + col])[b >> 1] = w;
+            }
+        }
+        if (lane == 0) ((uint32_t *)&sh.flag[buf])[tile] = flag;
     };
 
     int pg = page(st0, entry(st0));
-    load(pg);
+    load_k(pg, in_page);
+    load_v(pg, in_page);
     int next = entry(st0 + 1);
     // the wave's rows, one a lane (and l ^ 32)
     const int row0 = block * RB + wave * 32;
@@ -271,19 +267,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     // A stage's operands in runs of four, each read from the LDS while the run before it is multiplied: K of both 32 keys side by side
     // (two sums that do not wait for each other), then V.
     kv_h8 f[2][4];
-    auto read = [&](int buf, int run) {
+    auto read = [&](int buf, int half, int run) {
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-            if (run < G) f[run & 1][x] = sh.k[buf][x & 1][2 * run + (x >> 1)][lane];
-            else f[run & 1][x] = sh.v[buf][(4 * (run - G) + x) / G][(4 * (run - G) + x) % G][lane];
+            if (run < G) f[run & 1][x] = sh.k[buf][2 * half + (x & 1)][2 * run + (x >> 1)][lane];
+            else f[run & 1][x] = sh.v[buf][4 * half + (4 * (run - G) + x) / G][(4 * (run - G) + x) % G][lane];
         }
     };
-    auto work = [&](int buf, int key) {
-        const at_u4 fl = sh.flag[buf];
+    auto work = [&](int buf, int half, int key) {        // 64 keys
+        const at_u4 fl = sh.flag[buf][half];
         pr_f16 s[2];
 #pragma unroll
         for (int run = 0; run < G; run++) {
-            read(buf, run + 1);
+            read(buf, half, run + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int x = 0; x < 4; x++)
@@ -292,7 +288,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
                     s[x & 1] = pr_mfma(f[run & 1][x], qf[p][2 * run + (x >> 1)], run + p + (x >> 1) ? s[x & 1] : pr_all(zero));
         }
         const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
-        if ((flags & 0xaa) || key < lo_max || key + ST - 1 > hi_min) {
+        if ((flags & 0xaa) || key < lo_max || key + 63 > hi_min) {
             asm volatile("");
             const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
 #pragma unroll
@@ -325,7 +321,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         }
 #pragma unroll
         for (int run = G; run < 2 * G; run++) {
-            if (run + 1 < 2 * G) read(buf, run + 1);
+            if (run + 1 < 2 * G) read(buf, half, run + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int p = 0; p < PARTS; p++)
@@ -342,24 +338,40 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         if (flags & 0x55) nan = true;
     };
 
-    convert(0, st0, pg);                             // (without a stage: of a tile past the keys, or one that nothing reads)
-    int pn = page(st0 + 1, next);
-    load(pn);
+    // (without a stage: of a tile past the keys, or one that nothing reads)
+    convert_k(0);
+    convert_v(0, st0, pg);
+    pg = page(st0 + 1, next);
+    uint32_t in = in_page;
+    load_k(pg, in);
+    if (HALVES == 1) load_v(pg, in);
     next = entry(st0 + 2);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     int buf = 0;
 #pragma clang loop unroll(disable)
     for (int st = st0; st < st1; st++, buf ^= 1) {
         const int key = key0 + st * ST;
-        const bool mine = key <= hi_max && key + ST - 1 >= lo_min;
-        if (mine) read(buf, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        convert(buf ^ 1, st + 1, pn);
-        pn = page(st + 2, next);
-        load(pn);
-        next = entry(st + 3);
-        __builtin_amdgcn_sched_barrier(0);
-        if (mine) work(buf, key);
+#pragma unroll
+        for (int half = 0; half < HALVES; half++) {
+            const bool mine = key + 64 * half <= hi_max && key + 64 * half + 63 >= lo_min;
+            if (mine) read(buf, half, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            // the next stage's K, then its V (each loaded half a stage before)
+            if (half == 0) {
+                convert_k(buf ^ 1);
+                if (HALVES == 2) load_v(pg, in);
+            }
+            if (half == HALVES - 1) {
+                convert_v(buf ^ 1, st + 1, pg);
+                pg = page(st + 2, next);
+                in = in_page;
+                load_k(pg, in);
+                if (HALVES == 1) load_v(pg, in);
+                next = entry(st + 3);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (mine) work(buf, half, key + 64 * half);
+        }
         // LDS writes are done; loads that are on their way end in registers, which their uses wait for
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
