@@ -256,12 +256,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
 #pragma unroll
                 for (int j = 0; j < G; j++) qf[p][x * G + j] = half[x][p][j];
     }
-    pr_f16 o[G], l = pr_all(0.0f);
+    pr_f16 o[G];
+    float l = 0.0f;                                  // of the lane's half of the keys
 #pragma unroll
     for (int j = 0; j < G; j++) o[j] = pr_all(0.0f);
     const int lo_max = -pr_min32(-lo), lo_min = pr_min32(lo), hi_min = pr_min32(hi);
     const int hi_max = row0 < rows ? -pr_min32(-hi) : -1;      // (a wave without rows has nothing to do)
-    const kv_h8 ones = at_ones(0xff);
 
     bool nan = false;                                // V has had one
     // A stage's operands in runs of four, each read from the LDS while the run before it is multiplied: K of both 32 keys side by side
@@ -290,14 +290,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
         const uint32_t flags = (uint32_t)__builtin_amdgcn_readfirstlane((int)(fl[0] | fl[1] << 2 | fl[2] << 4 | fl[3] << 6));
         if ((flags & 0xaa) || key < lo_max || key + 63 > hi_min) {
             asm volatile("");
-            const int from = at_from(lo, key + 4 * h), to = at_from(hi, key + 4 * h);
+            // A lane's scores are of keys 8 (x / 4) + x % 4 behind its first: a bit for each that is seen, those of [lo, hi].
+            auto below = [&](int edge) {                 // bits of the keys below
+                const int e = (int)min(max((long)edge - (key + 4 * h), 0l), 64l), n = 4 * (e >> 3) + min(e & 7, 4);
+                return n > 31 ? ~0u : (1u << n) - 1;
+            };
+            uint32_t seen = below(hi + 1) & ~below(lo);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int last = flags >> (2 * t) & 2 ? -1 : to;                   // no page
+            for (int t = 0; t < 4; t++)
+                if (flags >> (2 * t) & 2) seen &= ~(0xffu << (8 * t));
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    s[t >> 1][8 * (t & 1) + i] = at_hide(s[t >> 1][8 * (t & 1) + i], at_hides(16 * t + 8 * (i >> 2) + (i & 3), from, last));
-            }
+            for (int x = 0; x < 32; x++) s[x >> 4][x & 15] = at_hide(s[x >> 4][x & 15], ~((int)(seen << (31 - x)) >> 31));
         }
         float top = s[0][0];
 #pragma unroll
@@ -319,6 +322,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
             pf[x >> 3][0][at] = (_Float16)p;
             if constexpr (PARTS == 2) pf[x >> 3][1][at] = (_Float16)(p - (float)pf[x >> 3][0][at]);
         }
+        // (the instruction's additions cut off what its largest term has no place for: short sums, which are added to nearest)
+        const kv_h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int y = 0; y < 8; y += 2) sum[c & 1] = __builtin_amdgcn_fdot2(kv_h2{pf[c][p][y], pf[c][p][y + 1]}, one, sum[c & 1], false);
+        l += sum[0] + sum[1];
 #pragma unroll
         for (int run = G; run < 2 * G; run++) {
             if (run + 1 < 2 * G) read(buf, half, run + 1);
@@ -331,10 +344,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
                     o[j] = pr_mfma(f[run & 1][x], pf[c][p], o[j]);
                 }
         }
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) l = pr_mfma(ones, pf[c][p], l);
         if (flags & 0x55) nan = true;
     };
 
@@ -381,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(
     const int r = row0 + (lane & 31);
     if (r >= rows) return;
     const int i = r / L.g, q_head = head * L.g + r - i * L.g;
-    const float sum = l[0];
+    const float sum = l + __shfl_xor(l, 32);
     // unit n = 8 x + 4 h + y holds values 2 G n .. : value 2 j + e is result 8 e + 4 x + y of o[j]
     if (P.parts > 1) {
         float *const to = prompt_piece<D, RB>(P, line * heads + head, part);
