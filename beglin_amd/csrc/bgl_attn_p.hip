@@ -469,8 +469,10 @@ static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
     PromptLaunch P;
     memset(&P, 0, sizeof P);
     P.A = L;
-    // as many blocks as the call's rows can make: a sequence has a last one that is not full
-    const long rows = (long)L.a.T * L.g, items = (rows / RB + std::min<long>(L.a.S, rows / ((long)L.limit + 1))) * L.c.heads;
+    // as many blocks as the call's rows can make: every sequence of this kernel's may have one that is not full
+    const long rows = (long)L.a.T * L.g, most = std::min<long>(L.a.S, rows / ((long)L.limit + 1));
+    const long items = ((rows - most) / RB + most) * L.c.heads;
+    if (!items) return 0;
     // few blocks: their keys in parts, of 256 keys at least
     const int at_once = 256;
     P.parts = (int)std::max<long>(1, std::min<long>({16, at_once / std::max(1l, items), ((long)std::max(1, L.a.max_len) + 255) / 256}));
