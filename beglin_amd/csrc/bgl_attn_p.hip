@@ -128,7 +128,7 @@ __device__ __forceinline__ void pr_nan(const AttnLaunch &L, const AttnSeq &q, in
 }
 
 template <int G, int WAVES, int PARTS>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 1) void k_attn_prompt(PromptLaunch P) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (PARTS == 1 && G <= 4) ? 2 : 1) void k_attn_prompt(PromptLaunch P) {
     using T = Prompt<G, WAVES, PARTS>;
     constexpr int D = T::D, RB = T::RB, ST = T::ST, HALVES = T::HALVES, KN = T::KN, VN = T::VN;
     const AttnLaunch &L = P.A;
@@ -463,34 +463,69 @@ __global__ __launch_bounds__(256) void k_attn_join(PromptLaunch P) {
 }
 
 // ================================================================================== host side
+// A launch's blocks of RB rows times heads, and the parts of their keys.
+struct PromptShape {
+    long items;
+    int parts;
+};
+static PromptShape prompt_shape(const AttnLaunch &L, int G, int RB) {
+    PromptShape h;
+    // as many blocks as the call's rows can make: every sequence of this kernel's may have one that is not full
+    const long rows = (long)L.a.T * L.g, most = std::min<long>(L.a.S, rows / ((long)L.limit + 1));
+    h.items = ((rows - most) / RB + most) * L.c.heads;
+    // Where blocks leave CUs idle their keys are split: 64 keys of a workgroup take some 1 + G / 4 us, the second launch 3 us, and a part's sums go
+    // out and in at 4 MB a us.  (512 rows of 32 heads of 128 over 4096 keys: 94 us in one part, 60 in four; over 512 keys 23 and 28 in two.)
+    const double keys = L.a.window ? std::min((double)L.a.max_len, (double)L.a.window + RB) : L.a.max_len, stages = std::max(1.0, keys / 64);
+    double best = 0;
+    h.parts = 1;
+    for (int p = 1; p <= 16 && p * h.items <= (p > 1 ? 256 : p * h.items); p++) {
+        const double us = stages / p * (1 + G / 4.0) + (p > 1 ? 3 + (double)rows * L.c.heads * p * (32 * G) * 8 / 4e6 : 0);
+        if (p == 1 || us < best) {
+            best = us;
+            h.parts = p;
+        }
+    }
+    return h;
+}
 template <int G, int WAVES, int PARTS>
-static int prompt_go(bgl_ctx *c, const AttnLaunch &L) {
+static int prompt_go(bgl_ctx *c, const AttnLaunch &L, const PromptShape &h) {
     constexpr int RB = Prompt<G, WAVES, PARTS>::RB, D = 32 * G;
     PromptLaunch P;
     memset(&P, 0, sizeof P);
     P.A = L;
-    // as many blocks as the call's rows can make: every sequence of this kernel's may have one that is not full
-    const long rows = (long)L.a.T * L.g, most = std::min<long>(L.a.S, rows / ((long)L.limit + 1));
-    const long items = ((rows - most) / RB + most) * L.c.heads;
-    if (!items) return 0;
-    // few blocks: their keys in parts, of 256 keys at least
-    const int at_once = 256;
-    P.parts = (int)std::max<long>(1, std::min<long>({16, at_once / std::max(1l, items), ((long)std::max(1, L.a.max_len) + 255) / 256}));
+    P.parts = h.parts;
+    if (!h.items) return 0;
     if (P.parts > 1) {
-        if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)items * P.parts * RB * (D + 2) * 4, false)) return rc;
+        if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)h.items * P.parts * RB * (D + 2) * 4, false)) return rc;
         P.A.part = (float *)c->attn_part.p;
     }
-    hipLaunchKernelGGL((k_attn_prompt<G, WAVES, PARTS>), dim3((unsigned)(items * P.parts)), dim3(64 * WAVES), 0, c->stream, P);
+    hipLaunchKernelGGL((k_attn_prompt<G, WAVES, PARTS>), dim3((unsigned)(h.items * P.parts)), dim3(64 * WAVES), 0, c->stream, P);
     if (P.parts > 1) {
         constexpr int per = 256 / (D / 4);
-        hipLaunchKernelGGL((k_attn_join<D, RB>), dim3((unsigned)items, (RB + per - 1) / per), dim3(256), 0, c->stream, P);
+        hipLaunchKernelGGL((k_attn_join<D, RB>), dim3((unsigned)h.items, (RB + per - 1) / per), dim3(256), 0, c->stream, P);
     }
     return 0;
 }
 template <int G>
 static int prompt_pick(bgl_ctx *c, const AttnLaunch &L) {
-    if (L.a.type == BGL_T_F32) return prompt_go<G, G <= 3 ? 8 : 4, 2>(c, L);
-    return prompt_go<G, G <= 4 ? 8 : 4, 1>(c, L);
+    if constexpr (G <= 4) {
+        const PromptShape h = prompt_shape(L, G, 256);
+        if (L.a.type != BGL_T_F32) {
+            // Blocks that are one round at most and not split: of half the size they fill more CUs, or two of them share one (32 heads of 128,
+            // prompts of 128, 512, 1024 and 2048 tokens: 13.5, 22.7, 37.5 and 70 us in blocks of 256 rows, 10.8, 19.5, 32.7 and 66 of 128; of 4096
+            // tokens 164 and 188: each block converts its keys).
+            if (h.parts == 1 && h.items <= 256) return prompt_go<G, 4, 1>(c, L, {prompt_shape(L, G, 128).items, 1});
+            return prompt_go<G, 8, 1>(c, L, h);
+        }
+        if constexpr (G <= 3) return prompt_go<G, 8, 2>(c, L, h);
+    }
+    if constexpr (G > 3) {
+        const PromptShape h = prompt_shape(L, G, 128);
+        if constexpr (G > 4) {
+            if (L.a.type != BGL_T_F32) return prompt_go<G, 4, 1>(c, L, h);
+        }
+        return prompt_go<G, 4, 2>(c, L, h);
+    }
 }
 
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L) {

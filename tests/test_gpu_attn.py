@@ -191,6 +191,18 @@ def test_many_rows(torch_dev, ctx, case):
     b.check(b.run(ctx, window=100, sink=True, max_rows=40, max_len=10 ** 6), window=100, sink=True)
     b.out.fill_(7.0)
     b.check(b.run(ctx, max_rows=1, max_len=longest))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, max_len=10 ** 6))                                           # the largest blocks, their keys in many parts
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_many_rows_of_many_heads(torch_dev, ctx, kind, D):
+    """More blocks than CUs, so the largest ones, in one part."""
+    b = Batch(torch_dev, ctx, [(70, 300), (60, 130), (40, 40), (5, 90), (110, 700), (35, 2000)], 90, 90, D, kind, 32)
+    b.check(b.run(ctx))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, sink=True, window=77), sink=True, window=77)
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -205,6 +217,8 @@ def test_nan_and_pages_that_are_gone_among_many_rows(torch_dev, ctx, kind, D, wi
     b.check(b.run(ctx, window=window), window=window)
     b.out.fill_(7.0)
     b.check(b.run(ctx, window=window, sink=True, max_rows=50, max_len=97), window=window, sink=True)
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, window=window, max_rows=50, max_len=10 ** 6), window=window)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
