@@ -1,12 +1,17 @@
 // bgl_attn_p.hip -- attention of many rows a sequence (prompts, chunks of them) over the paged cache in 4 bits: the same sums as
 // bgl_attn.hip's, bound by the matrix cores and by the exponentials, not by the cache's bytes.
 //
-// A workgroup takes RB rows of a head's group (tokens times heads of q) and goes over the keys that they see, 64 at a time.
+// A workgroup takes RB rows of a head's group (tokens times heads of q) and goes over the keys that they see, 64 or 128 at a time.
 // Its waves turn those keys' codes into fp16 operands once for all rows, in LDS: a record's order is the operands'
-// order, so lane l writes 16 bytes at 16 l and reads 16 bytes at 16 l, without a conflict and without a transposition.  Two
-// buffers: the next 64 keys are converted, and the ones after those loaded, while the matrix cores work on the present ones.
-// Each wave has 16 NT rows, as columns of S^T = K Q^T and O^T = V^T P^T; what a lane has of S^T is its part of P^T's operand.
-// A row's sum of weights is one more product, with ones in V's place: the vector units are the narrower side here.
+// order, so lane l writes 16 bytes at 16 l and reads 16 bytes at 16 l, without a transposition.  Two
+// buffers: the next keys are converted, and the ones after those loaded, while the matrix cores work on the present ones; one barrier a stage.
+// Each wave has 32 rows, as columns of S^T = K Q^T and O^T = V^T P^T; what a lane has of S^T is its part of P^T's operand.
+//
+// 4096 bf16 tokens of 32 heads of 128 over 8 of the cache: 164 us, 840 TFLOP/s of the rows' own products (a library's product of 8192^3
+// runs at 1180).  By counters the matrix units are busy 45% of that time and the vector units issue 50%: two waves a SIMD, which is what
+// 240 registers leave, hardly overlap them, and every instruction of the loop counts, scalar ones too (the same loop with 50 scalar
+// instructions more a stage: 181 us).  Tried and slower: the two waves of a SIMD in turns, half a stage apart (185 us); a stage's scores
+// between the products of the one before it; 16 x 16 tiles (190 us where these took 175); three waves a SIMD for heads of 64 (118 for 113).
 #include <string.h>
 
 #include <algorithm>
@@ -79,7 +84,7 @@ __device__ __forceinline__ bool prompt_block(const AttnLaunch &L, uint32_t x, Pr
 typedef float pr_f16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ pr_f16 pr_mfma(kv_h8 a, kv_h8 b, pr_f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ pr_f16 pr_all(float v) { return pr_f16{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
-// the larger value, and the sum, of a lane and the other lane of its row (l ^ 32)
+// the larger value of a lane and the other lane of its row (l ^ 32)
 __device__ __forceinline__ float pr_max2(float v) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
@@ -97,7 +102,7 @@ struct Prompt {
     };
 };
 
-// at_nan for 32 rows: keys key .. key + 15.
+// at_nan (bgl_attn.h) for 32 rows: keys key .. key + 15.
 template <int G>
 __device__ __forceinline__ void pr_nan(const AttnLaunch &L, const AttnSeq &q, int head, ucint table, int key, int lane, int lo, int hi, pr_f16 (&o)[G]) {
     const int n = lane & 15, h = lane >> 5, t = key >> 4, pg = key < q.len ? table[at_page(L, t)] : -1;

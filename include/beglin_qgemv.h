@@ -231,8 +231,9 @@ int  bgl_norm_dev(bgl_ctx *ctx, const bgl_norm *d);
  *     BGL_ROT_PAIRS  the same for values 2 i and 2 i + 1
  *     y_d = n_d for d >= rot, and everywhere with BGL_ROT_NONE (rope and pos unused)
  * Values are computed in double and rounded to fp32, then to out_type; those of a 16-bit out_type may be computed in
- * fp32.  q_w, k_w: fp32 [D], NULL: no factor.  rope: fp32 rows of rot values, n_pos of them; a token whose pos lies outside [0, n_pos) is skipped: nothing is written for it.  Value
- * d of head h of token t lies ld * t + hd * h + d values behind the pointer.  D is a multiple of 8 up to 512, rot of 16
+ * fp32.  q_w, k_w: fp32 [D], NULL: no factor.  rope: fp32 rows of rot values, n_pos of them; a token whose pos lies
+ * outside [0, n_pos) is skipped: nothing is written for it.  Value d of head h of token t lies ld * t + hd * h + d values
+ * behind the pointer.  D is a multiple of 8 up to 512, rot of 16
  * (HALF) or 8 (PAIRS).  q_out may be q, and k_out k, with the same type and strides; apart from that what is written
  * overlaps nothing that is read.  bgl_heads_dev: q with q_out, k with k_out, or both; v is not used. */
 typedef struct {
