@@ -13,6 +13,7 @@ struct AttnLaunch {
     uint32_t div_mul, div_shift; // t / ppt = (mulhi(t, div_mul) + t) >> div_shift for t < 2^31
     size_t page_bytes;           // of all heads
     int unit;                    // bgl_attn.hip: keys a unit, a multiple of AT_STEP
+    int least;                   // bgl_attn.hip: units a workgroup, at least (1 or 2)
     int limit;                   // sequences with more than this many rows times g are another launch's
     float scale2;                // |scale| * log2(e); a negative scale turns q's sign
     float *part;                 // bgl_attn.hip's partial sums: [2 * workgroups] pieces

@@ -235,8 +235,8 @@ __device__ __forceinline__ int attn_pause(int chunks, int run) { return chunks <
 // The line of units in runs: the first `more` workgroups have one unit more than the others' `each`.
 struct AttnRuns {
     uint32_t each, more, wgs;
-    __device__ AttnRuns(uint32_t total, uint32_t grid) {
-        wgs = min(grid, total);
+    __device__ AttnRuns(uint32_t total, uint32_t grid, uint32_t least) {
+        wgs = min(grid, total < 64 ? total : (total + least - 1) / least);
         each = wgs ? total / wgs : 0;
         more = total - each * wgs;
     }
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
         upto = at_scan(mine);
     }
     const __amdgpu_buffer_rsrc_t pieces = __builtin_amdgcn_make_buffer_rsrc(L.part, (short)0, AT_WG * 2 * PIECE * 4, 0x00020000);
-    const AttnRuns runs((uint32_t)__builtin_amdgcn_readlane(upto, 63), gridDim.x);
+    const AttnRuns runs((uint32_t)__builtin_amdgcn_readlane(upto, 63), gridDim.x, (uint32_t)L.least);
     const uint32_t w = blockIdx.x;
     if (w >= runs.wgs) return;
     const uint32_t end = runs.begin(w + 1);
@@ -571,9 +571,13 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.part = (float *)c->attn_part.p;
     L.sync = (int *)c->attn_sync.p;
     // Up to four steps stay together: a head whose keys are one unit needs no join (8 heads over 512 keys: 10.4 us in units of 128).
-    L.unit = a->max_len <= 4 * AT_STEP ? 4 * AT_STEP : AT_STEP;
-    const long units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * (((long)std::max(1, a->max_len) + L.unit - 1) / L.unit);
-    const unsigned wgs = (unsigned)std::min<long>(AT_WG, std::max<long>(1, units));
+    const long keys = a->window ? std::min((long)a->max_len, (long)a->window + rows) : a->max_len;
+    L.unit = keys <= 4 * AT_STEP ? 4 * AT_STEP : AT_STEP;
+    const long chunks = (std::max(1l, keys) + L.unit - 1) / L.unit, units = (long)a->S * kv->heads * ((rows + RB - 1) / RB) * chunks;
+    // Two units for a workgroup, where an item's pieces are large or many: half of them to join (2 sequences of 4096 keys, 2 heads of 128, 16 rows:
+    // 19.4 us in 128 workgroups, 15.8 in 64; 8 heads of 128, 4 rows: 8192 keys 15.2 and 13.7, 3000 keys 11.6 and 12.1).
+    L.least = chunks * std::min(rows, RB) * kv->D > 1 << 14 ? 2 : 1;
+    const unsigned wgs = (unsigned)std::min<long>(AT_WG, std::max<long>(1, units < 128 ? units : units / L.least));
     const int tok = prof_begin(c, 1);
     switch (G) {
     case 2: attn_pick<2>(c, L, nt, wgs); break;
