@@ -485,7 +485,8 @@ class Context:
     def attention(self, cache, q, out, start, lens, table, *, scale=None, causal=True, window=0, sink=None, max_rows=None, max_len=None):
         """out = attention of the rows q [T][heads][D] over the cache (bgl_attn_dev): sequence s has the rows start[s] ..
         start[s + 1] - 1 and lens[s] keys in the pages table[s]; int32 tensors [S + 1], [S], [S][pages].  scale None: 1 / sqrt(D).
-        sink: fp32 [heads].  max_rows, max_len: the most rows and keys of a sequence, where the program knows them."""
+        sink: fp32 [heads].  max_rows, max_len: the most rows and keys of a sequence, where the program knows them (None: as if every
+        sequence had a row, and as many keys as the table's pages hold); launch shapes go by them, no result does."""
         dev, who = self.device, "attention"
         if table.ndim != 2 or q.ndim != 3 or q.shape[2] != cache.dim or cache.device != dev:
             _refuse(f"attention: q [T][heads][{cache.dim}], table [S][pages], the cache on device {dev}")
@@ -495,7 +496,7 @@ class Context:
         a = capi.bgl_attn(S, T, nq, *_heads(q, shape, kind, dev, who), *_heads(out, shape, kind, dev, who), _row_type(kind, who),
                           _ints(start, S + 1, dev, who), _ints(lens, S, dev, who), _ints(table, S * ldt, dev, who), ldt,
                           D ** -0.5 if scale is None else scale, causal, window, _floats(sink, nq, dev, who),
-                          T if max_rows is None else max_rows, ldt * cache.page if max_len is None else max_len)
+                          max(1, T - S + 1) if max_rows is None else max_rows, ldt * cache.page if max_len is None else max_len)
         _check(lib().bgl_attn_dev(self.h, C.byref(cache.d), C.byref(a)), "bgl_attn_dev")
 
     # ---- MoE ----

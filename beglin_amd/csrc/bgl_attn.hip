@@ -8,9 +8,10 @@
 //   output   O^T = V^T P^T: what a lane has of S^T is, as weights, its part of P^T's operand: nothing is moved between lanes
 // but the row maxima; a row's statistics lie in the lanes that hold its sums.
 //
-// Work: 128 keys of one head and row block are a unit, 32 for each wave (or 512, where no sequence has more).  The units of all sequences lie in one line that
-// is cut into equal runs, one a workgroup, so a batch of very different lengths leaves no workgroup behind.  A head whose
-// keys end up in several runs is joined by whichever of them finishes last, in the order of its keys: the same bits every time.
+// Work: 128 keys of one head and row block are a unit, 32 for each wave (or 512, where no sequence has more).  The units of all
+// sequences lie in one line (short sequences apart, attn_pause) that is cut into equal runs, one a workgroup, so a batch of very
+// different lengths leaves no workgroup behind.  A head whose keys end up in several runs is joined by whichever of them
+// finishes last, in the order of its keys: the same bits every time.
 #include <string.h>
 
 #include <algorithm>

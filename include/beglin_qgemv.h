@@ -268,7 +268,7 @@ typedef struct {
 size_t bgl_kv_bytes(int pages, int page, int heads, int D);               /* 0: no such cache */
 /* Keys and values of d's T tokens into the cache, k normed and rotated as bgl_heads_dev does, v as it is; token t goes to
  * slot slots[t] = page id * page + place in the page.  Slots outside the cache: the token's keys and values are not
- * written.  The slots of one call are distinct.  With q and q_out the queries are normed and rotated in the same launch.
+ * written.  The slots of one call are distinct.  With q and q_out the queries are normed and rotated in the same call.
  * d->nk and d->D are the cache's; k_out has to be NULL. */
 int  bgl_kv_append_dev(bgl_ctx *ctx, const bgl_kv *kv, const bgl_heads *d, const int32_t *slots);
 /* The values of n slots, [n][heads] rows of D in `type`, as strided rows (see bgl_heads); k or v may be NULL.  Rows of

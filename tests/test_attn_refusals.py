@@ -32,7 +32,8 @@ BAD_KV = [dict(data=None), dict(data=(1 << 28) + 8), dict(pages=0), dict(page=0)
 BAD_ATTN = [dict(S=0), dict(T=0), dict(ldt=0), dict(nq=0), dict(nq=3), dict(nq=-2), dict(q=None), dict(out=None), dict(start=None), dict(len=None),
             dict(table=None), dict(type=5), dict(ldq=300), dict(hdq=64), dict(ldo=300), dict(hdo=-1), dict(window=-1),
             dict(window=5, causal=0), dict(max_rows=-1), dict(max_len=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(out=4096),
-            dict(T=1 << 30, nq=8, ldq=1024, ldo=1024), dict(ldt=(1 << 25) + 1), dict(ldt=1 << 30)]
+            dict(T=1 << 30, nq=8, ldq=1024, ldo=1024), dict(ldt=(1 << 25) + 1), dict(ldt=1 << 30),
+            dict(T=1 << 25, nq=32, ldq=4096, ldo=4096, max_rows=1 << 25)]
 
 
 def name(b):

@@ -286,6 +286,22 @@ def test_many_sequences(torch_dev, ctx):
     b.check(b.run(ctx, window=5, sink=True), window=5, sink=True)
 
 
+@pytest.mark.parametrize("case", [(30, 3000, 12, 1), (90, 900, 20, 1), (50, 2600, 40, 1), (25, 2000, 10, 4)], ids=str)
+def test_lengths_far_apart(torch_dev, ctx, case):
+    """Units for every workgroup several times over, and sequences of few of them between long ones."""
+    count, longest, heads, most = case
+    rng = np.random.default_rng(count)
+    lens = np.exp(rng.uniform(0, np.log(longest), count)).astype(int)
+    lens[::7] = longest
+    seqs = [(int(rng.integers(0, most + 1)) if most > 1 else 1, int(n)) for n in lens]
+    b = Batch(torch_dev, ctx, seqs, heads, heads, 64, "bf16", 32)
+    b.check(b.run(ctx, max_rows=most))
+    b.out.fill_(7.0)
+    b.check(b.run(ctx, max_rows=most, max_len=longest, window=700), window=700)
+    again = b.run(ctx, max_rows=most, max_len=longest, window=700)
+    assert np.array_equal(again[:b.T], b.run(ctx, max_rows=most, max_len=longest, window=700)[:b.T])
+
+
 def test_bad_starts_and_lengths_stay_in_bounds(torch_dev, ctx):
     """start and len are read on the device: rows outside [0, T) and keys outside the table do not exist."""
     torch = torch_dev
