@@ -27,7 +27,7 @@
     } while (0)
 
 #define AT_STEP 128              // keys that the four waves of a workgroup go over at once
-#define AT_WG 768                // workgroups at most
+#define AT_WG 512                // workgroups at most: two for each CU, so that all run at once (three, where registers allow it: 31.6 us for 30.0)
 #define AT_FEW 32                // rows of a head's group that a sequence of few rows has, at most
 #define AT_SC1 16                // the cache-policy bit of a buffer access of device scope
 
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
         __syncthreads();
         const bool whole = c0 == 0 && c1 == chunks;
         // Pieces go through accesses of device scope (sc1), which no XCD's L2 holds back or stale: no cache is written back or
-        // emptied (a fence of that scope in each of 768 workgroups took 200 us).
+        // emptied (a fence of that scope in each of some hundred workgroups took 200 us).
         auto piece = [&](uint32_t k, uint32_t first) { return (2 * k + (k == first)) * (uint32_t)(PIECE * 4); };
         auto get4 = [&](uint32_t at) { return __builtin_bit_cast(kv_f4, __builtin_amdgcn_raw_buffer_load_b128(pieces, at, 0, AT_SC1)); };
         auto get = [&](uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pieces, at, 0, AT_SC1)); };
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
             const uint32_t n = wB - wA + 1;
             uint32_t size = n;
             // (32 pieces of 4 rows of 128 values are faster joined at once, of 16 rows of 256 in two levels: 37 us and 31 in all)
-            if (n > AT_JOIN || n * (uint32_t)(rows * D) > 1u << 16) size = (uint32_t)ceilf(sqrtf((float)n));      // 28 of 768
+            if (n > AT_JOIN || n * (uint32_t)(rows * D) > 1u << 16) size = (uint32_t)ceilf(sqrtf((float)n));      // 23 of 512
             const uint32_t groups = (n + size - 1) / size;
             auto last = [&](int *count, uint32_t of) {   // whether the others have all written theirs
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                       // they are in memory
@@ -498,13 +498,7 @@ __global__ __launch_bounds__(256, 2) void k_attn(AttnLaunch L) {
 // ================================================================================== host side
 template <int G, int NT, int PARTS>
 static void attn_go(bgl_ctx *c, const AttnLaunch &L, unsigned wgs) {
-    // no more workgroups than run at once: the runs are equal
-    static const unsigned at_once = [] {
-        int n = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn<G, NT, PARTS>, 256, 0) != hipSuccess) n = 2;
-        return (unsigned)std::max(1, n) * 256u;
-    }();
-    hipLaunchKernelGGL((k_attn<G, NT, PARTS>), dim3(std::min(wgs, at_once)), dim3(256), 0, c->stream, L);
+    hipLaunchKernelGGL((k_attn<G, NT, PARTS>), dim3(wgs), dim3(256), 0, c->stream, L);
 }
 template <int G>
 static void attn_pick(bgl_ctx *c, const AttnLaunch &L, int nt, unsigned wgs) {
