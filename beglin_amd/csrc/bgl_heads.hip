@@ -5,7 +5,7 @@
 //   y_i = n_i c_i - n_j s_i,  y_j = n_j c_i + n_i s_i                            for the pairs (i, j) that are rotated
 //   groups of 32: m = fp16(min), s = fp16((max - m) (1/15)), c = rint((x - m) / s), value fp16(c s + m)
 //
-// Bound by memory where tokens are many: 4096 tokens of 40 heads of 128 in bf16, norms and rotation, 18.8 us, 4.6 TB/s.  4096 tokens'
+// Bound by memory where tokens are many: 4096 tokens of 40 heads of 128 in bf16, norms and rotation, 18.0 us, 4.8 TB/s.  4096 tokens'
 // keys and values of 8 heads into the cache take 13.7 us, 22 MB: the vector units issue 11 of them (doubles, codes).  Few tokens are a launch
 // and a chain of loads, position, its row of the table, the head: 8 tokens of 48 heads 4.8 us.
 // A code changes by one where a value lies within rounding of a border between codes.  So y is computed in double and rounded
@@ -256,11 +256,11 @@ __device__ __forceinline__ void hd_put_v(uint8_t *rec, int D, int tok, int li, c
 // lines of a record, go to one XCD (workgroups go round the eight), whose L2 then puts their bytes together.
 static __device__ __forceinline__ int hd_token(int x, int n) { return n < 128 ? x : (x & ~127) + ((x & 7) << 4) + (x >> 3 & 15); }
 
-// A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other.  FAST, EXACT: which rows the launch has, those
-// of hd_row_fast, the others and the cache's, or both: few tokens are one launch, many take one each, for the others' doubles would leave the
-// fast ones half as many waves (4096 tokens of 40 heads, bf16: 49 us together).
-template <int GL, bool FAST, bool EXACT>
-__global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
+// A workgroup takes a token, each GL lanes (D / 8 of them at work) one head after the other: rows that go to q_out and k_out, and what goes into
+// the cache.  FAST: rows of hd_row_fast are among them, for few tokens, which are one launch.  Of many the fast rows are k_heads_fast's: the
+// others' doubles would leave them half as many waves (4096 tokens of 40 heads, bf16: 49 us together).
+template <int GL, bool FAST>
+__global__ __launch_bounds__(256, 2) void k_heads(HeadsLaunch L) {
     const bgl_heads &d = L.d;
     const int t = hd_token(blockIdx.x, d.T), li = threadIdx.x & (GL - 1), per = (int)blockDim.x / GL;
     if (t >= d.T) return;
@@ -290,38 +290,101 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 4) void k_heads(HeadsLaunch L) {
     if (i < L.nq) {
         HdWeights g = hd_weights(d, d.q_w, turn, d0);
         const HdFast f(d, g, turn);
-        const bool fast = FAST && (!EXACT || hd_fast(d));
+        const bool fast = FAST && hd_fast(d);
         for (; i < L.nq; i += step) {
             float x[8], px[8], y[8];
             load(x, px, d.q, t * d.ldq + i * d.hdq);
             if (fast) hd_row_fast<GL>(y, L, x, px, f);
-            else if constexpr (EXACT) hd_row<GL>(y, L, x, px, g, turn);
+            else hd_row<GL>(y, L, x, px, g, turn);
             if (in) kv_store8(d.q_out, d.out_type, t * d.ldqo + i * d.hdqo + d0, y);
         }
     }
     if (i < L.nq + L.nk) {
         HdWeights g = hd_weights(d, d.k_w, turn, d0);
         const HdFast f(d, g, turn);
-        const bool fast = FAST && (!EXACT || (d.k_out && hd_fast(d)));
+        const bool fast = FAST && d.k_out && hd_fast(d);
         for (; i < L.nq + L.nk; i += step) {
             const int h = i - L.nq;
             float x[8], px[8], y[8];
             if (!d.k_out && !kept) continue;
             load(x, px, d.k, t * d.ldk + h * d.hdk);
             if (fast) hd_row_fast<GL>(y, L, x, px, f);
-            else if constexpr (EXACT) hd_row<GL>(y, L, x, px, g, turn);
+            else hd_row<GL>(y, L, x, px, g, turn);
             if (!in) continue;
             if (d.k_out) kv_store8(d.k_out, d.out_type, t * d.ldko + h * d.hdko + d0, y);
-            else if constexpr (EXACT) hd_put_k(kv_at(L.c, slot, h), d.D, tok, li, y);
+            else hd_put_k(kv_at(L.c, slot, h), d.D, tok, li, y);
         }
     }
-    if (!EXACT || !kept || !in) return;
+    if (!kept || !in) return;
     for (; i < L.nq + L.nk + L.nv; i += step) {
         const int h = i - L.nq - L.nk;
         float y[8];
         kv_load8(y, d.v, d.type, t * d.ldv + h * d.hdv + d0);
         hd_put_v(kv_at(L.c, slot, h), d.D, tok, li, y);
     }
+}
+
+// 8 values of a row and their partners, as they lie in memory.
+template <bool F32>
+struct HdRaw {
+    kv_mu4 x[1 + F32], p[1 + F32];
+    __device__ __forceinline__ void load(const char *row, int d0, int other) {
+#pragma unroll
+        for (int e = 0; e <= F32; e++) {
+            x[e] = ((const kv_mu4 *)(row + (F32 ? 4 : 2) * d0))[e];
+            p[e] = ((const kv_mu4 *)(row + (F32 ? 4 : 2) * other))[e];
+        }
+    }
+    static __device__ __forceinline__ void values(float (&v)[8], const kv_mu4 (&u)[1 + F32], int type) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (F32) v[j] = __uint_as_float(u[j >> 2][j & 3]);
+            else if (type == BGL_T_F16) v[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[0][j / 2] >> (16 * (j & 1))));
+            else v[j] = __uint_as_float(j & 1 ? u[0][j / 2] & 0xffff0000u : u[0][j / 2] << 16);
+        }
+    }
+};
+// The rows of hd_row_fast alone, each on its way while the one before it is worked on (4096 tokens of 40 heads: 18.1 us, 19.2 without).
+template <int GL, bool F32>
+__global__ __launch_bounds__(256, 4) void k_heads_fast(HeadsLaunch L) {
+    const bgl_heads &d = L.d;
+    const int t = hd_token(blockIdx.x, d.T), li = threadIdx.x & (GL - 1), per = (int)blockDim.x / GL;
+    if (t >= d.T) return;
+    const bool in = 8 * li < d.D;
+    const int d0 = in ? 8 * li : 0, q_end = L.nq, total = L.nq + L.nk, step = (int)gridDim.y * per;
+    const int pos = d.rot_kind != BGL_ROT_NONE ? d.pos[t] : 0;
+    if (d.rot_kind != BGL_ROT_NONE && (uint32_t)pos >= (uint32_t)d.n_pos) return;
+    HdTurn turn = hd_turn(d, d.rope + (size_t)pos * d.rot, d0);
+    constexpr int ES = F32 ? 4 : 2;
+    const char *const q0 = (const char *)d.q + t * d.ldq * ES, *const k0 = (const char *)d.k + t * d.ldk * ES;
+    const long hdq = d.hdq * ES, hdk = d.hdk * ES;
+    auto row = [=](int i) {                              // the last one past it
+        const int x = min(i, total - 1);
+        return x < q_end ? q0 + x * hdq : k0 + (x - q_end) * hdk;
+    };
+    HdRaw<F32> raw;
+    int i = (int)blockIdx.y * per + (int)threadIdx.x / GL;
+    raw.load(row(i), d0, turn.other);
+    auto go = [&](int end, const float *w, void *out, long ld, long hd, int first) {
+        if (i >= end) return;
+        const HdWeights g = hd_weights(d, w, turn, d0);
+        const HdFast f(d, g, turn);
+        for (; i < end; i += step) {
+            float x[8], px[8], y[8];
+            HdRaw<F32>::values(x, raw.x, d.type);
+            HdRaw<F32>::values(px, raw.p, d.type);
+            raw.load(row(i + step), d0, turn.other);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[j] = in ? x[j] : 0.0f;
+                px[j] = turn.on ? px[j] : 0.0f;
+            }
+            hd_row_fast<GL>(y, L, x, px, f);
+            if (in) kv_store8(out, d.out_type, t * ld + (i - first) * hd + d0, y);
+        }
+    };
+    go(q_end, d.q_w, d.q_out, d.ldqo, d.hdqo, 0);
+    go(total, d.k_w, d.k_out, d.ldko, d.hdko, q_end);
 }
 
 struct KvReadLaunch {
@@ -412,12 +475,16 @@ static int heads_launch(bgl_ctx *c, const HeadsLaunch &all) {
                 hipLaunchKernelGGL(kernel, dim3(hd_tokens(d.T), hd_parts(d.T, nq + nk + nv, block / GL)), dim3((unsigned)block), 0, c->stream, L);
             };
             const bool q_fast = all.nq && hd_fast(d), k_fast = all.nk && d.k_out && hd_fast(d), exact = all.nv || (all.nq && !q_fast) || (all.nk && !k_fast);
-            if (!exact) go(k_heads<GL, true, false>, all.nq, all.nk, 0);
-            else if (!q_fast) go(k_heads<GL, false, true>, all.nq, all.nk, all.nv);
-            else if ((long)a.T * all.nq < HD_MANY) go(k_heads<GL, true, true>, all.nq, all.nk, all.nv);
+            auto go_fast = [&](int nq, int nk) {
+                if (d.type == BGL_T_F32) go(k_heads_fast<GL, true>, nq, nk, 0);
+                else go(k_heads_fast<GL, false>, nq, nk, 0);
+            };
+            if (!exact) go_fast(all.nq, all.nk);
+            else if (!q_fast) go(k_heads<GL, false>, all.nq, all.nk, all.nv);
+            else if ((long)a.T * all.nq < HD_MANY) go(k_heads<GL, true>, all.nq, all.nk, all.nv);
             else {
-                go(k_heads<GL, true, false>, all.nq, 0, 0);
-                go(k_heads<GL, false, true>, 0, all.nk, all.nv);
+                go_fast(all.nq, 0);
+                go(k_heads<GL, false>, 0, all.nk, all.nv);
             }
         });
     }
