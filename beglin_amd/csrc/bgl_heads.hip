@@ -420,11 +420,11 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
         } else {
             if (!L.v) continue;
             const int b = tok >> 2, r = tok & 3;
-            const uint8_t *p = rec + kv_v_codes(D) + (b * (D / 2) + 4 * li) * 4 + r;
-            const uint16_t *q = (const uint16_t *)(rec + kv_v_steps(D)) + ((li >> 2) * 4 + b) * 8 + (r & 1) * 2 + (r >> 1);
-            const uint32_t s = q[0], m = q[4];
+            typedef unsigned int u4 __attribute__((ext_vector_type(4)));               // of all four tokens
+            const u4 w = *(const u4 *)(rec + kv_v_codes(D) + (b * (D / 2) + 4 * li) * 4), z = *(const u4 *)(rec + kv_v_steps(D) + ((li >> 2) * 4 + b) * 16);
+            const uint32_t s = (r & 1 ? z[1] : z[0]) >> (16 * (r >> 1)), m = (r & 1 ? z[3] : z[2]) >> (16 * (r >> 1));
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = kv_value(p[4 * (e >> 1)] >> (4 * (e & 1)) & 15u, s, m);
+            for (int e = 0; e < 8; e++) y[e] = kv_value(w[e >> 1] >> (8 * r + 4 * (e & 1)) & 15u, s, m);
             kv_store8(L.v, L.type, t * L.ldv + h * L.hdv + d0, y);
         }
     }
