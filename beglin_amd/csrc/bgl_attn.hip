@@ -548,16 +548,19 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
     const int G = kv->D / 32;
-    // Many rows of a head at once are the prompt kernel's, where they are told of; beside them sequences of few rows stay here.
+    // Many rows of a head at once are the prompt kernel's, where they are told of.  Beside them sequences of few rows stay here, unless they are
+    // few and see few keys: as blocks that are nearly empty they cost less than a launch (9 sequences, 4 of them short, window 512: 50 us in two
+    // launches, 38.6 in one; 200 rows and 15 of one, 1000 keys each: 45 and 30, 2000 keys: 76 and 53; 2000 rows and 31 of one, 3000 keys: 126 and 143).
     const bool prompt = rows > AT_FEW;
     if (prompt) {
-        L.limit = a->S > 1 ? AT_FEW : 0;
+        const bool alone = a->S == 1 || ((long)a->S * kv->heads <= 256 && (a->window ? std::min((long)a->max_len, a->window + 256l) : a->max_len) <= 2048);
+        L.limit = alone ? 0 : AT_FEW;
         const int tok = prof_begin(c, 1);
         const int rc = run_attn_prompt(c, L);
         prof_end(c, tok);
         if (rc) return rc;
         HIPCHK(hipGetLastError());
-        if (a->S == 1) return 0;
+        if (alone) return 0;
         rows = AT_FEW;
     }
     const int nt = rows > 16 && G <= 4 ? 2 : 1, RB = 16 * nt;
