@@ -513,6 +513,18 @@ static void attn_pick(bgl_ctx *c, const AttnLaunch &L, int nt, unsigned wgs) {
     else attn_go<G, 1, 1>(c, L, wgs);
 }
 
+// The scratch of k_attn, whose size is fixed.  A call that does without it (`needed` false) reserves it all the same, outside a capture: after any
+// eager call one of single rows can be captured.
+static int attn_scratch(bgl_ctx *c, bool needed) {
+    const size_t part = (size_t)2 * AT_WG * 32 * (128 + 2) * 4, sync = 3 * AT_WG * sizeof(int);
+    if (c->attn_part.bytes >= part && c->attn_sync.bytes >= sync) return 0;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (!needed) HIPCHK(hipStreamIsCapturing(c->stream, &cs));
+    if (cs != hipStreamCaptureStatusNone) return 0;
+    if (const int rc = dbuf_reserve(c, c->attn_part, part, false)) return rc;
+    return dbuf_reserve(c, c->attn_sync, sync, true);
+}
+
 extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (!c || !a || !a->q || !a->out || !a->start || !a->len || !a->table) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: NULL argument");
     if (const int rc = kv_check("bgl_attn_dev", kv)) return rc;
@@ -552,8 +564,11 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     // few and see few keys: as blocks that are nearly empty they cost less than a launch (9 sequences, 4 of them short, window 512: 50 us in two
     // launches, 38.6 in one; 200 rows and 15 of one, 1000 keys each: 45 and 30, 2000 keys: 76 and 53; 2000 rows and 31 of one, 3000 keys: 126 and 143).
     const bool prompt = rows > AT_FEW;
+    const bool alone =
+        prompt && (a->S == 1 || ((long)a->S * kv->heads <= 256 && (a->window ? std::min((long)a->max_len, a->window + 256l) : a->max_len) <= 2048));
+    // k_attn's scratch is there before the first launch: a call that fails has launched nothing.
+    if (const int rc = attn_scratch(c, !alone)) return rc;
     if (prompt) {
-        const bool alone = a->S == 1 || ((long)a->S * kv->heads <= 256 && (a->window ? std::min((long)a->max_len, a->window + 256l) : a->max_len) <= 2048);
         L.limit = alone ? 0 : AT_FEW;
         const int tok = prof_begin(c, 1);
         const int rc = run_attn_prompt(c, L);
@@ -564,9 +579,7 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
         rows = AT_FEW;
     }
     const int nt = rows > 16 && G <= 4 ? 2 : 1, RB = 16 * nt;
-    if (const int rc = dbuf_reserve(c, c->attn_part, (size_t)2 * AT_WG * 32 * (128 + 2) * 4, false)) return rc;
-    if (const int rc = dbuf_reserve(c, c->attn_sync, 3 * AT_WG * sizeof(int), true)) return rc;
-    L.part = (float *)c->attn_part.p;
+    L.part = (float *)c->attn_part.p;                    // (a prompt whose keys are split may have had it grow)
     L.sync = (int *)c->attn_sync.p;
     // Up to four steps stay together: a head whose keys are one unit needs no join (8 heads over 512 keys: 10.4 us in units of 128).
     const long keys = a->window ? std::min((long)a->max_len, (long)a->window + rows) : a->max_len;
