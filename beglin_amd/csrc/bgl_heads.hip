@@ -89,17 +89,19 @@ __device__ __forceinline__ HdTurn hd_turn(const bgl_heads &d, const float *rope,
     }
     return t;
 }
-// The norm's factors of a lane's values and of their partners.
+// The norm's factors of a lane's values and of their partners, but for what is added to all of them (nothing where there are no weights).
 struct HdWeights {
-    float w[8], pw[8];
+    float w[8], pw[8], add;
 };
 __device__ __forceinline__ HdWeights hd_weights(const bgl_heads &d, const float *w, const HdTurn &t, int d0) {
     HdWeights g;
 #pragma unroll
     for (int j = 0; j < 8; j++) g.w[j] = g.pw[j] = 1.0f;
+    g.add = 0.0f;
     if (d.norm == BGL_NORM_NONE || !w) return g;
     kv_load8(g.w, w, BGL_T_F32, d0);
     kv_load8(g.pw, w, BGL_T_F32, t.other);
+    g.add = d.w_add;
     return g;
 }
 
@@ -110,7 +112,7 @@ struct HdFast {
     float a[8], b[8];
     bool on;
     __device__ __forceinline__ HdFast(const bgl_heads &d, const HdWeights &g, const HdTurn &t) {
-        const float add = d.norm != BGL_NORM_NONE ? d.w_add : 0.0f;
+        const float add = g.add;
         on = t.on;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -184,7 +186,7 @@ __device__ __forceinline__ void hd_row(float (&y)[8], const HeadsLaunch &L, cons
         for (int j = 0; j < 8; j++) q = fma(v[j], v[j], q);
         inv = rsqrt(fma(hd_sum<GL>(q), L.one_over, (double)d.eps));
     }
-    const double add = d.norm != BGL_NORM_NONE ? (double)d.w_add : 0.0;
+    const double add = (double)g.add;
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] *= add != 0.0 ? (double)g.w[j] + add : (double)g.w[j];
     if (d.rot_kind == BGL_ROT_NONE) {
