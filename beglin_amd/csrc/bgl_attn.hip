@@ -172,10 +172,19 @@ struct AttnWave {
             for (int x = 0; x < 8; x++) {
                 const int h = x >> 2, r = x & 3;
                 const float p = at_exp2(fmaf(s[t][h][r], fac[t], off));
-                l[t] += p;
+                if constexpr (PARTS == 2) l[t] += p;
                 const int at = 4 * h + at_place(r);
                 pf[t][0][at] = (_Float16)p;
                 if constexpr (PARTS == 2) pf[t][1][at] = (_Float16)(p - (float)pf[t][0][at]);
+            }
+            // Weights rounded to fp16 are summed as what they are multiplied as, so that a row's add up to 1: their error is then that of an average
+            // of values (unrounded sums: a row whose keys all have the value v was up to 4e-4 v off).  Two parts are 2^-22 off p.
+            if constexpr (PARTS == 1) {
+                const kv_h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int y = 0; y < 8; y += 2) sum[y >> 2] = __builtin_amdgcn_fdot2(kv_h2{pf[t][0][y], pf[t][0][y + 1]}, one, sum[y >> 2], false);
+                l[t] += sum[0] + sum[1];
             }
         }
 #pragma unroll

@@ -284,8 +284,8 @@ int  bgl_kv_read_dev(bgl_ctx *ctx, const bgl_kv *kv, const int32_t *slots, int n
  * becomes 0; rows of no sequence are left as they are.  out overlaps nothing that is read.  Keys j >= ldt * page do not
  * exist (ldt * page is 2^30 at most).  start never goes back: a call where it does writes some rows or none.
  * Sums, maxima and products' accumulators are fp32.  With fp16 and bf16 rows the weights exp(..) are rounded to fp16
- * before they multiply v (queries and cached values are exact as operands); with fp32 rows they and the queries are held
- * as two fp16 parts each, 22 bits.
+ * before they multiply v and before they are summed, so a row's add up to 1 (queries and cached values are exact as
+ * operands); with fp32 rows they and the queries are held as two fp16 parts each, 22 bits.
  * max_rows and max_len: the most rows and keys of a sequence as far as the caller knows; launch shapes go by them, no
  * result needs them to be right.  Rows of one sequence are summed in an order that its lengths and the batch's give:
  * the same call gives the same bits.  The first call reserves the context's scratch for partial sums (one with many rows
