@@ -74,11 +74,6 @@ template <int CTRL>
 __device__ __forceinline__ int dpp_i(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false); }
 template <int CTRL>
 __device__ __forceinline__ float dpp_f(float v) { return __int_as_float(dpp_i<CTRL>(__float_as_int(v))); }
-template <int CTRL>
-__device__ __forceinline__ double dpp_d(double v) {
-    const int2 p = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(dpp_i<CTRL>(p.x), dpp_i<CTRL>(p.y)));
-}
 __device__ __forceinline__ float rlane_f(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
 __device__ __forceinline__ float wave_max_f32(float v) {

@@ -34,6 +34,13 @@ __device__ __forceinline__ float i8_kept(float v, int type) {
     return type == BGL_T_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
 }
 
+// dpp_f (bgl_device.h) for doubles, for the sums of norms
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const int2 p = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(dpp_i<CTRL>(p.x), dpp_i<CTRL>(p.y)));
+}
+
 // ------------------------------------------------------------------ the per-token quantizer
 // q4_quant_act_i8's arithmetic (q4gemv.h:177-213) with the whole row as the group: mx = max(1e-8, max|x|),
 // sc = mx / 127, inv = 1 / sc, code = sat8(trunc(x * inv +- 0.5)).  The maximum is taken on the bits of
