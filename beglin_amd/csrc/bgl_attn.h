@@ -295,3 +295,5 @@ __device__ __forceinline__ float attn_factor(float M, float sum, bool sink, floa
 
 // The prompt kernel (bgl_attn_p.hip): the call's sequences with more than L.limit rows times g, L.limit < INT32_MAX.
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L);
+// Whether it takes all of a call's sequences, as far as the call's hints tell.
+bool attn_prompt_alone(const AttnLaunch &L);

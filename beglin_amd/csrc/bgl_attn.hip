@@ -569,12 +569,9 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
     const int G = kv->D / 32;
-    // Many rows of a head at once are the prompt kernel's, where they are told of.  Beside them sequences of few rows stay here, unless they are
-    // few and see few keys: as blocks that are nearly empty they cost less than a launch (9 sequences, 4 of them short, window 512: 50 us in two
-    // launches, 38.6 in one; 200 rows and 15 of one, 1000 keys each: 45 and 30, 2000 keys: 76 and 53; 2000 rows and 31 of one, 3000 keys: 126 and 143).
-    const bool prompt = rows > AT_FEW;
-    const bool alone =
-        prompt && (a->S == 1 || ((long)a->S * kv->heads <= 256 && (a->window ? std::min((long)a->max_len, a->window + 256l) : a->max_len) <= 2048));
+    // Many rows of a head at once are the prompt kernel's, where they are told of.  Beside them sequences of few rows stay here, unless it
+    // costs less to take them along as blocks that are nearly empty.
+    const bool prompt = rows > AT_FEW, alone = prompt && attn_prompt_alone(L);
     // k_attn's scratch is there before the first launch: a call that fails has launched nothing.
     if (const int rc = attn_scratch(c, !alone)) return rc;
     if (prompt) {

@@ -533,6 +533,34 @@ static int prompt_pick(bgl_ctx *c, const AttnLaunch &L) {
     }
 }
 
+// What the prompt kernel costs, in us, for the sequences of more than `limit` rows times g if their rows see `keys` keys: rounds of blocks on the CUs,
+// 64 keys at a time.  From the hints, of the rows beside the longest sequence's as many for each of the others.
+static double prompt_us(AttnLaunch L, int limit, double keys) {
+    const int G = L.c.D / 32;
+    const bool f32 = L.a.type == BGL_T_F32, wide = G > 4 || (G > 3 && f32);            // one wave a SIMD
+    L.limit = limit;
+    int RB = wide ? 128 : 256, cap = 256;
+    const PromptShape h = prompt_shape(L, G, RB);
+    if (!wide && !f32 && h.parts == 1 && h.items <= 256) { RB = 128; cap = 512; }      // (prompt_pick)
+    const long most = std::min(L.a.T, std::max(1, L.a.max_rows)), others = (L.a.T - most) * L.g, S = L.a.S - 1, count = others > S * limit ? S : 0;
+    const long items = ((most * L.g + RB - 1) / RB + (count ? count + std::max(0l, others - count) / RB : 0)) * L.c.heads * h.parts;
+    if (L.a.window) keys = std::min(keys, (double)L.a.window + RB);
+    return 8 + (items + cap - 1) / cap * std::max(1.0, keys / 64) / h.parts * (1 + G / 4.0) * (wide ? 1.05 : 0.7) + (h.parts > 1 ? 6 : 0);
+}
+// One launch for all sequences, or k_attn for those of few rows (some 15 us with its launch, and the keys at 5 MB a us)?  Their keys are as many as the
+// longest sequence's for all that is known, but a prompt's may be its own rows only: the two costs' geometric mean stands for what two
+// launches take, and a tenth more, so that either choice is wrong by little.  Of 165 calls, heads of 64 to 256, 2 to 32 sequences, the slower form is
+// taken in 16 by more than 15%, at most by 54%; the rule before, S * heads <= 256 and 2048 keys at most: in 40, by up to 110%.  (32 heads over 8, us in one
+// launch and in two.  bf16, heads of 128: 200 rows and 15 of one, 1000 keys each, 29 and 45; 300 rows of three, 300 keys, and 5 of one, 1500 keys, 43 and 28;
+// 2000 rows and 31 of one, 3000 keys each, 147 and 130.  Heads of 256: 40 rows and 31 of one, 2048 keys each, 179 and 85.  fp32, heads of 128: the same 154 and 78.)
+bool attn_prompt_alone(const AttnLaunch &L) {
+    if (L.a.S == 1) return true;
+    const long few = L.a.window ? std::min((long)L.a.max_len, L.a.window + 32l) : L.a.max_len;
+    const double rest = 15 + (double)(L.a.S - 1) * few * L.c.heads * L.c.D * 1.25 / 5e6;
+    const double one = prompt_us(L, 0, L.a.max_len), far = prompt_us(L, 32, L.a.max_len), near = prompt_us(L, 32, std::min(L.a.max_len, L.a.max_rows));
+    return one * one <= 1.2 * (far + rest) * (near + rest);
+}
+
 int run_attn_prompt(bgl_ctx *c, const AttnLaunch &L) {
     switch (L.c.D / 32) {
     case 2: return prompt_pick<2>(c, L);

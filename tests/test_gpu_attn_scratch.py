@@ -92,25 +92,28 @@ def captured(torch, c, st, call, mark):
 @pytest.mark.parametrize("seqs,nk,longest", [([(90, 90), (1, 90), (40, 90)], 64, 4000), ([(90, 90), (1, 90), (40, 90)], 1, 4000), ([(90, 90), (1, 90)], 200, 90),
                                              ([(40, 3000)], 1, 3000)], ids=str)
 def test_a_refused_call_has_launched_nothing(torch_dev, seqs, nk, longest):
-    """A context's first call inside a capture, which needs scratch (two kernels, or keys in parts): refused as a whole."""
+    """A context's first call inside a capture: refused as a whole where it needs scratch (two kernels, or keys in parts), or captured as a whole."""
     import beglin_amd as B
     torch = torch_dev
     st = torch.cuda.Stream()
     with torch.cuda.stream(st):
         b = Seqs(torch, seqs, nk, nk, 64, torch.float16)
-        c = B.Context(0, st.cuda_stream)
-        mark = torch.zeros(4, device="cuda")
+        c, other = B.Context(0, st.cuda_stream), B.Context(0, st.cuda_stream)
+        mark, want = torch.zeros(4, device="cuda"), torch.empty_like(b.out)
+        b.call(other, want, max_len=longest)
         st.synchronize()
         g, code = captured(torch, c, st, lambda c: b.call(c, max_len=longest), mark)
-        assert code == B.E_CAPTURE
+        assert code in (0, B.E_CAPTURE) and (code or longest == 90)
         for i in range(3):
+            b.out.fill_(7.0)
             g.replay()
             st.synchronize()
-            assert (b.out == 7).all() and (mark == i + 1).all()
+            assert (mark == i + 1).all() and ((b.out == 7).all() if code else torch.equal(b.out, want))
         b.call(c, max_len=longest)
         st.synchronize()
-        assert torch.isfinite(b.out.float()).all() and not (b.out == 7).all(-1).any()
+        assert torch.equal(b.out, want)
         c.close()
+        other.close()
 
 
 def test_a_prompt_without_scratch_is_captured_first(torch_dev):
