@@ -548,15 +548,12 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if (!(a->scale == a->scale) || a->scale - a->scale != 0.0f) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: scale is not finite");
     if (a->q == a->out) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: out is q");
     if ((long)a->T * (a->nq / kv->heads) > INT32_MAX / 2) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of %d heads", a->T, a->nq);
-    // keys are numbered, and units counted, in 32 bits
+    // keys are numbered in 32 bits
     if ((long)a->ldt * kv->page > 1l << 30) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d pages of %d tokens a sequence", a->ldt, kv->page);
-    if ((double)kv->heads * ((double)a->T * (a->nq / kv->heads) / 16 + a->S) * ((double)a->ldt * kv->page / AT_STEP + 2 + AT_PAUSE) > 2e9)
-        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows over %d pages of %d tokens", a->T, a->ldt, kv->page);
     const int g = a->nq / kv->heads;
     int rows = (int)std::min<long>((long)std::min(std::max(1, a->max_rows), a->T) * g, INT32_MAX);
     if (rows > AT_FEW && ((double)a->T * g / 128 + a->S) * kv->heads > 1 << 22)        // a launch has less than 2^32 threads
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: prompts of T=%d rows of %d heads", a->T, a->nq);
-    HIPCHK(hipSetDevice(c->device));
     AttnLaunch L;
     memset(&L, 0, sizeof L);
     L.c = *kv;
@@ -572,6 +569,11 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     // Many rows of a head at once are the prompt kernel's, where they are told of.  Beside them sequences of few rows stay here, unless it
     // costs less to take them along as blocks that are nearly empty.
     const bool prompt = rows > AT_FEW, alone = prompt && attn_prompt_alone(L);
+    // k_attn counts its units in 32 bits: of all rows, or beside prompts of AT_FEW for each sequence
+    const double blocks = std::min((double)a->T * g / 16 + a->S, prompt ? a->S * (AT_FEW / 16.0) : INFINITY);
+    if (!alone && kv->heads * blocks * ((double)a->ldt * kv->page / AT_STEP + 2 + AT_PAUSE) > 2e9)
+        return bgl_fail(BGL_E_ARG, "bgl_attn_dev: T=%d rows of S=%d sequences over %d pages of %d tokens", a->T, a->S, a->ldt, kv->page);
+    HIPCHK(hipSetDevice(c->device));
     // k_attn's scratch is there before the first launch: a call that fails has launched nothing.
     if (const int rc = attn_scratch(c, !alone)) return rc;
     if (prompt) {
