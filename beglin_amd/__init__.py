@@ -445,8 +445,8 @@ class Context:
         if rope is None:
             rot = ROT_NONE
         elif rot:
-            if rope.ndim != 2:
-                _refuse(f"{who}: rope is fp32 [positions][rot]")
+            if rope.ndim != 2 or pos is None:
+                _refuse(f"{who}: rope is fp32 [positions][rot], with pos int32 [{T}]")
             n_pos, size = rope.shape
             table, at = _floats(rope, n_pos * size, dev, who), _ints(pos, T, dev, who)
         if norm:
