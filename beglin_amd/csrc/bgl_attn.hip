@@ -552,7 +552,9 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     if ((long)a->ldt * kv->page > 1l << 30) return bgl_fail(BGL_E_ARG, "bgl_attn_dev: %d pages of %d tokens a sequence", a->ldt, kv->page);
     const int g = a->nq / kv->heads;
     int rows = (int)std::min<long>((long)std::min(std::max(1, a->max_rows), a->T) * g, INT32_MAX);
-    if (rows > AT_FEW && ((double)a->T * g / 128 + a->S) * kv->heads > 1 << 22)        // a launch has less than 2^32 threads
+    // Many rows of a head at once are the prompt kernel's, where they are told of; its offsets inside a head's part of a page have 32 bits.
+    const bool prompt = rows > AT_FEW && (size_t)(kv->page / KV_TILE) * kv_record(kv->D) <= 1ull << 32;
+    if (prompt && ((double)a->T * g / 128 + a->S) * kv->heads > 1 << 22)        // a launch has less than 2^32 threads
         return bgl_fail(BGL_E_ARG, "bgl_attn_dev: prompts of T=%d rows of %d heads", a->T, a->nq);
     AttnLaunch L;
     memset(&L, 0, sizeof L);
@@ -566,9 +568,8 @@ extern "C" int bgl_attn_dev(bgl_ctx *c, const bgl_kv *kv, const bgl_attn *a) {
     L.scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     L.limit = INT32_MAX;
     const int G = kv->D / 32;
-    // Many rows of a head at once are the prompt kernel's, where they are told of.  Beside them sequences of few rows stay here, unless it
-    // costs less to take them along as blocks that are nearly empty.
-    const bool prompt = rows > AT_FEW, alone = prompt && attn_prompt_alone(L);
+    // Beside prompts sequences of few rows stay here, unless it costs less to take them along as blocks that are nearly empty.
+    const bool alone = prompt && attn_prompt_alone(L);
     // k_attn counts its units in 32 bits: of all rows, or beside prompts of AT_FEW for each sequence
     const double blocks = std::min((double)a->T * g / 16 + a->S, prompt ? a->S * (AT_FEW / 16.0) : INFINITY);
     if (!alone && kv->heads * blocks * ((double)a->ldt * kv->page / AT_STEP + 2 + AT_PAUSE) > 2e9)
