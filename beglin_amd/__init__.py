@@ -486,7 +486,8 @@ class Context:
         """out = attention of the rows q [T][heads][D] over the cache (bgl_attn_dev): sequence s has the rows start[s] ..
         start[s + 1] - 1 and lens[s] keys in the pages table[s]; int32 tensors [S + 1], [S], [S][pages].  scale None: 1 / sqrt(D).
         sink: fp32 [heads].  max_rows, max_len: the most rows and keys of a sequence, where the program knows them (None: as if every
-        sequence had a row, and as many keys as the table's pages hold); launch shapes go by them, no result does."""
+        sequence had a row, and as many keys as the table's pages hold); kernels and launch shapes go by them, and so the order of
+        sums, but no result needs them to be right."""
         dev, who = self.device, "attention"
         if table.ndim != 2 or q.ndim != 3 or q.shape[2] != cache.dim or cache.device != dev:
             _refuse(f"attention: q [T][heads][{cache.dim}], table [S][pages], the cache on device {dev}")

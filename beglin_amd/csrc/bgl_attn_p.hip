@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 || (PARTS == 1 && G <= 4) ? 
 #pragma unroll
             for (int j = 0; j < G; j++) o[j] *= g;
         }
-        kv_h8 pf[4][PARTS];
+        kv_h8 pf[4][PARTS];                              // (one part for 16-bit rows: bgl_attn.hip has both sides)
         const float off = AT_P2 - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
         for (int x = 0; x < 32; x++) {

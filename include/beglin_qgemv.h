@@ -282,17 +282,18 @@ int  bgl_kv_read_dev(bgl_ctx *ctx, const bgl_kv *kv, const int32_t *slots, int n
  *     out = sum_j exp(scale q.k_j) v_j / (sum_j exp(scale q.k_j) + exp(sink[h]))
  * for head h of nq, which reads head h / (nq / heads) of the cache; sink NULL: without that term.  A row that sees no key
  * becomes 0; rows of no sequence are left as they are.  out overlaps nothing that is read.  Keys j >= ldt * page do not
- * exist (ldt * page is 2^30 at most).  start never goes back: a call where it does writes some rows or none.
+ * exist (ldt * page is 2^30 at most): a len[s] above that, or below 0, counts as held to 0 .. ldt * page, as start is to 0 .. T.  start never
+ * goes back: a call where it does writes some rows or none.
  * Further limits, by the counters of a launch: nq and cache heads 65535 at most; T * (nq / heads) below 2^30; where max_rows * (nq / heads)
  * is over 32, heads * (T * (nq / heads) / 128 + S) up to 2^22; and heads * B * (ldt * page / 128 + 5) up to 2 * 10^9, B = T * (nq / heads) / 16 + S, or
  * 2 S at most where max_rows * (nq / heads) is over 32 (one prompt, S = 1, is not bound by the last).
  * Sums, maxima and products' accumulators are fp32.  With fp16 and bf16 rows the weights exp(..) are rounded to fp16
  * before they multiply v and before they are summed, so a row's add up to 1 (queries and cached values are exact as
  * operands); with fp32 rows they and the queries are held as two fp16 parts each, 22 bits.
- * max_rows and max_len: the most rows and keys of a sequence as far as the caller knows; launch shapes go by them, no
- * result needs them to be right.  Rows of one sequence are summed in an order that its lengths and the batch's give:
- * the same call gives the same bits.  The first call reserves the context's scratch for partial sums (one with many rows
- * may have to grow it), which the context's calls and the graphs captured from it share: let them run one after the other. */
+ * max_rows and max_len: the most rows and keys of a sequence as far as the caller knows; kernels and launch shapes go by them, and with
+ * those the order of sums, but no result needs them to be right.  Rows of one sequence are summed in an order that its lengths, the batch's and
+ * the hints give: the same call gives the same bits.  The first call outside a capture reserves the context's scratch for partial sums (one with
+ * many rows may have to grow it), which the context's calls and the graphs captured from it share: let them run one after the other. */
 typedef struct {
     int S, T, nq;                                  /* sequences; rows of q and out; heads of q, a multiple of the cache's */
     const void *q; long ldq, hdq;

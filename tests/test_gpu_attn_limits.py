@@ -44,3 +44,26 @@ def test_long_prompts_over_wide_tables(torch_dev, ctx, seqs, window):  # noqa: F
             for h in (0, 13, nq - 1):
                 F.attention_near(host(out[at + i:at + rows[-1] + 1, h]), host(q[at + i:at + rows[-1] + 1, h]), k[key % n, h // g], v[key % n, h // g], D ** -0.5, see,
                                  None, "float16", (at, i, h))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 50])
+@pytest.mark.parametrize("window", [0, 20])
+def test_lengths_outside_the_table(torch_dev, ctx, rows, window):  # noqa: F811
+    """A length above ldt * page counts as ldt * page, one below 0 as 0."""
+    import beglin_amd
+    torch = torch_dev
+    D, page, wide = 64, 16, 5
+    cache = beglin_amd.KVCache(2 * wide, page, 2, D)
+    n = 2 * wide * page
+    ctx.kv_append(cache, torch.arange(n, dtype=torch.int32, device="cuda"), torch.randn((n, 2, D), device="cuda"), torch.randn((n, 2, D), device="cuda"))
+    table = torch.arange(2 * wide, dtype=torch.int32, device="cuda").reshape(2, wide)
+    q = torch.randn((2 * rows, 4, D), device="cuda")
+    start = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device="cuda")
+    outs = []
+    for lens in ((wide * page, 0), (wide * page + 7, -3), (2 ** 31 - 1, -2 ** 31)):
+        out = torch.full_like(q, 7.0)
+        ctx.attention(cache, q, out, start, torch.tensor(lens, dtype=torch.int32, device="cuda"), table, window=window, max_rows=rows)
+        torch.cuda.synchronize()
+        outs.append(out)
+    assert torch.isfinite(outs[0]).all() and (outs[0][rows:] == 0).all() and (outs[0][:rows] != 0).any()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
