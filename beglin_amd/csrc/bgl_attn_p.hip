@@ -7,8 +7,8 @@
 // buffers: the next keys are converted, and the ones after those loaded, while the matrix cores work on the present ones; one barrier a stage.
 // Each wave has 32 rows, as columns of S^T = K Q^T and O^T = V^T P^T; what a lane has of S^T is its part of P^T's operand.
 //
-// 4096 bf16 tokens of 32 heads of 128 over 8 of the cache: 164 us, 840 TFLOP/s of the rows' own products (a library's product of 8192^3
-// runs at 1180).  By counters the matrix units are busy 45% of that time and the vector units issue 50%: two waves a SIMD, which is what
+// 4096 bf16 tokens of 32 heads of 128 over 8 of the cache: 151 us among other launches, 910 TFLOP/s of the rows' own products (a library's product of
+// 8192^3 runs at 1180); 160 to 184 us by itself time after time, when the clock falls.  By counters the matrix units are busy 45% of that time and the vector units issue 50%: two waves a SIMD, which is what
 // 240 registers leave, hardly overlap them, and every instruction of the loop counts, scalar ones too (the same loop with 50 scalar
 // instructions more a stage: 181 us).  Tried and slower: the two waves of a SIMD in turns, half a stage apart (185 us); a stage's scores
 // between the products of the one before it; 16 x 16 tiles (190 us where these took 175); three waves a SIMD for heads of 64 (118 for 113).
@@ -534,7 +534,8 @@ static int prompt_pick(bgl_ctx *c, const AttnLaunch &L) {
 }
 
 // What the prompt kernel costs, in us, for the sequences of more than `limit` rows times g if their rows see `keys` keys: rounds of blocks on the CUs,
-// 64 keys at a time.  From the hints, of the rows beside the longest sequence's as many for each of the others.
+// 64 keys at a time (0.7 (1 + G / 4) us measured with two waves a SIMD, half as much again with one) behind some 8 us, 6 more with a second launch.  From
+// the hints, of the rows beside the longest sequence's as many for each of the others.
 static double prompt_us(AttnLaunch L, int limit, double keys) {
     const int G = L.c.D / 32;
     const bool f32 = L.a.type == BGL_T_F32, wide = G > 4 || (G > 3 && f32);            // one wave a SIMD

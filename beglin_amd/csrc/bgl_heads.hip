@@ -6,7 +6,8 @@
 //   groups of 32: m = fp16(min), s = fp16((max - m) (1/15)), c = rint((x - m) / s), value fp16(c s + m)
 //
 // Bound by memory where tokens are many: 4096 tokens of 40 heads of 128 in bf16, norms and rotation, 18.0 us, 4.8 TB/s.  4096 tokens'
-// keys and values of 8 heads into the cache take 13.7 us, 22 MB: the vector units issue 11 of them (doubles, codes).  Few tokens are a launch
+// keys and values of 8 heads into the cache take 13.5 us, 22 MB: the vector units issue 8.4 of them (doubles, codes), waves wait half
+// of their time.  Layer norms of 16-bit outputs, in double, 31 us where RMS norms take 17; fp32 outputs 34 us, 4.9 TB/s.  Few tokens are a launch
 // and a chain of loads, position, its row of the table, the head: 8 tokens of 48 heads 4.8 us.
 // A code changes by one where a value lies within rounding of a border between codes.  So y is computed in double and rounded
 // once to fp32, and from there each step is one fp32 operation: the codes are the formula's.  (gfx950 issues double
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadLaunch L) {
 #define HD_MANY (1 << 14)         // heads of queries that are a launch of their own beside the cache's rows
 
 // Threads a workgroup.  A wave by itself takes a token's heads one after the other, so that the token's position and its row of the table are
-// waited for less often (4096 tokens: keys and values 13.7 us, 17.8 in workgroups of 256; 40 heads 18.8 and 20.8); few tokens start faster in few
+// waited for less often (4096 tokens: keys and values 13.5 us, 17.8 in workgroups of 256; 40 heads 18.8 and 20.8); few tokens start faster in few
 // workgroups (1 token 3.4 us, 3.8 in waves).
 static int hd_block(int T) { return T < 8 ? 256 : 64; }
 // Workgroups a token: as many as it takes to do every head at once, while the launch leaves units idle.
